@@ -127,7 +127,7 @@ def _quantise(x):
     2^-100 and 2^7."""
     x = x.float()
     mant, power = torch.frexp(x.abs().amax(-1))               # amax = mant * 2^power, mant in [0.5, 1); 448 = 0.875 * 2^9
-    b = (power - 9 + (mant > 0.875)).clamp(-100, 7) + 127
+    b = torch.where(mant > 0, power - 9 + (mant > 0.875), -100).clamp(-100, 7) + 127
     return (x / _power(b)).clamp(-448.0, 448.0).to(E4M3), b.to(torch.uint8)
 
 
