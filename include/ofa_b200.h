@@ -221,6 +221,88 @@ int ofa_ln_bwd_noalloc(void* dx, float* dgamma, const void* dy, const void* x, c
 int ofa_noalloc_max_rows(void);
 const char* ofa_noalloc_last_error(void);
 
+/* ---- serving over a paged cache ---------------------------------------------------------------------------------------
+ * No counterpart in the reference (its decoder keeps one contiguous cache and serves one sequence). Operators for hosts that serve many
+ * sequences from a model trained here: each is one or two ordinary kernel launches on `stream` (a cudaStream_t, or NULL) of the current device,
+ * allocates nothing, keeps nothing between calls, can be captured into a graph, and returns without waiting. All pointers are device pointers of the
+ * current device unless stated; strides are counted in elements and not negative. Errors: OFA_BAD_ARGUMENT or OFA_CUDA_ERROR, nothing launched, text
+ * in ofa_serving_last_error() (per thread).
+ *
+ * Cache: n_pages pages of page_size rows for each of n_kv_heads heads; k and v have the same strides, a row's head_dim (64 or 128) values lie side by
+ * side on a 16-byte boundary. OFA_KV_E4M3 rows are e4m3 numbers with one scale byte b for each row and head: they stand for code * 2^(b - 127); b is in
+ * 27 .. 134, or 255 for a row that held an infinity or a NaN and reads back as NaN. Magnitudes above 57,344 (448 * 2^7) are held as that, the
+ * codes 0x7f and 0xff are not used with other scales than 255. */
+enum { OFA_KV_BF16 = 0, OFA_KV_E4M3 = 1 };
+typedef struct {
+  int dtype, head_dim, n_kv_heads, page_size, n_pages;
+  void *k, *v;
+  long long page_stride, head_stride, row_stride;
+  unsigned char *k_scale, *v_scale;                                   /* OFA_KV_E4M3 */
+  long long scale_page_stride, scale_head_stride, scale_row_stride;
+} ofa_kv_cache;
+
+/* The sequences of a call. Rows q_start[i] .. q_start[i+1] of the call's n_rows belong to sequence i, whose context has kv_len[i] positions WITH
+ * them: row t of its n rows is position kv_len[i] - n + t, and position p is row p % page_size of page pages[i][p / page_size]. Sequences may bring no rows;
+ * rows that none brings (behind the last, padding) are neither read nor written. The arrays are read on the device, so a replayed graph sees their current values.
+ * What is wrong there cannot be refused on the host; it never becomes an access out of range, and sets bits of *status (or-ed; may be NULL):
+ * 1 a page number outside the cache, 2 a length below 0 or beyond the page table, 4 q_start not rising or beyond n_rows (that sequence is left out). */
+enum { OFA_KV_BAD_PAGE = 1, OFA_KV_BAD_LENGTH = 2, OFA_KV_BAD_ROWS = 4 };
+typedef struct {
+  int n_seqs, max_pages;              /* rows and columns of the page table */
+  const int *q_start, *kv_len;        /* [n_seqs + 1], [n_seqs] */
+  const int* pages;                   /* [n_seqs][max_pages] */
+  long long pages_stride;
+  int max_new, max_kv;                /* the longest chunk and context, as far as the host knows them (0: not). They choose how work is cut; results for longer ones are right too */
+  int* status;
+} ofa_kv_batch;
+
+/* Keys and values (bf16, [n_rows][n_kv_heads][head_dim]) to their pages, in the cache's type: to 8 bits with the smallest power of two by which the row's largest
+ * magnitude fits 448, rounded to nearest even. Rows whose position is negative or has no page are not kept. No two rows of a call may have the same
+ * place. */
+int ofa_kv_append(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const void* k, const void* v, int n_rows,
+                  long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream);
+/* The reverse: the rows of the call are read from their pages (all of a context with q_start counting kv_len) and are exact in bf16. Rows
+ * without a place read as zeros. */
+int ofa_kv_read(const ofa_kv_cache* cache, const ofa_kv_batch* batch, void* k, void* v, int n_rows,
+                long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream);
+
+/* out[row][h] = softmax over the cached keys that the row sees of scale * q.k, times their values; heads h of [g * n_heads / n_kv_heads ...) share key/value head g.
+ * causal: a row at position p sees positions <= p, and with window > 0 only those > p - window; otherwise all kv_len. The rows' own keys
+ * have to be in the cache (ofa_kv_append). lse (may be NULL, [n_rows][n_heads] fp32): the natural logarithm of the sum of exponentials. A row
+ * that sees no key gets zeros and -inf. Keys without a page are not seen. What a row does not see does not reach it, infinities and NaN included.
+ * workspace: ofa_paged_attention_workspace() bytes, 16-byte aligned, contents of no interest before and after; calls that may overlap need one each. */
+typedef struct {
+  int n_rows, n_heads;
+  const void* q;  long long q_row_stride, q_head_stride;     /* bf16 */
+  void* out;      long long out_row_stride, out_head_stride; /* bf16 */
+  float* lse;
+  float scale;
+  int causal, window;
+  void* workspace; size_t workspace_bytes;
+} ofa_paged_attention_args;
+int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const ofa_paged_attention_args* args, void* stream);
+size_t ofa_paged_attention_workspace(const ofa_kv_cache* cache, const ofa_kv_batch* batch, int n_rows, int n_heads);
+
+/* One pass over logits [n_rows][vocab] (OFA_DTYPE_BF16 or OFA_DTYPE_F32; out may be in), in fp32, in this order:
+ *   a token that stands in the row's history:  x > 0 ? x / repetition : x * repetition
+ *   x - frequency * n - presence * (n > 0), n = how often it stands there behind the prompt
+ *   x + the sum of the row's biases with this id
+ *   -inf where bit (id % 32) of mask[row][id / 32] is 0
+ * History: tokens[row][0 .. n_tokens[row]) (n_tokens NULL: max_tokens of them), the first n_prompt[row] of which are the prompt (NULL: none). Tokens and bias ids
+ * outside the vocabulary are passed over. NULL leaves a step out; repetition should be > 0. A row whose mask allows nothing is -inf throughout. */
+typedef struct {
+  int dtype, n_rows, vocab;
+  const void* in;  long long in_stride;
+  void* out;       long long out_stride;
+  const int* tokens; long long tokens_stride; int max_tokens;
+  const int *n_tokens, *n_prompt;
+  const float *repetition, *presence, *frequency;             /* [n_rows] */
+  const int* bias_ids; const float* bias; long long bias_stride; int max_bias;   /* [n_rows][max_bias] */
+  const unsigned* mask; long long mask_stride;                /* [n_rows][ceil(vocab / 32)] */
+} ofa_logits_args;
+int ofa_logits_process(const ofa_logits_args* args, void* stream);
+const char* ofa_serving_last_error(void);
+
 #ifdef __cplusplus
 }
 #endif

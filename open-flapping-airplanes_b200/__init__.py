@@ -12,5 +12,13 @@ from .tasks import DeviceBuffer, run_phases, gemm_phase, phase, bf16_round, to_b
 
 build = build_mod.build
 
-__all__ = ["build", "capi", "dp", "Megakernel", "OfaError", "default_config", "flat_from_named", "DeviceBuffer", "run_phases",
+
+def __getattr__(name):
+    if name == "serving":                # needs torch, which the rest of the package does without
+        import importlib
+        return importlib.import_module(__name__ + ".serving")
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+__all__ = ["build", "capi", "dp", "serving", "Megakernel", "OfaError", "default_config", "flat_from_named", "DeviceBuffer", "run_phases",
            "gemm_phase", "phase", "bf16_round", "to_bf16_bits", "from_bf16_bits", "PARAM_ORDER_DOC"]

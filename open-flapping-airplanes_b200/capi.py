@@ -42,6 +42,32 @@ class Dims(C.Structure):
     _fields_ = [("vocab", C.c_int), ("d_model", C.c_int), ("n_layer", C.c_int), ("n_head", C.c_int), ("ctx_len", C.c_int), ("batch", C.c_int)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("head_dim", C.c_int), ("n_kv_heads", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_longlong), ("head_stride", C.c_longlong), ("row_stride", C.c_longlong),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_page_stride", C.c_longlong), ("scale_head_stride", C.c_longlong), ("scale_row_stride", C.c_longlong)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("max_pages", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("pages_stride", C.c_longlong),
+                ("max_new", C.c_int), ("max_kv", C.c_int), ("status", C.c_void_p)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("n_heads", C.c_int), ("q", C.c_void_p), ("q_row_stride", C.c_longlong), ("q_head_stride", C.c_longlong),
+                ("out", C.c_void_p), ("out_row_stride", C.c_longlong), ("out_head_stride", C.c_longlong), ("lse", C.c_void_p),
+                ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LogitsArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("n_rows", C.c_int), ("vocab", C.c_int), ("inp", C.c_void_p), ("in_stride", C.c_longlong), ("out", C.c_void_p), ("out_stride", C.c_longlong),
+                ("tokens", C.c_void_p), ("tokens_stride", C.c_longlong), ("max_tokens", C.c_int), ("n_tokens", C.c_void_p), ("n_prompt", C.c_void_p),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_stride", C.c_longlong), ("max_bias", C.c_int), ("mask", C.c_void_p), ("mask_stride", C.c_longlong)]
+
+
+_MOVE = [C.POINTER(KvCache), C.POINTER(KvBatch), C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_longlong, C.c_longlong, C.c_void_p]
+
 # every symbol include/ofa_b200.h declares: name -> (restype, argtypes)
 PROTOTYPES = {
     "ofa_default_config": (C.c_int, [C.POINTER(Config), C.c_char_p]),
@@ -100,6 +126,12 @@ PROTOTYPES = {
     "ofa_ln_bwd_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "ofa_noalloc_max_rows": (C.c_int, []),
     "ofa_noalloc_last_error": (C.c_char_p, []),
+    "ofa_kv_append": (C.c_int, _MOVE),
+    "ofa_kv_read": (C.c_int, _MOVE),
+    "ofa_paged_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(PagedAttentionArgs), C.c_void_p]),
+    "ofa_paged_attention_workspace": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvBatch), C.c_int, C.c_int]),
+    "ofa_logits_process": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
+    "ofa_serving_last_error": (C.c_char_p, []),
     "ofa_debug_set_task_shuffle": (None, [C.c_uint]),
     "ofa_release_caches": (C.c_int, []),
     "ofa_run_phases": (C.c_int, [C.c_int, C.POINTER(Dims), C.POINTER(Phase), C.c_int, C.c_int, C.POINTER(C.c_float), C.POINTER(C.c_float), C.POINTER(Status)]),
@@ -107,6 +139,7 @@ PROTOTYPES = {
 
 OK, TIMEOUT, DEVICE_ABORT, CUDA_ERROR, BAD_CONFIG, BAD_ARGUMENT, NOT_LAUNCHED = range(7)
 DTYPE_BF16, DTYPE_F32 = 0, 1
+KV_BF16, KV_E4M3 = 0, 1
 MODE_TRAIN, MODE_FORWARD, MODE_NO_OPT, MODE_DECODE_ONLY = 0, 1, 2, 3
 (TK_DATA, TK_EMBED, TK_LN_FWD, TK_GEMM, TK_ATT_FWD, TK_ATT_PREP, TK_ATT_BWD, TK_CE, TK_CE_MEAN, TK_LN_BWD, TK_LN_DG, TK_EMB_WTE,
  TK_EMB_WPE, TK_ADAMW, TK_BARRIER) = range(15)

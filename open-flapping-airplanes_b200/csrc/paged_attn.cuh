@@ -1,0 +1,392 @@
+// Attention of few rows over a paged cache: a token, or a few, per sequence, where reading the keys and values is all that counts.
+//
+// For each row: O = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = scale log2(e) q.k_j, over the keys it sees, in one pass with a running
+// maximum m. The rows of a key/value head (new tokens x the query heads that share it) are taken 16 at a time, the M of one mma.sync: with few rows the
+// tensor pipe idles whatever feeds it, and what counts is bytes in flight and few steps between the last byte and the answer. A block's four warps take
+// every fourth step of 32 keys and meet once, at the end; `nsplit` blocks share the keys of a tile and meet in combine_kernel.
+//
+// A lane copies what it will itself feed to the mma, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
+// there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output columns
+// are free as long as both operands agree:
+//   scores   lane (r = lane / 4, c = lane % 4) holds of key r of 8 the dims c * 16 B + ... of every 64 B; q is fetched in the same order
+//   output   lane holds of keys 2c, 2c + 1, 2c + 8, 2c + 9 of 16 the dims r * 16 B + ..., two keys side by side make a word of the B operand, and column
+//            2c + e of the n-th 8-column product is dim (2c + e) * 8 + n
+// Rows of the 8-bit cache become bf16 with four instructions for two elements (paged::widen).
+//
+// A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
+// infinities and NaN are taken out of its values and added to the rows that see it. Rows past the context and of a bad page are never read.
+#pragma once
+#include "paged.cuh"
+
+namespace ofa {
+namespace paged {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int MAX_SPLIT = 64;
+
+struct AttnArgs {
+  Batch b;
+  Pool c;
+  const bf16* q; long long q_row, q_head;
+  bf16* out; long long o_row, o_head;
+  float* lse;                       // [n_rows][n_heads] or null
+  int n_heads, n_kv_heads, causal, window;
+  Div group;
+  float scale_log2;
+  int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
+  float* part;                      // nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ bool odd_bits(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }   // an infinity or a NaN in the pair
+__device__ __forceinline__ uint32_t without_odd(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+  return w;
+}
+
+template <int D, bool E4M3> struct Few {
+  static constexpr int KEYS = 32, WARPS = 4;
+  static constexpr int KP = D * (E4M3 ? 1 : 2) / 64;            // 16-byte pieces of a key that a lane holds
+  static constexpr int VB = D * (E4M3 ? 1 : 2) / 8;             // bytes of a value row that a lane holds
+  static constexpr int VW = VB >= 16 ? 16 : 8, VP = VB / VW;    // ... in pieces of VW
+  static constexpr int K_BYTES = 4 * KP * 512, V_BYTES = 8 * VB * 32;
+  static constexpr int SIDE = 3 * 128;                          // scale words of K and V, flags
+  static constexpr int STAGE = K_BYTES + V_BYTES + SIDE;
+  static constexpr int STAGES = K_BYTES + V_BYTES >= 16384 ? 3 : 4;
+  static constexpr int SMEM = WARPS * STAGES * STAGE;
+  static_assert(WARPS * 16 * (D + 2) * 4 <= SMEM, "the meeting of the warps does not fit");
+};
+
+// one held element as a float (the rare path)
+template <bool E4M3> __device__ float held(const char* row, int d, int scale) {
+  if constexpr (E4M3) return __uint_as_float(widen((uint32_t)*reinterpret_cast<const unsigned char*>(row + d) << 8, scale_bits(scale)) << 16);
+  return to_f(reinterpret_cast<const bf16*>(row)[d]);
+}
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ AttnArgs P) {
+  using F = Few<D, E4M3>;
+  constexpr int NT = D / 8, KS = D / 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const int split = (int)blockIdx.x % P.nsplit, tile0 = (int)blockIdx.x / P.nsplit % P.tiles, seq = (int)blockIdx.x / P.nsplit / P.tiles, kvh = blockIdx.y;
+  const Chunk ch = chunk_of(P.b, seq);
+  const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
+  if (ch.len > cap && threadIdx.x == 0) flag(P.b.status, ST_LENGTH);
+  unsigned char* ring = smem + warp * F::STAGES * F::STAGE;
+  const uint32_t ring_s = smem_u32(ring);
+  const char* kb = P.c.k + (long long)kvh * P.c.head_b;
+  const char* vb = P.c.v + (long long)kvh * P.c.head_b;
+
+  for (int tile = tile0; tile * 16 < ch.n * group; tile += P.tiles) {
+    // this thread's rows r and r + 8 of the tile
+    int pos[2];
+    uint32_t qf[KS][4];
+    const int t_last = min(ch.n - 1, (int)P.group.quot(tile * 16 + 15)), p_min = ch.p0 + (int)P.group.quot(tile * 16), p_max = ch.p0 + t_last;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int rr = tile * 16 + r + 8 * h, t = (int)P.group.quot(rr);
+      const bool on = t < ch.n;
+      pos[h] = on ? ch.p0 + t : p_max;
+      const bf16* src = P.q + (long long)(on ? ch.s + t : ch.s) * P.q_row + (long long)(kvh * group + rr - t * group) * P.q_head;
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        const int d = E4M3 ? ((s / 4) * 4 + c) * 16 + (s % 4) * 4 : ((s / 2) * 4 + c) * 8 + (s % 2) * 4;
+        const uint2 w = on ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+        qf[s][h] = w.x; qf[s][2 + h] = w.y;
+      }
+    }
+    const int hi = min(cap, P.causal ? p_max + 1 : ch.len), lo = P.window ? max(0, p_min - P.window + 1) : 0;
+    const int first = lo / F::KEYS, nst = max(0, (hi + F::KEYS - 1) / F::KEYS - first);
+    const int a = first + (int)((long long)nst * split / P.nsplit) + warp, b = first + (int)((long long)nst * (split + 1) / P.nsplit);
+    const int mine = b > a ? (b - a + F::WARPS - 1) / F::WARPS : 0;
+
+    float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < NT; t++) { o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f; }
+
+    auto issue = [&](int i) {                                    // the warp's i-th step: a lane looks up one key and copies its parts of all 32
+      const int p = (a + i * F::WARPS) * F::KEYS + lane;
+      int page = 0, at = 0;
+      const bool ok = p >= lo && p < hi && locate(P.b, seq, p, page, at);
+      const long long off = ok ? (long long)page * P.c.page_b + (long long)at * P.c.row_b : -1;
+      const int slot = i % F::STAGES;
+      const uint32_t dk = ring_s + slot * F::STAGE, dv = dk + F::K_BYTES, side = dv + F::V_BYTES;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const long long o2 = __shfl_sync(0xffffffffu, off, j * 8 + r);
+#pragma unroll
+        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, o2 >= 0 ? kb + o2 + x * 64 + c * 16 : kb, o2 >= 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const long long o2 = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8);
+#pragma unroll
+        for (int x = 0; x < F::VP; x++) {
+          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, o2 >= 0 ? vb + o2 + x * 128 + r * 16 : vb, o2 >= 0);
+          else cp8(dv + j * 256 + lane * 8, o2 >= 0 ? vb + o2 + r * 8 : vb, o2 >= 0);
+        }
+      }
+      uint32_t fl = ok ? 16u : 0u;
+      if constexpr (E4M3) {                                      // the aligned word around the scale byte; which byte of it is kept beside it
+        const long long so = ok ? (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row : 0;
+        const unsigned long long ka = reinterpret_cast<unsigned long long>(P.c.ks + so), va = reinterpret_cast<unsigned long long>(P.c.vs + so);
+        cp4(side + lane * 4, reinterpret_cast<const void*>(ka & ~3ull), ok);
+        cp4(side + 128 + lane * 4, reinterpret_cast<const void*>(va & ~3ull), ok);
+        fl |= (uint32_t)(ka & 3) | (uint32_t)(va & 3) << 2;
+      }
+      *reinterpret_cast<uint32_t*>(ring + slot * F::STAGE + F::K_BYTES + F::V_BYTES + 256 + lane * 4) = fl;
+    };
+
+    auto step = [&](int i) {
+      const int slot = i % F::STAGES, k0 = (a + i * F::WARPS) * F::KEYS;
+      unsigned char* sk = ring + slot * F::STAGE;
+      unsigned char* sv = sk + F::K_BYTES;
+      const uint32_t* side = reinterpret_cast<const uint32_t*>(sv + F::V_BYTES);
+      const uint32_t fl = side[64 + lane], valid = __ballot_sync(0xffffffffu, fl & 16u);
+      uint32_t kf = 0, vf = 0;                                   // 2^120 times the scales of this lane's key
+      if constexpr (E4M3) {
+        kf = scale_bits((side[lane] >> ((fl & 3) * 8)) & 255);
+        vf = scale_bits((side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255);
+      }
+      const bool mask = valid != 0xffffffffu || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 <= p_max - P.window);
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        uint32_t f = 0;
+        if constexpr (E4M3) { f = __shfl_sync(0xffffffffu, kf, j * 8 + r); f |= f << 16; }
+#pragma unroll
+        for (int x = 0; x < F::KP; x++) {
+          const uint4 w = *reinterpret_cast<const uint4*>(sk + (j * F::KP + x) * 512 + lane * 16);
+          if constexpr (E4M3) {
+            mma16816(s[j], qf[4 * x], widen_lo(w.x, f), widen_hi(w.x, f));
+            mma16816(s[j], qf[4 * x + 1], widen_lo(w.y, f), widen_hi(w.y, f));
+            mma16816(s[j], qf[4 * x + 2], widen_lo(w.z, f), widen_hi(w.z, f));
+            mma16816(s[j], qf[4 * x + 3], widen_lo(w.w, f), widen_hi(w.w, f));
+          } else {
+            mma16816(s[j], qf[2 * x], w.x, w.y);
+            mma16816(s[j], qf[2 * x + 1], w.z, w.w);
+          }
+        }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[j][e] *= P.scale_log2;
+          if (mask) {
+            const int kk = j * 8 + 2 * c + (e & 1), p = k0 + kk, h = e >> 1;
+            if (!((valid >> kk) & 1) || (P.causal && p > pos[h]) || (P.window && p <= pos[h] - P.window)) s[j][e] = -INFINITY;
+          }
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+        float al[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float mn = fmaxf(m[h], mx[h]);
+          al[h] = mn == -INFINITY ? 1.f : ex2_approx(m[h] - mn);
+          m[h] = mn; l[h] *= al[h];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) { o[t][0] *= al[0]; o[t][1] *= al[0]; o[t][2] *= al[1]; o[t][3] *= al[1]; }
+      }
+      const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};   // a row that has seen no key yet: 2^(-inf - 0) = 0
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[j][e] = ex2_approx(s[j][e] - ms[e >> 1]);
+        l[0] += s[j][0] + s[j][1]; l[1] += s[j][2] + s[j][3];
+      }
+      if (mask) {                                                // values that some row must not meet: none of them may be an infinity or a NaN
+        bool odd = false;
+        if constexpr (E4M3) { if (vf == 0x7fc0u && (fl & 16u)) { odd = true; vf = 0; } }
+        else {
+#pragma unroll 1
+          for (int x = 0; x < F::V_BYTES / 512; x++) {
+            uint4* w = reinterpret_cast<uint4*>(sv + x * 512 + lane * 16);
+            uint4 u = *w;
+            if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
+              odd = true;
+              *w = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+          for (int kk = 0; kk < F::KEYS; kk++) {
+            const int p = k0 + kk;
+            int page, at;
+            if (!((valid >> kk) & 1) || !locate(P.b, seq, p, page, at)) continue;
+            const char* row = vb + (long long)page * P.c.page_b + (long long)at * P.c.row_b;
+            const int sc = E4M3 ? P.c.vs[(long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row] : 0;
+            const bool see[2] = {!(P.causal && p > pos[0]) && !(P.window && p <= pos[0] - P.window), !(P.causal && p > pos[1]) && !(P.window && p <= pos[1] - P.window)};
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const int d = E4M3 ? (2 * c + e) * NT + t : (t / 8) * 64 + (2 * c + e) * 8 + t % 8;
+                const float x = held<E4M3>(row, d, sc);
+                if (!isfinite(x)) { if (see[0]) o[t][e] += x; if (see[1]) o[t][2 + e] += x; }
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; kb2++) {
+        // P is rounded to bf16 for the product (half a step, 2^-9 of each term, averaged over the keys); its sum l is taken before
+        const uint32_t pf[4] = {pack2f(s[2 * kb2][0], s[2 * kb2][1]), pack2f(s[2 * kb2][2], s[2 * kb2][3]), pack2f(s[2 * kb2 + 1][0], s[2 * kb2 + 1][1]), pack2f(s[2 * kb2 + 1][2], s[2 * kb2 + 1][3])};
+        uint32_t f01 = 0, f89 = 0;
+        if constexpr (E4M3) {
+          f01 = __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c) | __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 1) << 16;
+          f89 = __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 8) | __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 9) << 16;
+        }
+#pragma unroll
+        for (int x = 0; x < F::VP; x++) {
+          uint32_t w[4][F::VW / 4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if constexpr (F::VW == 16) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sv + ((kb2 * 4 + j) * F::VP + x) * 512 + lane * 16);
+              w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(sv + (kb2 * 4 + j) * 256 + lane * 8);
+              w[j][0] = u.x; w[j][1] = u.y;
+            }
+          }
+          if constexpr (E4M3) {
+#pragma unroll
+            for (int t = 0; t < F::VW; t++) {                    // byte t % 4 of both keys' words, to bytes 1 and 3
+              const unsigned sel = (unsigned)((t % 4) << 4 | (4 + t % 4) << 12);
+              mma16816(o[x * F::VW + t], pf, widen(__byte_perm(w[0][t / 4], w[1][t / 4], sel), f01), widen(__byte_perm(w[2][t / 4], w[3][t / 4], sel), f89));
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+              const unsigned sel = t & 1 ? 0x7632u : 0x5410u;
+              mma16816(o[x * 8 + t], pf, __byte_perm(w[0][t / 2], w[1][t / 2], sel), __byte_perm(w[2][t / 2], w[3][t / 2], sel));
+            }
+          }
+        }
+      }
+    };
+
+#pragma unroll
+    for (int i = 0; i < F::STAGES - 1; i++) { if (i < mine) issue(i); cp_commit(); }
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+      if (i + F::STAGES - 1 < mine) issue(i + F::STAGES - 1);
+      cp_commit();
+      cp_wait<F::STAGES - 1>();
+      step(i);
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; h++) { l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1); l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2); }
+
+    // the warps meet: 16 rows of D sums each, and {m, l}
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);
+    float2* sm = reinterpret_cast<float2*>(so + F::WARPS * 16 * D);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float* dst = so + (warp * 16 + r + 8 * h) * D;
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int t = 0; t < NT; t += 4) {
+          const int d = E4M3 ? (2 * c + e) * NT + t : (t / 8) * 64 + (2 * c + e) * 8 + t % 8;
+          *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][2 * h + e], o[t + 1][2 * h + e], o[t + 2][2 * h + e], o[t + 3][2 * h + e]);
+        }
+      if (c == 0) sm[warp * 16 + r + 8 * h] = make_float2(m[h], l[h]);
+    }
+    __syncthreads();
+    {
+      constexpr int DP = D / 8;                                  // eight threads a row
+      const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rr = tile * 16 + row, t = (int)P.group.quot(rr);
+      if (t < ch.n) {
+        float mm = -INFINITY, ll = 0.f, acc[DP] = {};
+#pragma unroll
+        for (int w = 0; w < F::WARPS; w++) mm = fmaxf(mm, sm[w * 16 + row].x);
+#pragma unroll
+        for (int w = 0; w < F::WARPS; w++) {
+          const float2 ml = sm[w * 16 + row];
+          const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);      // no key seen, or only scores of -inf: sums of 0, or not finite
+          ll += ml.y * f;
+#pragma unroll
+          for (int x = 0; x < DP; x++) acc[x] += so[(w * 16 + row) * D + part * DP + x] * f;
+        }
+        const int head = kvh * group + rr - t * group;
+        const long long g = (long long)(ch.s + t) * P.n_heads + head;
+        if (P.nsplit == 1) {
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * DP;
+#pragma unroll
+          for (int x = 0; x < DP; x++) acc[x] *= inv;
+#pragma unroll
+          for (int x = 0; x < DP; x += 8) *reinterpret_cast<uint4*>(dst + x) = pack8(acc + x);
+          if (P.lse && part == 0) P.lse[g] = ll == 0.f ? -INFINITY : mm * LN2 + logf(ll);
+        } else {
+          float* dst = P.part + (g * P.nsplit + split) * D + part * DP;
+#pragma unroll
+          for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(dst + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+          if (part == 0) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(mm, ll);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the splits of a row and head, in their order: a warp each. Rows that no sequence brought have no parts and are left as they are.
+template <int D> __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ AttnArgs P) {
+  const long long g = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int row = (int)(g / P.n_heads), head = (int)(g - (long long)row * P.n_heads);
+  const bool mine = row >= __ldg(P.b.q_start) && row < min(__ldg(P.b.q_start + P.b.n_seqs), P.b.n_rows);
+  cudaGridDependencySynchronize();
+  if (!mine) return;
+  const float2* ml = reinterpret_cast<const float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D) + g * P.nsplit;
+  float2 a = lane < P.nsplit ? ml[lane] : make_float2(-INFINITY, 0.f), b = lane + 32 < P.nsplit ? ml[lane + 32] : make_float2(-INFINITY, 0.f);
+  const float mm = warp_max(fmaxf(a.x, b.x));
+  const float fa = a.x == -INFINITY ? 1.f : ex2_approx(a.x - mm), fb = b.x == -INFINITY ? 1.f : ex2_approx(b.x - mm);
+  const float ll = warp_sum(a.y * fa + b.y * fb);
+  constexpr int DP = D / 32;
+  float acc[DP] = {};
+  const float* src = P.part + g * P.nsplit * D + lane * DP;
+  for (int s = 0; s < P.nsplit; s++) {
+    const float f = __shfl_sync(0xffffffffu, s < 32 ? fa : fb, s & 31);
+#pragma unroll
+    for (int x = 0; x < DP; x++) acc[x] += src[(long long)s * D + x] * f;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  bf16* dst = P.out + (long long)row * P.o_row + (long long)head * P.o_head + lane * DP;
+#pragma unroll
+  for (int x = 0; x < DP; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack2f(acc[x] * inv, acc[x + 1] * inv);
+  if (P.lse && lane == 0) P.lse[g] = ll == 0.f ? -INFINITY : mm * LN2 + logf(ll);
+}
+
+}  // namespace paged
+}  // namespace ofa

@@ -1,0 +1,99 @@
+// Rows of new keys and values to their pages, and back: one pass, bound by its bytes (or, for a step of a few tokens, by one launch and three
+// dependent loads: q_start, the page table, the row).
+//
+// A thread holds 16 bytes of a bf16 row, so a row of head_dim values is 8 or 16 neighbouring lanes: the largest magnitude is found as an unsigned maximum of
+// the bits without signs (an infinity or a NaN is then the largest) and shared with three or four shuffles; scaling by a power of two is exact, so the
+// only rounding is the one to e4m3 (to nearest, half a step 2^-4 relative). A block takes consecutive rows of the call; its threads compare the starts of
+// all sequences with them once and leave each row's page in shared memory.
+#pragma once
+#include <cuda_fp8.h>
+#include "paged.cuh"
+
+namespace ofa {
+namespace paged {
+
+struct MoveArgs {
+  Batch b;
+  Pool c;
+  bf16 *k, *v;                                        // rows of the call: read by append, written by read
+  long long k_row, k_head, v_row, v_head;             // strides in elements
+  int n_kv_heads, rows;                               // rows a block takes
+  Div pair;                                           // by 2 * n_kv_heads
+};
+constexpr int MOVE_ROWS = 64;                         // at most
+
+__device__ __forceinline__ unsigned max_bits(uint4 u) {
+  unsigned m = 0;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+  return m;
+}
+__device__ __forceinline__ uint32_t to_e4m3(uint32_t lo, uint32_t hi, float f) {
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&lo)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi));
+  const uint32_t x = __nv_cvt_float2_to_fp8x2(make_float2(a.x * f, a.y * f), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t y = __nv_cvt_float2_to_fp8x2(make_float2(b.x * f, b.y * f), __NV_SATFINITE, __NV_E4M3);
+  return x | y << 16;
+}
+
+template <int D, bool E4M3, bool READ>
+__global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ MoveArgs P) {
+  constexpr int LANES = D / 8;                        // of a row
+  __shared__ int2 place[MOVE_ROWS];                   // page and row in it; x = -1: nowhere, -2: no sequence's row
+  const int tid = threadIdx.x, r0 = blockIdx.x * P.rows, r1 = min(r0 + P.rows, P.b.n_rows);
+  if (tid < MOVE_ROWS) place[tid] = make_int2(-2, 0);
+  __syncthreads();
+  for (int i = tid; i < P.b.n_seqs; i += 256) {       // the sequence of each row
+    const int s = __ldg(P.b.q_start + i), e = __ldg(P.b.q_start + i + 1);
+    if (s < 0 || e < s || e > P.b.n_rows) { flag(P.b.status, ST_ROWS); continue; }
+    for (int row = max(s, r0); row < min(e, r1); row++) place[row - r0].x = i;
+  }
+  __syncthreads();
+  if (tid < MOVE_ROWS && place[tid].x >= 0) {
+    const int i = place[tid].x;
+    const Chunk ch = chunk_of(P.b, i);
+    const int pos = ch.p0 + r0 + tid - ch.s;
+    int page, at;
+    if (pos < 0 || !locate(P.b, i, pos, page, at)) page = -1, at = 0;
+    place[tid] = make_int2(page, at);
+  }
+  __syncthreads();
+  const int total = (r1 - r0) * 2 * P.n_kv_heads * LANES;
+  for (int base = 0; base < total; base += 256) {
+    const int it = base + tid, part = it % LANES, vec = it / LANES, row = (int)P.pair.quot(vec), wh = vec - row * 2 * P.n_kv_heads;
+    const bool is_v = wh >= P.n_kv_heads;
+    const int head = is_v ? wh - P.n_kv_heads : wh;
+    const int2 pl = it < total ? place[row] : make_int2(-2, 0);
+    bf16* x = it < total ? (is_v ? P.v + (long long)(r0 + row) * P.v_row + (long long)head * P.v_head : P.k + (long long)(r0 + row) * P.k_row + (long long)head * P.k_head) + part * 8 : nullptr;
+    char* held = (is_v ? P.c.v : P.c.k) + (long long)pl.x * P.c.page_b + (long long)head * P.c.head_b + (long long)pl.y * P.c.row_b + part * (E4M3 ? 8 : 16);
+    unsigned char* sc = E4M3 ? (is_v ? P.c.vs : P.c.ks) + (long long)pl.x * P.c.s_page + (long long)head * P.c.s_head + (long long)pl.y * P.c.s_row : nullptr;
+    if constexpr (READ) {
+      if (pl.x == -2) continue;
+      uint4 u = make_uint4(0, 0, 0, 0);               // a row that is nowhere reads as zeros
+      if (pl.x >= 0) {
+        if constexpr (E4M3) {
+          const uint2 w = *reinterpret_cast<const uint2*>(held);
+          uint32_t f = scale_bits(*sc); f |= f << 16;
+          u = make_uint4(widen_lo(w.x, f), widen_hi(w.x, f), widen_lo(w.y, f), widen_hi(w.y, f));
+        } else u = *reinterpret_cast<const uint4*>(held);
+      }
+      *reinterpret_cast<uint4*>(x) = u;
+    } else {
+      const uint4 u = pl.x >= 0 ? *reinterpret_cast<const uint4*>(x) : make_uint4(0, 0, 0, 0);
+      if constexpr (E4M3) {
+        unsigned m = max_bits(u);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int b = scale_byte(m);
+        const float f = __uint_as_float((uint32_t)(254 - (b == SCALE_NAN ? 127 : b)) << 23);          // 2^(127 - b)
+        if (pl.x >= 0) {
+          *reinterpret_cast<uint2*>(held) = b == SCALE_NAN ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : make_uint2(to_e4m3(u.x, u.y, f), to_e4m3(u.z, u.w, f));
+          if (part == 0) *sc = (unsigned char)b;
+        }
+      } else if (pl.x >= 0) *reinterpret_cast<uint4*>(held) = u;
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace ofa

@@ -1,0 +1,204 @@
+// Serving operators on the caller's stream (include/ofa_b200.h, "serving over a paged cache"): argument checks and launches. They allocate
+// nothing, keep nothing from one call to the next and touch no other stream, so they can be captured into graphs and run side by side.
+#include "../../include/ofa_b200.h"
+#include "logits.cuh"
+#include "paged_attn.cuh"
+#include "paged_move.cuh"
+#include <cuda_runtime.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+using namespace ofa;
+
+namespace {
+
+thread_local char g_error[256] = "";
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_error, sizeof g_error, fmt, ap);
+  va_end(ap);
+  return code;
+}
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
+}
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// ---- checks shared by the operators over a cache
+int check_cache(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, paged::Batch& B, paged::Pool& C) {
+  if (!c || !b) return fail(OFA_BAD_ARGUMENT, "null pointer");
+  if (c->dtype != OFA_KV_BF16 && c->dtype != OFA_KV_E4M3) return fail(OFA_BAD_ARGUMENT, "cache dtype %d is neither OFA_KV_BF16 nor OFA_KV_E4M3", c->dtype);
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(OFA_BAD_ARGUMENT, "head_dim %d: 64 and 128 are built", c->head_dim);
+  if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return fail(OFA_BAD_ARGUMENT, "n_kv_heads %d is outside 1 .. 65535", c->n_kv_heads);
+  if (c->page_size < 1 || c->n_pages < 0) return fail(OFA_BAD_ARGUMENT, "page_size %d, n_pages %d", c->page_size, c->n_pages);
+  if (n_rows < 0 || b->n_seqs < 0 || b->max_pages < 0 || b->max_new < 0 || b->max_kv < 0)
+    return fail(OFA_BAD_ARGUMENT, "negative size: n_rows %d, n_seqs %d, max_pages %d, max_new %d, max_kv %d", n_rows, b->n_seqs, b->max_pages, b->max_new, b->max_kv);
+  const bool e4m3 = c->dtype == OFA_KV_E4M3;
+  const long long es = e4m3 ? 1 : 2;
+  if (n_rows > 0 && b->n_seqs > 0) {
+    if (!b->q_start || !b->kv_len || (b->max_pages > 0 && !b->pages)) return fail(OFA_BAD_ARGUMENT, "null pointer in the batch");
+    if (c->n_pages > 0 && (!c->k || !c->v)) return fail(OFA_BAD_ARGUMENT, "null pointer in the cache");
+    if (e4m3 && c->n_pages > 0 && (!c->k_scale || !c->v_scale)) return fail(OFA_BAD_ARGUMENT, "an e4m3 cache needs scales");
+  }
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || (c->page_stride * es) % 16 || (c->head_stride * es) % 16 || (c->row_stride * es) % 16)
+    return fail(OFA_BAD_ARGUMENT, "cached rows start on 16-byte boundaries: pointers and strides");
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->scale_page_stride < 0 || c->scale_head_stride < 0 || c->scale_row_stride < 0)
+    return fail(OFA_BAD_ARGUMENT, "negative stride");
+  if (!aligned(b->q_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->pages, 4) || !aligned(b->status, 4)) return fail(OFA_BAD_ARGUMENT, "misaligned index array");
+  B.q_start = b->q_start; B.kv_len = b->kv_len; B.pages = b->pages; B.pages_stride = b->pages_stride;
+  B.n_seqs = b->n_seqs; B.max_pages = b->max_pages; B.n_pages = c->n_pages; B.n_rows = n_rows; B.page.set((unsigned)c->page_size); B.status = b->status;
+  C.k = static_cast<char*>(c->k); C.v = static_cast<char*>(c->v); C.ks = c->k_scale; C.vs = c->v_scale;
+  C.page_b = c->page_stride * es; C.head_b = c->head_stride * es; C.row_b = c->row_stride * es;
+  C.s_page = c->scale_page_stride; C.s_head = c->scale_head_stride; C.s_row = c->scale_row_stride;
+  return OFA_OK;
+}
+int check_rows(const char* name, const void* p, long long row, long long head) {
+  if (!p) return fail(OFA_BAD_ARGUMENT, "%s is null", name);
+  if (!aligned(p, 16) || row % 8 || head % 8 || row < 0 || head < 0) return fail(OFA_BAD_ARGUMENT, "rows of %s start on 16-byte boundaries: pointer and strides", name);
+  return OFA_OK;
+}
+
+template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void* k, void* v, int n_rows, long long k_row, long long k_head, long long v_row,
+                              long long v_head, void* stream) {
+  paged::MoveArgs P;
+  if (int rc = check_cache(c, b, n_rows, P.b, P.c)) return rc;
+  if (n_rows == 0 || b->n_seqs == 0) return OFA_OK;
+  if (int rc = check_rows("k", k, k_row, k_head)) return rc;
+  if (int rc = check_rows("v", v, v_row, v_head)) return rc;
+  P.k = static_cast<bf16*>(k); P.v = static_cast<bf16*>(v); P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
+  P.n_kv_heads = c->n_kv_heads; P.pair.set(2u * (unsigned)c->n_kv_heads);
+  // four pieces of 16 bytes for a thread where there are rows for it: a block then amortises the search for its sequences
+  const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / 8);
+  long long rows = (1024 + per_row - 1) / per_row;
+  while (rows > 1 && (n_rows + rows - 1) / rows < 148) rows--;
+  P.rows = (int)(rows < paged::MOVE_ROWS ? rows : paged::MOVE_ROWS);
+  const unsigned grid = (unsigned)((n_rows + P.rows - 1) / P.rows);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (c->dtype == OFA_KV_E4M3) {
+    if (c->head_dim == 64) paged::move_kernel<64, true, READ><<<grid, 256, 0, s>>>(P); else paged::move_kernel<128, true, READ><<<grid, 256, 0, s>>>(P);
+  } else {
+    if (c->head_dim == 64) paged::move_kernel<64, false, READ><<<grid, 256, 0, s>>>(P); else paged::move_kernel<128, false, READ><<<grid, 256, 0, s>>>(P);
+  }
+  return launched(READ ? "ofa_kv_read" : "ofa_kv_append");
+}
+
+// ---- attention
+struct Plan { int tiles, nsplit; size_t bytes; };
+
+// Blocks that share a tile's keys: as many as keep two blocks on each of 148 SMs busy, none with fewer than 8 steps of 32 keys (two for each of its four
+// warps). max_new and max_kv are what the caller says; without them a tile per sequence and the page table's width are assumed.
+Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
+  Plan p;
+  const long long group = n_heads / c->n_kv_heads;
+  const long long newest = b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows;
+  long long tiles = (newest * group + 15) / 16;
+  if (tiles > 4096) tiles = 4096;
+  const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
+  const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * (tiles > 0 ? tiles : 1);
+  long long ns = 2 * 148 / blocks;
+  if (ns > kv / 256) ns = kv / 256;
+  if (ns > paged::MAX_SPLIT) ns = paged::MAX_SPLIT;
+  p.tiles = (int)(tiles > 0 ? tiles : 1); p.nsplit = (int)(ns > 1 ? ns : 1);
+  p.bytes = p.nsplit > 1 ? (size_t)n_rows * n_heads * p.nsplit * (c->head_dim + 2) * 4 : 0;
+  return p;
+}
+
+template <int D, bool E4M3> cudaError_t few_rows(const paged::AttnArgs& P, cudaStream_t s) {
+  using F = paged::Few<D, E4M3>;
+  cudaError_t e = cudaFuncSetAttribute(paged::few_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+  if (e != cudaSuccess) return e;
+  paged::few_rows_kernel<D, E4M3><<<dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads), 128, F::SMEM, s>>>(P);
+  if (P.nsplit > 1) {
+    cudaLaunchAttribute after = {};
+    after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    after.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(((long long)P.b.n_rows * P.n_heads + 3) / 4)); lc.blockDim = dim3(128); lc.stream = s; lc.attrs = &after; lc.numAttrs = 1;
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if ((e = cudaLaunchKernelEx(&lc, paged::combine_kernel<D>, P)) != cudaSuccess) return e;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" const char* ofa_serving_last_error(void) { return g_error; }
+
+extern "C" int ofa_kv_append(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const void* k, const void* v, int n_rows, long long k_row_stride,
+                             long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream) {
+  return move<false>(cache, batch, const_cast<void*>(k), const_cast<void*>(v), n_rows, k_row_stride, k_head_stride, v_row_stride, v_head_stride, stream);
+}
+extern "C" int ofa_kv_read(const ofa_kv_cache* cache, const ofa_kv_batch* batch, void* k, void* v, int n_rows, long long k_row_stride, long long k_head_stride,
+                           long long v_row_stride, long long v_head_stride, void* stream) {
+  return move<true>(cache, batch, k, v, n_rows, k_row_stride, k_head_stride, v_row_stride, v_head_stride, stream);
+}
+
+extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const ofa_paged_attention_args* a, void* stream) {
+  paged::AttnArgs P;
+  if (!a) return fail(OFA_BAD_ARGUMENT, "null pointer");
+  if (int rc = check_cache(cache, batch, a->n_rows, P.b, P.c)) return rc;
+  if (a->n_heads < 1 || a->n_heads % cache->n_kv_heads) return fail(OFA_BAD_ARGUMENT, "n_heads %d is not a multiple of n_kv_heads %d", a->n_heads, cache->n_kv_heads);
+  if (a->window < 0 || (a->window && !a->causal)) return fail(OFA_BAD_ARGUMENT, "window %d: a window (> 0) needs causal attention", a->window);
+  if (!(a->scale > -1e30f && a->scale < 1e30f)) return fail(OFA_BAD_ARGUMENT, "scale is not finite");
+  const long long group = a->n_heads / cache->n_kv_heads;
+  if ((long long)a->n_rows * group > 0x7fffff00ll || (long long)a->n_rows * a->n_heads > 0x7fffff00ll * 4)
+    return fail(OFA_BAD_ARGUMENT, "%d rows of %d heads are too many for one call", a->n_rows, a->n_heads);
+  if (a->n_rows == 0 || batch->n_seqs == 0) return OFA_OK;
+  if (int rc = check_rows("q", a->q, a->q_row_stride, a->q_head_stride)) return rc;
+  if (int rc = check_rows("out", a->out, a->out_row_stride, a->out_head_stride)) return rc;
+  if (!aligned(a->lse, 4)) return fail(OFA_BAD_ARGUMENT, "lse is misaligned");
+  const Plan p = plan(cache, batch, a->n_rows, a->n_heads);
+  if (p.bytes && (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)))
+    return fail(OFA_BAD_ARGUMENT, "workspace of %zu bytes on a 16-byte boundary needed, %zu given", p.bytes, a->workspace ? a->workspace_bytes : 0);
+  if ((long long)batch->n_seqs * p.tiles * p.nsplit > 0x7fffffffll) return fail(OFA_BAD_ARGUMENT, "%d sequences are too many for one call", batch->n_seqs);
+  P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
+  P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
+  P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
+  P.scale_log2 = a->scale * paged::LOG2E; P.tiles = p.tiles; P.nsplit = p.nsplit; P.part = static_cast<float*>(a->workspace);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? few_rows<64, true>(P, s) : few_rows<128, true>(P, s);
+  else e = cache->head_dim == 64 ? few_rows<64, false>(P, s) : few_rows<128, false>(P, s);
+  return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
+}
+
+extern "C" size_t ofa_paged_attention_workspace(const ofa_kv_cache* cache, const ofa_kv_batch* batch, int n_rows, int n_heads) {
+  paged::Batch B;
+  paged::Pool C;
+  if (check_cache(cache, batch, n_rows, B, C) || n_heads < 1 || n_heads % cache->n_kv_heads || n_rows == 0) return 0;
+  return plan(cache, batch, n_rows, n_heads).bytes;
+}
+
+extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
+  if (!a) return fail(OFA_BAD_ARGUMENT, "null pointer");
+  if (a->dtype != OFA_DTYPE_BF16 && a->dtype != OFA_DTYPE_F32) return fail(OFA_BAD_ARGUMENT, "logits dtype %d is neither OFA_DTYPE_BF16 nor OFA_DTYPE_F32", a->dtype);
+  if (a->n_rows < 0 || a->vocab < 0 || a->max_tokens < 0 || a->max_bias < 0) return fail(OFA_BAD_ARGUMENT, "negative size: n_rows %d, vocab %d, max_tokens %d, max_bias %d", a->n_rows, a->vocab, a->max_tokens, a->max_bias);
+  if (a->n_rows > 65535) return fail(OFA_BAD_ARGUMENT, "n_rows %d: at most 65535", a->n_rows);
+  if (a->n_rows == 0 || a->vocab == 0) return OFA_OK;
+  const size_t es = a->dtype == OFA_DTYPE_F32 ? 4 : 2;
+  if (!a->in || !a->out) return fail(OFA_BAD_ARGUMENT, "logits are null");
+  if (!aligned(a->in, es) || !aligned(a->out, es)) return fail(OFA_BAD_ARGUMENT, "misaligned logits");
+  if (a->out_stride < a->vocab && a->n_rows > 1) return fail(OFA_BAD_ARGUMENT, "rows of out overlap: stride %lld, vocab %d", a->out_stride, a->vocab);
+  if (a->in_stride < 0 || a->tokens_stride < 0 || a->bias_stride < 0 || a->mask_stride < 0) return fail(OFA_BAD_ARGUMENT, "negative stride");
+  if ((a->repetition || a->presence || a->frequency) && !a->tokens && a->max_tokens > 0) return fail(OFA_BAD_ARGUMENT, "penalties need tokens");
+  if (!a->bias_ids != !a->bias) return fail(OFA_BAD_ARGUMENT, "bias_ids and bias come together");
+  if (!aligned(a->tokens, 4) || !aligned(a->n_tokens, 4) || !aligned(a->n_prompt, 4) || !aligned(a->repetition, 4) || !aligned(a->presence, 4) || !aligned(a->frequency, 4) ||
+      !aligned(a->bias_ids, 4) || !aligned(a->bias, 4) || !aligned(a->mask, 4)) return fail(OFA_BAD_ARGUMENT, "misaligned array");
+  logits::Args P;
+  P.in = a->in; P.out = a->out; P.in_row = a->in_stride; P.out_row = a->out_stride; P.vocab = a->vocab; P.stretch = 4096;
+  const bool history = a->tokens && a->max_tokens > 0 && (a->repetition || a->presence || a->frequency);
+  P.tokens = history ? a->tokens : nullptr; P.tokens_row = a->tokens_stride; P.max_tokens = a->max_tokens; P.n_tokens = a->n_tokens; P.n_prompt = a->n_prompt;
+  P.repetition = a->repetition; P.presence = a->presence; P.frequency = a->frequency;
+  P.bias_ids = a->max_bias > 0 ? a->bias_ids : nullptr; P.bias = a->bias; P.bias_row = a->bias_stride; P.max_bias = a->max_bias;
+  P.mask = a->mask; P.mask_row = a->mask_stride;
+  const unsigned smem = (unsigned)P.stretch * 4 * ((P.tokens != nullptr) + (P.bias_ids != nullptr));
+  const dim3 grid((unsigned)((a->vocab + P.stretch - 1) / P.stretch), (unsigned)a->n_rows);
+  const bool wide = aligned(a->in, 16) && aligned(a->out, 16) && (a->n_rows == 1 || ((a->in_stride * es) % 16 == 0 && (a->out_stride * es) % 16 == 0));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == OFA_DTYPE_F32) { if (wide) logits::process_kernel<float, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<float, false><<<grid, 256, smem, s>>>(P); }
+  else { if (wide) logits::process_kernel<bf16, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<bf16, false><<<grid, 256, smem, s>>>(P); }
+  return launched("ofa_logits_process");
+}

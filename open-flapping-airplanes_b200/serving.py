@@ -1,0 +1,219 @@
+"""Serving operators over a paged key/value cache, on the current stream of their tensors' device: the torch view of the "serving over a
+paged cache" part of include/ofa_b200.h, which says what each computes.
+
+    cache = KVCache.empty(n_pages, page_size, n_kv_heads, head_dim, "e4m3")     # one per layer
+    batch = KVBatch(q_start, kv_len, pages, max_new=..., max_kv=...)            # one per step, shared by the layers
+    kv_append(cache, batch, k, v)                                               # this step's keys and values to their pages
+    o = paged_attention(cache, batch, q)                                        # this step's queries over them
+    k, v = kv_read(cache, batch, n_rows)                                        # cached rows back as bf16
+    logits_process(logits, tokens=..., repetition=..., mask=..., out=logits)    # penalties, biases, a grammar's mask
+
+Nothing is copied, cast or made contiguous behind the caller's back: a tensor of another type, device or layout than an operator takes is refused with an
+OfaError. No call waits for the device or reads from it. Index tensors are int32 and are read by the kernels, so a captured graph sees what they hold when it
+is replayed.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import capi
+from .tasks import OfaError
+
+E4M3 = torch.float8_e4m3fn
+_TYPES = {"bf16": torch.bfloat16, "e4m3": E4M3}
+BAD_PAGE, BAD_LENGTH, BAD_ROWS = 1, 2, 4          # bits of a batch's status word
+
+
+def _refuse(msg):
+    raise OfaError(capi.BAD_ARGUMENT, msg)
+
+
+def _want(name, t, dtype, shape, device, inner=True):
+    """A CUDA tensor of this type and shape (None: any size) on `device` (None: any), its last axis dense."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(f"{name} has to be a CUDA tensor")
+    if t.dtype != dtype:
+        _refuse(f"{name} has to be {dtype}, not {t.dtype}")
+    s = t.shape
+    if len(s) != len(shape) or any(w is not None and w != n for w, n in zip(shape, s)):
+        _refuse(f"{name} has shape {tuple(s)}, not {tuple('any' if w is None else w for w in shape)}")
+    if device is not None and t.device != device:
+        _refuse(f"{name} is on {t.device}, not on {device}")
+    if inner and len(s) and s[-1] > 1 and t.stride(-1) != 1:
+        _refuse(f"the last axis of {name} has to be dense")
+
+
+def _call(fn, device, *args):
+    """fn(*args, current stream of `device`), with that device current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != capi.OK:
+        raise OfaError(rc, capi.load().ofa_serving_last_error().decode())
+
+
+class KVCache:
+    """Pages of keys and values: k and v [n_pages, n_kv_heads, page_size, head_dim], bf16 or float8_e4m3fn, any strides that keep rows on 16-byte
+    boundaries and are the same for both; for e4m3 also k_scale and v_scale [n_pages, n_kv_heads, page_size], uint8. The tensors stay the caller's."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        e4m3 = isinstance(k, torch.Tensor) and k.dtype == E4M3
+        _want("k", k, E4M3 if e4m3 else torch.bfloat16, (None,) * 4, None)
+        _want("v", v, k.dtype, k.shape, k.device)
+        if k.stride() != v.stride():
+            _refuse(f"k and v have different strides: {k.stride()} and {v.stride()}")
+        if e4m3:
+            _want("k_scale", k_scale, torch.uint8, k.shape[:3], k.device, inner=False)
+            _want("v_scale", v_scale, torch.uint8, k.shape[:3], k.device, inner=False)
+            if k_scale.stride() != v_scale.stride():
+                _refuse("k_scale and v_scale have different strides")
+        elif k_scale is not None or v_scale is not None:
+            _refuse("a bf16 cache has no scales")
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        if self.head_dim not in (64, 128):
+            _refuse(f"head_dim {self.head_dim}: 64 and 128 are built")
+        c = self.c = capi.KvCache()
+        c.dtype, c.head_dim, c.n_kv_heads, c.page_size, c.n_pages = capi.KV_E4M3 if e4m3 else capi.KV_BF16, self.head_dim, self.n_kv_heads, self.page_size, self.n_pages
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.page_stride, c.head_stride, c.row_stride = k.stride()[:3]
+        if e4m3:
+            c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            c.scale_page_stride, c.scale_head_stride, c.scale_row_stride = k_scale.stride()
+        self.ref = C.byref(c)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_kv_heads, head_dim, dtype="bf16", device="cuda"):
+        """A cache of its own; its rows are zeros."""
+        if dtype not in _TYPES:
+            _refuse(f"cache dtype {dtype!r} is neither 'bf16' nor 'e4m3'")
+        make = lambda *s, t: torch.zeros(s, dtype=t, device=device)  # noqa: E731
+        shape = (n_pages, n_kv_heads, page_size)
+        scales = [make(*shape, t=torch.uint8) for _ in range(2)] if dtype == "e4m3" else []
+        return cls(make(*shape, head_dim, t=_TYPES[dtype]), make(*shape, head_dim, t=_TYPES[dtype]), *scales)
+
+
+class KVBatch:
+    """The sequences of a step: q_start [n_seqs + 1], kv_len [n_seqs], pages [n_seqs, max_pages], int32 on the device. max_new and max_kv: the longest chunk
+    and context as far as the program knows them; they choose how the work is cut, not what is computed. status: an int32 tensor whose first element
+    collects BAD_PAGE, BAD_LENGTH and BAD_ROWS."""
+
+    def __init__(self, q_start, kv_len, pages, max_new=0, max_kv=0, status=None):
+        _want("pages", pages, torch.int32, (None, None), None)
+        n = pages.shape[0]
+        _want("kv_len", kv_len, torch.int32, (n,), pages.device)
+        _want("q_start", q_start, torch.int32, (n + 1,), pages.device)
+        if status is not None:
+            _want("status", status, torch.int32, (None,), pages.device)
+            if not status.numel():
+                _refuse("status is empty")
+        if max_new < 0 or max_kv < 0:
+            _refuse(f"max_new {max_new}, max_kv {max_kv}")
+        self.q_start, self.kv_len, self.pages, self.status, self.device = q_start, kv_len, pages, status, pages.device
+        c = self.c = capi.KvBatch()
+        c.n_seqs, c.max_pages, c.pages_stride = n, pages.shape[1], pages.stride(0)
+        c.q_start, c.kv_len, c.pages = q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr()
+        c.max_new, c.max_kv = min(max_new, 2 ** 31 - 1), min(max_kv, 2 ** 31 - 1)
+        c.status = status.data_ptr() if status is not None else None
+        self.ref = C.byref(c)
+
+
+def _same_device(cache, batch):
+    if cache.device != batch.device:
+        _refuse(f"the cache is on {cache.device}, the batch on {batch.device}")
+
+
+def kv_append(cache, batch, k, v):
+    """Rows k and v [n_rows, n_kv_heads, head_dim] (bf16; views of a fused projection will do) to their pages, in the cache's type."""
+    _same_device(cache, batch)
+    _want("k", k, torch.bfloat16, (None, cache.n_kv_heads, cache.head_dim), cache.device)
+    _want("v", v, torch.bfloat16, k.shape, cache.device)
+    _call(capi.load().ofa_kv_append, cache.device, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+
+
+def kv_read(cache, batch, n_rows=None, k=None, v=None):
+    """The batch's n_rows rows out of their pages, as bf16 [n_rows, n_kv_heads, head_dim] pairs (written into k and v where these are given)."""
+    _same_device(cache, batch)
+    if k is None or v is None:
+        if n_rows is None or k is not None or v is not None:
+            _refuse("kv_read needs n_rows, or k and v to write to")
+        k, v = (torch.empty((n_rows, cache.n_kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    _want("k", k, torch.bfloat16, (n_rows, cache.n_kv_heads, cache.head_dim), cache.device)
+    _want("v", v, torch.bfloat16, k.shape, cache.device)
+    _call(capi.load().ofa_kv_read, cache.device, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    return k, v
+
+
+def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0, with_lse=False):
+    """Attention of q [n_rows, n_heads, head_dim] (bf16) over the batch's pages; scale: 1/sqrt(head_dim) by default. Returns out, of q's shape, or with
+    with_lse (out, lse [n_rows, n_heads] fp32). Rows that no sequence brings are left as they were."""
+    _same_device(cache, batch)
+    _want("q", q, torch.bfloat16, (None, None, cache.head_dim), cache.device)
+    n_rows, n_heads = q.shape[:2]
+    if out is None:
+        out = torch.empty((n_rows, n_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
+    else:
+        _want("out", out, torch.bfloat16, q.shape, cache.device)
+    lse = torch.empty((n_rows, n_heads), dtype=torch.float32, device=cache.device) if with_lse else None
+    lib = capi.load()
+    a = capi.PagedAttentionArgs()
+    a.n_rows, a.n_heads, a.q, a.out = n_rows, n_heads, q.data_ptr(), out.data_ptr()
+    a.q_row_stride, a.q_head_stride, _ = q.stride()
+    a.out_row_stride, a.out_head_stride, _ = out.stride()
+    a.lse = lse.data_ptr() if with_lse else None
+    a.scale, a.causal, a.window = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale, bool(causal), window
+    need = lib.ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
+    if need:                                                   # the caller's allocator: a graph that captures the call keeps its own
+        work = torch.empty(need, dtype=torch.uint8, device=cache.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+    _call(lib.ofa_paged_attention, cache.device, cache.ref, batch.ref, C.byref(a))
+    return (out, lse) if with_lse else out
+
+
+def logits_process(logits, tokens=None, n_tokens=None, n_prompt=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias=None, mask=None, out=None):
+    """Penalties of repeated tokens, biases and a bit mask on logits [n_rows, vocab] (bf16 or fp32); returns out (a new tensor by default; out=logits works in place).
+    tokens [n_rows, max_tokens], n_tokens, n_prompt [n_rows], bias_ids [n_rows, n] and mask [n_rows, ceil(vocab / 32)] are int32, the rest fp32."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+        _refuse("logits have to be a bf16 or fp32 tensor")
+    _want("logits", logits, logits.dtype, (None, None), None)
+    rows, vocab = logits.shape
+    dev = logits.device
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    elif out is not logits:
+        _want("out", out, logits.dtype, logits.shape, dev)
+    a = capi.LogitsArgs()
+    a.dtype, a.n_rows, a.vocab = capi.DTYPE_F32 if logits.dtype == torch.float32 else capi.DTYPE_BF16, rows, vocab
+    a.inp, a.out, a.in_stride, a.out_stride = logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0)
+    if tokens is not None:
+        _want("tokens", tokens, torch.int32, (rows, None), dev)
+        a.tokens, a.tokens_stride, a.max_tokens = tokens.data_ptr(), tokens.stride(0), tokens.shape[1]
+        if n_tokens is not None:
+            _want("n_tokens", n_tokens, torch.int32, (rows,), dev)
+            a.n_tokens = n_tokens.data_ptr()
+        if n_prompt is not None:
+            _want("n_prompt", n_prompt, torch.int32, (rows,), dev)
+            a.n_prompt = n_prompt.data_ptr()
+    elif any(x is not None for x in (n_tokens, n_prompt, repetition, presence, frequency)):
+        _refuse("penalties and token counts need tokens")
+    for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if x is not None:
+            _want(name, x, torch.float32, (rows,), dev)
+            setattr(a, name, x.data_ptr())
+    if (bias_ids is None) != (bias is None):
+        _refuse("bias_ids and bias come together")
+    if bias is not None:
+        _want("bias_ids", bias_ids, torch.int32, (rows, None), dev)
+        _want("bias", bias, torch.float32, bias_ids.shape, dev)
+        if bias.stride(0) != bias_ids.stride(0) and rows > 1:
+            _refuse("bias and bias_ids have different strides")
+        a.bias_ids, a.bias, a.bias_stride, a.max_bias = bias_ids.data_ptr(), bias.data_ptr(), bias.stride(0), bias.shape[1]
+    if mask is not None:
+        _want("mask", mask, torch.int32, (rows, (vocab + 31) // 32), dev)
+        a.mask, a.mask_stride = mask.data_ptr(), mask.stride(0)
+    _call(capi.load().ofa_logits_process, dev, C.byref(a))
+    return out

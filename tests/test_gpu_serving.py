@@ -1,0 +1,476 @@
+"""Serving operators over a paged cache on the GPU: each against a plain form in 64 bits at the sizes, layouts and masks where it can go wrong, and a step
+of all of them as a program strings them together."""
+import math
+
+import pytest
+import torch
+
+import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def sv(ofa):
+    return ofa.serving
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def starts(new):
+    s = [0]
+    for n in new:
+        s.append(s[-1] + n)
+    return s
+
+
+def make(sv, new, kv, kv_heads, dim, page, dtype="bf16", layout="heads", seed=0, spare=2, **hints):
+    """A cache in use: pages anywhere, all its rows filled by kv_append's own rule on the host, and a batch of sequences."""
+    g = torch.Generator().manual_seed(seed)
+    per = [-(-max(k, 0) // page) for k in kv]
+    n_pages = sum(per) + spare
+    perm = torch.randperm(n_pages, generator=g).tolist()
+    cols = max(per + [1])
+    table, at = [], 0
+    for n in per:
+        table.append(perm[at:at + n] + [-1] * (cols - n))
+        at += n
+    shape = (n_pages, kv_heads, page) if layout == "heads" else (n_pages, page, kv_heads)
+    pools, scales = [], []
+    for _ in range(2):
+        x = (torch.randn(*shape, dim, generator=g) * torch.exp2(torch.randint(-3, 3, shape, generator=g).float())[..., None]).bfloat16()
+        if dtype == "e4m3":
+            q, b = ref.quantise(x)
+            x = q.float().to(torch.float8_e4m3fn)
+            scales.append(b.to(DEV) if layout == "heads" else b.to(DEV).transpose(1, 2))
+        x = x.to(DEV)
+        pools.append(x if layout == "heads" else x.transpose(1, 2))
+    cache = sv.KVCache(*pools, *scales)
+    st = starts(new)
+    batch = sv.KVBatch(i32(st), i32(kv), i32(table).view(len(kv), cols), status=torch.zeros(1, dtype=torch.int32, device=DEV), **hints)
+    return cache, batch, g
+
+
+def check_attention(sv, cache, batch, q, causal=True, window=0, scale=None):
+    got, lse = sv.paged_attention(cache, batch, q, causal=causal, window=window, scale=scale, with_lse=True)
+    want, want_lse, tol, tol_lse = ref.attention(cache, batch.q_start.tolist(), batch.kv_len.tolist(), batch.pages.cpu(), q,
+                                                 1 / math.sqrt(cache.head_dim) if scale is None else scale, causal, window)
+    rows = ~torch.isnan(want_lse[:, 0]) if want_lse.numel() else torch.zeros(0, dtype=torch.bool)
+    got, lse = got.double().cpu(), lse.double().cpu()
+    off = (got - want).abs()[rows]
+    assert torch.isfinite(got[rows]).all()
+    assert (off <= tol[rows]).all(), f"worst error is {float((off / tol[rows].clamp(min=1e-300)).max()):.3g} of its bound"
+    none = want_lse[rows] == -math.inf
+    assert torch.equal(none, lse[rows] == -math.inf)
+    off = (lse - want_lse).abs()[rows][~none]
+    assert (off <= tol_lse[rows][~none]).all(), f"lse: {float((off / tol_lse[rows][~none]).max()):.3g} of its bound"
+    return got, lse
+
+
+def queries(g, rows, heads, dim):
+    x = torch.randn(rows, (heads + 3) * dim, generator=g).bfloat16().to(DEV)
+    return x[:, dim:(heads + 1) * dim].view(rows, heads, dim)           # a view of something wider
+
+
+# ------------------------------------------------------------------------------------------------ append and read
+@pytest.mark.parametrize("layout", ["heads", "rows"])
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("new,kv,heads,dim,page", [([1], [1], 1, 64, 1), ([1, 0, 3, 1], [5, 9, 3, 129], 12, 64, 16), ([130, 7], [130, 200], 3, 128, 33),
+                                                   ([0], [4], 2, 64, 8), ([1] * 70, list(range(1, 71)), 2, 64, 24)])
+def test_rows_go_to_their_pages_and_come_back(sv, new, kv, heads, dim, page, dtype, layout):
+    cache, batch, g = make(sv, new, kv, heads, dim, page, dtype, layout)
+    rows = sum(new)
+    before = [t.clone() for t in (cache.k, cache.v)]
+    kvs = torch.randn(rows, 2 * heads * dim, generator=g) * torch.exp2(torch.randint(-30, 12, (rows, 1), generator=g).float())
+    kvs = kvs.bfloat16().to(DEV)
+    k, v = (t.view(rows, heads, dim) for t in kvs.split(heads * dim, 1))
+    sv.kv_append(cache, batch, k, v)
+    got = sv.kv_read(cache, batch, rows)
+    changed = torch.zeros(cache.n_pages, page, dtype=torch.bool)
+    at, table = 0, batch.pages.cpu()
+    for i, (n, length) in enumerate(zip(new, kv)):
+        for p in range(length - n, length):
+            pg, r = int(table[i, p // page]), p % page
+            changed[pg, r] = True
+            for name, x, back in (("k", k, got[0]), ("v", v, got[1])):
+                if dtype == "bf16":
+                    want = x[at].double().cpu()
+                else:
+                    q, b = ref.quantise(x[at])
+                    want = q * 2.0 ** (b.double() - 127)[:, None]
+                    assert torch.equal(getattr(cache, name + "_scale")[pg, :, r].cpu(), b)
+                    assert torch.equal(getattr(cache, name)[pg, :, r].double().cpu(), q)
+                assert torch.equal(ref.cached(cache, name, pg, r), want)
+                assert torch.equal(back[at].double().cpu(), want), "a read rounds nothing"
+            at += 1
+    for now, was in zip((cache.k, cache.v), before):                    # and nothing else is touched
+        same = (now.contiguous().view(torch.uint8) == was.contiguous().view(torch.uint8)).view(cache.n_pages, heads, page, -1).all(-1).all(1).cpu()
+        assert same[~changed].all()
+    assert int(batch.status) == 0
+
+
+def test_every_code_and_scale_reads_back_exactly(sv):
+    codes = torch.arange(256, dtype=torch.uint8, device=DEV).repeat(128 * 64 // 256)
+    for first in (27, 100, 127, 134 - 63 + 0):
+        k = codes.view(torch.float8_e4m3fn).view(1, 1, 128, 64).contiguous()
+        k = torch.where(torch.isnan(k.float()), torch.zeros_like(k.float()), k.float()).to(torch.float8_e4m3fn)
+        b = (first + torch.arange(128, device=DEV) % 64).clamp(max=134).to(torch.uint8).view(1, 1, 128)
+        cache = sv.KVCache(k, k.clone(), b, b.clone())
+        batch = sv.KVBatch(i32([0, 128]), i32([128]), i32([[0]]))
+        got = sv.kv_read(cache, batch, 128)[0].double()[:, 0]
+        want = k.double()[0, 0] * torch.tensor([2.0 ** (int(x) - 127) for x in b.flatten()], dtype=torch.float64, device=DEV)[:, None]
+        assert torch.equal(got, want)
+
+
+def test_rows_with_nan_infinity_zeros_and_the_largest_values(sv):
+    cache = sv.KVCache.empty(1, 8, 1, 64, "e4m3")
+    batch = sv.KVBatch(i32([0, 6]), i32([6]), i32([[0]]))
+    x = torch.randn(6, 1, 64).bfloat16()
+    x[0, 0, 3] = math.nan
+    x[1, 0, 63] = -math.inf
+    x[2] = 0
+    x[3, 0, 5] = 3.3e38                                                 # above 448 * 2^7: held as 57344
+    x[4] = x[4].float().mul(1e-36).bfloat16()                           # far below the smallest scale
+    x[5, 0, 0] = 448.0
+    x = x.to(DEV)
+    sv.kv_append(cache, batch, x, x)
+    assert cache.k_scale[0, 0, :6].tolist()[:4] == [255, 255, 27, 134] and int(cache.k_scale[0, 0, 4]) == 27
+    k, _ = sv.kv_read(cache, batch, 6)
+    k = k.double().cpu()[:, 0]
+    assert torch.isnan(k[0]).all() and torch.isnan(k[1]).all() and (k[2] == 0).all() and float(k[3, 5]) == 57344.0
+    assert (k[4].abs() <= 2.0 ** -109).all()
+    q, b = ref.quantise(x[5])
+    assert torch.equal(k[5], (q * 2.0 ** (b.double() - 127)[:, None])[0])
+
+
+# ------------------------------------------------------------------------------------------------ attention
+CASES = [
+    # new, kv, heads, kv_heads, dim, page
+    ([1], [1], 1, 1, 64, 16),
+    ([1], [1000], 12, 12, 64, 16),
+    ([1, 1, 1], [31, 32, 33], 4, 2, 128, 8),
+    ([1, 0, 1], [300, 50, 7], 8, 1, 64, 33),
+    ([3, 1, 17, 2], [3, 600, 40, 2], 12, 12, 64, 24),
+    ([5, 5], [257, 90], 32, 8, 128, 64),
+    ([16, 1], [16, 513], 24, 8, 64, 1),
+    ([33], [100], 3, 1, 128, 16),
+    ([70, 129], [70, 300], 4, 4, 64, 16),
+    ([200], [333], 6, 2, 128, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{len(c[0])}x{max(c[0])}of{max(c[1])}_h{c[2]}_{c[3]}_d{c[4]}_p{c[5]}")
+def test_attention(sv, case, dtype):
+    new, kv, heads, kv_heads, dim, page = case
+    cache, batch, g = make(sv, new, kv, kv_heads, dim, page, dtype, "rows" if len(new) % 2 else "heads", max_new=max(new), max_kv=max(kv))
+    check_attention(sv, cache, batch, queries(g, sum(new), heads, dim))
+    assert int(batch.status) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 200])
+@pytest.mark.parametrize("new", [[1, 1], [9, 40]])
+def test_window(sv, new, window, dtype):
+    cache, batch, g = make(sv, new, [500, 77], 2, 64, 16, dtype, max_new=max(new))
+    check_attention(sv, cache, batch, queries(g, sum(new), 4, 64), window=window)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [7, 150]])
+def test_without_causal_mask_and_with_another_scale(sv, new):
+    cache, batch, g = make(sv, new, [40, 333], 2, 128, 32)
+    check_attention(sv, cache, batch, queries(g, sum(new), 4, 128), causal=False, scale=0.3)
+    check_attention(sv, cache, batch, queries(g, sum(new), 4, 128), scale=-0.05)
+
+
+@pytest.mark.parametrize("hints", [{}, {"max_new": 1}, {"max_kv": 1}, {"max_new": 1, "max_kv": 1}, {"max_new": 10 ** 6, "max_kv": 10 ** 9}])
+def test_hints_change_no_result_beyond_rounding(sv, hints):
+    """max_new and max_kv only choose how the work is cut: too small, too large or absent, every row is computed"""
+    new, kv = [60, 1, 5], [900, 2000, 5]
+    cache, batch, g = make(sv, new, kv, 2, 64, 16, **hints)
+    check_attention(sv, cache, batch, queries(g, sum(new), 4, 64))
+
+
+@pytest.mark.parametrize("new", [[4, 2, 1], [40, 20, 1]])
+def test_rows_that_see_nothing(sv, new):
+    """A sequence shorter than what it brings has rows before its first position; one of length 0 has only such rows."""
+    cache, batch, g = make(sv, new, [2, 0, 1], 2, 64, 16)
+    got, lse = check_attention(sv, cache, batch, queries(g, sum(new), 2, 64))
+    assert (got[: new[0] - 2] == 0).all() and (lse[: new[0] - 2] == -math.inf).all()
+
+
+@pytest.mark.parametrize("new,heads", [([1, 1], 2), ([30, 1], 4)])
+def test_rows_of_no_sequence_are_left_alone(sv, new, heads):
+    cache, batch, g = make(sv, new, [300, 1200], 2, 64, 16)
+    rows = sum(new) + 5
+    q = queries(g, rows, heads, 64)
+    out = torch.full((rows, heads, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    sv.paged_attention(cache, batch, q, out=out)
+    assert (out[sum(new):] == 7).all()
+    k = torch.full((rows, 2, 64), 9.0, dtype=torch.bfloat16, device=DEV)
+    v = k.clone()
+    sv.kv_read(cache, batch, k=k, v=v)
+    assert (k[sum(new):] == 9).all() and (v[sum(new):] == 9).all() and not (k[:sum(new)] == 9).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("new,kv,window", [([5], [70], 0), ([1], [70], 20), ([20], [300], 40), ([150], [300], 0), ([150], [300], 33)])
+def test_what_a_row_does_not_see_does_not_reach_it(sv, new, kv, window, dtype):
+    """NaN and infinities in keys and values that some rows see and others do not, and in the unused rest of the last page"""
+    cache, batch, g = make(sv, new, kv, 1, 64, 64, dtype)
+    q = queries(g, new[0], 2, 64)
+    table = batch.pages.cpu()
+    where = lambda p: (int(table[0, p // 64]), 0, p % 64)  # noqa: E731
+    n, length = new[0], kv[0]
+
+    def spoil(p, value):
+        if dtype == "e4m3":
+            cache.k_scale[where(p)] = 255
+            cache.v_scale[where(p)] = 255
+        else:
+            cache.k[where(p)][3] = value
+            cache.v[where(p)][5] = value
+            cache.v[where(p)][6] = -value
+    spoiled = sorted({length - 1, length - n // 2 - 1} | ({max(0, length - n - window + 1 + n // 3), 0} if window else set())) if n > 1 else ([0] if window else [])
+    for p in spoiled:
+        spoil(p, math.nan if p % 2 else math.inf)
+    last = int(table[0, length // 64])                                   # the rest of the last page was never written
+    if dtype == "e4m3":
+        cache.k_scale[last, 0, length % 64:] = cache.v_scale[last, 0, length % 64:] = 255
+    else:
+        cache.k[last, 0, length % 64:] = cache.v[last, 0, length % 64:] = math.nan
+    got, lse = sv.paged_attention(cache, batch, q, window=window, with_lse=True)
+    got, lse = got.double().cpu(), lse.cpu()
+    want, _, tol, _ = ref.attention(cache, [0, n], kv, table, q, 1 / 8, True, window)
+    clean = torch.tensor([not any(p <= length - n + t and (not window or p > length - n + t - window) for p in spoiled) for t in range(n)])
+    assert clean.any()
+    assert torch.isfinite(got[clean]).all() and ((got - want).abs()[clean] <= tol[clean]).all()
+    if dtype == "e4m3":
+        assert torch.isnan(got[~clean]).all() and torch.isnan(lse[~clean]).all()
+    assert not torch.isfinite(got[~clean][..., 5]).any()
+
+
+@pytest.mark.parametrize("new", [[6], [100]])
+def test_infinite_values_reach_the_rows_that_see_them(sv, new):
+    cache, batch, g = make(sv, new, [160], 1, 64, 32)
+    table = batch.pages.cpu()
+    p = 160 - new[0] // 2
+    pg, r = int(table[0, p // 32]), p % 32
+    cache.v[pg, 0, r, 9] = math.inf
+    cache.v[pg, 0, r, 40] = math.nan
+    q = queries(g, new[0], 2, 64)
+    got = sv.paged_attention(cache, batch, q).float().cpu()
+    sees = torch.arange(160 - new[0], 160) >= p
+    assert (got[sees][:, :, 9] == math.inf).all() and torch.isnan(got[sees][:, :, 40]).all()
+    others = [d for d in range(64) if d not in (9, 40)]
+    want, _, tol, _ = ref.attention(cache, [0, new[0]], [160], table, q, 1 / 8)
+    assert torch.isfinite(got[~sees]).all()
+    assert ((got.double() - want).abs()[:, :, others] <= tol[:, :, others]).all()
+
+
+@pytest.mark.parametrize("new", [[2], [90]])
+def test_bad_tables_and_lengths_set_status_and_nothing_else(sv, new):
+    n = new[0]
+    cache, batch, g = make(sv, new, [200], 2, 64, 16)
+    q = queries(g, n, 4, 64)
+    batch.pages[0, 3], batch.pages[0, 7] = cache.n_pages, -5              # their keys are not seen
+    check_attention(sv, cache, batch, q)
+    assert int(batch.status) == sv.BAD_PAGE
+    long = sv.KVBatch(i32([0, n]), i32([10 ** 9]), batch.pages, status=torch.zeros(1, dtype=torch.int32, device=DEV))
+    sv.paged_attention(cache, long, q, window=1000)
+    k, v = sv.kv_read(cache, long, n)
+    assert int(long.status) & sv.BAD_LENGTH and (k == 0).all() and (v == 0).all()
+    before = cache.k.clone()
+    sv.kv_append(cache, long, q[:, :2], q[:, :2])
+    assert torch.equal(before, cache.k)
+    for st in ([0, n + 1], [-1, n], [n, 0]):
+        bad = sv.KVBatch(i32(st), i32([100]), batch.pages, status=torch.zeros(1, dtype=torch.int32, device=DEV))
+        out = torch.full((n, 4, 64), 3.0, dtype=torch.bfloat16, device=DEV)
+        sv.paged_attention(cache, bad, q, out=out)
+        sv.kv_append(cache, bad, q[:, :2], q[:, :2])
+        assert int(bad.status) & sv.BAD_ROWS and torch.equal(before, cache.k)
+    neg = sv.KVBatch(i32([0, n]), i32([-3]), batch.pages, status=torch.zeros(1, dtype=torch.int32, device=DEV))
+    assert (sv.paged_attention(cache, neg, q) == 0).all() and int(neg.status) & sv.BAD_LENGTH
+
+
+def test_a_long_cache_whose_offsets_pass_32_bits(sv):
+    """4.3 GB of keys: pages beyond 2^32 bytes are the ones in use"""
+    pages, page, heads, dim = 16500, 128, 8, 128
+    k = torch.empty(pages, heads, page, dim, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty_like(k)
+    cache = sv.KVCache(k, v)
+    table = i32([[pages - 1, pages - 3]])
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn(200, 2 * heads * dim, generator=g).bfloat16().to(DEV)
+    kk, vv = (t.view(200, heads, dim) for t in rows.split(heads * dim, 1))
+    full = sv.KVBatch(i32([0, 200]), i32([200]), table)
+    sv.kv_append(cache, full, kk, vv)
+    back = sv.kv_read(cache, full, 200)
+    assert torch.equal(back[0], kk) and torch.equal(back[1], vv)
+    for n in (1, 40):
+        batch = sv.KVBatch(i32([0, n]), i32([200]), table)
+        q = queries(g, n, 16, dim)
+        got = sv.paged_attention(cache, batch, q).double().cpu()
+        small = sv.KVCache(k[[pages - 1, pages - 3]].clone(), v[[pages - 1, pages - 3]].clone())
+        want, _, tol, _ = ref.attention(small, [0, n], [200], torch.tensor([[0, 1]]), q, 1 / math.sqrt(dim))
+        assert ((got - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------------------------------------ logits
+def logit_inputs(rows, vocab, history, biases, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, vocab, generator=g) * 4).to(dtype)
+    x[0, 0] = -math.inf
+    if vocab > 3:
+        x[0, 3] = torch.finfo(dtype).min
+    a = {}
+    if history:
+        a["tokens"] = torch.randint(-2, vocab + 2, (rows, history), generator=g).int()
+        a["tokens"][:, : history // 2] %= max(1, vocab // 7)              # repeats
+        a["n_tokens"] = torch.randint(0, history + 3, (rows,), generator=g).int()
+        a["n_prompt"] = torch.randint(0, history + 1, (rows,), generator=g).int()
+        a["repetition"] = 1 + torch.rand(rows, generator=g)
+        a["presence"], a["frequency"] = torch.rand(rows, generator=g), torch.rand(rows, generator=g) - 0.3
+    if biases:
+        a["bias_ids"] = torch.randint(-2, vocab + 2, (rows, biases), generator=g).int()
+        a["bias_ids"][:, -1] = a["bias_ids"][:, 0]                        # the same id twice
+        a["bias"] = torch.randn(rows, biases, generator=g) * 5
+    return x, a, torch.randint(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32), generator=g).int()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,history,biases,masked", [(1, 1, 3, 2, True), (3, 33, 40, 5, True), (2, 4097, 0, 0, True), (5, 8191, 300, 9, False), (1, 50304, 1000, 0, True),
+                                                              (4, 1000, 0, 3, False), (2, 777, 50, 0, False), (130, 64, 2, 1, True)])
+def test_logits(sv, rows, vocab, history, biases, masked, dtype):
+    x, a, mask = logit_inputs(rows, vocab, history, biases, dtype)
+    if masked:
+        mask[-1] = 0                                                      # a row that may take nothing
+        a["mask"] = mask
+    want, tol = ref.logits(x, **a)
+    half = ref.F32_HALF if dtype == torch.float32 else ref.BF16_HALF
+    tol = tol + half * (want.abs() + tol)
+    dev = {k: v.to(DEV) for k, v in a.items()}
+    got = sv.logits_process(x.to(DEV), **dev)
+    place = x.to(DEV)
+    assert sv.logits_process(place, out=place, **dev) is place
+    assert torch.equal(got, place)
+    got, fine = got.double().cpu(), torch.isfinite(want)
+    over = want.abs() >= torch.finfo(dtype).max                           # the lowest value times a factor is -inf in the type
+    same = fine & ~over
+    assert torch.equal(got[~fine], want[~fine])
+    assert ((got - want).abs()[same] <= tol[same]).all()
+    assert (got[fine & over] == -math.inf).all() or (got[fine & over] == torch.finfo(dtype).min).all()
+
+
+def test_logits_of_strided_rows(sv):
+    wide = torch.randn(4, 3000, device=DEV)
+    x = wide[:, 5:1006]
+    mask = torch.randint(-2 ** 31, 2 ** 31, (4, 40), device=DEV).int()[:, 3:35]
+    bias_ids, bias = torch.randint(0, 1001, (4, 6), device=DEV).int()[:, :4], torch.randn(4, 6, device=DEV)[:, :4]
+    want, tol = ref.logits(x, bias_ids=bias_ids.cpu(), bias=bias.cpu(), mask=mask)
+    before = wide.clone()
+    got = sv.logits_process(x, bias_ids=bias_ids, bias=bias, mask=mask)
+    assert torch.equal(wide, before)
+    fine = torch.isfinite(want)
+    assert torch.equal(got.cpu()[~fine].double(), want[~fine]) and ((got.cpu().double() - want).abs()[fine] <= (tol + want.abs() * ref.F32_HALF)[fine]).all()
+    sv.logits_process(x, bias_ids=bias_ids, bias=bias, mask=mask, out=x)
+    assert torch.equal(x, got) and torch.equal(wide[:, :5], before[:, :5]) and torch.equal(wide[:, 1006:], before[:, 1006:])
+
+
+# ------------------------------------------------------------------------------------------------ together
+def plain_step(sv, cache, lens, table, qkv, heads, kv_heads, dim):
+    n = [1] * len(lens)
+    return ref.attention(cache, starts(n), lens, table, qkv[:, : heads * dim].view(len(lens), heads, dim), 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_a_serving_run(sv, dtype):
+    """Prompts in one chunk, then tokens one at a time: append, attend, logits; the steps are also captured once and replayed with the lengths, tokens
+    and rows of each step, on another stream than the default one, and give the same bits."""
+    heads, kv_heads, dim, page, vocab, steps = 4, 2, 64, 16, 500, 5
+    prompt = [40, 3, 17]
+    kv = [p + steps for p in prompt]
+    cache, batch, g = make(sv, prompt, kv, kv_heads, dim, page, dtype)
+    width = (heads + 2 * kv_heads) * dim
+    head = torch.randn(heads * dim, vocab, generator=g).to(DEV) * 0.1
+
+    def step(c, b, x):
+        q, k, v = (t.view(x.shape[0], -1, dim) for t in x.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+        sv.kv_append(c, b, k, v)
+        return sv.paged_attention(c, b, q)
+    chunk = torch.randn(sum(prompt), width, generator=g).bfloat16().to(DEV)
+    first = sv.KVBatch(i32(starts(prompt)), i32(prompt), batch.pages, max_new=40)
+    o = step(cache, first, chunk)
+    want, _, tol, _ = ref.attention(cache, starts(prompt), prompt, batch.pages.cpu(), chunk[:, : heads * dim].view(-1, heads, dim), 1 / 8)
+    assert ((o.double().cpu() - want).abs() <= tol).all()
+
+    xs = [torch.randn(3, width, generator=g).bfloat16().to(DEV) for _ in range(steps)]
+    history = torch.zeros(3, steps, dtype=torch.int32, device=DEV)
+    pen = {"repetition": torch.full((3,), 1.3, device=DEV), "frequency": torch.full((3,), 0.2, device=DEV)}
+
+    def run(c, step_batch, lens, x, hist, made):
+        o = step(c, step_batch, x)
+        return o, sv.logits_process((o.reshape(3, -1).float() @ head), tokens=hist, n_tokens=made, **pen)
+    snapshot = [t.clone() for t in (cache.k, cache.v)] + ([cache.k_scale.clone(), cache.v_scale.clone()] if dtype == "e4m3" else [])
+    eager = []
+    for s in range(steps):
+        lens = [p + s + 1 for p in prompt]
+        b = sv.KVBatch(i32([0, 1, 2, 3]), i32(lens), batch.pages, max_new=1, max_kv=max(kv))
+        o, y = run(cache, b, lens, xs[s], history, i32([s] * 3))
+        want, _, tol, _ = plain_step(sv, cache, lens, batch.pages.cpu(), xs[s], heads, kv_heads, dim)
+        assert ((o.double().cpu() - want).abs() <= tol).all()
+        want, tol = ref.logits((o.reshape(3, -1).float() @ head), tokens=history.cpu(), n_tokens=[s] * 3, **{k: v.cpu() for k, v in pen.items()})
+        assert ((y.double().cpu() - want).abs() <= tol + want.abs() * ref.F32_HALF).all()
+        history[:, s] = y.argmax(-1).int()
+        eager.append((o.clone(), y.clone()))
+    for t, was in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), snapshot):
+        t.copy_(was)
+    made, length, x = i32([0] * 3), i32([p + 1 for p in prompt]), xs[0].clone()
+    hist = torch.zeros_like(history)
+    b = sv.KVBatch(i32([0, 1, 2, 3]), length, batch.pages, max_new=1, max_kv=max(kv))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        o, y = run(cache, b, None, x, hist, made)
+    for s in range(steps):
+        x.copy_(xs[s])
+        made.fill_(s)
+        length.copy_(i32([p + s + 1 for p in prompt]))
+        graph.replay()
+        assert torch.equal(o, eager[s][0]) and torch.equal(y, eager[s][1])
+        hist[:, s] = y.argmax(-1).int()
+
+
+def test_calls_on_two_streams_at_once(sv):
+    """Each with its own workspace: the same bits as one after the other"""
+    a = make(sv, [1, 1], [3000, 900], 2, 64, 16, seed=1)
+    b = make(sv, [3], [4000], 2, 64, 16, "e4m3", seed=2)
+    qa, qb = queries(a[2], 2, 8, 64), queries(b[2], 3, 8, 64)
+    want = sv.paged_attention(a[0], a[1], qa).clone(), sv.paged_attention(b[0], b[1], qb).clone()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            x = sv.paged_attention(a[0], a[1], qa)
+        with torch.cuda.stream(s2):
+            y = sv.paged_attention(b[0], b[1], qb)
+        got.append((x, y))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
+def test_empty_calls(sv):
+    cache, batch, _ = make(sv, [0, 0], [5, 0], 2, 64, 16)
+    e = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=DEV)
+    sv.kv_append(cache, batch, e, e)
+    assert sv.kv_read(cache, batch, 0)[0].shape == (0, 2, 64)
+    assert sv.paged_attention(cache, batch, e).shape == (0, 2, 64)
+    none = sv.KVBatch(i32([0]), torch.empty(0, dtype=torch.int32, device=DEV), torch.empty(0, 4, dtype=torch.int32, device=DEV))
+    assert sv.paged_attention(cache, none, e).shape == (0, 2, 64)
+    assert sv.logits_process(torch.empty(0, 10, device=DEV)).shape == (0, 10)
