@@ -12,7 +12,7 @@ LIB = os.path.join(CSRC, "libofa_b200.so")
 CLI = os.path.join(CSRC, "ofa_cli")              # the command-line host (csrc/ofa_cli.cpp), linked against LIB
 SOURCES = ["runtime.cu", "noalloc.cu", "serving.cu"]
 HEADERS = ["common.cuh", "task_api.h", "tickets.h", "elementwise.cuh", "gemm_tc.cuh", "attn_common.cuh", "attn_tc.cuh", "dp_nccl.inc", "simt_f32.cuh", "decode.cuh",
-           "megakernel.cuh", "paged.cuh", "paged_attn.cuh", "paged_move.cuh", "logits.cuh", os.path.join("..", "..", "include", "ofa_b200.h")]
+           "megakernel.cuh", "paged.cuh", "paged_attn.cuh", "paged_attn_tc.cuh", "paged_move.cuh", "logits.cuh", os.path.join("..", "..", "include", "ofa_b200.h")]
 
 
 def nvcc_path():

@@ -32,7 +32,8 @@ struct AttnArgs {
   float* lse;                       // [n_rows][n_heads] or null
   int n_heads, n_kv_heads, causal, window;
   Div group;
-  float scale_log2;
+  float scale_log2;                 // of many_rows_kernel: its magnitude, flip = the scale is negative
+  int flip;
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
   float* part;                      // nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
 };

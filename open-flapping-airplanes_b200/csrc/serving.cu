@@ -2,7 +2,7 @@
 // nothing, keep nothing from one call to the next and touch no other stream, so they can be captured into graphs and run side by side.
 #include "../../include/ofa_b200.h"
 #include "logits.cuh"
-#include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 #include "paged_move.cuh"
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -86,31 +86,45 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
 }
 
 // ---- attention
-struct Plan { int tiles, nsplit; size_t bytes; };
+struct Plan { bool many; int tiles, nsplit; size_t bytes; };
 
-// Blocks that share a tile's keys: as many as keep two blocks on each of 148 SMs busy, none with fewer than 8 steps of 32 keys (two for each of its four
-// warps). max_new and max_kv are what the caller says; without them a tile per sequence and the page table's width are assumed.
+// A chunk of more than 32 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 256 rows; fewer to the one that keeps more bytes
+// in flight. Blocks that share a tile's keys: as many as keep the SMs busy (one block of the first kernel on each of 148, two of the second), none with fewer than 512 keys
+// and 256. max_new and max_kv are what the caller says; without them one sequence with all rows and the page table's width are assumed.
 Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
   Plan p;
   const long long group = n_heads / c->n_kv_heads;
-  const long long newest = b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows;
-  long long tiles = (newest * group + 15) / 16;
+  const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
+  p.many = rows > 32;
+  long long tiles = p.many ? (rows + 255) / 256 : (rows + 15) / 16;
   if (tiles > 4096) tiles = 4096;
+  if (tiles < 1) tiles = 1;
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
-  const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * (tiles > 0 ? tiles : 1);
-  long long ns = 2 * 148 / blocks;
-  if (ns > kv / 256) ns = kv / 256;
+  const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles;
+  long long ns = (p.many ? 148 : 2 * 148) / blocks;
+  if (ns > kv / (p.many ? 512 : 256)) ns = kv / (p.many ? 512 : 256);
   if (ns > paged::MAX_SPLIT) ns = paged::MAX_SPLIT;
-  p.tiles = (int)(tiles > 0 ? tiles : 1); p.nsplit = (int)(ns > 1 ? ns : 1);
+  p.tiles = (int)tiles; p.nsplit = (int)(ns > 1 ? ns : 1);
   p.bytes = p.nsplit > 1 ? (size_t)n_rows * n_heads * p.nsplit * (c->head_dim + 2) * 4 : 0;
   return p;
 }
 
-template <int D, bool E4M3> cudaError_t few_rows(const paged::AttnArgs& P, cudaStream_t s) {
-  using F = paged::Few<D, E4M3>;
-  cudaError_t e = cudaFuncSetAttribute(paged::few_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-  if (e != cudaSuccess) return e;
-  paged::few_rows_kernel<D, E4M3><<<dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads), 128, F::SMEM, s>>>(P);
+template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, bool many, cudaStream_t s) {
+  const unsigned x = (unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), y = (unsigned)P.n_kv_heads;
+  cudaError_t e;
+  if (many) {
+    using F = paged::Tc<D>;
+    P.flip = P.scale_log2 < 0.f;
+    P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
+    e = cudaFuncSetAttribute(paged::many_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+    if (e != cudaSuccess) return e;
+    paged::many_rows_kernel<D, E4M3><<<dim3(x, y), 512, F::SMEM, s>>>(P);
+  } else {
+    using F = paged::Few<D, E4M3>;
+    e = cudaFuncSetAttribute(paged::few_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+    if (e != cudaSuccess) return e;
+    paged::few_rows_kernel<D, E4M3><<<dim3(x, y), 128, F::SMEM, s>>>(P);
+  }
   if (P.nsplit > 1) {
     cudaLaunchAttribute after = {};
     after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -157,11 +171,11 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
   P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
-  P.scale_log2 = a->scale * paged::LOG2E; P.tiles = p.tiles; P.nsplit = p.nsplit; P.part = static_cast<float*>(a->workspace);
+  P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0; P.tiles = p.tiles; P.nsplit = p.nsplit; P.part = static_cast<float*>(a->workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? few_rows<64, true>(P, s) : few_rows<128, true>(P, s);
-  else e = cache->head_dim == 64 ? few_rows<64, false>(P, s) : few_rows<128, false>(P, s);
+  if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p.many, s) : attend<128, true>(P, p.many, s);
+  else e = cache->head_dim == 64 ? attend<64, false>(P, p.many, s) : attend<128, false>(P, p.many, s);
   return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
 }
 

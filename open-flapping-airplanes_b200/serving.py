@@ -22,7 +22,7 @@ from .tasks import OfaError
 
 E4M3 = torch.float8_e4m3fn
 _TYPES = {"bf16": torch.bfloat16, "e4m3": E4M3}
-BAD_PAGE, BAD_LENGTH, BAD_ROWS = 1, 2, 4          # bits of a batch's status word
+BAD_PAGE, BAD_LENGTH, BAD_ROWS, TIMEOUT = 1, 2, 4, 8          # bits of a batch's status word
 
 
 def _refuse(msg):
@@ -100,7 +100,7 @@ class KVCache:
 class KVBatch:
     """The sequences of a step: q_start [n_seqs + 1], kv_len [n_seqs], pages [n_seqs, max_pages], int32 on the device. max_new and max_kv: the longest chunk
     and context as far as the program knows them; they choose how the work is cut, not what is computed. status: an int32 tensor whose first element
-    collects BAD_PAGE, BAD_LENGTH and BAD_ROWS."""
+    collects BAD_PAGE, BAD_LENGTH, BAD_ROWS and TIMEOUT."""
 
     def __init__(self, q_start, kv_len, pages, max_new=0, max_kv=0, status=None):
         _want("pages", pages, torch.int32, (None, None), None)
