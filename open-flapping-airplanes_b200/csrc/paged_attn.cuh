@@ -3,7 +3,7 @@
 // For each row: O = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = scale log2(e) q.k_j, over the keys it sees, in one pass with a running
 // maximum m. The rows of a key/value head (new tokens x the query heads that share it) are taken 16 at a time, the M of one mma.sync: with few rows the
 // tensor pipe idles whatever feeds it, and what counts is bytes in flight and few steps between the last byte and the answer. A block's four warps take
-// every fourth step of 32 keys and meet once, at the end; `nsplit` blocks share the keys of a tile and meet in combine_kernel.
+// every fourth step of 16 or 32 keys and meet once, at the end; `nsplit` blocks share the keys of a tile and meet in combine_kernel.
 //
 // A lane copies what it will itself feed to the mma, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
 // there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output columns
@@ -61,14 +61,17 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
 }
 
 template <int D, bool E4M3> struct Few {
-  static constexpr int KEYS = 32, WARPS = 4;
+  static constexpr int KEYS = D * (E4M3 ? 1 : 2) > 128 ? 16 : 32, WARPS = 4;      // of a step: 8 KB of keys and values a warp (4 KB: 8-bit rows of 64), so that
+                                                                // two blocks with three steps in flight for each warp fit an SM
+  static constexpr int NJ = KEYS / 8, NB = KEYS / 16;
   static constexpr int KP = D * (E4M3 ? 1 : 2) / 64;            // 16-byte pieces of a key that a lane holds
   static constexpr int VB = D * (E4M3 ? 1 : 2) / 8;             // bytes of a value row that a lane holds
   static constexpr int VW = VB >= 16 ? 16 : 8, VP = VB / VW;    // ... in pieces of VW
-  static constexpr int K_BYTES = 4 * KP * 512, V_BYTES = 8 * VB * 32;
+  static constexpr int K_BYTES = NJ * KP * 512, V_BYTES = NB * 4 * VB * 32;
   static constexpr int SIDE = 3 * 128;                          // scale words of K and V, flags
   static constexpr int STAGE = K_BYTES + V_BYTES + SIDE;
-  static constexpr int STAGES = K_BYTES + V_BYTES >= 16384 ? 3 : 4;
+  static constexpr int STAGES = K_BYTES + V_BYTES >= 8192 ? 3 : 4;
+  static constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
   static constexpr int SMEM = WARPS * STAGES * STAGE;
   static_assert(WARPS * 16 * (D + 2) * 4 <= SMEM, "the meeting of the warps does not fit");
 };
@@ -80,7 +83,7 @@ template <bool E4M3> __device__ float held(const char* row, int d, int scale) {
 }
 
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ AttnArgs P) {
+__global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant__ AttnArgs P) {
   using F = Few<D, E4M3>;
   constexpr int NT = D / 8, KS = D / 16;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -122,27 +125,28 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ A
     for (int t = 0; t < NT; t++) { o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f; }
 
     auto issue = [&](int i) {                                    // the warp's i-th step: a lane looks up one key and copies its parts of all 32
-      const int p = (a + i * F::WARPS) * F::KEYS + lane;
+      const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
       int page = 0, at = 0;
       const bool ok = p >= lo && p < hi && locate(P.b, seq, p, page, at);
       const long long off = ok ? (long long)page * P.c.page_b + (long long)at * P.c.row_b : -1;
       const int slot = i % F::STAGES;
       const uint32_t dk = ring_s + slot * F::STAGE, dv = dk + F::K_BYTES, side = dv + F::V_BYTES;
+      long long o_k[F::NJ], o_v[F::NB * 4];                       // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const long long o2 = __shfl_sync(0xffffffffu, off, j * 8 + r);
+      for (int j = 0; j < F::NJ; j++) o_k[j] = __shfl_sync(0xffffffffu, off, j * 8 + r);
 #pragma unroll
-        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, o2 >= 0 ? kb + o2 + x * 64 + c * 16 : kb, o2 >= 0);
-      }
+      for (int j = 0; j < F::NB * 4; j++) o_v[j] = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const long long o2 = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8);
+      for (int j = 0; j < F::NJ; j++)
+#pragma unroll
+        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, o_k[j] >= 0 ? kb + o_k[j] + x * 64 + c * 16 : kb, o_k[j] >= 0);
+#pragma unroll
+      for (int j = 0; j < F::NB * 4; j++)
 #pragma unroll
         for (int x = 0; x < F::VP; x++) {
-          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, o2 >= 0 ? vb + o2 + x * 128 + r * 16 : vb, o2 >= 0);
-          else cp8(dv + j * 256 + lane * 8, o2 >= 0 ? vb + o2 + r * 8 : vb, o2 >= 0);
+          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, o_v[j] >= 0 ? vb + o_v[j] + x * 128 + r * 16 : vb, o_v[j] >= 0);
+          else cp8(dv + j * 256 + lane * 8, o_v[j] >= 0 ? vb + o_v[j] + r * 8 : vb, o_v[j] >= 0);
         }
-      }
       uint32_t fl = ok ? 16u : 0u;
       if constexpr (E4M3) {                                      // the aligned word around the scale byte; which byte of it is kept beside it
         const long long so = ok ? (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row : 0;
@@ -159,16 +163,16 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ A
       unsigned char* sk = ring + slot * F::STAGE;
       unsigned char* sv = sk + F::K_BYTES;
       const uint32_t* side = reinterpret_cast<const uint32_t*>(sv + F::V_BYTES);
-      const uint32_t fl = side[64 + lane], valid = __ballot_sync(0xffffffffu, fl & 16u);
+      const uint32_t fl = side[64 + lane], valid = __ballot_sync(0xffffffffu, fl & 16u) & F::ALL;
       uint32_t kf = 0, vf = 0;                                   // 2^120 times the scales of this lane's key
       if constexpr (E4M3) {
         kf = scale_bits((side[lane] >> ((fl & 3) * 8)) & 255);
         vf = scale_bits((side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255);
       }
-      const bool mask = valid != 0xffffffffu || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 <= p_max - P.window);
-      float s[4][4];
+      const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 <= p_max - P.window);
+      float s[F::NJ][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < F::NJ; j++) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
         uint32_t f = 0;
         if constexpr (E4M3) { f = __shfl_sync(0xffffffffu, kf, j * 8 + r); f |= f << 16; }
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ A
       }
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < F::NJ; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           s[j][e] *= P.scale_log2;
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ A
       }
       const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};   // a row that has seen no key yet: 2^(-inf - 0) = 0
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < F::NJ; j++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) s[j][e] = ex2_approx(s[j][e] - ms[e >> 1]);
         l[0] += s[j][0] + s[j][1]; l[1] += s[j][2] + s[j][3];
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const __grid_constant__ A
         }
       }
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; kb2++) {
+      for (int kb2 = 0; kb2 < F::NB; kb2++) {
         // P is rounded to bf16 for the product (half a step, 2^-9 of each term, averaged over the keys); its sum l is taken before
         const uint32_t pf[4] = {pack2f(s[2 * kb2][0], s[2 * kb2][1]), pack2f(s[2 * kb2][2], s[2 * kb2][3]), pack2f(s[2 * kb2 + 1][0], s[2 * kb2 + 1][1]), pack2f(s[2 * kb2 + 1][2], s[2 * kb2 + 1][3])};
         uint32_t f01 = 0, f89 = 0;

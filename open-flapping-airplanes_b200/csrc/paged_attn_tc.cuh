@@ -28,7 +28,7 @@ enum { ST_TIMEOUT = 8 };
 template <int D> struct Tc {
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
   static constexpr int NST = D == 128 ? 4 : 8;                  // ring of K and V tiles
-  static constexpr int LAG = D == 128 ? 2 : 4;                  // tiles whose copies may be in flight when the next is begun
+  static constexpr int LAG = D == 128 ? 1 : 2;                  // tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
   static constexpr int Q_AT = 0, RING_AT = 2 * TILE, CTRL_AT = RING_AT + NST * TILE;
   static constexpr int SMEM = CTRL_AT + 512 + 1024;             // 1,024 for the alignment of the swizzle's atoms
@@ -48,10 +48,22 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < 10000000; i++) if (mbar_try(bar, parity)) return true;
   return false;
 }
+__device__ __forceinline__ bool elect_one() {                  // one thread of a converged warp
+  uint32_t e;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem desc]
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u64 desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
 template <bool INC, int N> __device__ __forceinline__ void set_regs() {
   if constexpr (INC) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }      // the lowest n bits
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) { return (uint32_t)((chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
 
 template <int D, bool E4M3>
@@ -61,7 +73,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   // the last pairs of tiles of a sequence have the most keys: they start first
   const int split = (int)blockIdx.x % P.nsplit, seq = (int)blockIdx.x / P.nsplit % P.b.n_seqs, kvh = blockIdx.y;
   const int turn = (int)blockIdx.x / P.nsplit / P.b.n_seqs;
@@ -141,7 +153,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
           u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
           *reinterpret_cast<uint4*>(dst + tile_at(r, q)) = u;
         }
-        fence_proxy_async();
+        fence_async_shared();
         attn_tc::warp_arrive(smem_u32(&ct.q_full));
       }
       const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + 256 + tile * D;
@@ -153,35 +165,25 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        // Half of the scores at a time: all 128 beside what else a thread keeps do not fit its registers. The second half stays there from the search of the maximum,
-        // the first is read again; probabilities go over the second, which by then has been read.
-        uint32_t s[2][32];
+        uint32_t s[4][32];
         const uint4 vw = *reinterpret_cast<const uint4*>(ct.valid[j % F::NV]);
-        const bool mask = partial(k, j) || (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu;
-        auto read = [&](int half) {
-          attn_tc::tmem_ld32_nw(ts + half * 64, s[0]);
-          attn_tc::tmem_ld32_nw(ts + half * 64 + 32, s[1]);
-          attn_tc::tmem_ld_wait();
-          if (mask) {
-            const int x1 = (P.causal ? pos - k0 : 127) - half * 64, x0 = (P.window ? pos - P.window + 1 - k0 : 0) - half * 64;
-            const uint32_t w[2] = {half ? vw.z : vw.x, half ? vw.w : vw.y};
 #pragma unroll
-            for (int q = 0; q < 2; q++)
+        for (int q = 0; q < 4; q++) attn_tc::tmem_ld32_nw(ts + q * 32, s[q]);
+        attn_tc::tmem_ld_wait();
+        if (partial(k, j) || (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu) {
+          const int x1 = P.causal ? pos - k0 : 127, x0 = P.window ? pos - P.window + 1 - k0 : 0;       // of the step's keys the row sees x0 .. x1
 #pragma unroll
-              for (int x = 0; x < 32; x++)
-                if (!((w[q] >> x) & 1) || q * 32 + x > x1 || q * 32 + x < x0) s[q][x] = 0xff800000u;
-          }
-        };
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int q = 0; q < 4; q++) {
+            const uint32_t w = (q == 0 ? vw.x : q == 1 ? vw.y : q == 2 ? vw.z : vw.w) & below(x1 + 1 - q * 32) & ~below(x0 - q * 32);
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          read(half);
-#pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            mx[x & 2] = attn_tc::max3(mx[x & 2], __uint_as_float(s[0][x]), __uint_as_float(s[0][x + 1]));
-            mx[(x & 2) + 1] = attn_tc::max3(mx[(x & 2) + 1], __uint_as_float(s[1][x]), __uint_as_float(s[1][x + 1]));
+            for (int x = 0; x < 32; x++) s[q][x] = w & (1u << x) ? s[q][x] : 0xff800000u;
           }
         }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 32; x += 2)
+#pragma unroll
+          for (int q = 0; q < 4; q++) mx[q] = attn_tc::max3(mx[q], __uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1]));
         const float m_true = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2);
         if (c == 0) m = m_true;
         else {
@@ -203,20 +205,16 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
         const u64 sc2 = attn_tc::f2(P.scale_log2, P.scale_log2), nm2 = attn_tc::f2(-ref, -ref);
         u64 sum[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int half = 1; half >= 0; half--) {
-          if (half == 0) read(0);
+        for (int q = 0; q < 4; q++) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int q = 0; q < 2; q++) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const float2 v = attn_tc::unf2(attn_tc::fma2(attn_tc::f2(__uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1])), sc2, nm2));
-              const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
-              sum[(x >> 1) & 3] = attn_tc::add2(sum[(x >> 1) & 3], attn_tc::f2(p0, p1));
-              pk[x >> 1] = pack2f(p0, p1);                       // rounded to bf16 for the product; the sum is taken before
-            }
-            attn_tc::tmem_st16(ts + 64 + half * 32 + q * 16, pk);
+          for (int x = 0; x < 32; x += 2) {
+            const float2 v = attn_tc::unf2(attn_tc::fma2(attn_tc::f2(__uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1])), sc2, nm2));
+            const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
+            sum[(x >> 1) & 3] = attn_tc::add2(sum[(x >> 1) & 3], attn_tc::f2(p0, p1));
+            pk[x >> 1] = pack2f(p0, p1);                         // rounded to bf16 for the product; the sum is taken before
           }
+          attn_tc::tmem_st16(ts + 64 + q * 16, pk);
         }
         attn_tc::tmem_st_wait();
         tc_fence_before();
@@ -281,46 +279,57 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     set_regs<false, 72>();
     const int tile = warp - 8;
     uint32_t uses = 0, done = 0, round = 0;                      // items through the ring, steps of the tile
+    // The whole warp walks, so that descriptors and addresses stay uniform, and one elected thread issues. What the loaders wrote is ordered before
+    // the products' reads by a fence here: in the loaders it would wait for every copy they have in flight.
+    const bool leader = elect_one();
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
-      if (lane == 0) {
-        const uint32_t ts = tmem + tile * 128, to = tmem + 256 + tile * D, sq = base + F::Q_AT + tile * F::TILE;
-        constexpr uint32_t I_S = umma_idesc(false, false, 128, 128), I_O = umma_idesc(false, true, 128, D);
-        ok = wait_for(smem_u32(&ct.q_full), round & 1);
-        uint32_t c = 0;
-        for (int j = k.A; j < k.B && ok; j++) {
-          const bool mine = j >= k.a[tile] && j < k.b[tile];
+      const int ka = k.a[tile], kb = k.b[tile];
+      const uint32_t ts = tmem + tile * 128, to = tmem + 256 + tile * D;
+      const u64 dq = umma_smem_desc(base + F::Q_AT + tile * F::TILE, 16, 1024);
+      constexpr uint32_t I_S = umma_idesc(false, false, 128, 128), I_O = umma_idesc(false, true, 128, D);
+      uint32_t c = 0;
+      auto slot_of = [&](int item) { return (uses + (uint32_t)item) % F::NST; };
+      auto filled = [&](int item) { return wait_for(smem_u32(&ct.full[slot_of(item)]), ((uses + (uint32_t)item) / F::NST) & 1); };
+      auto scores = [&](int j) {                                 // S = Q K_j^T, over the probabilities of the step before: one thread's products run in their order
+        const uint32_t slot = slot_of(2 * (j - k.A));
+        if (j < ka || j >= kb) { if (leader) mbar_arrive(smem_u32(&ct.empty[slot])); return; }
+        const u64 dk = umma_smem_desc(base + F::RING_AT + slot * F::TILE, 16, 1024);
+        if (leader) {
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            const uint32_t n = uses + 2 * (uint32_t)(j - k.A) + half, slot = n % F::NST;
-            const uint32_t sb = base + F::RING_AT + slot * F::TILE;
-            ok = ok && wait_for(smem_u32(&ct.full[slot]), (n / F::NST) & 1);
-            if (!ok) break;
-            if (!mine) { mbar_arrive(smem_u32(&ct.empty[slot])); continue; }
-            if (half == 0) {                                     // S = Q K_j^T, into columns whose probabilities the product before has read
-              if (c > 0) ok = wait_for(smem_u32(&ct.o_full[tile]), (done + c - 1) & 1);
-              if (!ok) break;
-              tc_fence_after();
+          for (int kk = 0; kk < D / 16; kk++) umma_bf16(ts, dq + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
+          umma_commit(smem_u32(&ct.s_full[tile]));
+          umma_commit(smem_u32(&ct.empty[slot]));
+        }
+      };
+      ok = wait_for(smem_u32(&ct.q_full), round & 1);
+      if (k.A < k.B) {
+        ok = ok && filled(0);
+        fence_async_shared();
+        if (ok) scores(k.A);
+      }
+      for (int j = k.A; j < k.B && ok; j++) {
+        const int item = 2 * (j - k.A) + 1;
+        ok = filled(item) && (j + 1 == k.B || filled(item + 1));
+        if (!ok) break;
+        fence_async_shared();                                    // what the loaders wrote, before it is read by the products
+        const uint32_t slot = slot_of(item);
+        if (j >= ka && j < kb) {                                 // O += P V_j
+          const u64 dv = umma_smem_desc(base + F::RING_AT + slot * F::TILE, 16384, 1024);
+          ok = wait_for(smem_u32(&ct.p_full[tile]), (done + c) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
 #pragma unroll
-              for (int kk = 0; kk < D / 16; kk++)
-                umma_bf16(ts, umma_smem_desc(sq + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024), umma_smem_desc(sb + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024), I_S, kk > 0 ? 1u : 0u);
-              umma_commit(smem_u32(&ct.s_full[tile]));
-            } else {                                             // O += P V_j
-              ok = wait_for(smem_u32(&ct.p_full[tile]), (done + c) & 1);
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll
-              for (int kk = 0; kk < 8; kk++)
-                asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                             ::"r"(to), "r"(ts + 64 + kk * 8), "l"(umma_smem_desc(sb + kk * 2048, 16384, 1024)), "r"(I_O), "r"((c > 0 || kk > 0) ? 1u : 0u) : "memory");
-              umma_commit(smem_u32(&ct.o_full[tile]));
-              c++;
-            }
+            for (int kk = 0; kk < 8; kk++) umma_bf16_ts(to, ts + 64 + kk * 8, dv + kk * 2048 / 16, I_O, (c > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(smem_u32(&ct.o_full[tile]));
             umma_commit(smem_u32(&ct.empty[slot]));
           }
-        }
+          c++;
+        } else if (leader) mbar_arrive(smem_u32(&ct.empty[slot]));
+        if (j + 1 < k.B) scores(j + 1);
       }
-      uses += 2u * (uint32_t)(k.B - k.A); done += (uint32_t)(k.b[tile] - k.a[tile]); round++;
+      uses += 2u * (uint32_t)(k.B - k.A); done += (uint32_t)(kb - ka); round++;
       if (!next(ok)) break;
     }
   } else {
@@ -329,81 +338,119 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     constexpr int CH = E4M3 ? D / 16 : D / 8, IT = 16 * CH / 32;      // 16-byte pieces of a held row, of 16 rows for each lane
     constexpr int LAG = E4M3 ? 0 : F::LAG;                       // rows in 8 bits are there when they are written
     const int w = warp - 10;
+    const char* kbase = P.c.k + (long long)kvh * P.c.head_b;
+    const char* vbase = P.c.v + (long long)kvh * P.c.head_b;
     uint32_t uses = 0;
+    // A step's 128 keys are eight units of 16 rows; a warp takes one or two, others in each step. Lanes 0 .. 15 (and 16 .. 31 again) look a unit's rows up, a step ahead.
+    struct Unit { long long off; uint32_t fk, fv; };
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
       const int total = 2 * (k.B - k.A);
-      for (int i = 0; i < total + LAG && ok; i++) {
-        if (i < total) {
+      auto look = [&](int j, int u) {
+        Unit x = {-1, 0, 0};
+        const int key = j * 128 + u * 16 + (lane & 15);
+        int page, at;
+        if (j < k.B && u < 8 && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) {
+          x.off = (long long)page * P.c.page_b + (long long)at * P.c.row_b;
+          if constexpr (E4M3) {
+            const long long so = (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row;
+            x.fk = __ldg(P.c.ks + so); x.fv = __ldg(P.c.vs + so);
+          }
+        }
+        return x;
+      };
+      auto fetch = [&](uint4 (&v)[4], const Unit& x, const char* src, int x0) {      // pieces x0 .. of the unit
+        constexpr int N = IT < 4 ? IT : 4;
+        long long o[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = __shfl_sync(0xffffffffu, x.off, ((x0 + i) * 32 + lane) / CH);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + lane % CH * 16) : make_uint4(0, 0, 0, 0);
+      };
+      auto put = [&](uint4 (&v)[4], uint32_t scale, unsigned char* dst, int j, int u, int x0, bool check) {     // check: values that some row must not meet
+        bool odd = false;
+        uint32_t f = 0;
+        if constexpr (E4M3) { f = scale_bits((int)scale); f |= f << 16; }
+#pragma unroll
+        for (int i = 0; i < (IT < 4 ? IT : 4); i++) {
+          const int idx = (x0 + i) * 32 + lane, row = u * 16 + idx / CH, q = idx % CH;
+          if constexpr (E4M3) {
+            uint32_t fr = __shfl_sync(0xffffffffu, f, idx / CH);
+            if (check && fr == 0x7fc07fc0u) { odd = true; fr = 0; }
+            *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * q)) = make_uint4(widen_lo(v[i].x, fr), widen_hi(v[i].x, fr), widen_lo(v[i].y, fr), widen_hi(v[i].y, fr));
+            *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * q + 1)) = make_uint4(widen_lo(v[i].z, fr), widen_hi(v[i].z, fr), widen_lo(v[i].w, fr), widen_hi(v[i].w, fr));
+          } else {
+            if (check && (odd_bits(v[i].x) || odd_bits(v[i].y) || odd_bits(v[i].z) || odd_bits(v[i].w))) {
+              odd = true;
+              v[i] = make_uint4(without_odd(v[i].x), without_odd(v[i].y), without_odd(v[i].z), without_odd(v[i].w));
+            }
+            *reinterpret_cast<uint4*>(dst + tile_at(row, q)) = v[i];
+          }
+        }
+        if (odd) { atomicMin(&ct.odd_lo, j * 128 + u * 16); atomicMax(&ct.odd_hi, min(k.hi - 1, j * 128 + u * 16 + 15)); }
+      };
+      int u = w;                                                 // the warp's units of the step: u, and u + 6 if there is one
+      Unit now[2] = {look(k.A, u), look(k.A, u + 6)};
+      uint4 v[4];
+      if constexpr (E4M3) fetch(v, now[0], kbase, 0);
+      int i = 0;
+      auto landed = [&](int item) {                              // of this warp's rows; the products may read a tile when all six have said so
+        if (item >= 0 && item < total) attn_tc::warp_arrive(smem_u32(&ct.full[(uses + (uint32_t)item) % F::NST]));
+      };
+      for (int j = k.A; j < k.B && ok; j++) {
+        const int un = (u + 4) % F::LOADERS;
+        const Unit then[2] = {look(j + 1, un), look(j + 1, un + 6)};
+        const bool part = partial(k, j);
+#pragma unroll
+        for (int half = 0; half < 2; half++, i++) {
           const uint32_t n = uses + (uint32_t)i, slot = n % F::NST;
-          const int j = k.A + (i >> 1);
-          const bool is_v = i & 1, part = partial(k, j);
+          const char* src = half ? vbase : kbase;
           ok = wait_for(smem_u32(&ct.empty[slot]), ((n / F::NST) & 1) ^ 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
-          const uint32_t dst_s = base + F::RING_AT + slot * F::TILE;
-          const char* src = (is_v ? P.c.v : P.c.k) + (long long)kvh * P.c.head_b;
-          for (int u = (w + F::LOADERS - (i * 8) % F::LOADERS) % F::LOADERS; u < 8; u += F::LOADERS) {
-            const int key = j * 128 + u * 16 + (lane & 15);
-            int page = 0, at = 0;
-            const bool there = key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at);
-            const long long off = there ? (long long)page * P.c.page_b + (long long)at * P.c.row_b : -1;
-            const uint32_t vb = __ballot_sync(0xffffffffu, there) & 0xffffu;
-            if (!is_v && lane == 0) ct.valid[j % F::NV][u] = (uint16_t)vb;
-            if (!E4M3 && !part) {
 #pragma unroll
-              for (int x = 0; x < IT; x++) {
-                const int idx = x * 32 + lane, row = idx / CH, q = idx % CH;
-                const long long o = __shfl_sync(0xffffffffu, off, row);
-                cp16(dst_s + tile_at(u * 16 + row, q), o >= 0 ? src + o + q * 16 : src, o >= 0);
-              }
+          for (int x = 0; x < 2; x++) {
+            const int uu = u + 6 * x;
+            if (uu >= 8) break;
+            if (half == 0) {
+              const uint32_t vb = __ballot_sync(0xffffffffu, now[x].off >= 0);
+              if (lane == 0) ct.valid[j % F::NV][uu] = (uint16_t)vb;
+            }
+            if constexpr (E4M3) {                                // the next unit's bytes are on their way while this one's are widened
+              uint4 vn[4];
+              if (x == 0 && u < 2) fetch(vn, now[1], src, 0);
+              else if (half == 0) fetch(vn, now[0], vbase, 0);
+              else fetch(vn, then[0], kbase, 0);
+              put(v, half ? now[x].fv : now[x].fk, dst, j, uu, 0, half && part);
+#pragma unroll
+              for (int y = 0; y < 4; y++) v[y] = vn[y];
+            } else if (part) {
+#pragma unroll 1
+              for (int x0 = 0; x0 < IT; x0 += 4) { fetch(v, now[x], src, x0); put(v, 0, dst, j, uu, x0, half); }
             } else {
-              uint32_t f = 0;
-              if (E4M3 && there) {
-                f = scale_bits((is_v ? P.c.vs : P.c.ks)[(long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row]);
-                f |= f << 16;
+              const uint32_t dst_s = smem_u32(dst);
+              long long o[IT];                                   // all the exchanges before the first copy: in turns each copy would wait for its own
+#pragma unroll
+              for (int y = 0; y < IT; y++) o[y] = __shfl_sync(0xffffffffu, now[x].off, (y * 32 + lane) / CH);
+#pragma unroll
+              for (int y = 0; y < IT; y++) {
+                const int row = (y * 32 + lane) / CH, q = lane % CH;
+                cp16(dst_s + tile_at(uu * 16 + row, q), o[y] >= 0 ? src + o[y] + q * 16 : src, o[y] >= 0);
               }
-              bool odd = false;
-#pragma unroll
-              for (int x0 = 0; x0 < IT; x0 += 4) {
-                constexpr int BT = IT < 4 ? IT : 4;
-                uint4 v[BT];
-#pragma unroll
-                for (int x = 0; x < BT; x++) {
-                  const int idx = (x0 + x) * 32 + lane, row = idx / CH, q = idx % CH;
-                  const long long o = __shfl_sync(0xffffffffu, off, row);
-                  v[x] = o >= 0 ? *reinterpret_cast<const uint4*>(src + o + q * 16) : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int x = 0; x < BT; x++) {
-                  const int idx = (x0 + x) * 32 + lane, row = idx / CH, q = idx % CH;
-                  if constexpr (E4M3) {
-                    uint32_t fr = __shfl_sync(0xffffffffu, f, row);
-                    if (is_v && part && fr == 0x7fc07fc0u) { odd = true; fr = 0; }
-                    *reinterpret_cast<uint4*>(dst + tile_at(u * 16 + row, 2 * q)) = make_uint4(widen_lo(v[x].x, fr), widen_hi(v[x].x, fr), widen_lo(v[x].y, fr), widen_hi(v[x].y, fr));
-                    *reinterpret_cast<uint4*>(dst + tile_at(u * 16 + row, 2 * q + 1)) = make_uint4(widen_lo(v[x].z, fr), widen_hi(v[x].z, fr), widen_lo(v[x].w, fr), widen_hi(v[x].w, fr));
-                  } else {
-                    if (is_v && (odd_bits(v[x].x) || odd_bits(v[x].y) || odd_bits(v[x].z) || odd_bits(v[x].w))) {
-                      odd = true;
-                      v[x] = make_uint4(without_odd(v[x].x), without_odd(v[x].y), without_odd(v[x].z), without_odd(v[x].w));
-                    }
-                    *reinterpret_cast<uint4*>(dst + tile_at(u * 16 + row, q)) = v[x];
-                  }
-                }
-              }
-              if (odd) { atomicMin(&ct.odd_lo, j * 128 + u * 16); atomicMax(&ct.odd_hi, min(k.hi - 1, j * 128 + u * 16 + 15)); }
             }
           }
+          cp_commit();
+          cp_wait<LAG>();
+          landed(i - LAG);
         }
-        cp_commit();
-        cp_wait<LAG>();
-        if (i >= LAG) {                                       // the copies of the tile LAG before this one have landed: the products may read it
-          fence_proxy_async();
-          attn_tc::warp_arrive(smem_u32(&ct.full[(uses + (uint32_t)(i - LAG)) % F::NST]));
-        }
+        u = un; now[0] = then[0]; now[1] = then[1];
       }
       cp_wait<0>();
+      if (ok) {
+#pragma unroll
+        for (int y = LAG; y > 0; y--) landed(total - y);
+      }
       uses += (uint32_t)total;
       if (!next(ok)) break;
     }
