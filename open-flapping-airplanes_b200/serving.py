@@ -44,16 +44,68 @@ def _want(name, t, dtype, shape, device, inner=True):
         _refuse(f"the last axis of {name} has to be dense")
 
 
-def _call(fn, device, *args):
-    """fn(*args, current stream of `device`), with that device current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
+# The current stream's handle and the current device, without an object around them (0.1 instead of 1.2 us a call)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+def _call(fn, index, *args):
+    """fn(*args, current stream of device `index`), with that device current."""
+    if _current() == index:
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
-    if rc != capi.OK:
-        raise OfaError(rc, capi.load().ofa_serving_last_error().decode())
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        raise OfaError(rc, _lib().ofa_serving_last_error().decode())
+
+
+_loaded = None
+
+
+def _lib():
+    global _loaded
+    if _loaded is None:
+        _loaded = capi.load()
+    return _loaded
+
+
+def _rows(name, t, shape, cache):
+    """The strides of bf16 rows [n_rows, heads, head_dim] on the cache's device; what is wrong with them otherwise."""
+    try:
+        if t.dtype is _BF16 and t.get_device() == cache.index and (shape is None or t.shape == shape):
+            s = t.stride()
+            if len(s) == 3 and s[2] == 1 and t.shape[2] == cache.head_dim:
+                return s
+    except AttributeError:
+        pass
+    _want(name, t, _BF16, (None, None, cache.head_dim) if shape is None else shape, cache.device)
+    return t.stride()                                           # a last axis of one element, any stride
+
+
+def _array(name, t, dtype, rows, index, device):
+    """A dense [rows] array's address."""
+    try:
+        if t.dtype is dtype and t.get_device() == index and t.shape == (rows,) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _want(name, t, dtype, (rows,), device)
+    return t.data_ptr()
+
+
+def _table(name, t, dtype, shape, index, device):
+    """(address, row stride) of a [rows, n] array with dense rows"""
+    try:
+        if t.dtype is dtype and t.get_device() == index:
+            s = t.stride()
+            if len(s) == 2 and s[1] == 1 and t.shape[0] == shape[0] and (shape[1] is None or t.shape[1] == shape[1]):
+                return t.data_ptr(), s[0]
+    except AttributeError:
+        pass
+    _want(name, t, dtype, shape, device)
+    return t.data_ptr(), t.stride(0)
 
 
 class KVCache:
@@ -73,10 +125,11 @@ class KVCache:
                 _refuse("k_scale and v_scale have different strides")
         elif k_scale is not None or v_scale is not None:
             _refuse("a bf16 cache has no scales")
-        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.k, self.v, self.k_scale, self.v_scale, self.device, self.index = k, v, k_scale, v_scale, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         if self.head_dim not in (64, 128):
             _refuse(f"head_dim {self.head_dim}: 64 and 128 are built")
+        self.scale = 1.0 / math.sqrt(self.head_dim)
         c = self.c = capi.KvCache()
         c.dtype, c.head_dim, c.n_kv_heads, c.page_size, c.n_pages = capi.KV_E4M3 if e4m3 else capi.KV_BF16, self.head_dim, self.n_kv_heads, self.page_size, self.n_pages
         c.k, c.v = k.data_ptr(), v.data_ptr()
@@ -113,7 +166,8 @@ class KVBatch:
                 _refuse("status is empty")
         if max_new < 0 or max_kv < 0:
             _refuse(f"max_new {max_new}, max_kv {max_kv}")
-        self.q_start, self.kv_len, self.pages, self.status, self.device = q_start, kv_len, pages, status, pages.device
+        self.q_start, self.kv_len, self.pages, self.status, self.device, self.index = q_start, kv_len, pages, status, pages.device, pages.get_device()
+        self._need = {}                                         # workspace sizes by what they depend on beside the batch
         c = self.c = capi.KvBatch()
         c.n_seqs, c.max_pages, c.pages_stride = n, pages.shape[1], pages.stride(0)
         c.q_start, c.kv_len, c.pages = q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr()
@@ -123,28 +177,31 @@ class KVBatch:
 
 
 def _same_device(cache, batch):
-    if cache.device != batch.device:
+    if cache.index != batch.index:
         _refuse(f"the cache is on {cache.device}, the batch on {batch.device}")
+
+
+def _move(fn, cache, batch, k, v, n_rows):
+    _same_device(cache, batch)
+    rows = k.shape[0] if n_rows is None and isinstance(k, torch.Tensor) and k.dim() else n_rows
+    shape = (rows, cache.n_kv_heads, cache.head_dim)
+    a, b = _rows("k", k, shape, cache), _rows("v", v, shape, cache)
+    _call(fn, cache.index, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), shape[0], a[0], a[1], b[0], b[1])
 
 
 def kv_append(cache, batch, k, v):
     """Rows k and v [n_rows, n_kv_heads, head_dim] (bf16; views of a fused projection will do) to their pages, in the cache's type."""
-    _same_device(cache, batch)
-    _want("k", k, torch.bfloat16, (None, cache.n_kv_heads, cache.head_dim), cache.device)
-    _want("v", v, torch.bfloat16, k.shape, cache.device)
-    _call(capi.load().ofa_kv_append, cache.device, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    _move(_lib().ofa_kv_append, cache, batch, k, v, None)
 
 
 def kv_read(cache, batch, n_rows=None, k=None, v=None):
     """The batch's n_rows rows out of their pages, as bf16 [n_rows, n_kv_heads, head_dim] pairs (written into k and v where these are given)."""
-    _same_device(cache, batch)
     if k is None or v is None:
         if n_rows is None or k is not None or v is not None:
             _refuse("kv_read needs n_rows, or k and v to write to")
-        k, v = (torch.empty((n_rows, cache.n_kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device) for _ in range(2))
-    _want("k", k, torch.bfloat16, (n_rows, cache.n_kv_heads, cache.head_dim), cache.device)
-    _want("v", v, torch.bfloat16, k.shape, cache.device)
-    _call(capi.load().ofa_kv_read, cache.device, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        shape = (n_rows, cache.n_kv_heads, cache.head_dim)
+        k, v = torch.empty(shape, dtype=_BF16, device=cache.device), torch.empty(shape, dtype=_BF16, device=cache.device)
+    _move(_lib().ofa_kv_read, cache, batch, k, v, n_rows)
     return k, v
 
 
@@ -152,68 +209,61 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
     """Attention of q [n_rows, n_heads, head_dim] (bf16) over the batch's pages; scale: 1/sqrt(head_dim) by default. Returns out, of q's shape, or with
     with_lse (out, lse [n_rows, n_heads] fp32). Rows that no sequence brings are left as they were."""
     _same_device(cache, batch)
-    _want("q", q, torch.bfloat16, (None, None, cache.head_dim), cache.device)
-    n_rows, n_heads = q.shape[:2]
+    sq = _rows("q", q, None, cache)
+    shape = q.shape
+    n_rows, n_heads = shape[0], shape[1]
     if out is None:
-        out = torch.empty((n_rows, n_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
-    else:
-        _want("out", out, torch.bfloat16, q.shape, cache.device)
-    lse = torch.empty((n_rows, n_heads), dtype=torch.float32, device=cache.device) if with_lse else None
-    lib = capi.load()
-    a = capi.PagedAttentionArgs()
-    a.n_rows, a.n_heads, a.q, a.out = n_rows, n_heads, q.data_ptr(), out.data_ptr()
-    a.q_row_stride, a.q_head_stride, _ = q.stride()
-    a.out_row_stride, a.out_head_stride, _ = out.stride()
-    a.lse = lse.data_ptr() if with_lse else None
-    a.scale, a.causal, a.window = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale, bool(causal), window
-    need = lib.ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
-    if need:                                                   # the caller's allocator: a graph that captures the call keeps its own
-        work = torch.empty(need, dtype=torch.uint8, device=cache.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-    _call(lib.ofa_paged_attention, cache.device, cache.ref, batch.ref, C.byref(a))
+        out = torch.empty(shape, dtype=_BF16, device=cache.device)
+    so = _rows("out", out, shape, cache)
+    lse = torch.empty((n_rows, n_heads), dtype=_F32, device=cache.device) if with_lse else None
+    lib = _lib()
+    key = (cache.c.dtype, cache.head_dim, cache.n_kv_heads, cache.page_size, n_rows, n_heads)
+    need = batch._need.get(key)
+    if need is None:
+        need = batch._need[key] = lib.ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
+    # from the caller's allocator: a graph that captures the call keeps its own
+    work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    a = capi.PagedAttentionArgs(n_rows, n_heads, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse.data_ptr() if with_lse else None,
+                                cache.scale if scale is None else scale, bool(causal), window, work.data_ptr() if need else None, need)
+    _call(lib.ofa_paged_attention, cache.index, cache.ref, batch.ref, C.byref(a))
     return (out, lse) if with_lse else out
 
 
 def logits_process(logits, tokens=None, n_tokens=None, n_prompt=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias=None, mask=None, out=None):
     """Penalties of repeated tokens, biases and a bit mask on logits [n_rows, vocab] (bf16 or fp32); returns out (a new tensor by default; out=logits works in place).
     tokens [n_rows, max_tokens], n_tokens, n_prompt [n_rows], bias_ids [n_rows, n] and mask [n_rows, ceil(vocab / 32)] are int32, the rest fp32."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F32, _BF16):
         _refuse("logits have to be a bf16 or fp32 tensor")
-    _want("logits", logits, logits.dtype, (None, None), None)
+    kind, dev, index = logits.dtype, logits.device, logits.get_device()
+    if index < 0 or logits.dim() != 2:
+        _want("logits", logits, kind, (None, None), None)
     rows, vocab = logits.shape
-    dev = logits.device
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
-    elif out is not logits:
-        _want("out", out, logits.dtype, logits.shape, dev)
-    a = capi.LogitsArgs()
-    a.dtype, a.n_rows, a.vocab = capi.DTYPE_F32 if logits.dtype == torch.float32 else capi.DTYPE_BF16, rows, vocab
-    a.inp, a.out, a.in_stride, a.out_stride = logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0)
+        out = torch.empty((rows, vocab), dtype=kind, device=dev)
+    src, src_row = _table("logits", logits, kind, (rows, vocab), index, dev)
+    dst, dst_row = _table("out", out, kind, (rows, vocab), index, dev)
+    text = text_row = most = made = first = ids = bias_row = n_bias = weight = words = words_row = 0
     if tokens is not None:
-        _want("tokens", tokens, torch.int32, (rows, None), dev)
-        a.tokens, a.tokens_stride, a.max_tokens = tokens.data_ptr(), tokens.stride(0), tokens.shape[1]
-        if n_tokens is not None:
-            _want("n_tokens", n_tokens, torch.int32, (rows,), dev)
-            a.n_tokens = n_tokens.data_ptr()
-        if n_prompt is not None:
-            _want("n_prompt", n_prompt, torch.int32, (rows,), dev)
-            a.n_prompt = n_prompt.data_ptr()
-    elif any(x is not None for x in (n_tokens, n_prompt, repetition, presence, frequency)):
+        text, text_row = _table("tokens", tokens, _I32, (rows, None), index, dev)
+        most = tokens.shape[1]
+        made = 0 if n_tokens is None else _array("n_tokens", n_tokens, _I32, rows, index, dev)
+        first = 0 if n_prompt is None else _array("n_prompt", n_prompt, _I32, rows, index, dev)
+    elif not (n_tokens is n_prompt is repetition is presence is frequency is None):
         _refuse("penalties and token counts need tokens")
-    for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if x is not None:
-            _want(name, x, torch.float32, (rows,), dev)
-            setattr(a, name, x.data_ptr())
+    rep = 0 if repetition is None else _array("repetition", repetition, _F32, rows, index, dev)
+    pres = 0 if presence is None else _array("presence", presence, _F32, rows, index, dev)
+    freq = 0 if frequency is None else _array("frequency", frequency, _F32, rows, index, dev)
     if (bias_ids is None) != (bias is None):
         _refuse("bias_ids and bias come together")
     if bias is not None:
-        _want("bias_ids", bias_ids, torch.int32, (rows, None), dev)
-        _want("bias", bias, torch.float32, bias_ids.shape, dev)
-        if bias.stride(0) != bias_ids.stride(0) and rows > 1:
+        ids, row = _table("bias_ids", bias_ids, _I32, (rows, None), index, dev)
+        n_bias = bias_ids.shape[1]
+        weight, bias_row = _table("bias", bias, _F32, (rows, n_bias), index, dev)
+        if bias_row != row and rows > 1:
             _refuse("bias and bias_ids have different strides")
-        a.bias_ids, a.bias, a.bias_stride, a.max_bias = bias_ids.data_ptr(), bias.data_ptr(), bias.stride(0), bias.shape[1]
     if mask is not None:
-        _want("mask", mask, torch.int32, (rows, (vocab + 31) // 32), dev)
-        a.mask, a.mask_stride = mask.data_ptr(), mask.stride(0)
-    _call(capi.load().ofa_logits_process, dev, C.byref(a))
+        words, words_row = _table("mask", mask, _I32, (rows, (vocab + 31) // 32), index, dev)
+    a = capi.LogitsArgs(capi.DTYPE_F32 if kind is _F32 else capi.DTYPE_BF16, rows, vocab, src, src_row, dst, dst_row, text, text_row, most, made, first, rep, pres, freq,
+                        ids, weight, bias_row, n_bias, words, words_row)
+    _call(_lib().ofa_logits_process, index, C.byref(a))
     return out
