@@ -3,7 +3,8 @@
 // For each row: O = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = scale log2(e) q.k_j, over the keys it sees, in one pass with a running
 // maximum m. The rows of a key/value head (new tokens x the query heads that share it) are taken 16 at a time, the M of one mma.sync: with few rows the
 // tensor pipe idles whatever feeds it, and what counts is bytes in flight and few steps between the last byte and the answer. A block's four warps take
-// every fourth step of 16 or 32 keys and meet once, at the end; `nsplit` blocks share the keys of a tile and meet in combine_kernel.
+// every fourth step of 16 or 32 keys and meet once, at the end; up to eight blocks that share the keys of a tile are a cluster and meet in shared memory, more leave their
+// parts in the workspace for combine_kernel.
 //
 // A lane copies what it will itself feed to the mma, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
 // there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output columns
@@ -35,7 +36,8 @@ struct AttnArgs {
   float scale_log2;                 // of many_rows_kernel: its magnitude, flip = the scale is negative
   int flip;
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
-  float* part;                      // nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
+  int cluster;                      // ... which are a cluster and meet in shared memory
+  float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
@@ -58,6 +60,16 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
   if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
   return w;
+}
+
+// Shared memory of the cluster's other blocks
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
+__device__ __forceinline__ float peer_f32(uint32_t a) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ float4 peer_f32x4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
 }
 
 template <int D, bool E4M3> struct Few {
@@ -331,35 +343,60 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
     {
       constexpr int DP = D / 8;                                  // eight threads a row
       const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rr = tile * 16 + row, t = (int)P.group.quot(rr);
-      if (t < ch.n) {
-        float mm = -INFINITY, ll = 0.f, acc[DP] = {};
+      float mm = -INFINITY, ll = 0.f, acc[DP] = {};
 #pragma unroll
-        for (int w = 0; w < F::WARPS; w++) mm = fmaxf(mm, sm[w * 16 + row].x);
+      for (int w = 0; w < F::WARPS; w++) mm = fmaxf(mm, sm[w * 16 + row].x);
 #pragma unroll
-        for (int w = 0; w < F::WARPS; w++) {
-          const float2 ml = sm[w * 16 + row];
-          const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);      // no key seen, or only scores of -inf: sums of 0, or not finite
-          ll += ml.y * f;
+      for (int w = 0; w < F::WARPS; w++) {
+        const float2 ml = sm[w * 16 + row];
+        const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);      // no key seen, or only scores of -inf: sums of 0, or not finite
+        ll += ml.y * f;
 #pragma unroll
-          for (int x = 0; x < DP; x++) acc[x] += so[(w * 16 + row) * D + part * DP + x] * f;
-        }
-        const int head = kvh * group + rr - t * group;
-        const long long g = (long long)(ch.s + t) * P.n_heads + head;
-        if (P.nsplit == 1) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * DP;
+        for (int x = 0; x < DP; x++) acc[x] += so[(w * 16 + row) * D + part * DP + x] * f;
+      }
+      const int head = kvh * group + rr - t * group;
+      const long long g = (long long)(ch.s + t) * P.n_heads + head;
+      bool last = t < ch.n;                                      // this thread writes the row's result
+      if (P.cluster) {                                           // the blocks of the cluster meet in each other's shared memory, rows dealt out among them
+        __syncthreads();
 #pragma unroll
-          for (int x = 0; x < DP; x++) acc[x] *= inv;
+        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(so + row * D + part * DP + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+        if (part == 0) sm[row] = make_float2(mm, ll);
+        cluster_sync();
+        last = last && row % P.nsplit == split;
+        if (last) {
+          const uint32_t at = smem_u32(so + row * D + part * DP), am = smem_u32(sm + row);
+          mm = -INFINITY; ll = 0.f;
+          for (int s = 0; s < P.nsplit; s++) mm = fmaxf(mm, peer_f32(peer(am, s)));
 #pragma unroll
-          for (int x = 0; x < DP; x += 8) *reinterpret_cast<uint4*>(dst + x) = pack8(acc + x);
-          if (P.lse && part == 0) P.lse[g] = ll == 0.f ? -INFINITY : mm * LN2 + logf(ll);
-        } else {
-          float* dst = P.part + (g * P.nsplit + split) * D + part * DP;
+          for (int x = 0; x < DP; x++) acc[x] = 0.f;
+          for (int s = 0; s < P.nsplit; s++) {
+            const float m1 = peer_f32(peer(am, s)), f = m1 == -INFINITY ? 1.f : ex2_approx(m1 - mm);
+            ll += peer_f32(peer(am, s) + 4) * f;
+            const uint32_t src = peer(at, s);
 #pragma unroll
-          for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(dst + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
-          if (part == 0) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(mm, ll);
+            for (int x = 0; x < DP; x += 4) {
+              const float4 v = peer_f32x4(src + x * 4);
+              acc[x] += v.x * f; acc[x + 1] += v.y * f; acc[x + 2] += v.z * f; acc[x + 3] += v.w * f;
+            }
+          }
         }
       }
+      if (last && (P.cluster || P.nsplit == 1)) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * DP;
+#pragma unroll
+        for (int x = 0; x < DP; x++) acc[x] *= inv;
+#pragma unroll
+        for (int x = 0; x < DP; x += 8) *reinterpret_cast<uint4*>(dst + x) = pack8(acc + x);
+        if (P.lse && part == 0) P.lse[g] = ll == 0.f ? -INFINITY : mm * LN2 + logf(ll);
+      } else if (last) {
+        float* dst = P.part + (g * P.nsplit + split) * D + part * DP;
+#pragma unroll
+        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(dst + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+        if (part == 0) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(mm, ll);
+      }
+      if (P.cluster) cluster_sync();                             // nobody's shared memory goes while another reads it
     }
     __syncthreads();
   }

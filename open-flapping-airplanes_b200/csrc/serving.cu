@@ -5,6 +5,7 @@
 #include "paged_attn_tc.cuh"
 #include "paged_move.cuh"
 #include <cuda_runtime.h>
+#include <atomic>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -86,7 +87,7 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
 }
 
 // ---- attention
-struct Plan { bool many; int tiles, nsplit; size_t bytes; };
+struct Plan { bool many, cluster; int tiles, nsplit; size_t bytes; };
 
 // A chunk of more than 32 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 256 rows; fewer to the one that keeps more bytes
 // in flight. Blocks that share a tile's keys: as many as keep the SMs busy (one block of the first kernel on each of 148, two of the second), none with fewer than 512 keys
@@ -104,37 +105,47 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   long long ns = (p.many ? 148 : 2 * 148) / blocks;
   if (ns > kv / (p.many ? 512 : 256)) ns = kv / (p.many ? 512 : 256);
   if (ns > paged::MAX_SPLIT) ns = paged::MAX_SPLIT;
+  p.cluster = !p.many && ns > 1 && ns < 16;
+  if (p.cluster) ns = ns >= 8 ? 8 : ns >= 4 ? 4 : 2;
   p.tiles = (int)tiles; p.nsplit = (int)(ns > 1 ? ns : 1);
-  p.bytes = p.nsplit > 1 ? (size_t)n_rows * n_heads * p.nsplit * (c->head_dim + 2) * 4 : 0;
+  p.bytes = p.nsplit > 1 && !p.cluster ? (size_t)n_rows * n_heads * p.nsplit * (c->head_dim + 2) * 4 : 0;
   return p;
 }
 
+// The limit of dynamic shared memory, raised once for each kernel and device
+template <auto KERNEL> cudaError_t allow(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, bool many, cudaStream_t s) {
-  const unsigned x = (unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), y = (unsigned)P.n_kv_heads;
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute at = {};
+  lc.gridDim = dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads); lc.stream = s; lc.attrs = &at;
   cudaError_t e;
   if (many) {
-    using F = paged::Tc<D>;
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    e = cudaFuncSetAttribute(paged::many_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-    if (e != cudaSuccess) return e;
-    paged::many_rows_kernel<D, E4M3><<<dim3(x, y), 512, F::SMEM, s>>>(P);
+    constexpr auto kernel = paged::many_rows_kernel<D, E4M3>;
+    lc.blockDim = dim3(512); lc.dynamicSmemBytes = paged::Tc<D>::SMEM;
+    if ((e = allow<kernel>(paged::Tc<D>::SMEM)) == cudaSuccess) e = cudaLaunchKernelEx(&lc, kernel, P);
   } else {
-    using F = paged::Few<D, E4M3>;
-    e = cudaFuncSetAttribute(paged::few_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-    if (e != cudaSuccess) return e;
-    paged::few_rows_kernel<D, E4M3><<<dim3(x, y), 128, F::SMEM, s>>>(P);
+    constexpr auto kernel = paged::few_rows_kernel<D, E4M3>;
+    if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
+    lc.blockDim = dim3(128); lc.dynamicSmemBytes = paged::Few<D, E4M3>::SMEM;
+    if ((e = allow<kernel>(paged::Few<D, E4M3>::SMEM)) == cudaSuccess) e = cudaLaunchKernelEx(&lc, kernel, P);
   }
-  if (P.nsplit > 1) {
-    cudaLaunchAttribute after = {};
-    after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    after.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)(((long long)P.b.n_rows * P.n_heads + 3) / 4)); lc.blockDim = dim3(128); lc.stream = s; lc.attrs = &after; lc.numAttrs = 1;
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    if ((e = cudaLaunchKernelEx(&lc, paged::combine_kernel<D>, P)) != cudaSuccess) return e;
+  if (e == cudaSuccess && P.nsplit > 1 && !P.cluster) {
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    lc.gridDim = dim3((unsigned)(((long long)P.b.n_rows * P.n_heads + 3) / 4)); lc.blockDim = dim3(128); lc.dynamicSmemBytes = 0; lc.numAttrs = 1;
+    e = cudaLaunchKernelEx(&lc, paged::combine_kernel<D>, P);
   }
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace
@@ -171,7 +182,7 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
   P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
-  P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0; P.tiles = p.tiles; P.nsplit = p.nsplit; P.part = static_cast<float*>(a->workspace);
+  P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.part = static_cast<float*>(a->workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p.many, s) : attend<128, true>(P, p.many, s);

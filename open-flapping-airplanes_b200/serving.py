@@ -200,7 +200,8 @@ def kv_read(cache, batch, n_rows=None, k=None, v=None):
         if n_rows is None or k is not None or v is not None:
             _refuse("kv_read needs n_rows, or k and v to write to")
         shape = (n_rows, cache.n_kv_heads, cache.head_dim)
-        k, v = torch.empty(shape, dtype=_BF16, device=cache.device), torch.empty(shape, dtype=_BF16, device=cache.device)
+        k = torch.empty(shape, dtype=_BF16, device=cache.device)
+        v = torch.empty_like(k)
     _move(_lib().ofa_kv_read, cache, batch, k, v, n_rows)
     return k, v
 
@@ -213,7 +214,7 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
     shape = q.shape
     n_rows, n_heads = shape[0], shape[1]
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=cache.device)
+        out = torch.empty_like(q)
     so = _rows("out", out, shape, cache)
     lse = torch.empty((n_rows, n_heads), dtype=_F32, device=cache.device) if with_lse else None
     lib = _lib()
@@ -239,7 +240,7 @@ def logits_process(logits, tokens=None, n_tokens=None, n_prompt=None, repetition
         _want("logits", logits, kind, (None, None), None)
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=kind, device=dev)
+        out = torch.empty_like(logits)
     src, src_row = _table("logits", logits, kind, (rows, vocab), index, dev)
     dst, dst_row = _table("out", out, kind, (rows, vocab), index, dev)
     text = text_row = most = made = first = ids = bias_row = n_bias = weight = words = words_row = 0
