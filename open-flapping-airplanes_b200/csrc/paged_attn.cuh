@@ -1,18 +1,24 @@
 // Attention of few rows over a paged cache: a token, or a few, per sequence, where reading the keys and values is all that counts.
 //
 // For each row: O = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = scale log2(e) q.k_j, over the keys it sees, in one pass with a running
-// maximum m. The rows of a key/value head (new tokens x the query heads that share it) are taken 16 at a time, the M of one mma.sync: with few rows the
-// tensor pipe idles whatever feeds it, and what counts is bytes in flight and few steps between the last byte and the answer. A block's four warps take
+// maximum m. The rows of a key/value head (new tokens x the query heads that share it) are taken 8 or 16 at a time, as columns: S^T = K Q^T and O^T = V^T P^T are
+// mma.sync products of 16 keys (or 16 head dims) by 8 rows, so that a single token of up to eight query heads wastes neither accumulators nor exponentials (with the rows as the
+// 16 of a product a step of 32 keys took about 2,000 clocks and twice the registers). With few rows the
+// tensor pipe idles whatever feeds it; what counts is bytes in flight, instructions per key and few steps between the last byte and the answer. A block's four warps take
 // every fourth step of 16 or 32 keys and meet once, at the end; up to eight blocks that share the keys of a tile are a cluster and meet in shared memory, more leave their
 // parts in the workspace for combine_kernel.
 //
-// A lane copies what it will itself feed to the mma, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
-// there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output columns
+// A lane copies what it will itself feed to the products, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
+// there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output's dims
 // are free as long as both operands agree:
 //   scores   lane (r = lane / 4, c = lane % 4) holds of key r of 8 the dims c * 16 B + ... of every 64 B; q is fetched in the same order
-//   output   lane holds of keys 2c, 2c + 1, 2c + 8, 2c + 9 of 16 the dims r * 16 B + ..., two keys side by side make a word of the B operand, and column
-//            2c + e of the n-th 8-column product is dim (2c + e) * 8 + n
-// Rows of the 8-bit cache become bf16 with four instructions for two elements (paged::widen).
+//   output   lane holds of keys 2c, 2c + 1, 2c + 8, 2c + 9 of 16 the dims r * 16 B + ...; two keys side by side make a word of the A operand, and rows r and r + 8
+//            of the t-th product are two neighbouring dims
+// The scores' accumulator has keys down the lanes, the second product wants them along a lane: movmatrix turns 8 x 8 of them.
+//
+// Rows of the 8-bit cache enter the products as bf16 of 2^-120 times their codes (paged::raw_pair, three instructions for two elements); the keys' scales multiply the
+// scores, the values' scales the probabilities. So that nothing underflows, q is brought to 2^60 by a power of two for each row, and probabilities carry 2^100 (the result
+// 2^-20 of what it should be, made good at the end).
 //
 // A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
 // infinities and NaN are taken out of its values and added to the rows that see it. Rows past the context and of a bad page are never read.
@@ -72,20 +78,20 @@ __device__ __forceinline__ float4 peer_f32x4(uint32_t a) {
   return v;
 }
 
-template <int D, bool E4M3> struct Few {
-  static constexpr int KEYS = D * (E4M3 ? 1 : 2) > 128 ? 16 : 32, WARPS = 4;      // of a step: 8 KB of keys and values a warp (4 KB: 8-bit rows of 64), so that
-                                                                // two blocks with three steps in flight for each warp fit an SM
-  static constexpr int NJ = KEYS / 8, NB = KEYS / 16;
+template <int D, bool E4M3, int NR> struct Few {
+  static constexpr int KEYS = D * (E4M3 ? 1 : 2) > 128 ? 16 : 32, WARPS = 4, ROWS = 8 * NR;      // of a step: at most 8 KB of keys and values a warp
+  static constexpr int NB = KEYS / 16;
   static constexpr int KP = D * (E4M3 ? 1 : 2) / 64;            // 16-byte pieces of a key that a lane holds
   static constexpr int VB = D * (E4M3 ? 1 : 2) / 8;             // bytes of a value row that a lane holds
   static constexpr int VW = VB >= 16 ? 16 : 8, VP = VB / VW;    // ... in pieces of VW
-  static constexpr int K_BYTES = NJ * KP * 512, V_BYTES = NB * 4 * VB * 32;
+  static constexpr int K_BYTES = 2 * NB * KP * 512, V_BYTES = NB * 4 * VB * 32;
   static constexpr int SIDE = 3 * 128;                          // scale words of K and V, flags
   static constexpr int STAGE = K_BYTES + V_BYTES + SIDE;
-  static constexpr int STAGES = K_BYTES + V_BYTES >= 8192 ? 3 : 4;
+  static constexpr int STAGES = K_BYTES + V_BYTES >= 8192 ? 2 : 3;
   static constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
+  static constexpr int PAD = D + 8;                             // floats of a row where the warps meet
   static constexpr int SMEM = WARPS * STAGES * STAGE;
-  static_assert(WARPS * 16 * (D + 2) * 4 <= SMEM, "the meeting of the warps does not fit");
+  static_assert(WARPS * ROWS * (PAD + 2) * 4 <= SMEM, "the meeting of the warps does not fit");
 };
 
 // one held element as a float (the rare path)
@@ -94,10 +100,10 @@ template <bool E4M3> __device__ float held(const char* row, int d, int scale) {
   return to_f(reinterpret_cast<const bf16*>(row)[d]);
 }
 
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant__ AttnArgs P) {
-  using F = Few<D, E4M3>;
-  constexpr int NT = D / 8, KS = D / 16;
+template <int D, bool E4M3, int NR>
+__global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __grid_constant__ AttnArgs P) {
+  using F = Few<D, E4M3, NR>;
+  constexpr int MT = D / 16, KS = D / 16;                        // products of 16 dims of the output, of 16 dims of a score
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const int split = (int)blockIdx.x % P.nsplit, tile0 = (int)blockIdx.x / P.nsplit % P.tiles, seq = (int)blockIdx.x / P.nsplit / P.tiles, kvh = blockIdx.y;
@@ -108,23 +114,51 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
   const uint32_t ring_s = smem_u32(ring);
   const char* kb = P.c.k + (long long)kvh * P.c.head_b;
   const char* vb = P.c.v + (long long)kvh * P.c.head_b;
+  // the dim of row r (or r + 8: the one behind it) in the t-th product of the output
+  auto dim_of = [&](int t) { return E4M3 ? r * (D / 8) + 2 * t : (t / 4) * 64 + r * 8 + (t % 4) * 2; };
 
-  for (int tile = tile0; tile * 16 < ch.n * group; tile += P.tiles) {
-    // this thread's rows r and r + 8 of the tile
-    int pos[2];
-    uint32_t qf[KS][4];
-    const int t_last = min(ch.n - 1, (int)P.group.quot(tile * 16 + 15)), p_min = ch.p0 + (int)P.group.quot(tile * 16), p_max = ch.p0 + t_last;
+  for (int tile = tile0; tile * F::ROWS < ch.n * group; tile += P.tiles) {
+    const int t_last = min(ch.n - 1, (int)P.group.quot(tile * F::ROWS + F::ROWS - 1)), p_min = ch.p0 + (int)P.group.quot(tile * F::ROWS), p_max = ch.p0 + t_last;
+    uint32_t qf[NR][KS][2];                                      // row r of every eight
+    float rowf[NR][2];                                           // what the raw scores of rows 2c and 2c + 1 of every eight are multiplied by
+    int pos[NR][2];                                              // and where they stand
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int rr = tile * 16 + r + 8 * h, t = (int)P.group.quot(rr);
+    for (int n = 0; n < NR; n++) {
+      const int rr = tile * F::ROWS + n * 8 + r, t = (int)P.group.quot(rr);
       const bool on = t < ch.n;
-      pos[h] = on ? ch.p0 + t : p_max;
       const bf16* src = P.q + (long long)(on ? ch.s + t : ch.s) * P.q_row + (long long)(kvh * group + rr - t * group) * P.q_head;
 #pragma unroll
       for (int s = 0; s < KS; s++) {
         const int d = E4M3 ? ((s / 4) * 4 + c) * 16 + (s % 4) * 4 : ((s / 2) * 4 + c) * 8 + (s % 2) * 4;
         const uint2 w = on ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-        qf[s][h] = w.x; qf[s][2 + h] = w.y;
+        qf[n][s][0] = w.x; qf[n][s][1] = w.y;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int t2 = (int)P.group.quot(tile * F::ROWS + n * 8 + 2 * c + h);
+        pos[n][h] = t2 < ch.n ? ch.p0 + t2 : p_max;
+        rowf[n][h] = P.scale_log2;
+      }
+      if constexpr (E4M3) {
+        unsigned mag = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) mag = max(mag, max(qf[n][s][h] & 0x7fffu, qf[n][s][h] >> 16 & 0x7fffu));
+        mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
+        mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
+        // largest magnitude to 2^60 ..; beyond these bounds the scores' factor would leave fp32, and need not
+        const int shift = mag >= 0x7f80u ? 0 : min(max(60 - ((int)(mag >> 7) - 127), -7), 120);
+        const float up = __uint_as_float((uint32_t)(127 + shift) << 23), down = __uint_as_float((uint32_t)(247 - shift) << 23);      // 2^shift, 2^(120 - shift)
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[n][s][h]));
+            qf[n][s][h] = pack2f(v.x * up, v.y * up);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; h++) rowf[n][h] *= __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
       }
     }
     const int hi = min(cap, P.causal ? p_max + 1 : ch.len), lo = P.window ? max(0, p_min - P.window + 1) : 0;
@@ -132,24 +166,28 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
     const int a = first + (int)((long long)nst * split / P.nsplit) + warp, b = first + (int)((long long)nst * (split + 1) / P.nsplit);
     const int mine = b > a ? (b - a + F::WARPS - 1) / F::WARPS : 0;
 
-    float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[NR][MT][4], m[NR][2], l[NR][2];
 #pragma unroll
-    for (int t = 0; t < NT; t++) { o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f; }
+    for (int n = 0; n < NR; n++) {
+      m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < MT; t++) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
+    }
 
-    auto issue = [&](int i) {                                    // the warp's i-th step: a lane looks up one key and copies its parts of all 32
+    auto issue = [&](int i) {                                    // the warp's i-th step: a lane looks up one key and copies its parts of all
       const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
       int page = 0, at = 0;
       const bool ok = p >= lo && p < hi && locate(P.b, seq, p, page, at);
       const long long off = ok ? (long long)page * P.c.page_b + (long long)at * P.c.row_b : -1;
       const int slot = i % F::STAGES;
       const uint32_t dk = ring_s + slot * F::STAGE, dv = dk + F::K_BYTES, side = dv + F::V_BYTES;
-      long long o_k[F::NJ], o_v[F::NB * 4];                       // all the exchanges before the first copy: in turns each copy would wait for its own
+      long long o_k[2 * F::NB], o_v[F::NB * 4];                  // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-      for (int j = 0; j < F::NJ; j++) o_k[j] = __shfl_sync(0xffffffffu, off, j * 8 + r);
+      for (int j = 0; j < 2 * F::NB; j++) o_k[j] = __shfl_sync(0xffffffffu, off, j * 8 + r);
 #pragma unroll
       for (int j = 0; j < F::NB * 4; j++) o_v[j] = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8);
 #pragma unroll
-      for (int j = 0; j < F::NJ; j++)
+      for (int j = 0; j < 2 * F::NB; j++)
 #pragma unroll
         for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, o_k[j] >= 0 ? kb + o_k[j] + x * 64 + c * 16 : kb, o_k[j] >= 0);
 #pragma unroll
@@ -176,71 +214,94 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
       unsigned char* sv = sk + F::K_BYTES;
       const uint32_t* side = reinterpret_cast<const uint32_t*>(sv + F::V_BYTES);
       const uint32_t fl = side[64 + lane], valid = __ballot_sync(0xffffffffu, fl & 16u) & F::ALL;
-      uint32_t kf = 0, vf = 0;                                   // 2^120 times the scales of this lane's key
+      float kf = 1.f, vf = 1.f;                                  // of this lane's key: its scale, 2^100 times its values' scale
       if constexpr (E4M3) {
-        kf = scale_bits((side[lane] >> ((fl & 3) * 8)) & 255);
-        vf = scale_bits((side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255);
+        const int k8 = (side[lane] >> ((fl & 3) * 8)) & 255, v8 = (side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255;
+        kf = __uint_as_float(k8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)min(max(k8, 1), E_MAX + 127) << 23);
+        vf = __uint_as_float(v8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)(min(v8, E_MAX + 127) + 100) << 23);
       }
       const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 <= p_max - P.window);
-      float s[F::NJ][4];
+      float s[F::NB][NR][4];
+      float fk[F::NB][2], fv[F::NB][2];
 #pragma unroll
-      for (int j = 0; j < F::NJ; j++) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-        uint32_t f = 0;
-        if constexpr (E4M3) { f = __shfl_sync(0xffffffffu, kf, j * 8 + r); f |= f << 16; }
+      for (int kk = 0; kk < F::NB; kk++) {
+#pragma unroll
+        for (int n = 0; n < NR; n++) s[kk][n][0] = s[kk][n][1] = s[kk][n][2] = s[kk][n][3] = 0.f;
+        if constexpr (E4M3) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) { fk[kk][h] = __shfl_sync(0xffffffffu, kf, kk * 16 + h * 8 + r); fv[kk][h] = __shfl_sync(0xffffffffu, vf, kk * 16 + h * 8 + r); }
+        }
 #pragma unroll
         for (int x = 0; x < F::KP; x++) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sk + (j * F::KP + x) * 512 + lane * 16);
+          const uint4 wa = *reinterpret_cast<const uint4*>(sk + (2 * kk * F::KP + x) * 512 + lane * 16), wb = *reinterpret_cast<const uint4*>(sk + ((2 * kk + 1) * F::KP + x) * 512 + lane * 16);
           if constexpr (E4M3) {
-            mma16816(s[j], qf[4 * x], widen_lo(w.x, f), widen_hi(w.x, f));
-            mma16816(s[j], qf[4 * x + 1], widen_lo(w.y, f), widen_hi(w.y, f));
-            mma16816(s[j], qf[4 * x + 2], widen_lo(w.z, f), widen_hi(w.z, f));
-            mma16816(s[j], qf[4 * x + 3], widen_lo(w.w, f), widen_hi(w.w, f));
+            const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+              const uint32_t af[4] = {raw_pair(ua[y], 0, raw_sel(0, 1)), raw_pair(ub[y], 0, raw_sel(0, 1)), raw_pair(ua[y], 0, raw_sel(2, 3)), raw_pair(ub[y], 0, raw_sel(2, 3))};
+#pragma unroll
+              for (int n = 0; n < NR; n++) mma16816(s[kk][n], af, qf[n][4 * x + y][0], qf[n][4 * x + y][1]);
+            }
           } else {
-            mma16816(s[j], qf[2 * x], w.x, w.y);
-            mma16816(s[j], qf[2 * x + 1], w.z, w.w);
+            const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+              mma16816(s[kk][n], a0, qf[n][2 * x][0], qf[n][2 * x][1]);
+              mma16816(s[kk][n], a1, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
+            }
           }
         }
       }
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[NR][2];
 #pragma unroll
-      for (int j = 0; j < F::NJ; j++)
+      for (int n = 0; n < NR; n++) {
+        mx[n][0] = mx[n][1] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          s[j][e] *= P.scale_log2;
-          if (mask) {
-            const int kk = j * 8 + 2 * c + (e & 1), p = k0 + kk, h = e >> 1;
-            if (!((valid >> kk) & 1) || (P.causal && p > pos[h]) || (P.window && p <= pos[h] - P.window)) s[j][e] = -INFINITY;
+        for (int kk = 0; kk < F::NB; kk++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float& x = s[kk][n][e];
+            x *= rowf[n][e & 1];
+            if constexpr (E4M3) x *= fk[kk][e >> 1];
+            if (mask) {
+              const int at = kk * 16 + (e >> 1) * 8 + r, p = k0 + at, q = pos[n][e & 1];
+              if (!((valid >> at) & 1) || (P.causal && p > q) || (P.window && p <= q - P.window)) x = -INFINITY;
+            }
+            mx[n][e & 1] = fmaxf(mx[n][e & 1], x);
           }
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-        }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
       }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-        float al[2];
+      bool up = false;
+#pragma unroll
+      for (int n = 0; n < NR; n++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const float mn = fmaxf(m[h], mx[h]);
-          al[h] = mn == -INFINITY ? 1.f : ex2_approx(m[h] - mn);
-          m[h] = mn; l[h] *= al[h];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx[n][h] = fmaxf(mx[n][h], __shfl_xor_sync(0xffffffffu, mx[n][h], d));
+          up |= mx[n][h] > m[n][h];
         }
+      if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) { o[t][0] *= al[0]; o[t][1] *= al[0]; o[t][2] *= al[1]; o[t][3] *= al[1]; }
-      }
-      const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};   // a row that has seen no key yet: 2^(-inf - 0) = 0
+        for (int n = 0; n < NR; n++) {
+          float al[2];
 #pragma unroll
-      for (int j = 0; j < F::NJ; j++) {
+          for (int h = 0; h < 2; h++) {
+            const float mn = fmaxf(m[n][h], mx[n][h]);
+            al[h] = mn == -INFINITY ? 1.f : ex2_approx(m[n][h] - mn);
+            m[n][h] = mn; l[n][h] *= al[h];
+          }
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[j][e] = ex2_approx(s[j][e] - ms[e >> 1]);
-        l[0] += s[j][0] + s[j][1]; l[1] += s[j][2] + s[j][3];
+          for (int t = 0; t < MT; t++) { o[n][t][0] *= al[0]; o[n][t][1] *= al[1]; o[n][t][2] *= al[0]; o[n][t][3] *= al[1]; }
+        }
       }
       if (mask) {                                                // values that some row must not meet: none of them may be an infinity or a NaN
         bool odd = false;
-        if constexpr (E4M3) { if (vf == 0x7fc0u && (fl & 16u)) { odd = true; vf = 0; } }
-        else {
+        if constexpr (E4M3) {
+          odd = vf != vf && (fl & 16u);
+#pragma unroll
+          for (int kk = 0; kk < F::NB; kk++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) if (fv[kk][h] != fv[kk][h]) fv[kk][h] = 0.f;
+        } else {
 #pragma unroll 1
           for (int x = 0; x < F::V_BYTES / 512; x++) {
             uint4* w = reinterpret_cast<uint4*>(sv + x * 512 + lane * 16);
@@ -259,26 +320,33 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
             if (!((valid >> kk) & 1) || !locate(P.b, seq, p, page, at)) continue;
             const char* row = vb + (long long)page * P.c.page_b + (long long)at * P.c.row_b;
             const int sc = E4M3 ? P.c.vs[(long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row] : 0;
-            const bool see[2] = {!(P.causal && p > pos[0]) && !(P.window && p <= pos[0] - P.window), !(P.causal && p > pos[1]) && !(P.window && p <= pos[1] - P.window)};
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int t = 0; t < MT; t++)
 #pragma unroll
               for (int e = 0; e < 2; e++) {
-                const int d = E4M3 ? (2 * c + e) * NT + t : (t / 8) * 64 + (2 * c + e) * 8 + t % 8;
-                const float x = held<E4M3>(row, d, sc);
-                if (!isfinite(x)) { if (see[0]) o[t][e] += x; if (see[1]) o[t][2 + e] += x; }
+                const float x = held<E4M3>(row, dim_of(t) + e, sc);
+                if (isfinite(x)) continue;
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+#pragma unroll
+                  for (int h = 0; h < 2; h++) if (!(P.causal && p > pos[n][h]) && !(P.window && p <= pos[n][h] - P.window)) o[n][t][2 * e + h] += x;
               }
           }
         }
       }
 #pragma unroll
-      for (int kb2 = 0; kb2 < F::NB; kb2++) {
-        // P is rounded to bf16 for the product (half a step, 2^-9 of each term, averaged over the keys); its sum l is taken before
-        const uint32_t pf[4] = {pack2f(s[2 * kb2][0], s[2 * kb2][1]), pack2f(s[2 * kb2][2], s[2 * kb2][3]), pack2f(s[2 * kb2 + 1][0], s[2 * kb2 + 1][1]), pack2f(s[2 * kb2 + 1][2], s[2 * kb2 + 1][3])};
-        uint32_t f01 = 0, f89 = 0;
-        if constexpr (E4M3) {
-          f01 = __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c) | __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 1) << 16;
-          f89 = __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 8) | __shfl_sync(0xffffffffu, vf, kb2 * 16 + 2 * c + 9) << 16;
+      for (int kk = 0; kk < F::NB; kk++) {
+        uint32_t pf[NR][2];                                      // P^T: rounded to bf16 for the product (half a step, 2^-8 of each term); the sum l is taken before
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];      // a row that has seen no key yet: 2^(-inf - 0) = 0
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float p0 = ex2_approx(s[kk][n][2 * h] - m0), p1 = ex2_approx(s[kk][n][2 * h + 1] - m1);
+            l[n][0] += p0; l[n][1] += p1;
+            if constexpr (E4M3) { p0 *= fv[kk][h]; p1 *= fv[kk][h]; }
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[n][h]) : "r"(pack2f(p0, p1)));
+          }
         }
 #pragma unroll
         for (int x = 0; x < F::VP; x++) {
@@ -286,73 +354,78 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             if constexpr (F::VW == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sv + ((kb2 * 4 + j) * F::VP + x) * 512 + lane * 16);
+              const uint4 u = *reinterpret_cast<const uint4*>(sv + ((kk * 4 + j) * F::VP + x) * 512 + lane * 16);
               w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w;
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(sv + (kb2 * 4 + j) * 256 + lane * 8);
+              const uint2 u = *reinterpret_cast<const uint2*>(sv + (kk * 4 + j) * 256 + lane * 8);
               w[j][0] = u.x; w[j][1] = u.y;
             }
           }
-          if constexpr (E4M3) {
+          constexpr int TP = E4M3 ? F::VW / 2 : 4;               // products of a piece
 #pragma unroll
-            for (int t = 0; t < F::VW; t++) {                    // byte t % 4 of both keys' words, to bytes 1 and 3
-              const unsigned sel = (unsigned)((t % 4) << 4 | (4 + t % 4) << 12);
-              mma16816(o[x * F::VW + t], pf, widen(__byte_perm(w[0][t / 4], w[1][t / 4], sel), f01), widen(__byte_perm(w[2][t / 4], w[3][t / 4], sel), f89));
+          for (int t = 0; t < TP; t++) {
+            uint32_t af[4];
+            if constexpr (E4M3) {                                // bytes 2t and 2t + 1 of a piece, of two keys each
+              const int y = t / 2, z = (t % 2) * 2;
+              af[0] = raw_pair(w[0][y], w[1][y], raw_sel(z, 4 + z)); af[1] = raw_pair(w[0][y], w[1][y], raw_sel(z + 1, 5 + z));
+              af[2] = raw_pair(w[2][y], w[3][y], raw_sel(z, 4 + z)); af[3] = raw_pair(w[2][y], w[3][y], raw_sel(z + 1, 5 + z));
+            } else {
+              af[0] = __byte_perm(w[0][t], w[1][t], 0x5410); af[1] = __byte_perm(w[0][t], w[1][t], 0x7632);
+              af[2] = __byte_perm(w[2][t], w[3][t], 0x5410); af[3] = __byte_perm(w[2][t], w[3][t], 0x7632);
             }
-          } else {
 #pragma unroll
-            for (int t = 0; t < 8; t++) {
-              const unsigned sel = t & 1 ? 0x7632u : 0x5410u;
-              mma16816(o[x * 8 + t], pf, __byte_perm(w[0][t / 2], w[1][t / 2], sel), __byte_perm(w[2][t / 2], w[3][t / 2], sel));
-            }
+            for (int n = 0; n < NR; n++) mma16816(o[n][x * TP + t], af, pf[n][0], pf[n][1]);
           }
         }
       }
     };
 
-#pragma unroll
-    for (int i = 0; i < F::STAGES - 1; i++) { if (i < mine) issue(i); cp_commit(); }
+    // One copy of each part of the code: a short context runs through it once, fetching it from L2
 #pragma unroll 1
-    for (int i = 0; i < mine; i++) {
-      if (i + F::STAGES - 1 < mine) issue(i + F::STAGES - 1);
+    for (int i = 0; i < mine + F::STAGES - 1; i++) {
+      if (i < mine) issue(i);
       cp_commit();
-      cp_wait<F::STAGES - 1>();
-      step(i);
+      if (i >= F::STAGES - 1) { cp_wait<F::STAGES - 1>(); step(i - (F::STAGES - 1)); }
     }
     cp_wait<0>();
 #pragma unroll
-    for (int h = 0; h < 2; h++) { l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1); l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2); }
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], d);
 
-    // the warps meet: 16 rows of D sums each, and {m, l}
+    // the warps meet: rows of D sums each, and {m, l}
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem);
-    float2* sm = reinterpret_cast<float2*>(so + F::WARPS * 16 * D);
+    float2* sm = reinterpret_cast<float2*>(so + F::WARPS * F::ROWS * F::PAD);
+    constexpr float MEND = E4M3 ? 1048576.f : 1.f;               // 2^20
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float* dst = so + (warp * 16 + r + 8 * h) * D;
+    for (int n = 0; n < NR; n++)
 #pragma unroll
-      for (int e = 0; e < 2; e++)
+      for (int h = 0; h < 2; h++) {
+        const int row = warp * F::ROWS + n * 8 + 2 * c + h;
 #pragma unroll
-        for (int t = 0; t < NT; t += 4) {
-          const int d = E4M3 ? (2 * c + e) * NT + t : (t / 8) * 64 + (2 * c + e) * 8 + t % 8;
-          *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][2 * h + e], o[t + 1][2 * h + e], o[t + 2][2 * h + e], o[t + 3][2 * h + e]);
-        }
-      if (c == 0) sm[warp * 16 + r + 8 * h] = make_float2(m[h], l[h]);
-    }
+        for (int t = 0; t < MT; t++) *reinterpret_cast<float2*>(so + row * F::PAD + dim_of(t)) = make_float2(o[n][t][h] * MEND, o[n][t][2 + h] * MEND);
+        if (r == 0) sm[row] = make_float2(m[n][h], l[n][h]);
+      }
     __syncthreads();
     {
-      constexpr int DP = D / 8;                                  // eight threads a row
-      const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rr = tile * 16 + row, t = (int)P.group.quot(rr);
+      constexpr int TPR = 128 / F::ROWS, DP = D / TPR;           // threads a row, dims a thread: a thread's are 4 side by side in every 4 * TPR
+      const int row = threadIdx.x / TPR, part = threadIdx.x % TPR, rr = tile * F::ROWS + row, t = (int)P.group.quot(rr);
       float mm = -INFINITY, ll = 0.f, acc[DP] = {};
 #pragma unroll
-      for (int w = 0; w < F::WARPS; w++) mm = fmaxf(mm, sm[w * 16 + row].x);
+      for (int w = 0; w < F::WARPS; w++) mm = fmaxf(mm, sm[w * F::ROWS + row].x);
 #pragma unroll
       for (int w = 0; w < F::WARPS; w++) {
-        const float2 ml = sm[w * 16 + row];
+        const float2 ml = sm[w * F::ROWS + row];
         const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);      // no key seen, or only scores of -inf: sums of 0, or not finite
         ll += ml.y * f;
 #pragma unroll
-        for (int x = 0; x < DP; x++) acc[x] += so[(w * 16 + row) * D + part * DP + x] * f;
+        for (int x = 0; x < DP; x += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(so + (w * F::ROWS + row) * F::PAD + x * TPR + part * 4);
+          acc[x] += v.x * f; acc[x + 1] += v.y * f; acc[x + 2] += v.z * f; acc[x + 3] += v.w * f;
+        }
       }
       const int head = kvh * group + rr - t * group;
       const long long g = (long long)(ch.s + t) * P.n_heads + head;
@@ -360,12 +433,12 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
       if (P.cluster) {                                           // the blocks of the cluster meet in each other's shared memory, rows dealt out among them
         __syncthreads();
 #pragma unroll
-        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(so + row * D + part * DP + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(so + row * F::PAD + x * TPR + part * 4) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
         if (part == 0) sm[row] = make_float2(mm, ll);
         cluster_sync();
         last = last && row % P.nsplit == split;
         if (last) {
-          const uint32_t at = smem_u32(so + row * D + part * DP), am = smem_u32(sm + row);
+          const uint32_t at = smem_u32(so + row * F::PAD + part * 4), am = smem_u32(sm + row);
           mm = -INFINITY; ll = 0.f;
           for (int s = 0; s < P.nsplit; s++) mm = fmaxf(mm, peer_f32(peer(am, s)));
 #pragma unroll
@@ -376,7 +449,7 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
             const uint32_t src = peer(at, s);
 #pragma unroll
             for (int x = 0; x < DP; x += 4) {
-              const float4 v = peer_f32x4(src + x * 4);
+              const float4 v = peer_f32x4(src + x * TPR * 4);
               acc[x] += v.x * f; acc[x + 1] += v.y * f; acc[x + 2] += v.z * f; acc[x + 3] += v.w * f;
             }
           }
@@ -384,16 +457,14 @@ __global__ void __launch_bounds__(128, 2) few_rows_kernel(const __grid_constant_
       }
       if (last && (P.cluster || P.nsplit == 1)) {
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * DP;
+        bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * 4;
 #pragma unroll
-        for (int x = 0; x < DP; x++) acc[x] *= inv;
-#pragma unroll
-        for (int x = 0; x < DP; x += 8) *reinterpret_cast<uint4*>(dst + x) = pack8(acc + x);
+        for (int x = 0; x < DP; x += 4) *reinterpret_cast<uint2*>(dst + x * TPR) = make_uint2(pack2f(acc[x] * inv, acc[x + 1] * inv), pack2f(acc[x + 2] * inv, acc[x + 3] * inv));
         if (P.lse && part == 0) P.lse[g] = ll == 0.f ? -INFINITY : mm * LN2 + logf(ll);
       } else if (last) {
-        float* dst = P.part + (g * P.nsplit + split) * D + part * DP;
+        float* dst = P.part + (g * P.nsplit + split) * D + part * 4;
 #pragma unroll
-        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(dst + x) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+        for (int x = 0; x < DP; x += 4) *reinterpret_cast<float4*>(dst + x * TPR) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
         if (part == 0) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(mm, ll);
       }
       if (P.cluster) cluster_sync();                             // nobody's shared memory goes while another reads it

@@ -87,22 +87,23 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
 }
 
 // ---- attention
-struct Plan { bool many, cluster; int tiles, nsplit; size_t bytes; };
+struct Plan { bool many, cluster; int rows, tiles, nsplit; size_t bytes; };      // rows: of a tile
 
 // A chunk of more than 32 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 256 rows; fewer to the one that keeps more bytes
-// in flight. Blocks that share a tile's keys: as many as keep the SMs busy (one block of the first kernel on each of 148, two of the second), none with fewer than 512 keys
+// in flight. Blocks that share a tile's keys: as many as keep the SMs busy (one block of the first kernel on each of 148, three of the second), none with fewer than 512 keys
 // and 256. max_new and max_kv are what the caller says; without them one sequence with all rows and the page table's width are assumed.
 Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
   Plan p;
   const long long group = n_heads / c->n_kv_heads;
   const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
   p.many = rows > 32;
-  long long tiles = p.many ? (rows + 255) / 256 : (rows + 15) / 16;
+  p.rows = p.many ? 256 : rows > 8 ? 16 : 8;
+  long long tiles = (rows + p.rows - 1) / p.rows;
   if (tiles > 4096) tiles = 4096;
   if (tiles < 1) tiles = 1;
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
   const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles;
-  long long ns = (p.many ? 148 : 2 * 148) / blocks;
+  long long ns = (p.many ? 148 : 3 * 148) / blocks;
   if (ns > kv / (p.many ? 512 : 256)) ns = kv / (p.many ? 512 : 256);
   if (ns > paged::MAX_SPLIT) ns = paged::MAX_SPLIT;
   p.cluster = !p.many && ns > 1 && ns < 16;
@@ -122,22 +123,23 @@ template <auto KERNEL> cudaError_t allow(int bytes) {
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }
-template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, bool many, cudaStream_t s) {
+template <auto KERNEL> cudaError_t launch(cudaLaunchConfig_t& lc, int threads, int smem, const paged::AttnArgs& P) {
+  lc.blockDim = dim3((unsigned)threads); lc.dynamicSmemBytes = (size_t)smem;
+  const cudaError_t e = allow<KERNEL>(smem);
+  return e == cudaSuccess ? cudaLaunchKernelEx(&lc, KERNEL, P) : e;
+}
+template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p, cudaStream_t s) {
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute at = {};
   lc.gridDim = dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads); lc.stream = s; lc.attrs = &at;
   cudaError_t e;
-  if (many) {
+  if (p.many) {
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    constexpr auto kernel = paged::many_rows_kernel<D, E4M3>;
-    lc.blockDim = dim3(512); lc.dynamicSmemBytes = paged::Tc<D>::SMEM;
-    if ((e = allow<kernel>(paged::Tc<D>::SMEM)) == cudaSuccess) e = cudaLaunchKernelEx(&lc, kernel, P);
+    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, 512, paged::Tc<D>::SMEM, P);
   } else {
-    constexpr auto kernel = paged::few_rows_kernel<D, E4M3>;
     if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
-    lc.blockDim = dim3(128); lc.dynamicSmemBytes = paged::Few<D, E4M3>::SMEM;
-    if ((e = allow<kernel>(paged::Few<D, E4M3>::SMEM)) == cudaSuccess) e = cudaLaunchKernelEx(&lc, kernel, P);
+    e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(lc, 128, paged::Few<D, E4M3, 1>::SMEM, P) : launch<paged::few_rows_kernel<D, E4M3, 2>>(lc, 128, paged::Few<D, E4M3, 2>::SMEM, P);
   }
   if (e == cudaSuccess && P.nsplit > 1 && !P.cluster) {
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -185,8 +187,8 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.part = static_cast<float*>(a->workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p.many, s) : attend<128, true>(P, p.many, s);
-  else e = cache->head_dim == 64 ? attend<64, false>(P, p.many, s) : attend<128, false>(P, p.many, s);
+  if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p, s) : attend<128, true>(P, p, s);
+  else e = cache->head_dim == 64 ? attend<64, false>(P, p, s) : attend<128, false>(P, p, s);
   return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
 }
 

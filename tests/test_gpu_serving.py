@@ -474,3 +474,24 @@ def test_empty_calls(sv):
     none = sv.KVBatch(i32([0]), torch.empty(0, dtype=torch.int32, device=DEV), torch.empty(0, 4, dtype=torch.int32, device=DEV))
     assert sv.paged_attention(cache, none, e).shape == (0, 2, 64)
     assert sv.logits_process(torch.empty(0, 10, device=DEV)).shape == (0, 10)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_over_codes_of_every_size(sv, dim, rows):
+    """8-bit rows of subnormal codes, of the smallest and largest scales, and queries of any magnitude: nothing underflows or overflows on the way. Scales of keys and
+    queries are opposite, so that scores are of order one."""
+    g = torch.Generator().manual_seed(3)
+    n = 96
+    codes = torch.randint(0, 256, (2, n, dim), generator=g).to(torch.uint8)
+    codes[:, : n // 3] &= 0x87                                            # subnormal
+    codes[(codes & 0x7f) == 0x7f] = 0x7e
+    for e in (-100, -60, 0, 7):
+        k = codes[0].view(torch.float8_e4m3fn).view(1, 1, n, dim).to(DEV)
+        v = codes[1].view(torch.float8_e4m3fn).view(1, 1, n, dim).to(DEV)
+        ks = torch.full((1, 1, n), e + 127, dtype=torch.uint8, device=DEV)
+        vs = torch.randint(27, 135, (1, 1, n), generator=g).to(torch.uint8).to(DEV) if e == 0 else ks.clone()
+        cache = sv.KVCache(k, v, ks, vs)
+        batch = sv.KVBatch(i32([0, rows]), i32([n]), i32([[0]]), max_new=rows)
+        q = (torch.randn(rows, 2, dim, generator=g) * 2.0 ** (-e - 8)).bfloat16().to(DEV)
+        check_attention(sv, cache, batch, q)
