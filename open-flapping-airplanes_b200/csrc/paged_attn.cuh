@@ -30,6 +30,7 @@ namespace paged {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int MAX_SPLIT = 64;
+constexpr float RESCALE_LOG2 = 8.f;
 
 struct AttnArgs {
   Batch b;
@@ -40,7 +41,7 @@ struct AttnArgs {
   int n_heads, n_kv_heads, causal, window;
   Div group;
   float scale_log2;                 // of many_rows_kernel: its magnitude, flip = the scale is negative
-  int flip;
+  int flip, wide;                   // wide: offsets of 2^35 bytes and more
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
   int cluster;                      // ... which are a cluster and meet in shared memory
   float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
@@ -68,6 +69,12 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
   return w;
 }
 
+// A row's offset (a multiple of 16 bytes, -1: no row) from another lane: one exchange where the cache's offsets over 16 fit 31 bits
+__device__ __forceinline__ long long from_lane(long long off, int lane, bool wide) {
+  if (wide) return __shfl_sync(0xffffffffu, off, lane);
+  const int v = __shfl_sync(0xffffffffu, (int)(off >> 4), lane);
+  return v < 0 ? -1ll : (long long)v << 4;
+}
 // Shared memory of the cluster's other blocks
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
@@ -85,7 +92,7 @@ template <int D, bool E4M3, int NR> struct Few {
   static constexpr int VB = D * (E4M3 ? 1 : 2) / 8;             // bytes of a value row that a lane holds
   static constexpr int VW = VB >= 16 ? 16 : 8, VP = VB / VW;    // ... in pieces of VW
   static constexpr int K_BYTES = 2 * NB * KP * 512, V_BYTES = NB * 4 * VB * 32;
-  static constexpr int SIDE = 3 * 128;                          // scale words of K and V, flags
+  static constexpr int SIDE = E4M3 ? 256 : 0;                   // scale words of K and V
   static constexpr int STAGE = K_BYTES + V_BYTES + SIDE;
   static constexpr int STAGES = K_BYTES + V_BYTES >= 8192 ? 2 : 3;
   static constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
@@ -174,46 +181,69 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       for (int t = 0; t < MT; t++) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
     }
 
-    auto issue = [&](int i) {                                    // the warp's i-th step: a lane looks up one key and copies its parts of all
+    // the page of this lane's key in the warp's i-th step; asked for a step ahead
+    auto page_of = [&](int i) {
       const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
-      int page = 0, at = 0;
-      const bool ok = p >= lo && p < hi && locate(P.b, seq, p, page, at);
-      const long long off = ok ? (long long)page * P.c.page_b + (long long)at * P.c.row_b : -1;
+      if (i >= mine || p < lo || p >= hi) return -1;
+      return __ldg(P.b.pages + (long long)seq * P.b.pages_stride + P.b.page.quot((unsigned)p));      // p < cap: within the table
+    };
+    int page = page_of(0);
+    uint32_t keys[F::STAGES], scale_at[F::STAGES];               // of the steps on their way, the last one first: which of their keys are there; where in their words a lane's scales are
+    auto issue = [&](int i) {                                    // the warp's i-th step: a lane places one key and copies its parts of all
+      const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
+      const int at = p - (int)(P.b.page.quot((unsigned)p) * P.b.page.d);
+      const bool inside = p >= lo && p < hi, ok = inside && (unsigned)page < (unsigned)P.b.n_pages;
+      if (inside && !ok) flag(P.b.status, ST_PAGE);
+      const int pg = page;
+      page = page_of(i + 1);
+      const long long off = ok ? (long long)pg * P.c.page_b + (long long)at * P.c.row_b : -1;
       const int slot = i % F::STAGES;
       const uint32_t dk = ring_s + slot * F::STAGE, dv = dk + F::K_BYTES, side = dv + F::V_BYTES;
       long long o_k[2 * F::NB], o_v[F::NB * 4];                  // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-      for (int j = 0; j < 2 * F::NB; j++) o_k[j] = __shfl_sync(0xffffffffu, off, j * 8 + r);
+      for (int j = 0; j < 2 * F::NB; j++) o_k[j] = from_lane(off, j * 8 + r, P.wide);
 #pragma unroll
-      for (int j = 0; j < F::NB * 4; j++) o_v[j] = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8);
+      for (int j = 0; j < F::NB * 4; j++) o_v[j] = from_lane(off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8, P.wide);
 #pragma unroll
-      for (int j = 0; j < 2 * F::NB; j++)
+      for (int j = 0; j < 2 * F::NB; j++) {
+        const bool on = o_k[j] >= 0;
+        const char* src = kb + (on ? o_k[j] : 0) + c * 16;
 #pragma unroll
-        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, o_k[j] >= 0 ? kb + o_k[j] + x * 64 + c * 16 : kb, o_k[j] >= 0);
+        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, src + x * 64, on);
+      }
 #pragma unroll
-      for (int j = 0; j < F::NB * 4; j++)
+      for (int j = 0; j < F::NB * 4; j++) {
+        const bool on = o_v[j] >= 0;
+        const char* src = vb + (on ? o_v[j] : 0) + r * F::VW;
 #pragma unroll
         for (int x = 0; x < F::VP; x++) {
-          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, o_v[j] >= 0 ? vb + o_v[j] + x * 128 + r * 16 : vb, o_v[j] >= 0);
-          else cp8(dv + j * 256 + lane * 8, o_v[j] >= 0 ? vb + o_v[j] + r * 8 : vb, o_v[j] >= 0);
+          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, src + x * 128, on);
+          else cp8(dv + j * 256 + lane * 8, src, on);
         }
-      uint32_t fl = ok ? 16u : 0u;
+      }
+      uint32_t fl = __ballot_sync(0xffffffffu, ok) & F::ALL, bytes = 0;
       if constexpr (E4M3) {                                      // the aligned word around the scale byte; which byte of it is kept beside it
-        const long long so = ok ? (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row : 0;
+        const long long so = ok ? (long long)pg * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row : 0;
         const unsigned long long ka = reinterpret_cast<unsigned long long>(P.c.ks + so), va = reinterpret_cast<unsigned long long>(P.c.vs + so);
         cp4(side + lane * 4, reinterpret_cast<const void*>(ka & ~3ull), ok);
         cp4(side + 128 + lane * 4, reinterpret_cast<const void*>(va & ~3ull), ok);
-        fl |= (uint32_t)(ka & 3) | (uint32_t)(va & 3) << 2;
+        bytes = (uint32_t)(ka & 3) | (uint32_t)(va & 3) << 2;
       }
-      *reinterpret_cast<uint32_t*>(ring + slot * F::STAGE + F::K_BYTES + F::V_BYTES + 256 + lane * 4) = fl;
+#pragma unroll
+      for (int x = F::STAGES - 1; x > 0; x--) { keys[x] = keys[x - 1]; scale_at[x] = scale_at[x - 1]; }
+      keys[0] = fl; scale_at[0] = bytes;
     };
 
+    auto skip = [&]() {
+#pragma unroll
+      for (int x = F::STAGES - 1; x > 0; x--) { keys[x] = keys[x - 1]; scale_at[x] = scale_at[x - 1]; }
+    };
     auto step = [&](int i) {
       const int slot = i % F::STAGES, k0 = (a + i * F::WARPS) * F::KEYS;
       unsigned char* sk = ring + slot * F::STAGE;
       unsigned char* sv = sk + F::K_BYTES;
       const uint32_t* side = reinterpret_cast<const uint32_t*>(sv + F::V_BYTES);
-      const uint32_t fl = side[64 + lane], valid = __ballot_sync(0xffffffffu, fl & 16u) & F::ALL;
+      const uint32_t valid = keys[F::STAGES - 1], fl = scale_at[F::STAGES - 1];
       float kf = 1.f, vf = 1.f;                                  // of this lane's key: its scale, 2^100 times its values' scale
       if constexpr (E4M3) {
         const int k8 = (side[lane] >> ((fl & 3) * 8)) & 255, v8 = (side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255;
@@ -227,6 +257,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       for (int kk = 0; kk < F::NB; kk++) {
 #pragma unroll
         for (int n = 0; n < NR; n++) s[kk][n][0] = s[kk][n][1] = s[kk][n][2] = s[kk][n][3] = 0.f;
+        float s2[NR][4] = {};                                    // two chains of products
         if constexpr (E4M3) {
 #pragma unroll
           for (int h = 0; h < 2; h++) { fk[kk][h] = __shfl_sync(0xffffffffu, kf, kk * 16 + h * 8 + r); fv[kk][h] = __shfl_sync(0xffffffffu, vf, kk * 16 + h * 8 + r); }
@@ -240,17 +271,21 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             for (int y = 0; y < 4; y++) {
               const uint32_t af[4] = {raw_pair(ua[y], 0, raw_sel(0, 1)), raw_pair(ub[y], 0, raw_sel(0, 1)), raw_pair(ua[y], 0, raw_sel(2, 3)), raw_pair(ub[y], 0, raw_sel(2, 3))};
 #pragma unroll
-              for (int n = 0; n < NR; n++) mma16816(s[kk][n], af, qf[n][4 * x + y][0], qf[n][4 * x + y][1]);
+              for (int n = 0; n < NR; n++) mma16816(y & 1 ? s2[n] : s[kk][n], af, qf[n][4 * x + y][0], qf[n][4 * x + y][1]);
             }
           } else {
             const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
 #pragma unroll
             for (int n = 0; n < NR; n++) {
               mma16816(s[kk][n], a0, qf[n][2 * x][0], qf[n][2 * x][1]);
-              mma16816(s[kk][n], a1, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
+              mma16816(s2[n], a1, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
             }
           }
         }
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[kk][n][e] += s2[n][e];
       }
       float mx[NR][2];
 #pragma unroll
@@ -270,21 +305,19 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             mx[n][e & 1] = fmaxf(mx[n][e & 1], x);
           }
       }
+      // The reference that a row's exponentials are taken against is raised only when some score has passed it by 2^8 (they stay below 256, exact enough in fp32 sums and
+      // bf16): in most steps one vote replaces the search of the maximum over the lanes.
       bool up = false;
 #pragma unroll
-      for (int n = 0; n < NR; n++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) mx[n][h] = fmaxf(mx[n][h], __shfl_xor_sync(0xffffffffu, mx[n][h], d));
-          up |= mx[n][h] > m[n][h];
-        }
+      for (int n = 0; n < NR; n++) up |= mx[n][0] > m[n][0] + RESCALE_LOG2 || mx[n][1] > m[n][1] + RESCALE_LOG2;
       if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
         for (int n = 0; n < NR; n++) {
           float al[2];
 #pragma unroll
           for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx[n][h] = fmaxf(mx[n][h], __shfl_xor_sync(0xffffffffu, mx[n][h], d));
             const float mn = fmaxf(m[n][h], mx[n][h]);
             al[h] = mn == -INFINITY ? 1.f : ex2_approx(m[n][h] - mn);
             m[n][h] = mn; l[n][h] *= al[h];
@@ -296,7 +329,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       if (mask) {                                                // values that some row must not meet: none of them may be an infinity or a NaN
         bool odd = false;
         if constexpr (E4M3) {
-          odd = vf != vf && (fl & 16u);
+          odd = vf != vf && ((valid >> (lane & (F::KEYS - 1))) & 1);
 #pragma unroll
           for (int kk = 0; kk < F::NB; kk++)
 #pragma unroll
@@ -383,7 +416,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
     // One copy of each part of the code: a short context runs through it once, fetching it from L2
 #pragma unroll 1
     for (int i = 0; i < mine + F::STAGES - 1; i++) {
-      if (i < mine) issue(i);
+      if (i < mine) issue(i); else skip();
       cp_commit();
       if (i >= F::STAGES - 1) { cp_wait<F::STAGES - 1>(); step(i - (F::STAGES - 1)); }
     }

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
         const float m_true = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2);
         if (c == 0) m = m_true;
         else {
-          const bool grow = m_true > m + attn_tc::RESCALE_LOG2;
+          const bool grow = m_true > m + RESCALE_LOG2;
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? ex2_approx(m - m_true) : 1.f;
             if (grow) { m = m_true; l *= alpha; }
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
         constexpr int N = IT < 4 ? IT : 4;
         long long o[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) o[i] = __shfl_sync(0xffffffffu, x.off, ((x0 + i) * 32 + lane) / CH);
+        for (int i = 0; i < N; i++) o[i] = from_lane(x.off, ((x0 + i) * 32 + lane) / CH, P.wide);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + lane % CH * 16) : make_uint4(0, 0, 0, 0);
       };
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
               const uint32_t dst_s = smem_u32(dst);
               long long o[IT];                                   // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-              for (int y = 0; y < IT; y++) o[y] = __shfl_sync(0xffffffffu, now[x].off, (y * 32 + lane) / CH);
+              for (int y = 0; y < IT; y++) o[y] = from_lane(now[x].off, (y * 32 + lane) / CH, P.wide);
 #pragma unroll
               for (int y = 0; y < IT; y++) {
                 const int row = (y * 32 + lane) / CH, q = lane % CH;

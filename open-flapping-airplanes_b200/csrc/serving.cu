@@ -184,7 +184,8 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
   P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
-  P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.part = static_cast<float*>(a->workspace);
+  P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0;
+  P.wide = (long long)cache->n_pages * P.c.page_b + (long long)cache->page_size * P.c.row_b >= 1ll << 35; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.part = static_cast<float*>(a->workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p, s) : attend<128, true>(P, p, s);
