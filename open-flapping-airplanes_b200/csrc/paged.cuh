@@ -14,7 +14,7 @@
 namespace ofa {
 namespace paged {
 
-enum { ST_PAGE = 1, ST_LENGTH = 2, ST_ROWS = 4 };     // bits of the caller's status word
+enum { ST_PAGE = 1, ST_LENGTH = 2, ST_ROWS = 4, ST_TIMEOUT = 8 };     // bits of the caller's status word
 
 // n / d for 0 <= n < 2^31 (d >= 1): a multiplication instead of a division of 20 instructions
 struct Div {

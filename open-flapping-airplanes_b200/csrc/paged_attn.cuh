@@ -8,11 +8,13 @@
 // every fourth step of 16 or 32 keys and meet once, at the end; up to eight blocks that share the keys of a tile are a cluster and meet in shared memory, more leave their
 // parts in the workspace for combine_kernel.
 //
-// A lane copies what it will itself feed to the products, 16 bytes at a time, into its own slots of a ring in shared memory (cp.async), and reads it back from
-// there: no barrier, no bank conflict, no exchange between lanes. That works because the order of the sum over head dims and the order of the output's dims
-// are free as long as both operands agree:
-//   scores   lane (r = lane / 4, c = lane % 4) holds of key r of 8 the dims c * 16 B + ... of every 64 B; q is fetched in the same order
-//   output   lane holds of keys 2c, 2c + 1, 2c + 8, 2c + 9 of 16 the dims r * 16 B + ...; two keys side by side make a word of the A operand, and rows r and r + 8
+// Each warp has a ring of steps in shared memory. Where a page holds a multiple of 8 rows, boxes of 8 or 16 rows come through the copy engine, one instruction for
+// 1 or 2 KB; other pages are gathered by cp.async, 16 bytes a lane. (Gathering everything kept the load/store pipe busy with the copies themselves: 29 clocks for
+// 512 bytes, with the reads behind them, 4.8 TB/s over long contexts.) Rows lie 128 bytes wide, their 16-byte pieces permuted by the row number (the copy engine's
+// swizzle), and operands are read in an order that meets no bank conflict; the order of the sum over head dims and the order of the output's dims are free as long as both
+// operands agree:
+//   scores   lane (r = lane / 4, c = lane % 4) reads of key r of 8 the pieces 2c and 2c + 1 of every 128 bytes; q is fetched in the same order
+//   output   lane reads of keys 2c, 2c + 1, 2c + 8, 2c + 9 of 16 the piece r; two keys side by side make a word of the A operand, and rows r and r + 8
 //            of the t-th product are two neighbouring dims
 // The scores' accumulator has keys down the lanes, the second product wants them along a lane: movmatrix turns 8 x 8 of them.
 //
@@ -23,6 +25,7 @@
 // A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
 // infinities and NaN are taken out of its values and added to the rows that see it. Rows past the context and of a bad page are never read.
 #pragma once
+#include <cuda.h>
 #include "paged.cuh"
 
 namespace ofa {
@@ -42,6 +45,8 @@ struct AttnArgs {
   Div group;
   float scale_log2;                 // of many_rows_kernel: its magnitude, flip = the scale is negative
   int flip, wide;                   // wide: offsets of 2^35 bytes and more
+  alignas(64) CUtensorMap km, vm;   // the pages in boxes of `run` rows x 128 bytes (64: 8-bit rows of 64)
+  int run;                          // 16, 8, or 0: pages of other sizes, no maps
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
   int cluster;                      // ... which are a cluster and meet in shared memory
   float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
@@ -75,6 +80,17 @@ __device__ __forceinline__ long long from_lane(long long off, int lane, bool wid
   const int v = __shfl_sync(0xffffffffu, (int)(off >> 4), lane);
   return v < 0 ? -1ll : (long long)v << 4;
 }
+// A bounded wait without a call (a function with an ABI of its own does not go with setmaxnreg). A try sleeps for about 300 clocks, the limit is a second or a few.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 10000000; i++) if (mbar_try(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Shared memory of the cluster's other blocks
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
@@ -86,19 +102,23 @@ __device__ __forceinline__ float4 peer_f32x4(uint32_t a) {
 }
 
 template <int D, bool E4M3, int NR> struct Few {
-  static constexpr int KEYS = D * (E4M3 ? 1 : 2) > 128 ? 16 : 32, WARPS = 4, ROWS = 8 * NR;      // of a step: at most 8 KB of keys and values a warp
+  static constexpr int RB = D * (E4M3 ? 1 : 2);                 // bytes of a row
+  static constexpr int KEYS = RB > 128 ? 16 : 32, WARPS = 4, ROWS = 8 * NR;      // of a step: at most 8 KB of keys and values a warp
   static constexpr int NB = KEYS / 16;
-  static constexpr int KP = D * (E4M3 ? 1 : 2) / 64;            // 16-byte pieces of a key that a lane holds
-  static constexpr int VB = D * (E4M3 ? 1 : 2) / 8;             // bytes of a value row that a lane holds
-  static constexpr int VW = VB >= 16 ? 16 : 8, VP = VB / VW;    // ... in pieces of VW
-  static constexpr int K_BYTES = 2 * NB * KP * 512, V_BYTES = NB * 4 * VB * 32;
-  static constexpr int SIDE = E4M3 ? 256 : 0;                   // scale words of K and V
-  static constexpr int STAGE = K_BYTES + V_BYTES + SIDE;
-  static constexpr int STAGES = K_BYTES + V_BYTES >= 8192 ? 2 : 3;
+  static constexpr int W = RB > 128 ? 128 : RB, HALVES = RB / W;                 // rows lie W bytes wide, in one or two parts
+  static constexpr int KP = RB / 64;                            // 16-byte pieces of a key that a lane reads
+  static constexpr int VB = RB / 8, VW = VB >= 16 ? 16 : 8, VP = VB / VW;        // bytes of a value row that a lane reads, in pieces of VW
+  static constexpr int TILE = KEYS * RB, STAGE = 2 * TILE;      // K, then V
+  static constexpr int STAGES = STAGE >= 8192 ? 2 : 3;
   static constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
   static constexpr int PAD = D + 8;                             // floats of a row where the warps meet
-  static constexpr int SMEM = WARPS * STAGES * STAGE;
-  static_assert(WARPS * ROWS * (PAD + 2) * 4 <= SMEM, "the meeting of the warps does not fit");
+  static constexpr int BARS_AT = WARPS * STAGES * STAGE, SMEM = BARS_AT + WARPS * STAGES * 8 + 1024;      // 1,024 for the alignment of the swizzle's atoms
+  static_assert(WARPS * ROWS * (PAD + 2) * 4 <= BARS_AT, "the meeting of the warps does not fit");
+  // where piece `chunk` (16 bytes) of a row lies
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
+    if constexpr (W == 64) return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+    else return (uint32_t)((chunk >> 3) * (KEYS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  }
 };
 
 // one held element as a float (the rare path)
@@ -111,8 +131,14 @@ template <int D, bool E4M3, int NR>
 __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __grid_constant__ AttnArgs P) {
   using F = Few<D, E4M3, NR>;
   constexpr int MT = D / 16, KS = D / 16;                        // products of 16 dims of the output, of 16 dims of a score
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(16) unsigned char raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const uint32_t bars = smem_u32(smem + F::BARS_AT) + warp * F::STAGES * 8;
+  if (lane < F::STAGES) mbar_init(bars + lane * 8, 1);
+  mbar_fence_init();
+  __syncwarp();
+  uint32_t used = 0;                                             // steps of this warp so far: phases of its barriers
   const int split = (int)blockIdx.x % P.nsplit, tile0 = (int)blockIdx.x / P.nsplit % P.tiles, seq = (int)blockIdx.x / P.nsplit / P.tiles, kvh = blockIdx.y;
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
@@ -136,7 +162,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       const bf16* src = P.q + (long long)(on ? ch.s + t : ch.s) * P.q_row + (long long)(kvh * group + rr - t * group) * P.q_head;
 #pragma unroll
       for (int s = 0; s < KS; s++) {
-        const int d = E4M3 ? ((s / 4) * 4 + c) * 16 + (s % 4) * 4 : ((s / 2) * 4 + c) * 8 + (s % 2) * 4;
+        const int d = !E4M3 ? (s / 4) * 64 + (2 * c + s / 2 % 2) * 8 + s % 2 * 4 : D == 128 ? (2 * c + s / 4) * 16 + s % 4 * 4 : c * 16 + s * 4;
         const uint2 w = on ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
         qf[n][s][0] = w.x; qf[n][s][1] = w.y;
       }
@@ -181,72 +207,70 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       for (int t = 0; t < MT; t++) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
     }
 
-    // the page of this lane's key in the warp's i-th step; asked for a step ahead
+    // the page of this lane's key in the warp's i-th step (of its run of keys, as far as the tile reaches into it); asked for a step ahead
+    const int run = P.run ? P.run : 1;
     auto page_of = [&](int i) {
       const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
-      if (i >= mine || p < lo || p >= hi) return -1;
-      return __ldg(P.b.pages + (long long)seq * P.b.pages_stride + P.b.page.quot((unsigned)p));      // p < cap: within the table
+      if (i >= mine || (p | (run - 1)) < lo || (p & -run) >= hi) return -1;
+      return __ldg(P.b.pages + (long long)seq * P.b.pages_stride + P.b.page.quot((unsigned)(p & -run)));      // below cap: within the table
     };
     int page = page_of(0);
-    uint32_t keys[F::STAGES], scale_at[F::STAGES];               // of the steps on their way, the last one first: which of their keys are there; where in their words a lane's scales are
-    auto issue = [&](int i) {                                    // the warp's i-th step: a lane places one key and copies its parts of all
+    uint32_t keys[F::STAGES], ks8[F::STAGES], vs8[F::STAGES];    // of the steps on their way, the last one first: which keys are there, scale bytes of this lane's
+    auto issue = [&](int i) {                                    // the warp's i-th step
+#pragma unroll
+      for (int x = F::STAGES - 1; x > 0; x--) { keys[x] = keys[x - 1]; ks8[x] = ks8[x - 1]; vs8[x] = vs8[x - 1]; }
+      if (i >= mine) return;
       const int p = (a + i * F::WARPS) * F::KEYS + (lane & (F::KEYS - 1));
-      const int at = p - (int)(P.b.page.quot((unsigned)p) * P.b.page.d);
-      const bool inside = p >= lo && p < hi, ok = inside && (unsigned)page < (unsigned)P.b.n_pages;
-      if (inside && !ok) flag(P.b.status, ST_PAGE);
-      const int pg = page;
+      const int at = p - (int)(P.b.page.quot((unsigned)p) * P.b.page.d), pg = page;
+      const bool inside = p >= lo && p < hi, there = (unsigned)pg < (unsigned)P.b.n_pages, ok = inside && there;
+      if (inside && !there) flag(P.b.status, ST_PAGE);
       page = page_of(i + 1);
-      const long long off = ok ? (long long)pg * P.c.page_b + (long long)at * P.c.row_b : -1;
-      const int slot = i % F::STAGES;
-      const uint32_t dk = ring_s + slot * F::STAGE, dv = dk + F::K_BYTES, side = dv + F::V_BYTES;
-      long long o_k[2 * F::NB], o_v[F::NB * 4];                  // all the exchanges before the first copy: in turns each copy would wait for its own
-#pragma unroll
-      for (int j = 0; j < 2 * F::NB; j++) o_k[j] = from_lane(off, j * 8 + r, P.wide);
-#pragma unroll
-      for (int j = 0; j < F::NB * 4; j++) o_v[j] = from_lane(off, (j >> 2) * 16 + (j & 1) + 2 * c + ((j >> 1) & 1) * 8, P.wide);
-#pragma unroll
-      for (int j = 0; j < 2 * F::NB; j++) {
-        const bool on = o_k[j] >= 0;
-        const char* src = kb + (on ? o_k[j] : 0) + c * 16;
-#pragma unroll
-        for (int x = 0; x < F::KP; x++) cp16(dk + (j * F::KP + x) * 512 + lane * 16, src + x * 64, on);
+      keys[0] = __ballot_sync(0xffffffffu, ok) & F::ALL;
+      if constexpr (E4M3) {
+        const long long so = (long long)pg * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row;
+        ks8[0] = ok ? __ldg(P.c.ks + so) : 127; vs8[0] = ok ? __ldg(P.c.vs + so) : 127;
       }
+      const uint32_t slot = (used + (uint32_t)i) % F::STAGES, dk = ring_s + slot * F::STAGE, dv = dk + F::TILE;
+      if (P.run) {                                               // the first lane of a run asks for its boxes
+        const bool first_of = there && lane < F::KEYS && (lane & (run - 1)) == 0;
+        const uint32_t bar = bars + slot * 8, n = __popc(__ballot_sync(0xffffffffu, first_of));
+        if (lane == 0) mbar_expect_tx(bar, n * (uint32_t)(run * F::RB * 2));
+        __syncwarp();
+        if (first_of) {
 #pragma unroll
-      for (int j = 0; j < F::NB * 4; j++) {
-        const bool on = o_v[j] >= 0;
-        const char* src = vb + (on ? o_v[j] : 0) + r * F::VW;
+          for (int h = 0; h < F::HALVES; h++) {
+            tma_load_4d(dk + h * (F::KEYS * 128) + lane * F::W, &P.km, bar, h * 64, at, kvh, pg);
+            tma_load_4d(dv + h * (F::KEYS * 128) + lane * F::W, &P.vm, bar, h * 64, at, kvh, pg);
+          }
+        }
+      } else {
+        constexpr int CH = F::RB / 16, N = F::KEYS * CH / 32;
+        const long long off = ok ? (long long)pg * P.c.page_b + (long long)at * P.c.row_b : -1;
+        long long o[N];                                          // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-        for (int x = 0; x < F::VP; x++) {
-          if constexpr (F::VW == 16) cp16(dv + (j * F::VP + x) * 512 + lane * 16, src + x * 128, on);
-          else cp8(dv + j * 256 + lane * 8, src, on);
+        for (int x = 0; x < N; x++) o[x] = from_lane(off, (x * 32 + lane) / CH, P.wide);
+#pragma unroll
+        for (int x = 0; x < N; x++) {
+          const bool on = o[x] >= 0;
+          const long long src = (on ? o[x] : 0) + lane % CH * 16;
+          const uint32_t to = F::at((x * 32 + lane) / CH, lane % CH);
+          cp16(dk + to, kb + src, on);
+          cp16(dv + to, vb + src, on);
         }
       }
-      uint32_t fl = __ballot_sync(0xffffffffu, ok) & F::ALL, bytes = 0;
-      if constexpr (E4M3) {                                      // the aligned word around the scale byte; which byte of it is kept beside it
-        const long long so = ok ? (long long)pg * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row : 0;
-        const unsigned long long ka = reinterpret_cast<unsigned long long>(P.c.ks + so), va = reinterpret_cast<unsigned long long>(P.c.vs + so);
-        cp4(side + lane * 4, reinterpret_cast<const void*>(ka & ~3ull), ok);
-        cp4(side + 128 + lane * 4, reinterpret_cast<const void*>(va & ~3ull), ok);
-        bytes = (uint32_t)(ka & 3) | (uint32_t)(va & 3) << 2;
-      }
-#pragma unroll
-      for (int x = F::STAGES - 1; x > 0; x--) { keys[x] = keys[x - 1]; scale_at[x] = scale_at[x - 1]; }
-      keys[0] = fl; scale_at[0] = bytes;
     };
-
-    auto skip = [&]() {
-#pragma unroll
-      for (int x = F::STAGES - 1; x > 0; x--) { keys[x] = keys[x - 1]; scale_at[x] = scale_at[x - 1]; }
-    };
+    bool fine = true;
     auto step = [&](int i) {
-      const int slot = i % F::STAGES, k0 = (a + i * F::WARPS) * F::KEYS;
+      const uint32_t slot = (used + (uint32_t)i) % F::STAGES;
+      const int k0 = (a + i * F::WARPS) * F::KEYS;
       unsigned char* sk = ring + slot * F::STAGE;
-      unsigned char* sv = sk + F::K_BYTES;
-      const uint32_t* side = reinterpret_cast<const uint32_t*>(sv + F::V_BYTES);
-      const uint32_t valid = keys[F::STAGES - 1], fl = scale_at[F::STAGES - 1];
+      unsigned char* sv = sk + F::TILE;
+      if (P.run) { if (!wait_for(bars + slot * 8, ((used + (uint32_t)i) / F::STAGES) & 1)) fine = false; }
+      else { cp_wait<F::STAGES - 1>(); __syncwarp(); }
+      const uint32_t valid = keys[F::STAGES - 1];
       float kf = 1.f, vf = 1.f;                                  // of this lane's key: its scale, 2^100 times its values' scale
       if constexpr (E4M3) {
-        const int k8 = (side[lane] >> ((fl & 3) * 8)) & 255, v8 = (side[32 + lane] >> (((fl >> 2) & 3) * 8)) & 255;
+        const int k8 = (int)ks8[F::STAGES - 1], v8 = (int)vs8[F::STAGES - 1];
         kf = __uint_as_float(k8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)min(max(k8, 1), E_MAX + 127) << 23);
         vf = __uint_as_float(v8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)(min(v8, E_MAX + 127) + 100) << 23);
       }
@@ -264,7 +288,8 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         }
 #pragma unroll
         for (int x = 0; x < F::KP; x++) {
-          const uint4 wa = *reinterpret_cast<const uint4*>(sk + (2 * kk * F::KP + x) * 512 + lane * 16), wb = *reinterpret_cast<const uint4*>(sk + ((2 * kk + 1) * F::KP + x) * 512 + lane * 16);
+          const int chunk = F::W == 64 ? c : x / 2 * 8 + 2 * c + x % 2;
+          const uint4 wa = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + r, chunk)), wb = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + 8 + r, chunk));
           if constexpr (E4M3) {
             const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
@@ -336,7 +361,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             for (int h = 0; h < 2; h++) if (fv[kk][h] != fv[kk][h]) fv[kk][h] = 0.f;
         } else {
 #pragma unroll 1
-          for (int x = 0; x < F::V_BYTES / 512; x++) {
+          for (int x = 0; x < F::TILE / 512; x++) {
             uint4* w = reinterpret_cast<uint4*>(sv + x * 512 + lane * 16);
             uint4 u = *w;
             if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
@@ -346,6 +371,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
           }
         }
         if (__any_sync(0xffffffffu, odd)) {
+          fence_async_shared();                                  // what was taken out, before the copy engine writes there again
 #pragma unroll 1
           for (int kk = 0; kk < F::KEYS; kk++) {
             const int p = k0 + kk;
@@ -387,10 +413,10 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             if constexpr (F::VW == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sv + ((kk * 4 + j) * F::VP + x) * 512 + lane * 16);
+              const uint4 u = *reinterpret_cast<const uint4*>(sv + F::at(kk * 16 + 2 * c + (j & 1) + (j >> 1) * 8, x * 8 + r));
               w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w;
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(sv + (kk * 4 + j) * 256 + lane * 8);
+              const uint2 u = *reinterpret_cast<const uint2*>(sv + F::at(kk * 16 + 2 * c + (j & 1) + (j >> 1) * 8, r >> 1) + (r & 1) * 8);
               w[j][0] = u.x; w[j][1] = u.y;
             }
           }
@@ -416,10 +442,13 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
     // One copy of each part of the code: a short context runs through it once, fetching it from L2
 #pragma unroll 1
     for (int i = 0; i < mine + F::STAGES - 1; i++) {
-      if (i < mine) issue(i); else skip();
-      cp_commit();
-      if (i >= F::STAGES - 1) { cp_wait<F::STAGES - 1>(); step(i - (F::STAGES - 1)); }
+      issue(i);
+      if (!P.run) cp_commit();
+      if (i >= F::STAGES - 1) step(i - (F::STAGES - 1));
+      __syncwarp();                                              // all lanes have read what the next copies overwrite
     }
+    used += (uint32_t)mine;
+    if (!fine) flag(P.b.status, ST_TIMEOUT);
     cp_wait<0>();
 #pragma unroll
     for (int n = 0; n < NR; n++)
@@ -502,6 +531,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       }
       if (P.cluster) cluster_sync();                             // nobody's shared memory goes while another reads it
     }
+    fence_async_shared();
     __syncthreads();
   }
 }

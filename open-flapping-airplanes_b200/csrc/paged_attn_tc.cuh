@@ -23,8 +23,6 @@
 namespace ofa {
 namespace paged {
 
-enum { ST_TIMEOUT = 8 };
-
 template <int D> struct Tc {
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
   static constexpr int NST = D == 128 ? 4 : 8;                  // ring of K and V tiles
@@ -42,18 +40,11 @@ struct TcCtrl {
 };
 static_assert(sizeof(TcCtrl) <= 512, "control area");
 
-// A bounded wait without a call: a function with an ABI of its own does not go with setmaxnreg. A try sleeps for about 300 clocks, the limit is a second or a few.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
-#pragma unroll 1
-  for (int i = 0; i < 10000000; i++) if (mbar_try(bar, parity)) return true;
-  return false;
-}
 __device__ __forceinline__ bool elect_one() {                  // one thread of a converged warp
   uint32_t e;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e != 0;
 }
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // D[tmem] (+)= A[tmem] * B[smem desc]
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u64 desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"

@@ -113,6 +113,22 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   return p;
 }
 
+// The pages as boxes of `run` rows for the copy engine; false where the driver will not have them, which leaves the other way of fetching them
+bool map_pages(CUtensorMap* m, const void* base, const ofa_kv_cache* c, const paged::Pool& C, int run) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess ? (Encode)f : (Encode) nullptr;
+  }();
+  const bool e4m3 = c->dtype == OFA_KV_E4M3;
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)C.row_b, (cuuint64_t)C.head_b, (cuuint64_t)C.page_b};
+  const cuuint32_t box[4] = {(cuuint32_t)(e4m3 ? c->head_dim : 64), (cuuint32_t)run, 1, 1}, one[4] = {1, 1, 1, 1};
+  return encode && encode(m, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          e4m3 && c->head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // The limit of dynamic shared memory, raised once for each kernel and device
 template <auto KERNEL> cudaError_t allow(int bytes) {
   static std::atomic<unsigned long long> done{0};
@@ -186,6 +202,8 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
   P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0;
   P.wide = (long long)cache->n_pages * P.c.page_b + (long long)cache->page_size * P.c.row_b >= 1ll << 35; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.part = static_cast<float*>(a->workspace);
+  P.run = cache->n_pages == 0 ? 0 : cache->page_size % 16 == 0 ? 16 : cache->page_size % 8 == 0 ? 8 : 0;
+  if (P.run && !(map_pages(&P.km, cache->k, cache, P.c, P.run) && map_pages(&P.vm, cache->v, cache, P.c, P.run))) P.run = 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p, s) : attend<128, true>(P, p, s);
