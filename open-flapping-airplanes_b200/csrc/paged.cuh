@@ -82,14 +82,22 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, uint32_t f) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(f));
   return r;
 }
-// Without the multiplication: two e4m3 numbers as bf16 of 2^-120 times their codes' values, three instructions. sel places them in bytes 1 and 3 and the first one's sign in
-// byte 2, so that one arithmetic shift moves both and brings their signs. Factors are then applied to what is computed from them.
+// the largest magnitude's bits of eight bf16 numbers; an infinity or a NaN is the largest
+__device__ __forceinline__ unsigned max_bits(uint4 u) {
+  unsigned m = 0;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+  return m;
+}
+// Without the multiplication: two e4m3 numbers as bf16 of 2^-120 times their codes' values, three instructions. sel places them in bytes 0 and 2 with their signs
+// in the bytes above, so that one shift moves both. Factors are then applied to what is computed from them.
 __device__ __forceinline__ uint32_t raw_pair(uint32_t x, uint32_t y, uint32_t sel) {
   uint32_t w;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(sel));
-  return (uint32_t)((int)w >> 4) & 0x87f087f0u;
+  return (w << 4) & 0x87f087f0u;
 }
-__host__ __device__ constexpr uint32_t raw_sel(int a, int b) { return (uint32_t)(a << 4 | (8 | a) << 8 | b << 12); }      // of bytes a and b of the eight in (x, y)
+__host__ __device__ constexpr uint32_t raw_sel(int a, int b) { return (uint32_t)(a | (8 | a) << 4 | b << 8 | (8 | b) << 12); }      // of bytes a and b of the eight in (x, y)
 // elements 2x, 2x+1 of the four in w
 __device__ __forceinline__ uint32_t widen_lo(uint32_t w, uint32_t f) { return widen(__byte_perm(w, 0, 0x1404), f); }
 __device__ __forceinline__ uint32_t widen_hi(uint32_t w, uint32_t f) { return widen(__byte_perm(w, 0, 0x3424), f); }

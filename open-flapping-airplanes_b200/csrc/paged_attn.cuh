@@ -18,14 +18,17 @@
 //            of the t-th product are two neighbouring dims
 // The scores' accumulator has keys down the lanes, the second product wants them along a lane: movmatrix turns 8 x 8 of them.
 //
-// Rows of the 8-bit cache enter the products as bf16 of 2^-120 times their codes (paged::raw_pair, three instructions for two elements); the keys' scales multiply the
-// scores, the values' scales the probabilities. So that nothing underflows, q is brought to 2^60 by a power of two for each row, and probabilities carry 2^100 (the result
-// 2^-20 of what it should be, made good at the end).
+// Keys of the 8-bit cache are operands as they are: a row of q is brought to 128 .. 256 by a power of two and split into two e4m3 numbers, the second holding
+// 16 times what the first leaves, which is all 8 bits of a bf16 number down to 2^-13 of the row's largest and 2^-21 of that below (products of e4m3 numbers are summed in fp32 as
+// exactly as those of bf16). Values enter as bf16 of 2^-120 times their codes (paged::raw_pair, three instructions for two elements). Keys' scales multiply the scores, values'
+// scales the probabilities, which carry 2^100 so that nothing underflows (the result is 2^-20 of what it should be, made good at the end). Widening the keys like the
+// values left the byte and logic instructions of the integer pipe, two clocks each, as the bound: 10 of them for four elements.
 //
 // A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
 // infinities and NaN are taken out of its values and added to the rows that see it. Rows past the context and of a bad page are never read.
 #pragma once
 #include <cuda.h>
+#include <cuda_fp8.h>
 #include "paged.cuh"
 
 namespace ofa {
@@ -66,6 +69,20 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// four values as e4m3 numbers, to nearest; what they leave comes back in their place
+__device__ __forceinline__ uint32_t split_e4m3(float (&v)[4]) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)((i < 2 ? lo : hi) >> (i & 1) * 8 & 255), __NV_E4M3);
+    v[i] -= __half2float(*reinterpret_cast<const __half*>(&h));
+  }
+  return lo | hi << 16;
 }
 __device__ __forceinline__ bool odd_bits(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }   // an infinity or a NaN in the pair
 __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
@@ -130,7 +147,7 @@ template <bool E4M3> __device__ float held(const char* row, int d, int scale) {
 template <int D, bool E4M3, int NR>
 __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __grid_constant__ AttnArgs P) {
   using F = Few<D, E4M3, NR>;
-  constexpr int MT = D / 16, KS = D / 16;                        // products of 16 dims of the output, of 16 dims of a score
+  constexpr int MT = D / 16, KS = E4M3 ? D / 32 : D / 16;        // products of 16 dims of the output; of 16 (32: 8-bit keys) dims of a score
   extern __shared__ __align__(16) unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
@@ -152,7 +169,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 
   for (int tile = tile0; tile * F::ROWS < ch.n * group; tile += P.tiles) {
     const int t_last = min(ch.n - 1, (int)P.group.quot(tile * F::ROWS + F::ROWS - 1)), p_min = ch.p0 + (int)P.group.quot(tile * F::ROWS), p_max = ch.p0 + t_last;
-    uint32_t qf[NR][KS][2];                                      // row r of every eight
+    uint32_t qf[NR][KS][2], ql[NR][KS][2];                       // row r of every eight; 8-bit keys: 16 times what qf leaves
     float rowf[NR][2];                                           // what the raw scores of rows 2c and 2c + 1 of every eight are multiplied by
     int pos[NR][2];                                              // and where they stand
 #pragma unroll
@@ -160,11 +177,14 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       const int rr = tile * F::ROWS + n * 8 + r, t = (int)P.group.quot(rr);
       const bool on = t < ch.n;
       const bf16* src = P.q + (long long)(on ? ch.s + t : ch.s) * P.q_row + (long long)(kvh * group + rr - t * group) * P.q_head;
+      uint4 qv[E4M3 ? KS : 1];
 #pragma unroll
       for (int s = 0; s < KS; s++) {
-        const int d = !E4M3 ? (s / 4) * 64 + (2 * c + s / 2 % 2) * 8 + s % 2 * 4 : D == 128 ? (2 * c + s / 4) * 16 + s % 4 * 4 : c * 16 + s * 4;
-        const uint2 w = on ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-        qf[n][s][0] = w.x; qf[n][s][1] = w.y;
+        if constexpr (E4M3) qv[s] = on ? *reinterpret_cast<const uint4*>(src + (D == 128 ? (2 * c + s / 2) * 16 : c * 16) + s % 2 * 8) : make_uint4(0, 0, 0, 0);
+        else {
+          const uint2 w = on ? *reinterpret_cast<const uint2*>(src + (s / 4) * 64 + (2 * c + s / 2 % 2) * 8 + s % 2 * 4) : make_uint2(0, 0);
+          qf[n][s][0] = w.x; qf[n][s][1] = w.y;
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -175,21 +195,26 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
       if constexpr (E4M3) {
         unsigned mag = 0;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) mag = max(mag, max(qf[n][s][h] & 0x7fffu, qf[n][s][h] >> 16 & 0x7fffu));
+        for (int s = 0; s < KS; s++) mag = max(mag, max_bits(qv[s]));
         mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
         mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
-        // largest magnitude to 2^60 ..; beyond these bounds the scores' factor would leave fp32, and need not
-        const int shift = mag >= 0x7f80u ? 0 : min(max(60 - ((int)(mag >> 7) - 127), -7), 120);
-        const float up = __uint_as_float((uint32_t)(127 + shift) << 23), down = __uint_as_float((uint32_t)(247 - shift) << 23);      // 2^shift, 2^(120 - shift)
+        const int shift = min(7 - ((int)(mag >> 7) - 127), 120);                     // largest magnitude to 2^7 ..
+        const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
+        float down = __uint_as_float((uint32_t)(127 - shift) << 23);
+        if (mag >= 0x7f80u) down = __uint_as_float(0x7fc00000u);                     // an infinity or a NaN in the row
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int s = 0; s < KS; s++) {
+          const uint32_t w[4] = {qv[s].x, qv[s].y, qv[s].z, qv[s].w};
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[n][s][h]));
-            qf[n][s][h] = pack2f(v.x * up, v.y * up);
+            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[2 * h])), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[2 * h + 1]));
+            float v[4] = {x.x * up, x.y * up, y.x * up, y.y * up};
+            qf[n][s][h] = split_e4m3(v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] *= 16.f;
+            ql[n][s][h] = split_e4m3(v);
           }
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) rowf[n][h] *= __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
       }
@@ -291,12 +316,13 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
           const int chunk = F::W == 64 ? c : x / 2 * 8 + 2 * c + x % 2;
           const uint4 wa = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + r, chunk)), wb = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + 8 + r, chunk));
           if constexpr (E4M3) {
-            const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+            const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-              const uint32_t af[4] = {raw_pair(ua[y], 0, raw_sel(0, 1)), raw_pair(ub[y], 0, raw_sel(0, 1)), raw_pair(ua[y], 0, raw_sel(2, 3)), raw_pair(ub[y], 0, raw_sel(2, 3))};
-#pragma unroll
-              for (int n = 0; n < NR; n++) mma16816(y & 1 ? s2[n] : s[kk][n], af, qf[n][4 * x + y][0], qf[n][4 * x + y][1]);
+            for (int n = 0; n < NR; n++) {
+              mma16832_e4m3(s[kk][n], a0, qf[n][2 * x][0], qf[n][2 * x][1]);
+              mma16832_e4m3(s2[n], a0, ql[n][2 * x][0], ql[n][2 * x][1]);
+              mma16832_e4m3(s[kk][n], a1, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
+              mma16832_e4m3(s2[n], a1, ql[n][2 * x + 1][0], ql[n][2 * x + 1][1]);
             }
           } else {
             const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
@@ -310,7 +336,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 #pragma unroll
         for (int n = 0; n < NR; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[kk][n][e] += s2[n][e];
+          for (int e = 0; e < 4; e++) s[kk][n][e] += E4M3 ? s2[n][e] * 0.0625f : s2[n][e];
       }
       float mx[NR][2];
 #pragma unroll

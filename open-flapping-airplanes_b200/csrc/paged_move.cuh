@@ -22,13 +22,6 @@ struct MoveArgs {
 };
 constexpr int MOVE_ROWS = 64;                         // at most
 
-__device__ __forceinline__ unsigned max_bits(uint4 u) {
-  unsigned m = 0;
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
-  return m;
-}
 __device__ __forceinline__ uint32_t to_e4m3(uint32_t lo, uint32_t hi, float f) {
   const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&lo)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi));
   const uint32_t x = __nv_cvt_float2_to_fp8x2(make_float2(a.x * f, a.y * f), __NV_SATFINITE, __NV_E4M3);
