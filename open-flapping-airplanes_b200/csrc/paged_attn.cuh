@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   using F = Few<D, E4M3, NR>;
   constexpr int MT = D / 16, KS = E4M3 ? D / 32 : D / 16;        // products of 16 dims of the output; of 16 (32: 8-bit keys) dims of a score
   extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = raw + (-(int)smem_u32(raw) & 1023);      // by an offset: through an integer the pointer would lose its address space
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const uint32_t bars = smem_u32(smem + F::BARS_AT) + warp * F::STAGES * 8;
   if (lane < F::STAGES) mbar_init(bars + lane * 8, 1);
@@ -164,6 +164,9 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   const uint32_t ring_s = smem_u32(ring);
   const char* kb = P.c.k + (long long)kvh * P.c.head_b;
   const char* vb = P.c.v + (long long)kvh * P.c.head_b;
+  // where this lane's pieces lie in a tile: keys' rows r, values' rows 2c and 2c + 1; rows 8 further are 8 W bytes further
+  const uint32_t ka0 = F::at(r, F::W == 64 ? c : 2 * c), ka1 = F::W == 64 ? ka0 : F::at(r, 2 * c + 1);
+  const uint32_t va0 = F::at(2 * c, F::W == 64 ? r >> 1 : r) + (F::VW == 8 ? (r & 1) * 8 : 0), va1 = F::at(2 * c + 1, F::W == 64 ? r >> 1 : r) + (F::VW == 8 ? (r & 1) * 8 : 0);
   // the dim of row r (or r + 8: the one behind it) in the t-th product of the output
   auto dim_of = [&](int t) { return E4M3 ? r * (D / 8) + 2 * t : (t / 4) * 64 + r * 8 + (t % 4) * 2; };
 
@@ -313,8 +316,8 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         }
 #pragma unroll
         for (int x = 0; x < F::KP; x++) {
-          const int chunk = F::W == 64 ? c : x / 2 * 8 + 2 * c + x % 2;
-          const uint4 wa = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + r, chunk)), wb = *reinterpret_cast<const uint4*>(sk + F::at(kk * 16 + 8 + r, chunk));
+          const unsigned char* src = sk + (x & 1 ? ka1 : ka0) + x / 2 * (F::KEYS * 128) + kk * 16 * F::W;
+          const uint4 wa = *reinterpret_cast<const uint4*>(src), wb = *reinterpret_cast<const uint4*>(src + 8 * F::W);
           if constexpr (E4M3) {
             const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
 #pragma unroll
@@ -438,11 +441,12 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
           uint32_t w[4][F::VW / 4];
 #pragma unroll
           for (int j = 0; j < 4; j++) {
+            const unsigned char* src = sv + (j & 1 ? va1 : va0) + x * (F::KEYS * 128) + (kk * 16 + (j >> 1) * 8) * F::W;
             if constexpr (F::VW == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sv + F::at(kk * 16 + 2 * c + (j & 1) + (j >> 1) * 8, x * 8 + r));
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
               w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w;
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(sv + F::at(kk * 16 + 2 * c + (j & 1) + (j >> 1) * 8, r >> 1) + (r & 1) * 8);
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
               w[j][0] = u.x; w[j][1] = u.y;
             }
           }

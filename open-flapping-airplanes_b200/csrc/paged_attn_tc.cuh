@@ -61,7 +61,7 @@ template <int D, bool E4M3>
 __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant__ AttnArgs P) {
   using F = Tc<D>;
   extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = raw + (-(int)smem_u32(raw) & 1023);      // by an offset: through an integer the pointer would lose its address space
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
