@@ -1,10 +1,10 @@
 // Rows of new keys and values to their pages, and back: one pass, bound by its bytes (or, for a step of a few tokens, by one launch and three
 // dependent loads: q_start, the page table, the row).
 //
-// A thread holds 16 bytes of a bf16 row, so a row of head_dim values is 8 or 16 neighbouring lanes: the largest magnitude is found as an unsigned maximum of
-// the bits without signs (an infinity or a NaN is then the largest) and shared with three or four shuffles; scaling by a power of two is exact, so the
+// A thread holds 8 values of a row (16 of an 8-bit one: 16 bytes where it is held), so a row is 4 to 16 neighbouring lanes: the largest magnitude is found as an
+// unsigned maximum of the bits without signs (an infinity or a NaN is then the largest) and shared by shuffles; scaling by a power of two is exact, so the
 // only rounding is the one to e4m3 (to nearest, half a step 2^-4 relative). A block takes consecutive rows of the call; its threads compare the starts of
-// all sequences with them once and leave each row's page in shared memory.
+// all sequences with them once and leave each row's page in shared memory. Four pieces a thread are asked for before the first is worked on.
 #pragma once
 #include <cuda_fp8.h>
 #include "paged.cuh"
@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t to_e4m3(uint32_t lo, uint32_t hi, float f) {
 
 template <int D, bool E4M3, bool READ>
 __global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ MoveArgs P) {
-  constexpr int LANES = D / 8;                        // of a row
+  constexpr int PIECE = E4M3 ? 16 : 8, LANES = D / PIECE;      // values a thread holds of a row, lanes of a row
   __shared__ int2 place[MOVE_ROWS];                   // page and row in it; x = -1: nowhere, -2: no sequence's row
   const int tid = threadIdx.x, r0 = blockIdx.x * P.rows, r1 = min(r0 + P.rows, P.b.n_rows);
   if (tid < MOVE_ROWS) place[tid] = make_int2(-2, 0);
@@ -51,39 +51,56 @@ __global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ MoveA
     place[tid] = make_int2(page, at);
   }
   __syncthreads();
+  constexpr int U = 4;                                // pieces that a thread has on their way
   const int total = (r1 - r0) * 2 * P.n_kv_heads * LANES;
-  for (int base = 0; base < total; base += 256) {
-    const int it = base + tid, part = it % LANES, vec = it / LANES, row = (int)P.pair.quot(vec), wh = vec - row * 2 * P.n_kv_heads;
-    const bool is_v = wh >= P.n_kv_heads;
-    const int head = is_v ? wh - P.n_kv_heads : wh;
-    const int2 pl = it < total ? place[row] : make_int2(-2, 0);
-    bf16* x = it < total ? (is_v ? P.v + (long long)(r0 + row) * P.v_row + (long long)head * P.v_head : P.k + (long long)(r0 + row) * P.k_row + (long long)head * P.k_head) + part * 8 : nullptr;
-    char* held = (is_v ? P.c.v : P.c.k) + (long long)pl.x * P.c.page_b + (long long)head * P.c.head_b + (long long)pl.y * P.c.row_b + part * (E4M3 ? 8 : 16);
-    unsigned char* sc = E4M3 ? (is_v ? P.c.vs : P.c.ks) + (long long)pl.x * P.c.s_page + (long long)head * P.c.s_head + (long long)pl.y * P.c.s_row : nullptr;
-    if constexpr (READ) {
-      if (pl.x == -2) continue;
-      uint4 u = make_uint4(0, 0, 0, 0);               // a row that is nowhere reads as zeros
-      if (pl.x >= 0) {
-        if constexpr (E4M3) {
-          const uint2 w = *reinterpret_cast<const uint2*>(held);
-          uint32_t f = scale_bits(*sc); f |= f << 16;
-          u = make_uint4(widen_lo(w.x, f), widen_hi(w.x, f), widen_lo(w.y, f), widen_hi(w.y, f));
-        } else u = *reinterpret_cast<const uint4*>(held);
+  for (int base = 0; base < total; base += 256 * U) {
+    bf16* x[U];
+    char* held[U];
+    unsigned char* sc[U];
+    int state[U];                                     // -2 no row, -1 a row without a place, 0 a row with one
+    uint4 a[U], b[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const int it = base + i * 256 + tid, part = it % LANES, vec = it / LANES, row = (int)P.pair.quot(vec), wh = vec - row * 2 * P.n_kv_heads;
+      const bool is_v = wh >= P.n_kv_heads;
+      const int head = is_v ? wh - P.n_kv_heads : wh;
+      const int2 pl = it < total ? place[row] : make_int2(-2, 0);
+      state[i] = min(pl.x, 0);
+      x[i] = (is_v ? P.v + (long long)(r0 + row) * P.v_row + (long long)head * P.v_head : P.k + (long long)(r0 + row) * P.k_row + (long long)head * P.k_head) + part * PIECE;
+      held[i] = (is_v ? P.c.v : P.c.k) + (long long)pl.x * P.c.page_b + (long long)head * P.c.head_b + (long long)pl.y * P.c.row_b + part * 16;
+      if (E4M3) sc[i] = (is_v ? P.c.vs : P.c.ks) + (long long)pl.x * P.c.s_page + (long long)head * P.c.s_head + (long long)pl.y * P.c.s_row;
+      a[i] = b[i] = make_uint4(0, 0, 0, 0);           // a row that is nowhere reads as zeros
+      if (state[i] == 0) {
+        if constexpr (READ) {
+          a[i] = *reinterpret_cast<const uint4*>(held[i]);
+          if (E4M3) b[i].x = *sc[i];
+        } else {
+          a[i] = reinterpret_cast<const uint4*>(x[i])[0];
+          if (E4M3) b[i] = reinterpret_cast<const uint4*>(x[i])[1];
+        }
       }
-      *reinterpret_cast<uint4*>(x) = u;
-    } else {
-      const uint4 u = pl.x >= 0 ? *reinterpret_cast<const uint4*>(x) : make_uint4(0, 0, 0, 0);
-      if constexpr (E4M3) {
-        unsigned m = max_bits(u);
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      if constexpr (READ) {
+        if (state[i] == -2) continue;
+        if constexpr (E4M3) {
+          uint32_t f = scale_bits((int)b[i].x); f |= f << 16;
+          reinterpret_cast<uint4*>(x[i])[0] = make_uint4(widen_lo(a[i].x, f), widen_hi(a[i].x, f), widen_lo(a[i].y, f), widen_hi(a[i].y, f));
+          reinterpret_cast<uint4*>(x[i])[1] = make_uint4(widen_lo(a[i].z, f), widen_hi(a[i].z, f), widen_lo(a[i].w, f), widen_hi(a[i].w, f));
+        } else *reinterpret_cast<uint4*>(x[i]) = a[i];
+      } else if constexpr (E4M3) {
+        unsigned m = max(max_bits(a[i]), max_bits(b[i]));
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int b = scale_byte(m);
-        const float f = __uint_as_float((uint32_t)(254 - (b == SCALE_NAN ? 127 : b)) << 23);          // 2^(127 - b)
-        if (pl.x >= 0) {
-          *reinterpret_cast<uint2*>(held) = b == SCALE_NAN ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : make_uint2(to_e4m3(u.x, u.y, f), to_e4m3(u.z, u.w, f));
-          if (part == 0) *sc = (unsigned char)b;
+        const int s = scale_byte(m);
+        const float f = __uint_as_float((uint32_t)(254 - (s == SCALE_NAN ? 127 : s)) << 23);          // 2^(127 - s)
+        if (state[i] == 0) {
+          *reinterpret_cast<uint4*>(held[i]) = s == SCALE_NAN ? make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu)
+                                                              : make_uint4(to_e4m3(a[i].x, a[i].y, f), to_e4m3(a[i].z, a[i].w, f), to_e4m3(b[i].x, b[i].y, f), to_e4m3(b[i].z, b[i].w, f));
+          if (tid % LANES == 0) *sc[i] = (unsigned char)s;
         }
-      } else if (pl.x >= 0) *reinterpret_cast<uint4*>(held) = u;
+      } else if (state[i] == 0) *reinterpret_cast<uint4*>(held[i]) = a[i];
     }
   }
 }

@@ -72,7 +72,7 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
   P.k = static_cast<bf16*>(k); P.v = static_cast<bf16*>(v); P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
   P.n_kv_heads = c->n_kv_heads; P.pair.set(2u * (unsigned)c->n_kv_heads);
   // four pieces of 16 bytes for a thread where there are rows for it: a block then amortises the search for its sequences
-  const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / 8);
+  const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / (c->dtype == OFA_KV_E4M3 ? 16 : 8));
   long long rows = (1024 + per_row - 1) / per_row;
   while (rows > 1 && (n_rows + rows - 1) / rows < 148) rows--;
   P.rows = (int)(rows < paged::MOVE_ROWS ? rows : paged::MOVE_ROWS);
@@ -166,6 +166,16 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   return e;
 }
 
+// Four vectors a thread where that still gives every SM several blocks, else one: each block reads its row's whole history
+template <class T, bool WIDE> void process(const logits::Args& P, int rows, cudaStream_t s) {
+  const int vn = Vec<T>::N, span = P.vocab + (WIDE ? vn - 1 : 0);
+  const bool large = (long long)rows * ((span + 1024 * vn - 1) / (1024 * vn)) >= 4 * 148;
+  const int stretch = (large ? 1024 : 256) * vn;
+  const dim3 grid((unsigned)((span + stretch - 1) / stretch), (unsigned)rows);
+  const unsigned smem = P.tokens || P.bias_ids ? (unsigned)stretch * 4 : 0;
+  if (large) logits::process_kernel<T, 4, WIDE><<<grid, 256, smem, s>>>(P); else logits::process_kernel<T, 1, WIDE><<<grid, 256, smem, s>>>(P);
+}
+
 }  // namespace
 
 extern "C" const char* ofa_serving_last_error(void) { return g_error; }
@@ -234,17 +244,16 @@ extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
   if (!aligned(a->tokens, 4) || !aligned(a->n_tokens, 4) || !aligned(a->n_prompt, 4) || !aligned(a->repetition, 4) || !aligned(a->presence, 4) || !aligned(a->frequency, 4) ||
       !aligned(a->bias_ids, 4) || !aligned(a->bias, 4) || !aligned(a->mask, 4)) return fail(OFA_BAD_ARGUMENT, "misaligned array");
   logits::Args P;
-  P.in = a->in; P.out = a->out; P.in_row = a->in_stride; P.out_row = a->out_stride; P.vocab = a->vocab; P.stretch = 4096;
+  P.in = a->in; P.out = a->out; P.in_row = a->in_stride; P.out_row = a->out_stride; P.vocab = a->vocab;
   const bool history = a->tokens && a->max_tokens > 0 && (a->repetition || a->presence || a->frequency);
   P.tokens = history ? a->tokens : nullptr; P.tokens_row = a->tokens_stride; P.max_tokens = a->max_tokens; P.n_tokens = a->n_tokens; P.n_prompt = a->n_prompt;
   P.repetition = a->repetition; P.presence = a->presence; P.frequency = a->frequency;
   P.bias_ids = a->max_bias > 0 ? a->bias_ids : nullptr; P.bias = a->bias; P.bias_row = a->bias_stride; P.max_bias = a->max_bias;
   P.mask = a->mask; P.mask_row = a->mask_stride;
-  const unsigned smem = (unsigned)P.stretch * 4 * ((P.tokens != nullptr) + (P.bias_ids != nullptr));
-  const dim3 grid((unsigned)((a->vocab + P.stretch - 1) / P.stretch), (unsigned)a->n_rows);
-  const bool wide = aligned(a->in, 16) && aligned(a->out, 16) && (a->n_rows == 1 || ((a->in_stride * es) % 16 == 0 && (a->out_stride * es) % 16 == 0));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == OFA_DTYPE_F32) { if (wide) logits::process_kernel<float, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<float, false><<<grid, 256, smem, s>>>(P); }
-  else { if (wide) logits::process_kernel<bf16, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<bf16, false><<<grid, 256, smem, s>>>(P); }
+  // whole 16-byte vectors where rows of in and out lie alike against their boundaries (an odd vocabulary moves both from row to row)
+  const bool wide = (reinterpret_cast<uintptr_t>(a->in) - reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 && (a->n_rows == 1 || ((a->in_stride - a->out_stride) * (long long)es) % 16 == 0);
+  if (a->dtype == OFA_DTYPE_F32) wide ? process<float, true>(P, a->n_rows, s) : process<float, false>(P, a->n_rows, s);
+  else wide ? process<bf16, true>(P, a->n_rows, s) : process<bf16, false>(P, a->n_rows, s);
   return launched("ofa_logits_process");
 }

@@ -495,3 +495,24 @@ def test_attention_over_codes_of_every_size(sv, dim, rows):
         batch = sv.KVBatch(i32([0, rows]), i32([n]), i32([[0]]), max_new=rows)
         q = (torch.randn(rows, 2, dim, generator=g) * 2.0 ** (-e - 8)).bfloat16().to(DEV)
         check_attention(sv, cache, batch, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,pad", [(3, 8200, 1), (600, 4103, 0), (9, 2049, 3), (2, 7, 5), (200, 12289, 2)])
+def test_logits_of_rows_between_boundaries(sv, rows, vocab, pad, dtype):
+    """Odd vocabularies and offsets: rows start anywhere against 16 bytes, in one tensor alike and in the other not"""
+    x, a, mask = logit_inputs(rows, vocab, 20, 3, dtype)
+    a["mask"] = mask
+    dev = {k: v.to(DEV) for k, v in a.items()}
+    half = ref.F32_HALF if dtype == torch.float32 else ref.BF16_HALF
+    some = sorted({0, 1, rows // 2, rows - 1})
+    want, tol = ref.logits(x[some], **{k: v[some] for k, v in a.items()})
+    for shift in (0, pad):
+        space = torch.zeros(rows * (vocab + pad) + 8, dtype=dtype, device=DEV)
+        y = space[shift: shift + rows * (vocab + pad)].view(rows, vocab + pad)[:, :vocab]
+        y.copy_(x.to(DEV))
+        for out in (None, torch.empty_like(x.to(DEV)), y):
+            got = sv.logits_process(y, out=out, **dev)[some].double().cpu()
+            fine = torch.isfinite(want) & (want.abs() < torch.finfo(dtype).max)
+            assert torch.equal(got[want == -math.inf], want[want == -math.inf])
+            assert ((got - want).abs()[fine] <= (tol + half * (want.abs() + tol))[fine]).all()
