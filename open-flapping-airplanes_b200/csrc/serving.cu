@@ -248,7 +248,7 @@ extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
   const bool history = a->tokens && a->max_tokens > 0 && (a->repetition || a->presence || a->frequency);
   P.tokens = history ? a->tokens : nullptr; P.tokens_row = a->tokens_stride; P.max_tokens = a->max_tokens; P.n_tokens = a->n_tokens; P.n_prompt = a->n_prompt;
   P.repetition = a->repetition; P.presence = a->presence; P.frequency = a->frequency;
-  P.bias_ids = a->max_bias > 0 ? a->bias_ids : nullptr; P.bias = a->bias; P.bias_row = a->bias_stride; P.max_bias = a->max_bias;
+  P.bias_ids = a->max_bias > 0 ? a->bias_ids : nullptr; P.bias = a->bias; P.bias_row = a->bias_stride; P.max_bias = a->bias_ids ? a->max_bias : 0;
   P.mask = a->mask; P.mask_row = a->mask_stride;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // whole 16-byte vectors where rows of in and out lie alike against their boundaries (an odd vocabulary moves both from row to row)
