@@ -6,16 +6,18 @@
 //                    back over them as bf16, the A operand of the second product
 //   warps 8, 9       one thread each issues a tile's products: S = Q K_j^T, then O += P V_j. Two threads because one issues a tcgen05.mma only every
 //                    ~96 clocks, and a 128 x 128 x 16 product takes 64
-//   warps 10-15      fetch keys and values into a ring of tiles in the layout the products read (128-byte swizzle)
-// Tensor memory, 512 columns: S 0 / 128 (P in their last 64), O 256 / 256 + D. Rows of pages are gathered by cp.async, 16 bytes at a time, so pages
-// may have any size and end inside a tile; 8-bit rows become bf16 in the loaders' registers, once for the 256 rows.
+//   warp 10          asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
+//                    (128-byte swizzle), 8-bit rows into a ring of their own
+//   warps 11-15      widen 8-bit rows from there into the tiles, once for the 256 rows; look at values that some row must not meet; and gather the rows of pages that are no
+//                    multiple of 8 by cp.async, 16 bytes a lane
+// Tensor memory, 512 columns: S 0 / 128 (P in their last 64), O 256 / 256 + D.
 //
 // A row's probabilities are taken against a reference that is raised only when the true maximum has passed it by 2^8 (they stay below 256: exact enough in fp32 sums and
 // bf16), and only then is the row of O multiplied in tensor memory. Before S of the next step is issued the issuer has seen the product before it complete, so a softmax thread
 // that has its scores may also rewrite its row of O.
 //
-// Keys that some rows of the block see and others do not (the diagonal, the window's edge, the end of the context) come in tiles whose loaders look at
-// every value: infinities and NaN are left out and added at the end to the rows that see them.
+// Keys that some rows of the block see and others do not (the diagonal, the window's edge, the end of the context) come in tiles whose values are all looked
+// at: infinities and NaN are taken out and added at the end to the rows that see them.
 #pragma once
 #include "attn_tc.cuh"
 #include "paged_attn.cuh"
@@ -23,22 +25,28 @@
 namespace ofa {
 namespace paged {
 
-template <int D> struct Tc {
+template <int D, bool E4M3> struct Tc {
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
-  static constexpr int NST = D == 128 ? 4 : 8;                  // ring of K and V tiles
-  static constexpr int LAG = D == 128 ? 1 : 2;                  // tiles whose copies may be in flight when the next is begun
+  static constexpr int NST = D == 64 ? 8 : E4M3 ? 3 : 4;        // ring of K and V tiles
+  static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 4 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
+  static constexpr int LAG = D == 128 ? 1 : 2;                  // gathered tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
-  static constexpr int Q_AT = 0, RING_AT = 2 * TILE, CTRL_AT = RING_AT + NST * TILE;
-  static constexpr int SMEM = CTRL_AT + 512 + 1024;             // 1,024 for the alignment of the swizzle's atoms
-  static constexpr int LOADERS = 6;
+  static constexpr int Q_AT = 0, RING_AT = 2 * TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
+  static constexpr int SMEM = CTRL_AT + 640 + 1024;             // 1,024 for the alignment of the swizzle's atoms
+  static constexpr int WORKERS = 5;
+  static __device__ __forceinline__ uint32_t raw_at(int row, int chunk) {      // a 16-byte piece of an 8-bit row
+    return D == 64 ? (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)) : (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
+  }
 };
 struct TcCtrl {
   u64 q_full, full[8], empty[8], s_full[2], p_full[2], o_full[2];
+  u64 look[8];                                                  // bf16: a tile that the workers look through has landed
+  u64 raw_full[4], raw_empty[4];
   uint32_t tmem, dead;
   int odd_lo, odd_hi;
-  alignas(16) uint16_t valid[8][8];
+  alignas(16) uint8_t valid[8][16];                             // by step, a bit for each key
 };
-static_assert(sizeof(TcCtrl) <= 512, "control area");
+static_assert(sizeof(TcCtrl) <= 640, "control area");
 
 __device__ __forceinline__ bool elect_one() {                  // one thread of a converged warp
   uint32_t e;
@@ -54,12 +62,13 @@ template <bool INC, int N> __device__ __forceinline__ void set_regs() {
   if constexpr (INC) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, int n) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory"); }
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }      // the lowest n bits
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) { return (uint32_t)((chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant__ AttnArgs P) {
-  using F = Tc<D>;
+  using F = Tc<D, E4M3>;
   extern __shared__ __align__(16) unsigned char raw[];
   unsigned char* smem = raw + (-(int)smem_u32(raw) & 1023);      // by an offset: through an integer the pointer would lose its address space
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
@@ -75,7 +84,8 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
   if (turn >= npair) return;
   if (tid == 0) {
     mbar_init(smem_u32(&ct.q_full), 8);
-    for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::LOADERS); mbar_init(smem_u32(&ct.empty[s]), 2); }
+    for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::WORKERS); mbar_init(smem_u32(&ct.empty[s]), 2); mbar_init(smem_u32(&ct.look[s]), 1); }
+    for (int s = 0; s < 4; s++) { mbar_init(smem_u32(&ct.raw_full[s]), 1); mbar_init(smem_u32(&ct.raw_empty[s]), F::WORKERS); }
     for (int i = 0; i < 2; i++) { mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.p_full[i]), 4); mbar_init(smem_u32(&ct.o_full[i]), 1); }
     ct.odd_lo = 0x7fffffff; ct.odd_hi = -1; ct.dead = 0;
     mbar_fence_init();
@@ -323,125 +333,213 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
       uses += 2u * (uint32_t)(k.B - k.A); done += (uint32_t)(kb - ka); round++;
       if (!next(ok)) break;
     }
-  } else {
-    // ------------------------------------------------------------------------------------------ loaders
+  } else if (warp == 10) {
+    // ------------------------------------------------------------------------------------------ copies
     set_regs<false, 72>();
-    constexpr int CH = E4M3 ? D / 16 : D / 8, IT = 16 * CH / 32;      // 16-byte pieces of a held row, of 16 rows for each lane
-    constexpr int LAG = E4M3 ? 0 : F::LAG;                       // rows in 8 bits are there when they are written
-    const int w = warp - 10;
-    const char* kbase = P.c.k + (long long)kvh * P.c.head_b;
-    const char* vbase = P.c.v + (long long)kvh * P.c.head_b;
+    const int run = P.run ? P.run : 8, nrun = 128 / run;         // a lane for each run of a step's keys
     uint32_t uses = 0;
-    // A step's 128 keys are eight units of 16 rows; a warp takes one or two, others in each step. Lanes 0 .. 15 (and 16 .. 31 again) look a unit's rows up, a step ahead.
-    struct Unit { long long off; uint32_t fk, fv; };
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
-      const int total = 2 * (k.B - k.A);
-      auto look = [&](int j, int u) {
-        Unit x = {-1, 0, 0};
-        const int key = j * 128 + u * 16 + (lane & 15);
-        int page, at;
-        if (j < k.B && u < 8 && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) {
-          x.off = (long long)page * P.c.page_b + (long long)at * P.c.row_b;
-          if constexpr (E4M3) {
-            const long long so = (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row;
-            x.fk = __ldg(P.c.ks + so); x.fv = __ldg(P.c.vs + so);
+      if (P.run) {
+        auto reaches = [&](int j) { const int key = j * 128 + lane * run; return lane < nrun && j < k.B && key + run > k.lo && key < k.hi; };
+        auto page_of = [&](int j) { return reaches(j) ? __ldg(P.b.pages + (long long)seq * P.b.pages_stride + P.b.page.quot((unsigned)(j * 128 + lane * run))) : -1; };      // below cap
+        int page = page_of(k.A);
+        for (int j = k.A; j < k.B && ok; j++) {
+          const int pg = page, key = j * 128 + lane * run, at = key - (int)(P.b.page.quot((unsigned)key) * P.b.page.d);
+          page = page_of(j + 1);
+          const bool there = (unsigned)pg < (unsigned)P.b.n_pages, bad = reaches(j) && !there;
+          if (bad) flag(P.b.status, ST_PAGE);
+          const bool any_bad = __any_sync(0xffffffffu, bad);
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * (uint32_t)(run * D * (E4M3 ? 1 : 2));
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const uint32_t n = uses + 2 * (uint32_t)(j - k.A) + half, slot = n % F::NST, rs = n % F::RS;
+            if constexpr (E4M3) ok = wait_for(smem_u32(&ct.raw_empty[rs]), ((n / F::RS) & 1) ^ 1);
+            else ok = wait_for(smem_u32(&ct.empty[slot]), ((n / F::NST) & 1) ^ 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (half == 0 && lane < nrun) {                      // which keys are there
+              const uint32_t bits = there ? below(k.hi - key) & ~below(k.lo - key) : 0u;
+              if (run == 16) *reinterpret_cast<uint16_t*>(&ct.valid[j % F::NV][lane * 2]) = (uint16_t)bits;
+              else ct.valid[j % F::NV][lane] = (uint8_t)bits;
+            }
+            const CUtensorMap* map = half ? &P.vm : &P.km;
+            if constexpr (E4M3) {
+              if (lane == 0) mbar_expect_tx(smem_u32(&ct.raw_full[rs]), bytes);
+              __syncwarp();
+              if (there) tma_load_4d(base + F::RAW_AT + rs * F::RAW + lane * run * D, map, smem_u32(&ct.raw_full[rs]), 0, at, kvh, pg);
+            } else {
+              unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
+              if (half && any_bad) {                             // values of rows that are not there: zeros
+                if (bad)
+                  for (int x = 0; x < run * 8; x++)
+                    for (int h = 0; h < D / 64; h++) *reinterpret_cast<uint4*>(dst + h * 16384 + lane * run * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_shared();
+                __syncwarp();
+              }
+              const bool look = half && partial(k, j);
+              const uint32_t bar = smem_u32(look ? &ct.look[slot] : &ct.full[slot]);
+              if (lane == 0) {
+                if (!look) mbar_arrive_n(bar, F::WORKERS - 1);
+                mbar_expect_tx(bar, bytes);
+              }
+              __syncwarp();
+              if (there) {
+#pragma unroll
+                for (int h = 0; h < D / 64; h++) tma_load_4d(base + F::RING_AT + slot * F::TILE + h * 16384 + lane * run * 128, map, bar, h * 64, at, kvh, pg);
+              }
+            }
           }
+        }
+      }
+      uses += 2u * (uint32_t)(k.B - k.A);
+      if (!next(ok)) break;
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------ workers
+    set_regs<false, 72>();
+    const int w = warp - 11;
+    constexpr int CH = E4M3 ? D / 16 : D / 8, IT = 8 * CH / 32 > 0 ? 8 * CH / 32 : 1;      // 16-byte pieces of a held row; of 8 rows, for each lane
+    constexpr int LAG = F::LAG;
+    const char* kbase = P.c.k + (long long)kvh * P.c.head_b;
+    const char* vbase = P.c.v + (long long)kvh * P.c.head_b;
+    uint32_t uses = 0, looks = 0;                                // looks: a bit for each slot, the phase of its barrier
+    // A step's 128 keys are 16 units of 8 rows, dealt out to the workers through all items. Lanes 0 .. 7 (and 8 .. 15 again, and so on) place a unit's rows.
+    struct Unit { long long off; uint32_t f; };
+    for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
+      const Walk k = walk(pair);
+      const int total = 2 * (k.B - k.A), units = total * 16;
+      auto place = [&](int e, bool scale) {                      // of unit e of all: item e / 16
+        Unit x = {-1, 0};
+        const int item = e >> 4, key = (k.A + (item >> 1)) * 128 + (e & 15) * 8 + (lane & 7);
+        int page, at;
+        if (e < units && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) {
+          x.off = (long long)page * P.c.page_b + (long long)at * P.c.row_b;
+          if (E4M3 && scale) x.f = 256u | __ldg((item & 1 ? P.c.vs : P.c.ks) + (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row);
         }
         return x;
       };
-      auto fetch = [&](uint4 (&v)[4], const Unit& x, const char* src, int x0) {      // pieces x0 .. of the unit
-        constexpr int N = IT < 4 ? IT : 4;
-        long long o[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = from_lane(x.off, ((x0 + i) * 32 + lane) / CH, P.wide);
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + lane % CH * 16) : make_uint4(0, 0, 0, 0);
+      auto odd_at = [&](int key) { atomicMin(&ct.odd_lo, key); atomicMax(&ct.odd_hi, min(k.hi - 1, key)); };
+      auto tile_free = [&](int item) {
+        const uint32_t n = uses + (uint32_t)item;
+        ok = wait_for(smem_u32(&ct.empty[n % F::NST]), ((n / F::NST) & 1) ^ 1);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
       };
-      auto put = [&](uint4 (&v)[4], uint32_t scale, unsigned char* dst, int j, int u, int x0, bool check) {     // check: values that some row must not meet
-        bool odd = false;
-        uint32_t f = 0;
-        if constexpr (E4M3) { f = scale_bits((int)scale); f |= f << 16; }
+      auto done_with = [&](int item) { attn_tc::warp_arrive(smem_u32(&ct.full[(uses + (uint32_t)item) % F::NST])); };
+      if constexpr (E4M3) {
+        // 8-bit rows, from their ring; where the copy engine does not bring them, by this warp's own copies, RS - 1 items ahead
+        auto gather = [&](int item) {
+          if (item < total) {
+            const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
+            ok = ok && wait_for(smem_u32(&ct.raw_empty[rs]), ((n / F::RS) & 1) ^ 1);       // the rows that this warp writes there are others than it read
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            for (int e = item * 16 + (w + 5 - item * 16 % 5) % 5; e < item * 16 + 16; e += 5) {
+              const Unit x = place(e, false);
+              if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][e & 15] = (uint8_t)vb; }
+              long long o[IT];
 #pragma unroll
-        for (int i = 0; i < (IT < 4 ? IT : 4); i++) {
-          const int idx = (x0 + i) * 32 + lane, row = u * 16 + idx / CH, q = idx % CH;
-          if constexpr (E4M3) {
-            uint32_t fr = __shfl_sync(0xffffffffu, f, idx / CH);
-            if (check && fr == 0x7fc07fc0u) { odd = true; fr = 0; }
-            *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * q)) = make_uint4(widen_lo(v[i].x, fr), widen_hi(v[i].x, fr), widen_lo(v[i].y, fr), widen_hi(v[i].y, fr));
-            *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * q + 1)) = make_uint4(widen_lo(v[i].z, fr), widen_hi(v[i].z, fr), widen_lo(v[i].w, fr), widen_hi(v[i].w, fr));
-          } else {
-            if (check && (odd_bits(v[i].x) || odd_bits(v[i].y) || odd_bits(v[i].z) || odd_bits(v[i].w))) {
-              odd = true;
-              v[i] = make_uint4(without_odd(v[i].x), without_odd(v[i].y), without_odd(v[i].z), without_odd(v[i].w));
+              for (int i = 0; i < IT; i++) o[i] = from_lane(x.off, (i * 32 + lane) / CH & 7, P.wide);
+#pragma unroll
+              for (int i = 0; i < IT; i++)
+                if (i * 32 + lane < 8 * CH)
+                  cp16(base + F::RAW_AT + rs * F::RAW + F::raw_at((e & 15) * 8 + (i * 32 + lane) / CH, lane % CH), (item & 1 ? vbase : kbase) + (o[i] >= 0 ? o[i] : 0) + lane % CH * 16, o[i] >= 0);
             }
-            *reinterpret_cast<uint4*>(dst + tile_at(row, q)) = v[i];
           }
-        }
-        if (odd) { atomicMin(&ct.odd_lo, j * 128 + u * 16); atomicMax(&ct.odd_hi, min(k.hi - 1, j * 128 + u * 16 + 15)); }
-      };
-      int u = w;                                                 // the warp's units of the step: u, and u + 6 if there is one
-      Unit now[2] = {look(k.A, u), look(k.A, u + 6)};
-      uint4 v[4];
-      if constexpr (E4M3) fetch(v, now[0], kbase, 0);
-      int i = 0;
-      auto landed = [&](int item) {                              // of this warp's rows; the products may read a tile when all six have said so
-        if (item >= 0 && item < total) attn_tc::warp_arrive(smem_u32(&ct.full[(uses + (uint32_t)item) % F::NST]));
-      };
-      for (int j = k.A; j < k.B && ok; j++) {
-        const int un = (u + 4) % F::LOADERS;
-        const Unit then[2] = {look(j + 1, un), look(j + 1, un + 6)};
-        const bool part = partial(k, j);
+          cp_commit();
+        };
+        if (!P.run) for (int i = 0; i < F::RS - 1; i++) gather(i);
+        int e = (w + 5 - 0) % 5;
+        Unit x = place(e, true);
+        for (int item = 0; item < total && ok; item++) {
+          const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
+          const int j = k.A + (item >> 1);
+          const bool check = (item & 1) && partial(k, j);
+          if (P.run) ok = wait_for(smem_u32(&ct.raw_full[rs]), (n / F::RS) & 1);
+          else { gather(item + F::RS - 1); cp_wait<F::RS - 1>(); __syncwarp(); }
+          if (!__all_sync(0xffffffffu, ok) || !tile_free(item)) { ok = false; break; }
+          const unsigned char* src = smem + F::RAW_AT + rs * F::RAW;
+          unsigned char* dst = smem + F::RING_AT + n % F::NST * F::TILE;
+#pragma unroll 1
+          for (; e < item * 16 + 16; e += 5) {
+            const Unit y = place(e + 5, true);                   // the next unit's scales are on their way
+            uint32_t f = x.f ? scale_bits((int)(x.f & 255)) : 0u;      // rows that are not there become zeros
+            f |= f << 16;
+            if (check && f == 0x7fc07fc0u) { odd_at(j * 128 + (e & 15) * 8 + (lane & 7)); f = 0; }
 #pragma unroll
-        for (int half = 0; half < 2; half++, i++) {
-          const uint32_t n = uses + (uint32_t)i, slot = n % F::NST;
-          const char* src = half ? vbase : kbase;
-          ok = wait_for(smem_u32(&ct.empty[slot]), ((n / F::NST) & 1) ^ 1);
+            for (int i = 0; i < IT; i++) {
+              const int row = (i * 32 + lane) / CH & 7, q = lane % CH, r = (e & 15) * 8 + row;
+              const uint32_t fr = __shfl_sync(0xffffffffu, f, row);
+              if (i * 32 + lane < 8 * CH) {
+                const uint4 v = *reinterpret_cast<const uint4*>(src + F::raw_at(r, q));
+                *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * q)) = make_uint4(widen_lo(v.x, fr), widen_hi(v.x, fr), widen_lo(v.y, fr), widen_hi(v.y, fr));
+                *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * q + 1)) = make_uint4(widen_lo(v.z, fr), widen_hi(v.z, fr), widen_lo(v.w, fr), widen_hi(v.w, fr));
+              }
+            }
+            x = y;
+          }
+          done_with(item);
+          attn_tc::warp_arrive(smem_u32(&ct.raw_empty[rs]));
+        }
+      } else if (P.run) {
+        // look through the values of steps that not every row sees whole
+        for (int j = k.A; j < k.B && ok; j++) {
+          if (!partial(k, j)) continue;
+          const int item = 2 * (j - k.A) + 1;
+          const uint32_t slot = (uses + (uint32_t)item) % F::NST;
+          ok = wait_for(smem_u32(&ct.look[slot]), looks >> slot & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const int uu = u + 6 * x;
-            if (uu >= 8) break;
-            if (half == 0) {
-              const uint32_t vb = __ballot_sync(0xffffffffu, now[x].off >= 0);
-              if (lane == 0) ct.valid[j % F::NV][uu] = (uint16_t)vb;
+          looks ^= 1u << slot;
+          unsigned char* tile = smem + F::RING_AT + slot * F::TILE;
+#pragma unroll 4
+          for (int c = w * 32 + lane; c < F::TILE / 16; c += F::WORKERS * 32) {
+            const uint4 u = *reinterpret_cast<const uint4*>(tile + c * 16);
+            if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
+              *reinterpret_cast<uint4*>(tile + c * 16) = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
+              odd_at(j * 128 + (c * 16 & 16383) / 128);
             }
-            if constexpr (E4M3) {                                // the next unit's bytes are on their way while this one's are widened
-              uint4 vn[4];
-              if (x == 0 && u < 2) fetch(vn, now[1], src, 0);
-              else if (half == 0) fetch(vn, now[0], vbase, 0);
-              else fetch(vn, then[0], kbase, 0);
-              put(v, half ? now[x].fv : now[x].fk, dst, j, uu, 0, half && part);
-#pragma unroll
-              for (int y = 0; y < 4; y++) v[y] = vn[y];
-            } else if (part) {
-#pragma unroll 1
-              for (int x0 = 0; x0 < IT; x0 += 4) { fetch(v, now[x], src, x0); put(v, 0, dst, j, uu, x0, half); }
-            } else {
-              const uint32_t dst_s = smem_u32(dst);
+          }
+          done_with(item);
+        }
+      } else {
+        // gather
+        for (int item = 0; item < total + LAG && ok; item++) {
+          if (item < total) {
+            if (!tile_free(item)) break;
+            const int j = k.A + (item >> 1);
+            const char* src = item & 1 ? vbase : kbase;
+            const uint32_t slot = (uses + (uint32_t)item) % F::NST;
+            unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
+            for (int e = item * 16 + (w + 5 - item * 16 % 5) % 5; e < item * 16 + 16; e += 5) {
+              const Unit x = place(e, false);
+              if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[j % F::NV][e & 15] = (uint8_t)vb; }
               long long o[IT];                                   // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-              for (int y = 0; y < IT; y++) o[y] = from_lane(now[x].off, (y * 32 + lane) / CH, P.wide);
+              for (int i = 0; i < IT; i++) o[i] = from_lane(x.off, (i * 32 + lane) / CH, P.wide);
+              const bool check = (item & 1) && partial(k, j);
 #pragma unroll
-              for (int y = 0; y < IT; y++) {
-                const int row = (y * 32 + lane) / CH, q = lane % CH;
-                cp16(dst_s + tile_at(uu * 16 + row, q), o[y] >= 0 ? src + o[y] + q * 16 : src, o[y] >= 0);
+              for (int i = 0; i < IT; i++) {
+                const int row = (e & 15) * 8 + (i * 32 + lane) / CH, q = lane % CH;
+                if (!check) cp16(smem_u32(dst) + tile_at(row, q), src + (o[i] >= 0 ? o[i] : 0) + q * 16, o[i] >= 0);
+                else {
+                  uint4 u = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + q * 16) : make_uint4(0, 0, 0, 0);
+                  if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
+                    odd_at(j * 128 + row);
+                    u = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
+                  }
+                  *reinterpret_cast<uint4*>(dst + tile_at(row, q)) = u;
+                }
               }
             }
           }
           cp_commit();
           cp_wait<LAG>();
-          landed(i - LAG);
+          if (item >= LAG) done_with(item - LAG);
         }
-        u = un; now[0] = then[0]; now[1] = then[1];
       }
       cp_wait<0>();
-      if (ok) {
-#pragma unroll
-        for (int y = LAG; y > 0; y--) landed(total - y);
-      }
       uses += (uint32_t)total;
       if (!next(ok)) break;
     }

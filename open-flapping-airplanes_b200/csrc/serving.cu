@@ -152,7 +152,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   if (p.many) {
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, 512, paged::Tc<D>::SMEM, P);
+    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, 512, paged::Tc<D, E4M3>::SMEM, P);
   } else {
     if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
     e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(lc, 128, paged::Few<D, E4M3, 1>::SMEM, P) : launch<paged::few_rows_kernel<D, E4M3, 2>>(lc, 128, paged::Few<D, E4M3, 2>::SMEM, P);
