@@ -3,9 +3,11 @@
 // The rows of a key/value head (new tokens x the query heads that share it) are taken 256 at a time by a block of 16 warps, two tiles of 128 rows that walk the
 // same keys 128 at a time, half a step apart: while the softmax warps of one tile work, the tensor pipe works for the other.
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row (= tensor-memory lane): reads its 128 scores, keeps maximum and sum, writes the probabilities
-//                    back over them as bf16, the A operand of the second product
-//   warps 8, 9       one thread each issues a tile's products: S = Q K_j^T, then O += P V_j. Two threads because one issues a tcgen05.mma only every
-//                    ~96 clocks, and a 128 x 128 x 16 product takes 64
+//                    back over the second half of them as bf16, the A operand of the second product
+//   warps 8, 9       one thread each issues a tile's products, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
+//                    soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores
+//                    (4,096 tokens over 16,384 keys, heads of 128: 854 us with whole steps in turns, HALVES_US so; steps of 64 keys with two buffers of scores waited least but
+//                    their fixed cost, 420 clocks, came twice: 928)
 //   warp 10          asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
 //                    (128-byte swizzle), 8-bit rows into a ring of their own
 //   warps 11-15      widen 8-bit rows from there into the tiles, once for the 256 rows; look at values that some row must not meet; and gather the rows of pages that are no
@@ -39,7 +41,7 @@ template <int D, bool E4M3> struct Tc {
   }
 };
 struct TcCtrl {
-  u64 q_full, full[8], empty[8], s_full[2], p_full[2], o_full[2];
+  u64 q_full, full[8], empty[8], sa_full[2], s_full[2], s_free[2], pa_full[2], p_full[2], o_full[2];      // a: the first half
   u64 look[8];                                                  // bf16: a tile that the workers look through has landed
   u64 raw_full[4], raw_empty[4];
   uint32_t tmem, dead;
@@ -86,7 +88,10 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     mbar_init(smem_u32(&ct.q_full), 8);
     for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::WORKERS); mbar_init(smem_u32(&ct.empty[s]), 2); mbar_init(smem_u32(&ct.look[s]), 1); }
     for (int s = 0; s < 4; s++) { mbar_init(smem_u32(&ct.raw_full[s]), 1); mbar_init(smem_u32(&ct.raw_empty[s]), F::WORKERS); }
-    for (int i = 0; i < 2; i++) { mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.p_full[i]), 4); mbar_init(smem_u32(&ct.o_full[i]), 1); }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&ct.sa_full[i]), 1); mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.s_free[i]), 4);
+      mbar_init(smem_u32(&ct.pa_full[i]), 4); mbar_init(smem_u32(&ct.p_full[i]), 4); mbar_init(smem_u32(&ct.o_full[i]), 1);
+    }
     ct.odd_lo = 0x7fffffff; ct.odd_hi = -1; ct.dead = 0;
     mbar_fence_init();
   }
@@ -162,15 +167,23 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
       const int n = k.b[tile] - k.a[tile];
       for (int c = 0; c < n; c++) {
         const int j = k.a[tile] + c, k0 = j * 128;
-        ok = wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
+        uint32_t s[4][32];
+        ok = wait_for(smem_u32(&ct.sa_full[tile]), (done + c) & 1);
+        tc_fence_after();
+        if (__all_sync(0xffffffffu, ok)) {
+          attn_tc::tmem_ld32_nw(ts, s[0]);
+          attn_tc::tmem_ld32_nw(ts + 32, s[1]);
+        }
+        ok = ok && wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[4][32];
-        const uint4 vw = *reinterpret_cast<const uint4*>(ct.valid[j % F::NV]);
-#pragma unroll
-        for (int q = 0; q < 4; q++) attn_tc::tmem_ld32_nw(ts + q * 32, s[q]);
+        attn_tc::tmem_ld32_nw(ts + 64, s[2]);
+        attn_tc::tmem_ld32_nw(ts + 96, s[3]);
         attn_tc::tmem_ld_wait();
+        tc_fence_before();
+        attn_tc::warp_arrive(smem_u32(&ct.s_free[tile]));        // the first half of the next scores may overwrite these
+        const uint4 vw = *reinterpret_cast<const uint4*>(ct.valid[j % F::NV]);
         if (partial(k, j) || (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu) {
           const int x1 = P.causal ? pos - k0 : 127, x0 = P.window ? pos - P.window + 1 - k0 : 0;       // of the step's keys the row sees x0 .. x1
 #pragma unroll
@@ -216,6 +229,11 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
             pk[x >> 1] = pack2f(p0, p1);                         // rounded to bf16 for the product; the sum is taken before
           }
           attn_tc::tmem_st16(ts + 64 + q * 16, pk);
+          if (q == 1) {
+            attn_tc::tmem_st_wait();
+            tc_fence_before();
+            attn_tc::warp_arrive(smem_u32(&ct.pa_full[tile]));
+          }
         }
         attn_tc::tmem_st_wait();
         tc_fence_before();
@@ -288,48 +306,64 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
       const int ka = k.a[tile], kb = k.b[tile];
       const uint32_t ts = tmem + tile * 128, to = tmem + 256 + tile * D;
       const u64 dq = umma_smem_desc(base + F::Q_AT + tile * F::TILE, 16, 1024);
-      constexpr uint32_t I_S = umma_idesc(false, false, 128, 128), I_O = umma_idesc(false, true, 128, D);
+      constexpr uint32_t I_S = umma_idesc(false, false, 128, 64), I_O = umma_idesc(false, true, 128, D);
       uint32_t c = 0;
       auto slot_of = [&](int item) { return (uses + (uint32_t)item) % F::NST; };
       auto filled = [&](int item) { return wait_for(smem_u32(&ct.full[slot_of(item)]), ((uses + (uint32_t)item) / F::NST) & 1); };
-      auto scores = [&](int j) {                                 // S = Q K_j^T, over the probabilities of the step before: one thread's products run in their order
+      auto scores = [&](int j, int half) {                       // S = Q K_j^T for 64 keys; one thread's products run in their order
         const uint32_t slot = slot_of(2 * (j - k.A));
-        if (j < ka || j >= kb) { if (leader) mbar_arrive(smem_u32(&ct.empty[slot])); return; }
-        const u64 dk = umma_smem_desc(base + F::RING_AT + slot * F::TILE, 16, 1024);
+        const u64 dk = umma_smem_desc(base + F::RING_AT + slot * F::TILE + half * 8192, 16, 1024);
         if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; kk++) umma_bf16(ts, dq + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
-          umma_commit(smem_u32(&ct.s_full[tile]));
-          umma_commit(smem_u32(&ct.empty[slot]));
+          for (int kk = 0; kk < D / 16; kk++)
+            umma_bf16(ts + half * 64, dq + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
+          umma_commit(smem_u32(half ? &ct.s_full[tile] : &ct.sa_full[tile]));
+          if (half) umma_commit(smem_u32(&ct.empty[slot]));
         }
       };
+      auto pass = [&](int item) {                                // a tile that this issuer has no use for
+        if (!filled(item)) return false;
+        if (leader) mbar_arrive(smem_u32(&ct.empty[slot_of(item)]));
+        return true;
+      };
       ok = wait_for(smem_u32(&ct.q_full), round & 1);
-      if (k.A < k.B) {
-        ok = ok && filled(0);
-        fence_async_shared();
-        if (ok) scores(k.A);
+      for (int item = 0; item < 2 * ((kb > ka ? ka : k.B) - k.A) && ok; item++) ok = pass(item);
+      if (ka < kb && ok) {
+        ok = filled(2 * (ka - k.A));
+        fence_async_shared();                                    // what the workers wrote, before it is read by the products
+        if (ok) { scores(ka, 0); scores(ka, 1); }
       }
-      for (int j = k.A; j < k.B && ok; j++) {
+      for (int j = ka; j < kb && ok; j++, c++) {
         const int item = 2 * (j - k.A) + 1;
-        ok = filled(item) && (j + 1 == k.B || filled(item + 1));
+        ok = filled(item) && (j + 1 == kb || filled(item + 1));
         if (!ok) break;
-        fence_async_shared();                                    // what the loaders wrote, before it is read by the products
+        fence_async_shared();
+        if (j + 1 < kb) {
+          ok = wait_for(smem_u32(&ct.s_free[tile]), (done + c) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          scores(j + 1, 0);
+        }
         const uint32_t slot = slot_of(item);
-        if (j >= ka && j < kb) {                                 // O += P V_j
-          const u64 dv = umma_smem_desc(base + F::RING_AT + slot * F::TILE, 16384, 1024);
-          ok = wait_for(smem_u32(&ct.p_full[tile]), (done + c) & 1);
+        const u64 dv = umma_smem_desc(base + F::RING_AT + slot * F::TILE, 16384, 1024);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {                   // O += P V_j
+          ok = ok && wait_for(smem_u32(half ? &ct.p_full[tile] : &ct.pa_full[tile]), (done + c) & 1);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++) umma_bf16_ts(to, ts + 64 + kk * 8, dv + kk * 2048 / 16, I_O, (c > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(smem_u32(&ct.o_full[tile]));
-            umma_commit(smem_u32(&ct.empty[slot]));
+            for (int kk = half * 4; kk < half * 4 + 4; kk++) umma_bf16_ts(to, ts + 64 + kk * 8, dv + kk * 2048 / 16, I_O, (c > 0 || kk > 0) ? 1u : 0u);
           }
-          c++;
-        } else if (leader) mbar_arrive(smem_u32(&ct.empty[slot]));
-        if (j + 1 < k.B) scores(j + 1);
+        }
+        if (!ok) break;
+        if (leader) {
+          umma_commit(smem_u32(&ct.o_full[tile]));
+          umma_commit(smem_u32(&ct.empty[slot]));
+        }
+        if (j + 1 < kb) scores(j + 1, 1);
       }
+      if (kb > ka) for (int item = 2 * (kb - k.A); item < 2 * (k.B - k.A) && ok; item++) ok = pass(item);
       uses += 2u * (uint32_t)(k.B - k.A); done += (uint32_t)(kb - ka); round++;
       if (!next(ok)) break;
     }
