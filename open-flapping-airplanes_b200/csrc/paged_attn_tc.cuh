@@ -2,7 +2,7 @@
 //
 // The rows of a key/value head (new tokens x the query heads that share it) are taken 256 at a time by a block of 16 warps, two tiles of 128 rows that walk the
 // same keys 128 at a time, half a step apart: while the softmax warps of one tile work, the tensor pipe works for the other.
-//   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row (= tensor-memory lane): reads its 128 scores, keeps maximum and sum, writes the probabilities
+//   softmax, four warps a tile:  of tile 0 and 1, a thread per row (= tensor-memory lane): reads its 128 scores, keeps maximum and sum, writes the probabilities
 //                    back over the second half of them as bf16, the A operand of the second product
 //   warps 8, 9       one thread each issues a tile's products, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
 //                    soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores
@@ -28,14 +28,17 @@ namespace ofa {
 namespace paged {
 
 template <int D, bool E4M3> struct Tc {
+  static constexpr int NT = D == 64 ? 1 : 2, BLOCKS = D == 64 ? 2 : 1;      // tiles of 128 rows a block, blocks an SM
+  static constexpr int WORKERS = NT == 1 ? 2 : 5, WARPS = 5 * NT + 1 + WORKERS, THREADS = 32 * WARPS;
+  static constexpr int SOFT_REGS = 184, REST_REGS = 72;         // of a softmax thread, of another: together twice the launch's 128
+  static constexpr int TMEM = NT * 256, O_AT = NT * 128;        // columns; S of a tile at tile * 128, O behind them
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
-  static constexpr int NST = D == 64 ? 8 : E4M3 ? 3 : 4;        // ring of K and V tiles
-  static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 4 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
-  static constexpr int LAG = D == 128 ? 1 : 2;                  // gathered tiles whose copies may be in flight when the next is begun
+  static constexpr int NST = E4M3 && D == 128 ? 3 : 4;          // ring of K and V tiles
+  static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 2 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
+  static constexpr int LAG = 1;                                 // gathered tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
-  static constexpr int Q_AT = 0, RING_AT = 2 * TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
+  static constexpr int Q_AT = 0, RING_AT = NT * TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
   static constexpr int SMEM = CTRL_AT + 640 + 1024;             // 1,024 for the alignment of the swizzle's atoms
-  static constexpr int WORKERS = 5;
   static __device__ __forceinline__ uint32_t raw_at(int row, int chunk) {      // a 16-byte piece of an 8-bit row
     return D == 64 ? (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)) : (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
   }
@@ -69,8 +72,9 @@ __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) { return (uint32_t)((chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
 
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant__ AttnArgs P) {
+__global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) many_rows_kernel(const __grid_constant__ AttnArgs P) {
   using F = Tc<D, E4M3>;
+  constexpr int NT = F::NT, WK = F::WORKERS;
   extern __shared__ __align__(16) unsigned char raw[];
   unsigned char* smem = raw + (-(int)smem_u32(raw) & 1023);      // by an offset: through an integer the pointer would lose its address space
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
@@ -82,32 +86,32 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);
-  const int npair = (ch.n * group + 255) / 256;
+  const int npair = (ch.n * group + NT * 128 - 1) / (NT * 128);      // pairs of tiles, or tiles
   if (turn >= npair) return;
   if (tid == 0) {
-    mbar_init(smem_u32(&ct.q_full), 8);
-    for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::WORKERS); mbar_init(smem_u32(&ct.empty[s]), 2); mbar_init(smem_u32(&ct.look[s]), 1); }
+    mbar_init(smem_u32(&ct.q_full), 4 * NT);
+    for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::WORKERS); mbar_init(smem_u32(&ct.empty[s]), NT); mbar_init(smem_u32(&ct.look[s]), 1); }
     for (int s = 0; s < 4; s++) { mbar_init(smem_u32(&ct.raw_full[s]), 1); mbar_init(smem_u32(&ct.raw_empty[s]), F::WORKERS); }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < NT; i++) {
       mbar_init(smem_u32(&ct.sa_full[i]), 1); mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.s_free[i]), 4);
       mbar_init(smem_u32(&ct.pa_full[i]), 4); mbar_init(smem_u32(&ct.p_full[i]), 4); mbar_init(smem_u32(&ct.o_full[i]), 1);
     }
     ct.odd_lo = 0x7fffffff; ct.odd_hi = -1; ct.dead = 0;
     mbar_fence_init();
   }
-  if (warp == 8) tmem_alloc(smem_u32(&ct.tmem), 512);
+  if (warp == 4 * NT) tmem_alloc(smem_u32(&ct.tmem), F::TMEM);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ct.tmem;
   // Steps of 128 keys that the block walks for a pair of tiles, and those [a, b) that each tile takes part in
-  struct Walk { int a[2], b[2], lo, hi, A, B, p_low, p_high; };
+  struct Walk { int a[NT], b[NT], lo, hi, A, B, p_low, p_high; };
   auto walk = [&](int pair) {
     Walk k;
     k.lo = 0x7fffffff; k.hi = 0; k.p_low = k.p_high = 0;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int r0 = (pair * 2 + i) * 128;
+    for (int i = 0; i < NT; i++) {
+      const int r0 = (pair * NT + i) * 128;
       if (r0 >= ch.n * group) { k.a[i] = k.b[i] = 0; continue; }
       const int pmin = ch.p0 + (int)P.group.quot(r0), pmax = ch.p0 + min(ch.n - 1, (int)P.group.quot(r0 + 127));
       const int h = min(cap, P.causal ? pmax + 1 : ch.len), l = P.window ? max(0, pmin - P.window + 1) : 0;
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     const int first = k.lo / 128, nst = k.hi > k.lo ? (k.hi + 127) / 128 - first : 0;
     k.A = first + (int)((long long)nst * split / P.nsplit); k.B = first + (int)((long long)nst * (split + 1) / P.nsplit);
 #pragma unroll
-    for (int i = 0; i < 2; i++) { k.a[i] = max(k.a[i], k.A); k.b[i] = max(k.a[i], min(k.b[i], k.B)); }
+    for (int i = 0; i < NT; i++) { k.a[i] = max(k.a[i], k.A); k.b[i] = max(k.a[i], min(k.b[i], k.B)); }
     return k;
   };
   // a step that not every row of the block sees whole
@@ -139,14 +143,14 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
   };
   bool ok = true;
 
-  if (warp < 8) {
+  if (warp < 4 * NT) {
     // ------------------------------------------------------------------------------------------ softmax: a thread a row
-    set_regs<true, 184>();
+    set_regs<true, F::SOFT_REGS>();
     const int tile = warp >> 2, e = warp & 3, r = e * 32 + lane;
     uint32_t done = 0;                                           // steps of this tile so far: phases of its barriers
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
-      const int rr = (pair * 2 + tile) * 128 + r, t = (int)P.group.quot(rr);
+      const int rr = (pair * NT + tile) * 128 + r, t = (int)P.group.quot(rr);
       const bool on = t < ch.n;
       const int pos = ch.p0 + (on ? t : ch.n - 1), head = kvh * group + rr - t * group;
       {                                                          // the row of Q, its sign turned if scores are scaled by a negative number
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
         fence_async_shared();
         attn_tc::warp_arrive(smem_u32(&ct.q_full));
       }
-      const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + 256 + tile * D;
+      const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + F::O_AT + tile * D;
       float m = -INFINITY, l = 0.f;
       const int n = k.b[tile] - k.a[tile];
       for (int c = 0; c < n; c++) {
@@ -293,10 +297,10 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
       done += (uint32_t)n;
       if (!next(ok)) break;
     }
-  } else if (warp < 10) {
+  } else if (warp < 5 * NT) {
     // ------------------------------------------------------------------------------------------ products
-    set_regs<false, 72>();
-    const int tile = warp - 8;
+    set_regs<false, F::REST_REGS>();
+    const int tile = warp - 4 * NT;
     uint32_t uses = 0, done = 0, round = 0;                      // items through the ring, steps of the tile
     // The whole warp walks, so that descriptors and addresses stay uniform, and one elected thread issues. What the loaders wrote is ordered before
     // the products' reads by a fence here: in the loaders it would wait for every copy they have in flight.
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
       const int ka = k.a[tile], kb = k.b[tile];
-      const uint32_t ts = tmem + tile * 128, to = tmem + 256 + tile * D;
+      const uint32_t ts = tmem + tile * 128, to = tmem + F::O_AT + tile * D;
       const u64 dq = umma_smem_desc(base + F::Q_AT + tile * F::TILE, 16, 1024);
       constexpr uint32_t I_S = umma_idesc(false, false, 128, 64), I_O = umma_idesc(false, true, 128, D);
       uint32_t c = 0;
@@ -367,9 +371,9 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
       uses += 2u * (uint32_t)(k.B - k.A); done += (uint32_t)(kb - ka); round++;
       if (!next(ok)) break;
     }
-  } else if (warp == 10) {
+  } else if (warp == 5 * NT) {
     // ------------------------------------------------------------------------------------------ copies
-    set_regs<false, 72>();
+    set_regs<false, F::REST_REGS>();
     const int run = P.run ? P.run : 8, nrun = 128 / run;         // a lane for each run of a step's keys
     uint32_t uses = 0;
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
@@ -431,8 +435,8 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
     }
   } else {
     // ------------------------------------------------------------------------------------------ workers
-    set_regs<false, 72>();
-    const int w = warp - 11;
+    set_regs<false, F::REST_REGS>();
+    const int w = warp - 5 * NT - 1;
     constexpr int CH = E4M3 ? D / 16 : D / 8, IT = 8 * CH / 32 > 0 ? 8 * CH / 32 : 1;      // 16-byte pieces of a held row; of 8 rows, for each lane
     constexpr int LAG = F::LAG;
     const char* kbase = P.c.k + (long long)kvh * P.c.head_b;
@@ -469,7 +473,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
             ok = ok && wait_for(smem_u32(&ct.raw_empty[rs]), ((n / F::RS) & 1) ^ 1);       // the rows that this warp writes there are others than it read
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
-            for (int e = item * 16 + (w + 5 - item * 16 % 5) % 5; e < item * 16 + 16; e += 5) {
+            for (int e = item * 16 + (w + WK - item * 16 % WK) % WK; e < item * 16 + 16; e += WK) {
               const Unit x = place(e, false);
               if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][e & 15] = (uint8_t)vb; }
               long long o[IT];
@@ -484,7 +488,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
           cp_commit();
         };
         if (!P.run) for (int i = 0; i < F::RS - 1; i++) gather(i);
-        int e = (w + 5 - 0) % 5;
+        int e = w;
         Unit x = place(e, true);
         for (int item = 0; item < total && ok; item++) {
           const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
@@ -496,8 +500,8 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
           const unsigned char* src = smem + F::RAW_AT + rs * F::RAW;
           unsigned char* dst = smem + F::RING_AT + n % F::NST * F::TILE;
 #pragma unroll 1
-          for (; e < item * 16 + 16; e += 5) {
-            const Unit y = place(e + 5, true);                   // the next unit's scales are on their way
+          for (; e < item * 16 + 16; e += WK) {
+            const Unit y = place(e + WK, true);                   // the next unit's scales are on their way
             uint32_t f = x.f ? scale_bits((int)(x.f & 255)) : 0u;      // rows that are not there become zeros
             f |= f << 16;
             if (check && f == 0x7fc07fc0u) { odd_at(j * 128 + (e & 15) * 8 + (lane & 7)); f = 0; }
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
             const char* src = item & 1 ? vbase : kbase;
             const uint32_t slot = (uses + (uint32_t)item) % F::NST;
             unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
-            for (int e = item * 16 + (w + 5 - item * 16 % 5) % 5; e < item * 16 + 16; e += 5) {
+            for (int e = item * 16 + (w + WK - item * 16 % WK) % WK; e < item * 16 + 16; e += WK) {
               const Unit x = place(e, false);
               if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[j % F::NV][e & 15] = (uint8_t)vb; }
               long long o[IT];                                   // all the exchanges before the first copy: in turns each copy would wait for its own
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(512, 1) many_rows_kernel(const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 4 * NT) tmem_dealloc(tmem, F::TMEM);
 }
 
 }  // namespace paged

@@ -97,13 +97,14 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   const long long group = n_heads / c->n_kv_heads;
   const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
   p.many = rows > 32;
-  p.rows = p.many ? 256 : rows > 8 ? 16 : 8;
+  const int tiles_of = c->head_dim == 64 ? 1 : 2;      // tiles of 128 rows a block of the tensor-core kernel, of which an SM holds 2 / tiles_of
+  p.rows = p.many ? 128 * tiles_of : rows > 8 ? 16 : 8;
   long long tiles = (rows + p.rows - 1) / p.rows;
   if (tiles > 4096) tiles = 4096;
   if (tiles < 1) tiles = 1;
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
   const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles;
-  long long ns = (p.many ? 148 : 3 * 148) / blocks;
+  long long ns = (p.many ? 148 * 2 / tiles_of : 3 * 148) / blocks;
   if (ns > kv / (p.many ? 512 : 256)) ns = kv / (p.many ? 512 : 256);
   if (ns > paged::MAX_SPLIT) ns = paged::MAX_SPLIT;
   p.cluster = !p.many && ns > 1 && ns < 16;
@@ -152,7 +153,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   if (p.many) {
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, 512, paged::Tc<D, E4M3>::SMEM, P);
+    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, paged::Tc<D, E4M3>::THREADS, paged::Tc<D, E4M3>::SMEM, P);
   } else {
     if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
     e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(lc, 128, paged::Few<D, E4M3, 1>::SMEM, P) : launch<paged::few_rows_kernel<D, E4M3, 2>>(lc, 128, paged::Few<D, E4M3, 2>::SMEM, P);
