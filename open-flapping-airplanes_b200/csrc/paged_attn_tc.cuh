@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  // the last pairs of tiles of a sequence have the most keys: they start first
-  const int split = (int)blockIdx.x % P.nsplit, seq = (int)blockIdx.x / P.nsplit % P.b.n_seqs, kvh = blockIdx.y;
-  const int turn = (int)blockIdx.x / P.nsplit / P.b.n_seqs;
+  // the last tiles of all sequences and heads, which have the most keys, start first
+  const int split = (int)blockIdx.x % P.nsplit, kvh = (int)blockIdx.x / P.nsplit % P.n_kv_heads, seq = (int)blockIdx.x / P.nsplit / P.n_kv_heads % P.b.n_seqs;
+  const int turn = (int)blockIdx.x / P.nsplit / P.n_kv_heads / P.b.n_seqs;
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);
@@ -153,15 +153,21 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
       const int rr = (pair * NT + tile) * 128 + r, t = (int)P.group.quot(rr);
       const bool on = t < ch.n;
       const int pos = ch.p0 + (on ? t : ch.n - 1), head = kvh * group + rr - t * group;
-      {                                                          // the row of Q, its sign turned if scores are scaled by a negative number
+      unsigned char* qt = smem + F::Q_AT + tile * F::TILE;
+      constexpr int CQ = D / 8;                                  // 16-byte pieces of a row
+      {                                                          // the warp's 32 rows of Q, whole rows side by side, their sign turned if scores are scaled by a negative number
         const uint32_t flip = P.flip ? 0x80008000u : 0u;
-        const bf16* src = P.q + (long long)(ch.s + t) * P.q_row + (long long)head * P.q_head;
-        unsigned char* dst = smem + F::Q_AT + tile * F::TILE;
+        const long long at = on ? (long long)(ch.s + t) * P.q_row + (long long)head * P.q_head : -1;
+        uint4 u[CQ];
 #pragma unroll
-        for (int q = 0; q < D / 8; q++) {
-          uint4 u = on ? reinterpret_cast<const uint4*>(src)[q] : make_uint4(0, 0, 0, 0);
-          u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
-          *reinterpret_cast<uint4*>(dst + tile_at(r, q)) = u;
+        for (int q = 0; q < CQ; q++) {
+          const long long o = __shfl_sync(0xffffffffu, at, (q * 32 + lane) / CQ);
+          u[q] = o >= 0 ? *reinterpret_cast<const uint4*>(P.q + o + lane % CQ * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < CQ; q++) {
+          u[q].x ^= flip; u[q].y ^= flip; u[q].z ^= flip; u[q].w ^= flip;
+          *reinterpret_cast<uint4*>(qt + tile_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ)) = u[q];
         }
         fence_async_shared();
         attn_tc::warp_arrive(smem_u32(&ct.q_full));
@@ -254,7 +260,6 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         const int olo = *reinterpret_cast<volatile int*>(&ct.odd_lo), ohi = *reinterpret_cast<volatile int*>(&ct.odd_hi);
         const long long g = (long long)(ch.s + t) * P.n_heads + head;
         const float inv = P.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head;
         float* part = P.part + (g * P.nsplit + split) * D;
 #pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
@@ -277,17 +282,26 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
               }
             }
           }
-          if (on && P.nsplit == 1) {
+          if (P.nsplit == 1) {                                   // through the tile of Q, which is not needed any more, so that rows leave whole
 #pragma unroll
             for (int x = 0; x < 32; x += 8) {
               float f[8];
 #pragma unroll
               for (int y = 0; y < 8; y++) f[y] = __uint_as_float(o[x + y]) * inv;
-              *reinterpret_cast<uint4*>(dst + q * 32 + x) = pack8(f);
+              *reinterpret_cast<uint4*>(qt + tile_at(r, (q * 32 + x) / 8)) = pack8(f);
             }
           } else if (on) {
 #pragma unroll
             for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + q * 32 + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+          }
+        }
+        if (P.nsplit == 1) {
+          __syncwarp();
+          const long long at = on ? (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head : -1;
+#pragma unroll
+          for (int q = 0; q < CQ; q++) {
+            const long long d = __shfl_sync(0xffffffffu, at, (q * 32 + lane) / CQ);
+            if (d >= 0) *reinterpret_cast<uint4*>(P.out + d + lane % CQ * 8) = *reinterpret_cast<const uint4*>(qt + tile_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ));
           }
         }
         if (on && P.nsplit > 1) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(m, l);

@@ -151,6 +151,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   lc.gridDim = dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads); lc.stream = s; lc.attrs = &at;
   cudaError_t e;
   if (p.many) {
+    lc.gridDim = dim3(lc.gridDim.x * lc.gridDim.y);             // heads among the tiles, for the order in which blocks start
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
     e = launch<paged::many_rows_kernel<D, E4M3>>(lc, paged::Tc<D, E4M3>::THREADS, paged::Tc<D, E4M3>::SMEM, P);
@@ -207,7 +208,7 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   const Plan p = plan(cache, batch, a->n_rows, a->n_heads);
   if (p.bytes && (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)))
     return fail(OFA_BAD_ARGUMENT, "workspace of %zu bytes on a 16-byte boundary needed, %zu given", p.bytes, a->workspace ? a->workspace_bytes : 0);
-  if ((long long)batch->n_seqs * p.tiles * p.nsplit > 0x7fffffffll) return fail(OFA_BAD_ARGUMENT, "%d sequences are too many for one call", batch->n_seqs);
+  if ((long long)batch->n_seqs * p.tiles * p.nsplit * (p.many ? cache->n_kv_heads : 1) > 0x7fffffffll) return fail(OFA_BAD_ARGUMENT, "%d sequences are too many for one call", batch->n_seqs);
   P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
   P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
