@@ -456,20 +456,24 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
     const char* kbase = P.c.k + (long long)kvh * P.c.head_b;
     const char* vbase = P.c.v + (long long)kvh * P.c.head_b;
     uint32_t uses = 0, looks = 0;                                // looks: a bit for each slot, the phase of its barrier
-    // A step's 128 keys are 16 units of 8 rows, dealt out to the workers through all items. Lanes 0 .. 7 (and 8 .. 15 again, and so on) place a unit's rows.
-    struct Unit { long long off; uint32_t f; };
+    // A span's 128 keys are 16 units of 8 rows, dealt out to the workers through all items: unit e of all is e % 16 of item e / 16 and the work of worker e % WORKERS. A
+    // lane places one row, up to four units of an item at once: its page is asked for two items ahead, its scale one.
+    constexpr int UNITS = (16 + WK - 1) / WK, GROUPS = (UNITS + 3) / 4;
+    struct Row { int page, at; };
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
-      const int total = 2 * (k.B - k.A), units = total * 16;
-      auto place = [&](int e, bool scale) {                      // of unit e of all: item e / 16
-        Unit x = {-1, 0};
-        const int item = e >> 4, key = (k.A + (item >> 1)) * 128 + (e & 15) * 8 + (lane & 7);
+      const int total = 2 * (k.B - k.A);
+      auto unit0 = [&](int item) { return (w + WK - item * 16 % WK) % WK; };               // the first unit of this worker
+      auto row_of = [&](int item, int gr) {                                                // this lane's row of its unit number gr * 4 + lane / 8
+        const int u = unit0(item) + (gr * 4 + (lane >> 3)) * WK, key = (k.A + (item >> 1)) * 128 + u * 8 + (lane & 7);
+        Row x = {-1, 0};
         int page, at;
-        if (e < units && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) {
-          x.off = (long long)page * P.c.page_b + (long long)at * P.c.row_b;
-          if (E4M3 && scale) x.f = 256u | __ldg((item & 1 ? P.c.vs : P.c.ks) + (long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row);
-        }
+        if (item < total && u < 16 && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) x = {page, at};
         return x;
+      };
+      auto offset = [&](const Row& x) { return x.page >= 0 ? (long long)x.page * P.c.page_b + (long long)x.at * P.c.row_b : -1ll; };
+      auto scale = [&](const Row& x, int item) {
+        return x.page >= 0 ? 256u | __ldg((item & 1 ? P.c.vs : P.c.ks) + (long long)x.page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)x.at * P.c.s_row) : 0u;
       };
       auto odd_at = [&](int key) { atomicMin(&ct.odd_lo, key); atomicMax(&ct.odd_hi, min(k.hi - 1, key)); };
       auto tile_free = [&](int item) {
@@ -487,49 +491,65 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             ok = ok && wait_for(smem_u32(&ct.raw_empty[rs]), ((n / F::RS) & 1) ^ 1);       // the rows that this warp writes there are others than it read
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
-            for (int e = item * 16 + (w + WK - item * 16 % WK) % WK; e < item * 16 + 16; e += WK) {
-              const Unit x = place(e, false);
-              if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][e & 15] = (uint8_t)vb; }
-              long long o[IT];
+#pragma unroll 1
+            for (int gr = 0; gr < GROUPS; gr++) {
+              const long long off = offset(row_of(item, gr));
+              const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
+#pragma unroll 1
+              for (int y = 0; y < 4; y++) {
+                const int u = unit0(item) + (gr * 4 + y) * WK;
+                if (u >= 16) break;
+                if (!(item & 1) && lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][u] = (uint8_t)(there >> y * 8);
+                long long o[IT];
 #pragma unroll
-              for (int i = 0; i < IT; i++) o[i] = from_lane(x.off, (i * 32 + lane) / CH & 7, P.wide);
+                for (int i = 0; i < IT; i++) o[i] = from_lane(off, y * 8 + ((i * 32 + lane) / CH & 7), P.wide);
 #pragma unroll
-              for (int i = 0; i < IT; i++)
-                if (i * 32 + lane < 8 * CH)
-                  cp16(base + F::RAW_AT + rs * F::RAW + F::raw_at((e & 15) * 8 + (i * 32 + lane) / CH, lane % CH), (item & 1 ? vbase : kbase) + (o[i] >= 0 ? o[i] : 0) + lane % CH * 16, o[i] >= 0);
+                for (int i = 0; i < IT; i++)
+                  cp16(base + F::RAW_AT + rs * F::RAW + F::raw_at(u * 8 + (i * 32 + lane) / CH, lane % CH), (item & 1 ? vbase : kbase) + (o[i] >= 0 ? o[i] : 0) + lane % CH * 16, o[i] >= 0);
+              }
             }
           }
           cp_commit();
         };
         if (!P.run) for (int i = 0; i < F::RS - 1; i++) gather(i);
-        int e = w;
-        Unit x = place(e, true);
+        Row ahead[GROUPS];
+        uint32_t next_f[GROUPS];
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; gr++) { next_f[gr] = scale(row_of(0, gr), 0); ahead[gr] = row_of(1, gr); }
         for (int item = 0; item < total && ok; item++) {
           const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
           const int j = k.A + (item >> 1);
           const bool check = (item & 1) && partial(k, j);
+          uint32_t f[GROUPS];
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; gr++) {
+            f[gr] = next_f[gr];
+            next_f[gr] = scale(ahead[gr], item + 1);
+            ahead[gr] = row_of(item + 2, gr);
+          }
           if (P.run) ok = wait_for(smem_u32(&ct.raw_full[rs]), (n / F::RS) & 1);
           else { gather(item + F::RS - 1); cp_wait<F::RS - 1>(); __syncwarp(); }
           if (!__all_sync(0xffffffffu, ok) || !tile_free(item)) { ok = false; break; }
           const unsigned char* src = smem + F::RAW_AT + rs * F::RAW;
           unsigned char* dst = smem + F::RING_AT + n % F::NST * F::TILE;
-#pragma unroll 1
-          for (; e < item * 16 + 16; e += WK) {
-            const Unit y = place(e + WK, true);                   // the next unit's scales are on their way
-            uint32_t f = x.f ? scale_bits((int)(x.f & 255)) : 0u;      // rows that are not there become zeros
-            f |= f << 16;
-            if (check && f == 0x7fc07fc0u) { odd_at(j * 128 + (e & 15) * 8 + (lane & 7)); f = 0; }
 #pragma unroll
-            for (int i = 0; i < IT; i++) {
-              const int row = (i * 32 + lane) / CH & 7, q = lane % CH, r = (e & 15) * 8 + row;
-              const uint32_t fr = __shfl_sync(0xffffffffu, f, row);
-              if (i * 32 + lane < 8 * CH) {
+          for (int gr = 0; gr < GROUPS; gr++) {
+            uint32_t mine = f[gr] ? scale_bits((int)(f[gr] & 255)) : 0u;      // rows that are not there become zeros
+            if (check && mine == 0x7fc0u) { odd_at(j * 128 + (unit0(item) + (gr * 4 + (lane >> 3)) * WK) * 8 + (lane & 7)); mine = 0; }
+            mine |= mine << 16;
+#pragma unroll 1
+            for (int y = 0; y < 4; y++) {
+              const int u = unit0(item) + (gr * 4 + y) * WK;
+              if (u >= 16) break;
+#pragma unroll
+              for (int i = 0; i < IT; i++) {
+                const int row = (i * 32 + lane) / CH, q = lane % CH, r = u * 8 + row;
+                const uint32_t fr = __shfl_sync(0xffffffffu, mine, y * 8 + row);
                 const uint4 v = *reinterpret_cast<const uint4*>(src + F::raw_at(r, q));
                 *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * q)) = make_uint4(widen_lo(v.x, fr), widen_hi(v.x, fr), widen_lo(v.y, fr), widen_hi(v.y, fr));
                 *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * q + 1)) = make_uint4(widen_lo(v.z, fr), widen_hi(v.z, fr), widen_lo(v.w, fr), widen_hi(v.w, fr));
               }
             }
-            x = y;
           }
           done_with(item);
           attn_tc::warp_arrive(smem_u32(&ct.raw_empty[rs]));
@@ -557,6 +577,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         }
       } else {
         // gather
+        long long now[GROUPS];
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; gr++) now[gr] = offset(row_of(0, gr));
         for (int item = 0; item < total + LAG && ok; item++) {
           if (item < total) {
             if (!tile_free(item)) break;
@@ -564,24 +587,32 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             const char* src = item & 1 ? vbase : kbase;
             const uint32_t slot = (uses + (uint32_t)item) % F::NST;
             unsigned char* dst = smem + F::RING_AT + slot * F::TILE;
-            for (int e = item * 16 + (w + WK - item * 16 % WK) % WK; e < item * 16 + 16; e += WK) {
-              const Unit x = place(e, false);
-              if (!(item & 1)) { const uint32_t vb = __ballot_sync(0xffffffffu, x.off >= 0); if (lane == 0) ct.valid[j % F::NV][e & 15] = (uint8_t)vb; }
-              long long o[IT];                                   // all the exchanges before the first copy: in turns each copy would wait for its own
+            const bool check = (item & 1) && partial(k, j);
 #pragma unroll
-              for (int i = 0; i < IT; i++) o[i] = from_lane(x.off, (i * 32 + lane) / CH, P.wide);
-              const bool check = (item & 1) && partial(k, j);
+            for (int gr = 0; gr < GROUPS; gr++) {
+              const long long off = now[gr];
+              now[gr] = offset(row_of(item + 1, gr));
+              const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
+#pragma unroll 1
+              for (int y = 0; y < 4; y++) {
+                const int u = unit0(item) + (gr * 4 + y) * WK;
+                if (u >= 16) break;
+                if (!(item & 1) && lane == 0) ct.valid[j % F::NV][u] = (uint8_t)(there >> y * 8);
+                long long o[IT];                                 // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
-              for (int i = 0; i < IT; i++) {
-                const int row = (e & 15) * 8 + (i * 32 + lane) / CH, q = lane % CH;
-                if (!check) cp16(smem_u32(dst) + tile_at(row, q), src + (o[i] >= 0 ? o[i] : 0) + q * 16, o[i] >= 0);
-                else {
-                  uint4 u = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + q * 16) : make_uint4(0, 0, 0, 0);
-                  if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
-                    odd_at(j * 128 + row);
-                    u = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
+                for (int i = 0; i < IT; i++) o[i] = from_lane(off, y * 8 + (i * 32 + lane) / CH, P.wide);
+#pragma unroll
+                for (int i = 0; i < IT; i++) {
+                  const int row = u * 8 + (i * 32 + lane) / CH, q = lane % CH;
+                  if (!check) cp16(smem_u32(dst) + tile_at(row, q), src + (o[i] >= 0 ? o[i] : 0) + q * 16, o[i] >= 0);
+                  else {
+                    uint4 v = o[i] >= 0 ? *reinterpret_cast<const uint4*>(src + o[i] + q * 16) : make_uint4(0, 0, 0, 0);
+                    if (odd_bits(v.x) || odd_bits(v.y) || odd_bits(v.z) || odd_bits(v.w)) {
+                      odd_at(j * 128 + row);
+                      v = make_uint4(without_odd(v.x), without_odd(v.y), without_odd(v.z), without_odd(v.w));
+                    }
+                    *reinterpret_cast<uint4*>(dst + tile_at(row, q)) = v;
                   }
-                  *reinterpret_cast<uint4*>(dst + tile_at(row, q)) = u;
                 }
               }
             }
