@@ -28,13 +28,13 @@ namespace ofa {
 namespace paged {
 
 template <int D, bool E4M3> struct Tc {
-  static constexpr int NT = D == 64 ? 1 : 2, BLOCKS = D == 64 ? 2 : 1;      // tiles of 128 rows a block, blocks an SM
+  static constexpr int NT = D == 64 && !E4M3 ? 1 : 2, BLOCKS = 3 - NT;      // tiles of 128 rows a block, blocks an SM
   static constexpr int WORKERS = NT == 1 ? 2 : 5, WARPS = 5 * NT + 1 + WORKERS, THREADS = 32 * WARPS;
   static constexpr int SOFT_REGS = 184, REST_REGS = 72;         // of a softmax thread, of another: together twice the launch's 128
   static constexpr int TMEM = NT * 256, O_AT = NT * 128;        // columns; S of a tile at tile * 128, O behind them
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
-  static constexpr int NST = E4M3 && D == 128 ? 3 : 4;          // ring of K and V tiles
-  static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 2 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
+  static constexpr int NST = E4M3 ? (D == 128 ? 3 : 6) : 4;           // ring of K and V tiles
+  static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 4 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
   static constexpr int LAG = 1;                                 // gathered tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
   static constexpr int Q_AT = 0, RING_AT = NT * TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
@@ -260,7 +260,6 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         const int olo = *reinterpret_cast<volatile int*>(&ct.odd_lo), ohi = *reinterpret_cast<volatile int*>(&ct.odd_hi);
         const long long g = (long long)(ch.s + t) * P.n_heads + head;
         const float inv = P.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        float* part = P.part + (g * P.nsplit + split) * D;
 #pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
           uint32_t o[32];
@@ -290,9 +289,18 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
               for (int y = 0; y < 8; y++) f[y] = __uint_as_float(o[x + y]) * inv;
               *reinterpret_cast<uint4*>(qt + tile_at(r, (q * 32 + x) / 8)) = pack8(f);
             }
-          } else if (on) {
+          } else {                                               // 128 bytes of each of the warp's rows, the same way
+            unsigned char* mine = qt + e * 4096;
 #pragma unroll
-            for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + q * 32 + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            for (int x = 0; x < 8; x++) *reinterpret_cast<uint4*>(mine + lane * 128 + ((x ^ (lane & 7)) << 4)) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+              const int row = x * 4 + (lane >> 3);
+              const long long d = __shfl_sync(0xffffffffu, on ? g : -1ll, row);
+              if (d >= 0) *reinterpret_cast<uint4*>(P.part + (d * P.nsplit + split) * D + q * 32 + (lane & 7) * 4) = *reinterpret_cast<const uint4*>(mine + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+            }
+            __syncwarp();
           }
         }
         if (P.nsplit == 1) {
@@ -464,11 +472,22 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
       const Walk k = walk(pair);
       const int total = 2 * (k.B - k.A);
       auto unit0 = [&](int item) { return (w + WK - item * 16 % WK) % WK; };               // the first unit of this worker
-      auto row_of = [&](int item, int gr) {                                                // this lane's row of its unit number gr * 4 + lane / 8
+      auto row_of = [&](int item, int gr) {                                                // this lane's row of its unit number gr * 4 + lane / 8; its page is not looked at yet
         const int u = unit0(item) + (gr * 4 + (lane >> 3)) * WK, key = (k.A + (item >> 1)) * 128 + u * 8 + (lane & 7);
         Row x = {-1, 0};
-        int page, at;
-        if (item < total && u < 16 && key >= k.lo && key < k.hi && locate(P.b, seq, key, page, at)) x = {page, at};
+        if (item < total && u < 16 && key >= k.lo && key < k.hi) {                         // below cap: within the table
+          const unsigned idx = P.b.page.quot((unsigned)key);
+          x.at = key - (int)(idx * P.b.page.d);
+          x.page = __ldg(P.b.pages + (long long)seq * P.b.pages_stride + idx);
+          x.at |= 1 << 31;                                                                 // there should be one
+        }
+        return x;
+      };
+      auto known = [&](Row x) {                                                            // and now it is
+        const bool want = x.at < 0;
+        x.at &= 0x7fffffff;
+        if (want && (unsigned)x.page >= (unsigned)P.b.n_pages) { flag(P.b.status, ST_PAGE); x.page = -1; }
+        if (!want) x.page = -1;
         return x;
       };
       auto offset = [&](const Row& x) { return x.page >= 0 ? (long long)x.page * P.c.page_b + (long long)x.at * P.c.row_b : -1ll; };
@@ -493,7 +512,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             if (!ok) return;
 #pragma unroll 1
             for (int gr = 0; gr < GROUPS; gr++) {
-              const long long off = offset(row_of(item, gr));
+              const long long off = offset(known(row_of(item, gr)));
               const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {
@@ -515,7 +534,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         Row ahead[GROUPS];
         uint32_t next_f[GROUPS];
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; gr++) { next_f[gr] = scale(row_of(0, gr), 0); ahead[gr] = row_of(1, gr); }
+        for (int gr = 0; gr < GROUPS; gr++) { next_f[gr] = scale(known(row_of(0, gr)), 0); ahead[gr] = row_of(1, gr); }
         for (int item = 0; item < total && ok; item++) {
           const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
           const int j = k.A + (item >> 1);
@@ -524,7 +543,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
 #pragma unroll
           for (int gr = 0; gr < GROUPS; gr++) {
             f[gr] = next_f[gr];
-            next_f[gr] = scale(ahead[gr], item + 1);
+            next_f[gr] = scale(known(ahead[gr]), item + 1);
             ahead[gr] = row_of(item + 2, gr);
           }
           if (P.run) ok = wait_for(smem_u32(&ct.raw_full[rs]), (n / F::RS) & 1);
@@ -537,7 +556,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             uint32_t mine = f[gr] ? scale_bits((int)(f[gr] & 255)) : 0u;      // rows that are not there become zeros
             if (check && mine == 0x7fc0u) { odd_at(j * 128 + (unit0(item) + (gr * 4 + (lane >> 3)) * WK) * 8 + (lane & 7)); mine = 0; }
             mine |= mine << 16;
-#pragma unroll 1
+#pragma unroll
             for (int y = 0; y < 4; y++) {
               const int u = unit0(item) + (gr * 4 + y) * WK;
               if (u >= 16) break;
@@ -577,9 +596,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         }
       } else {
         // gather
-        long long now[GROUPS];
+        Row now[GROUPS];
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; gr++) now[gr] = offset(row_of(0, gr));
+        for (int gr = 0; gr < GROUPS; gr++) now[gr] = row_of(0, gr);
         for (int item = 0; item < total + LAG && ok; item++) {
           if (item < total) {
             if (!tile_free(item)) break;
@@ -590,8 +609,8 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             const bool check = (item & 1) && partial(k, j);
 #pragma unroll
             for (int gr = 0; gr < GROUPS; gr++) {
-              const long long off = now[gr];
-              now[gr] = offset(row_of(item + 1, gr));
+              const long long off = offset(known(now[gr]));
+              now[gr] = row_of(item + 1, gr);
               const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {

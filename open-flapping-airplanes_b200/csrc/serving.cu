@@ -5,6 +5,7 @@
 #include "paged_attn_tc.cuh"
 #include "paged_move.cuh"
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <atomic>
 #include <stdarg.h>
 #include <stdio.h>
@@ -92,22 +93,24 @@ struct Plan { bool many, cluster; int rows, tiles, nsplit; size_t bytes; };     
 // A chunk of more than 32 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 128 or 256 rows; fewer to the one that keeps more bytes
 // in flight. max_new and max_kv are what the caller says; without them one sequence with all rows and the page table's width are assumed.
 //
-// How many blocks share a tile's keys: the number for which the rounds of blocks on the SMs times a block's time, in units of 128 keys, is least. What a block costs beside its keys
-// (its first loads one after the other, the meeting at its end) measured 3 units of the tensor-core kernel and 6 of the other, a second launch to join parts 3, and parts pass through memory at
-// 5 TB/s, a unit being 1.6 us. Up to eight blocks of the few-row kernel are a cluster and need no parts. (64 tokens over 1,024 to 4,096 8-bit keys: 88 us in one round and a bit, 84 with two
-// blocks a tile, 97 with four; a token over 1,000 keys, 12 heads of 64: 11.1, 8.7, 6.9 and 6.3 us with one, two, four and eight.)
+// How many blocks share a tile's keys: the number for which the call should take least, in units of 128 keys of a block: one block's time where all run at once, else all blocks' time over
+// the places for them and half a block's more for the end. What a block costs beside its keys (its first loads one after the other, the meeting at its end) measured 3 units of the tensor-core
+// kernel and 6 of the other, a second launch to join parts 3, and parts pass through memory at 5 TB/s, a unit being 1.6 us. Up to eight blocks of the few-row kernel are a cluster and need no parts.
+// (64 tokens over 1,024 to 4,096 8-bit keys: 88 us with one block a tile, 84 with two, 97 with four; a token over 1,000 keys, 12 heads of 64: 11.1, 8.7, 6.9 and 6.3 us with one, two, four and
+// eight; 4,096 tokens over 16,384 keys: 889 us with one, 914 with two.)
 Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
   Plan p;
   const long long group = n_heads / c->n_kv_heads;
   const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
   p.many = rows > 32;
-  const int tiles_of = c->head_dim == 64 ? 1 : 2;      // tiles of 128 rows a block of the tensor-core kernel, of which an SM holds 2 / tiles_of
+  const int tiles_of = c->head_dim == 64 && c->dtype == OFA_KV_BF16 ? 1 : 2;      // tiles of 128 rows a block of the tensor-core kernel, of which an SM holds 2 / tiles_of
   p.rows = p.many ? 128 * tiles_of : rows > 8 ? 16 : 8;
   long long tiles = (rows + p.rows - 1) / p.rows;
   if (tiles > 4096) tiles = 4096;
   if (tiles < 1) tiles = 1;
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
   const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles, units = (kv + 127) / 128;
+  const long long fewer = p.many ? std::min(rows / group, kv) / 256 : 0;       // units that a chunk's blocks have less on average than the last one
   const long long slots = 148 * (p.many ? 2 / tiles_of : p.rows == 8 ? 3 : 2), fixed = p.many ? 3 : 6;
   const size_t part = (size_t)n_rows * n_heads * (c->head_dim + 2) * 4;      // bytes of one split's parts
   p.nsplit = 1;
@@ -115,7 +118,8 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   for (int ns : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
     const bool cluster = !p.many && ns <= 8;
     if (ns > 1 && (ns > units || (cluster && (ns & (ns - 1))) || blocks * ns > 0x7fffffffll)) continue;
-    const double t = (double)((blocks * ns + slots - 1) / slots * (fixed + (units + ns - 1) / ns)) + (ns > 1 && !cluster ? 3 + 2.0 * part * ns / 8e6 : 0.0);
+    const double block = fixed + (double)((units + ns - 1) / ns), mean = fixed + (double)(units - fewer) / ns;
+    const double t = (blocks * ns <= slots ? block : blocks * ns * mean / slots + block / 2) + (ns > 1 && !cluster ? 3 + 2.0 * part * ns / 8e6 : 0.0);
     if (ns == 1 || t < best) { best = t; p.nsplit = ns; p.cluster = cluster && ns > 1; }
   }
   p.tiles = (int)tiles;
