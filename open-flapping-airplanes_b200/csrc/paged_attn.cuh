@@ -51,6 +51,7 @@ struct AttnArgs {
   alignas(64) CUtensorMap km, vm;   // the pages in boxes of `run` rows x 128 bytes (64: 8-bit rows of 64)
   int run;                          // 16, 8, or 0: pages of other sizes, no maps
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
+  int by_head;                      // many_rows_kernel: the order of its blocks
   int cluster;                      // ... which are a cluster and meet in shared memory
   float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
 };

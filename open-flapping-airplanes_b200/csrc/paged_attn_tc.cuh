@@ -6,7 +6,7 @@
 //                    back over the second half of them as bf16, the A operand of the second product
 //   warps 8, 9       one thread each issues a tile's products, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
 //                    soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores
-//                    (4,096 tokens over 16,384 keys, heads of 128: 854 us with whole steps in turns, HALVES_US so; steps of 64 keys with two buffers of scores waited least but
+//                    (4,096 tokens over 16,384 keys, heads of 128: 854 us with whole steps in turns, 862 so; steps of 64 keys with two buffers of scores waited least but
 //                    their fixed cost, 420 clocks, came twice: 928)
 //   warp 10          asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
 //                    (128-byte swizzle), 8-bit rows into a ring of their own
@@ -44,7 +44,7 @@ template <int D, bool E4M3> struct Tc {
   }
 };
 struct TcCtrl {
-  u64 q_full, full[8], empty[8], sa_full[2], s_full[2], s_free[2], pa_full[2], p_full[2], o_full[2];      // a: the first half
+  u64 q_full, full[8], empty[8], s_full[2], s_free[2], pa_full[2], p_full[2], o_full[2];      // a: the first half
   u64 look[8];                                                  // bf16: a tile that the workers look through has landed
   u64 raw_full[4], raw_empty[4];
   uint32_t tmem, dead;
@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  // the last tiles of all sequences and heads, which have the most keys, start first
-  const int split = (int)blockIdx.x % P.nsplit, kvh = (int)blockIdx.x / P.nsplit % P.n_kv_heads, seq = (int)blockIdx.x / P.nsplit / P.n_kv_heads % P.b.n_seqs;
-  const int turn = (int)blockIdx.x / P.nsplit / P.n_kv_heads / P.b.n_seqs;
+  // The last tiles, which have the most keys, start first: over all sequences and heads, or, where their keys and values together would not stay in L2, head by head
+  const int split = (int)blockIdx.x % P.nsplit, rest = (int)blockIdx.x / P.nsplit, streams = P.n_kv_heads * P.b.n_seqs;
+  const int turn = P.by_head ? rest % P.tiles : rest / streams, stream = P.by_head ? rest / P.tiles : rest % streams, kvh = stream % P.n_kv_heads, seq = stream / P.n_kv_heads;
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
     for (int s = 0; s < F::NST; s++) { mbar_init(smem_u32(&ct.full[s]), F::WORKERS); mbar_init(smem_u32(&ct.empty[s]), NT); mbar_init(smem_u32(&ct.look[s]), 1); }
     for (int s = 0; s < 4; s++) { mbar_init(smem_u32(&ct.raw_full[s]), 1); mbar_init(smem_u32(&ct.raw_empty[s]), F::WORKERS); }
     for (int i = 0; i < NT; i++) {
-      mbar_init(smem_u32(&ct.sa_full[i]), 1); mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.s_free[i]), 4);
+      mbar_init(smem_u32(&ct.s_full[i]), 1); mbar_init(smem_u32(&ct.s_free[i]), 4);
       mbar_init(smem_u32(&ct.pa_full[i]), 4); mbar_init(smem_u32(&ct.p_full[i]), 4); mbar_init(smem_u32(&ct.o_full[i]), 1);
     }
     ct.odd_lo = 0x7fffffff; ct.odd_hi = -1; ct.dead = 0;
@@ -178,16 +178,12 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
       for (int c = 0; c < n; c++) {
         const int j = k.a[tile] + c, k0 = j * 128;
         uint32_t s[4][32];
-        ok = wait_for(smem_u32(&ct.sa_full[tile]), (done + c) & 1);
-        tc_fence_after();
-        if (__all_sync(0xffffffffu, ok)) {
-          attn_tc::tmem_ld32_nw(ts, s[0]);
-          attn_tc::tmem_ld32_nw(ts + 32, s[1]);
-        }
-        ok = ok && wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
+        ok = wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
+        attn_tc::tmem_ld32_nw(ts, s[0]);
+        attn_tc::tmem_ld32_nw(ts + 32, s[1]);
         attn_tc::tmem_ld32_nw(ts + 64, s[2]);
         attn_tc::tmem_ld32_nw(ts + 96, s[3]);
         attn_tc::tmem_ld_wait();
@@ -227,7 +223,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         }
         const float ref = m == -INFINITY ? 0.f : m;              // no key seen yet: 2^(-inf - 0) = 0
         const u64 sc2 = attn_tc::f2(P.scale_log2, P.scale_log2), nm2 = attn_tc::f2(-ref, -ref);
-        u64 sum[4] = {0, 0, 0, 0};
+        u64 sum[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; q++) {
           uint32_t pk[16];
@@ -235,7 +231,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
           for (int x = 0; x < 32; x += 2) {
             const float2 v = attn_tc::unf2(attn_tc::fma2(attn_tc::f2(__uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1])), sc2, nm2));
             const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
-            sum[(x >> 1) & 3] = attn_tc::add2(sum[(x >> 1) & 3], attn_tc::f2(p0, p1));
+            sum[(x >> 1) & 1] = attn_tc::add2(sum[(x >> 1) & 1], attn_tc::f2(p0, p1));
             pk[x >> 1] = pack2f(p0, p1);                         // rounded to bf16 for the product; the sum is taken before
           }
           attn_tc::tmem_st16(ts + 64 + q * 16, pk);
@@ -248,8 +244,8 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         attn_tc::tmem_st_wait();
         tc_fence_before();
         attn_tc::warp_arrive(smem_u32(&ct.p_full[tile]));
-        const float2 s0 = attn_tc::unf2(attn_tc::add2(sum[0], sum[1])), s1 = attn_tc::unf2(attn_tc::add2(sum[2], sum[3]));
-        l += (s0.x + s0.y) + (s1.x + s1.y);
+        const float2 s0 = attn_tc::unf2(attn_tc::add2(sum[0], sum[1]));
+        l += s0.x + s0.y;
       }
       if (ok && n > 0) {
         ok = wait_for(smem_u32(&ct.o_full[tile]), (done + n - 1) & 1);
@@ -343,8 +339,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++)
             umma_bf16(ts + half * 64, dq + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
-          umma_commit(smem_u32(half ? &ct.s_full[tile] : &ct.sa_full[tile]));
-          if (half) umma_commit(smem_u32(&ct.empty[slot]));
+          if (half) { umma_commit(smem_u32(&ct.s_full[tile])); umma_commit(smem_u32(&ct.empty[slot])); }
         }
       };
       auto pass = [&](int item) {                                // a tile that this issuer has no use for
