@@ -5,6 +5,7 @@
 import os
 import shutil
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -13,6 +14,10 @@ CLI = os.path.join(CSRC, "ofa_cli")              # the command-line host (csrc/o
 SOURCES = ["runtime.cu", "noalloc.cu", "serving.cu"]
 HEADERS = ["common.cuh", "task_api.h", "tickets.h", "elementwise.cuh", "gemm_tc.cuh", "attn_common.cuh", "attn_tc.cuh", "dp_nccl.inc", "simt_f32.cuh", "decode.cuh",
            "megakernel.cuh", "paged.cuh", "paged_attn.cuh", "paged_attn_tc.cuh", "paged_move.cuh", "logits.cuh", os.path.join("..", "..", "include", "ofa_b200.h")]
+
+
+HOST_SRC = os.path.join(CSRC, "serving_py.cpp")  # the torch view's calls of the serving operators, a CPython extension
+HOST = os.path.join(HERE, "_serving" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
 def nvcc_path():
@@ -63,3 +68,19 @@ def build_cli(force=False):
     if r.returncode != 0:
         raise RuntimeError("building ofa_cli failed:\n" + r.stdout + r.stderr)
     return CLI
+
+
+def build_host(force=False):
+    """Compile csrc/serving_py.cpp for this Python next to the package's modules. Returns the path, or None where Python's headers are missing: serving.py then makes the same
+    calls itself, more slowly."""
+    hdr = os.path.join(CSRC, "..", "..", "include", "ofa_b200.h")
+    inc = sysconfig.get_paths()["include"]
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if not force and os.path.exists(HOST) and os.path.getmtime(HOST) >= max(os.path.getmtime(HOST_SRC), os.path.getmtime(hdr)):
+        return HOST
+    if not cxx or not os.path.exists(os.path.join(inc, "Python.h")):
+        return None
+    r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + inc, "-o", HOST, HOST_SRC], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building " + HOST + " failed:\n" + r.stdout + r.stderr)
+    return HOST

@@ -71,6 +71,34 @@ def _lib():
     return _loaded
 
 
+def _bind():
+    """The extension that build.build_host() compiles, bound to the loaded library; None where there is none. Its functions return an entry point's code, or None for
+    arguments that are not plainly right: the code below then finds out what is wrong with them."""
+    try:
+        from . import _serving
+    except ImportError:
+        return None
+    lib = _lib()
+    addr = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
+    _serving.bind(addr(lib.ofa_kv_append), addr(lib.ofa_kv_read), addr(lib.ofa_paged_attention), addr(lib.ofa_logits_process), _BF16, _F32, _I32, torch.uint8, _stream, _current)
+    return _serving
+
+
+_fast_module = ()
+
+
+def _fast():
+    global _fast_module
+    if _fast_module == ():
+        _fast_module = _bind()
+    return _fast_module
+
+
+def _done(rc):
+    if rc:
+        raise OfaError(rc, _lib().ofa_serving_last_error().decode())
+
+
 def _rows(name, t, shape, cache):
     """The strides of bf16 rows [n_rows, heads, head_dim] on the cache's device; what is wrong with them otherwise."""
     try:
@@ -137,7 +165,7 @@ class KVCache:
         if e4m3:
             c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
             c.scale_page_stride, c.scale_head_stride, c.scale_row_stride = k_scale.stride()
-        self.ref = C.byref(c)
+        self.ref, self.address = C.byref(c), C.addressof(c)
 
     @classmethod
     def empty(cls, n_pages, page_size, n_kv_heads, head_dim, dtype="bf16", device="cuda"):
@@ -173,7 +201,7 @@ class KVBatch:
         c.q_start, c.kv_len, c.pages = q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr()
         c.max_new, c.max_kv = min(max_new, 2 ** 31 - 1), min(max_kv, 2 ** 31 - 1)
         c.status = status.data_ptr() if status is not None else None
-        self.ref = C.byref(c)
+        self.ref, self.address = C.byref(c), C.addressof(c)
 
 
 def _same_device(cache, batch):
@@ -181,8 +209,14 @@ def _same_device(cache, batch):
         _refuse(f"the cache is on {cache.device}, the batch on {batch.device}")
 
 
-def _move(fn, cache, batch, k, v, n_rows):
+def _move(read, cache, batch, k, v, n_rows):
     _same_device(cache, batch)
+    f = _fast()
+    if f is not None:
+        rc = f.move(read, cache.address, batch.address, cache.n_kv_heads, cache.head_dim, cache.index, -1 if n_rows is None else n_rows, k, v)
+        if rc is not None:
+            return _done(rc)
+    fn = _lib().ofa_kv_read if read else _lib().ofa_kv_append
     rows = k.shape[0] if n_rows is None and isinstance(k, torch.Tensor) and k.dim() else n_rows
     shape = (rows, cache.n_kv_heads, cache.head_dim)
     a, b = _rows("k", k, shape, cache), _rows("v", v, shape, cache)
@@ -191,7 +225,7 @@ def _move(fn, cache, batch, k, v, n_rows):
 
 def kv_append(cache, batch, k, v):
     """Rows k and v [n_rows, n_kv_heads, head_dim] (bf16; views of a fused projection will do) to their pages, in the cache's type."""
-    _move(_lib().ofa_kv_append, cache, batch, k, v, None)
+    _move(False, cache, batch, k, v, None)
 
 
 def kv_read(cache, batch, n_rows=None, k=None, v=None):
@@ -200,9 +234,9 @@ def kv_read(cache, batch, n_rows=None, k=None, v=None):
         if n_rows is None or k is not None or v is not None:
             _refuse("kv_read needs n_rows, or k and v to write to")
         shape = (n_rows, cache.n_kv_heads, cache.head_dim)
-        k = torch.empty(shape, dtype=_BF16, device=cache.device)
+        k = torch.empty_strided(shape, (cache.n_kv_heads * cache.head_dim, cache.head_dim, 1), dtype=_BF16, device=cache.device)
         v = torch.empty_like(k)
-    _move(_lib().ofa_kv_read, cache, batch, k, v, n_rows)
+    _move(True, cache, batch, k, v, n_rows)
     return k, v
 
 
@@ -210,23 +244,32 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
     """Attention of q [n_rows, n_heads, head_dim] (bf16) over the batch's pages; scale: 1/sqrt(head_dim) by default. Returns out, of q's shape, or with
     with_lse (out, lse [n_rows, n_heads] fp32). Rows that no sequence brings are left as they were."""
     _same_device(cache, batch)
-    sq = _rows("q", q, None, cache)
-    shape = q.shape
-    n_rows, n_heads = shape[0], shape[1]
+    try:
+        n_rows, n_heads, _ = q.shape
+    except (AttributeError, ValueError):
+        _rows("q", q, None, cache)
+        raise
     if out is None:
+        if not q.is_cuda or q.dtype is not _BF16:
+            _rows("q", q, None, cache)
         out = torch.empty_like(q)
-    so = _rows("out", out, shape, cache)
-    lse = torch.empty((n_rows, n_heads), dtype=_F32, device=cache.device) if with_lse else None
-    lib = _lib()
+    lse = torch.empty_strided((n_rows, n_heads), (n_heads, 1), dtype=_F32, device=cache.device) if with_lse else None
     key = (cache.c.dtype, cache.head_dim, cache.n_kv_heads, cache.page_size, n_rows, n_heads)
     need = batch._need.get(key)
     if need is None:
-        need = batch._need[key] = lib.ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
+        need = batch._need[key] = _lib().ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
     # from the caller's allocator: a graph that captures the call keeps its own
-    work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-    a = capi.PagedAttentionArgs(n_rows, n_heads, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse.data_ptr() if with_lse else None,
-                                cache.scale if scale is None else scale, bool(causal), window, work.data_ptr() if need else None, need)
-    _call(lib.ofa_paged_attention, cache.index, cache.ref, batch.ref, C.byref(a))
+    work = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=cache.device) if need else None
+    scale = cache.scale if scale is None else scale
+    f = _fast()
+    rc = f.attend(cache.address, batch.address, cache.head_dim, cache.index, q, out, lse, work, scale, causal, window) if f is not None else None
+    if rc is not None:
+        _done(rc)
+    else:
+        sq, so = _rows("q", q, None, cache), _rows("out", out, q.shape, cache)
+        a = capi.PagedAttentionArgs(n_rows, n_heads, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse.data_ptr() if with_lse else None, scale, bool(causal), window,
+                                    work.data_ptr() if need else None, need)
+        _call(_lib().ofa_paged_attention, cache.index, cache.ref, batch.ref, C.byref(a))
     return (out, lse) if with_lse else out
 
 
@@ -235,6 +278,13 @@ def logits_process(logits, tokens=None, n_tokens=None, n_prompt=None, repetition
     tokens [n_rows, max_tokens], n_tokens, n_prompt [n_rows], bias_ids [n_rows, n] and mask [n_rows, ceil(vocab / 32)] are int32, the rest fp32."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F32, _BF16):
         _refuse("logits have to be a bf16 or fp32 tensor")
+    f = _fast()
+    if f is not None and logits.is_cuda:
+        y = torch.empty_like(logits) if out is None else out
+        rc = f.process(logits, y, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias, mask)
+        if rc is not None:
+            _done(rc)
+            return y
     kind, dev, index = logits.dtype, logits.device, logits.get_device()
     if index < 0 or logits.dim() != 2:
         _want("logits", logits, kind, (None, None), None)
