@@ -25,7 +25,8 @@
 // values left the byte and logic instructions of the integer pipe, two clocks each, as the bound: 10 of them for four elements.
 //
 // A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
-// infinities and NaN are taken out of its values and added to the rows that see it. Rows past the context and of a bad page are never read.
+// infinities and NaN are taken out of its values and added to the rows that see it. What lies behind the context in its last page may be fetched and counts nowhere; nothing
+// of a bad page is read.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -395,13 +396,16 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             uint4* w = reinterpret_cast<uint4*>(sv + x * 512 + lane * 16);
             uint4 u = *w;
             if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
-              odd = true;
+              odd |= valid >> ((x * 512 + lane * 16) / F::W % F::KEYS) & 1;
               *w = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
             }
           }
         }
-        if (__any_sync(0xffffffffu, odd)) {
+        if constexpr (!E4M3) {
           fence_async_shared();                                  // what was taken out, before the copy engine writes there again
+          __syncwarp();
+        }
+        if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll 1
           for (int kk = 0; kk < F::KEYS; kk++) {
             const int p = k0 + kk;

@@ -1,21 +1,24 @@
 // Attention of many rows over a paged cache on the 5th-generation tensor cores: chunks of new tokens, where the products count.
 //
-// The rows of a key/value head (new tokens x the query heads that share it) are taken 256 at a time by a block of 16 warps, two tiles of 128 rows that walk the
-// same keys 128 at a time, half a step apart: while the softmax warps of one tile work, the tensor pipe works for the other.
-//   softmax, four warps a tile:  of tile 0 and 1, a thread per row (= tensor-memory lane): reads its 128 scores, keeps maximum and sum, writes the probabilities
-//                    back over the second half of them as bf16, the A operand of the second product
-//   warps 8, 9       one thread each issues a tile's products, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
-//                    soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores
-//                    (4,096 tokens over 16,384 keys, heads of 128: 854 us with whole steps in turns, 862 so; steps of 64 keys with two buffers of scores waited least but
-//                    their fixed cost, 420 clocks, came twice: 928)
-//   warp 10          asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
-//                    (128-byte swizzle), 8-bit rows into a ring of their own
-//   warps 11-15      widen 8-bit rows from there into the tiles, once for the 256 rows; look at values that some row must not meet; and gather the rows of pages that are no
-//                    multiple of 8 by cp.async, 16 bytes a lane
-// Tensor memory, 512 columns: S 0 / 128 (P in their last 64), O 256 / 256 + D.
+// The rows of a key/value head (new tokens x the query heads that share it) are taken 128 at a time, a tile, and walk their keys 128 at a time. A block has two tiles, half
+// a step apart, so that the tensor pipe works for one while the softmax warps of the other do; heads of 64 with bf16 rows, whose tiles are small, have one tile a block and two blocks
+// an SM, which also covers a block's start and end (four prompts of 1,024 tokens, 12 heads: 32.1 -> 29.0 us). Roles of a block's warps:
+//   softmax    four warps a tile, a thread per row (= tensor-memory lane): reads its 128 scores once, keeps maximum and sum, writes the probabilities
+//              back over the second half of them as bf16, the A operand of the second product
+//   products   a warp a tile, one thread of which issues, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
+//              soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores. (4,096 tokens over
+//              16,384 keys, heads of 128: 843 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
+//              two threads a row, four softmax warps a scheduler: 910, bound by issue; a third of the exponentials by a polynomial on the multiply-add pipe: 970 and more, for registers and issue.)
+//              One thread a tile because one issues a tcgen05.mma only every ~96 clocks and a 128 x 128 x 16 product takes 64
+//   copies     one warp asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
+//              (128-byte swizzle), 8-bit rows into a ring of their own
+//   workers    widen 8-bit rows from there into the tiles, once for the block's rows; look at values that some row must not meet; and gather the rows of pages that are no
+//              multiple of 8 by cp.async, 16 bytes a lane
+// What bounds it: 128 keys of two tiles of heads of 128 take 3,400 clocks, of which the tensor pipe works 2,048 and the special-function unit, for 32,768 exponentials, as many.
+// Tensor memory: S of a tile in 128 columns (P in their last 64), O behind all S.
 //
 // A row's probabilities are taken against a reference that is raised only when the true maximum has passed it by 2^8 (they stay below 256: exact enough in fp32 sums and
-// bf16), and only then is the row of O multiplied in tensor memory. Before S of the next step is issued the issuer has seen the product before it complete, so a softmax thread
+// bf16), and only then is the row of O multiplied in tensor memory. A step's scores are complete only when the product before them is, since one thread's products run in their order: a softmax thread
 // that has its scores may also rewrite its row of O.
 //
 // Keys that some rows of the block see and others do not (the diagonal, the window's edge, the end of the context) come in tiles whose values are all looked
@@ -584,7 +587,8 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
             const uint4 u = *reinterpret_cast<const uint4*>(tile + c * 16);
             if (odd_bits(u.x) || odd_bits(u.y) || odd_bits(u.z) || odd_bits(u.w)) {
               *reinterpret_cast<uint4*>(tile + c * 16) = make_uint4(without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w));
-              odd_at(j * 128 + (c * 16 & 16383) / 128);
+              const int row = (c * 16 & 16383) / 128;            // what lies behind the context in its last page counts nowhere
+              if (ct.valid[j % F::NV][row >> 3] >> (row & 7) & 1) odd_at(j * 128 + row);
             }
           }
           done_with(item);

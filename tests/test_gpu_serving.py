@@ -516,3 +516,123 @@ def test_logits_of_rows_between_boundaries(sv, rows, vocab, pad, dtype):
             fine = torch.isfinite(want) & (want.abs() < torch.finfo(dtype).max)
             assert torch.equal(got[want == -math.inf], want[want == -math.inf])
             assert ((got - want).abs()[fine] <= (tol + half * (want.abs() + tol))[fine]).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("page", [16, 8, 33])
+def test_a_cache_full_of_nan_behind_the_contexts(sv, page, new):
+    """Pages that were never written, or held another sequence, may hold anything: contexts end in the middle of boxes, tiles and pages."""
+    for length in (new, 45, 130, 256, 300):
+        if length < new:
+            continue
+        cols = -(-length // page)
+        cache = sv.KVCache(torch.full((cols, 2, page, 64), math.nan, dtype=torch.bfloat16, device=DEV), torch.full((cols, 2, page, 64), -math.inf, dtype=torch.bfloat16, device=DEV))
+        g = torch.Generator().manual_seed(length)
+        table = i32([torch.randperm(cols, generator=g).tolist()])
+        rows = torch.randn(length, 2, 64, generator=g).bfloat16().to(DEV)
+        sv.kv_append(cache, sv.KVBatch(i32([0, length]), i32([length]), table), rows, rows * 2)
+        check_attention(sv, cache, sv.KVBatch(i32([0, new]), i32([length]), table, max_new=new), queries(g, new, 4, 64))
+
+
+def test_thousands_of_sequences(sv):
+    """Every block finds its rows among all sequences"""
+    n = 3000
+    g = torch.Generator().manual_seed(5)
+    new = torch.randint(0, 3, (n,), generator=g).tolist()
+    kv = [k + int(x) for k, x in zip(new, torch.randint(0, 30, (n,), generator=g))]
+    per = [-(-k // 8) for k in kv]
+    cols, total = max(per), sum(per)
+    perm, at, table = torch.randperm(total, generator=g).tolist(), 0, []
+    for p in per:
+        table.append(perm[at:at + p] + [-1] * (cols - p))
+        at += p
+    cache = sv.KVCache.empty(total, 8, 1, 64)
+    full = sv.KVBatch(i32(starts(kv)), i32(kv), i32(table))
+    k, v = (torch.randn(sum(kv), 1, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    sv.kv_append(cache, full, k, v)
+    back = sv.kv_read(cache, full, sum(kv))
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+    q = queries(g, sum(new), 2, 64)
+    o, lse = sv.paged_attention(cache, sv.KVBatch(i32(starts(new)), i32(kv), i32(table), max_new=2), q, with_lse=True)
+    st = starts(new)
+    some = [i for i in range(n) if new[i]][::97]
+    for i in some:
+        s, e = starts(kv[:i + 1])[-2:]
+        want, _, tol, _ = dense(q[st[i]:st[i + 1]], k[s:e], v[s:e])
+        assert ((o[st[i]:st[i + 1]].double().cpu() - want).abs() <= tol).all()
+
+
+def dense(q, k, v):
+    """attention of one sequence whose keys and values lie side by side"""
+    class One:
+        n_pages, page_size, n_kv_heads, head_dim, k_scale = 1, k.shape[0], k.shape[1], k.shape[2], None
+    One.k, One.v = k.transpose(0, 1)[None], v.transpose(0, 1)[None]
+    return ref.attention(One, [0, q.shape[0]], [k.shape[0]], torch.tensor([[0]]), q, 1 / math.sqrt(k.shape[2]))
+
+
+def test_calls_without_the_extension_give_the_same(sv, monkeypatch):
+    cache, batch, g = make(sv, [3, 30], [70, 90], 2, 64, 16, "e4m3", max_new=30)
+    q = queries(g, 33, 4, 64)
+    rows = torch.randn(33, 2, 64, generator=g).bfloat16().to(DEV)
+    x, a, mask = logit_inputs(5, 300, 20, 3, torch.float32)
+    a = {k: v.to(DEV) for k, v in a.items()} | {"mask": mask.to(DEV)}
+
+    def all_of_them():
+        sv.kv_append(cache, batch, rows, rows)
+        return (*sv.kv_read(cache, batch, 33), *sv.paged_attention(cache, batch, q, window=50, with_lse=True), sv.logits_process(x.to(DEV), **a))
+    assert sv._fast() is not None
+    one = all_of_them()
+    monkeypatch.setattr(sv, "_fast_module", None)
+    for u, w in zip(one, all_of_them()):
+        assert torch.equal(u, w)
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_tensors_that_do_not_fit_are_refused(sv, ofa, monkeypatch, extension):
+    """and nothing is written"""
+    if not extension:
+        monkeypatch.setattr(sv, "_fast_module", None)
+    cache, batch, g = make(sv, [2, 1], [20, 9], 2, 64, 16)
+    q, k = queries(g, 3, 4, 64), torch.randn(3, 2, 64, generator=g).bfloat16().to(DEV)
+    before = cache.k.clone(), cache.v.clone()
+    wide = torch.randn(3, 2, 128, device=DEV).bfloat16()
+    for bad in (k.float(), k.half(), k[:, :1], k[..., :32], wide[..., ::2], k.cpu(), k[0], None, "k", k.transpose(0, 1)):
+        with pytest.raises(ofa.OfaError):
+            sv.kv_append(cache, batch, bad, k)
+        with pytest.raises(ofa.OfaError):
+            sv.kv_append(cache, batch, k, bad)
+    for bad in (q.float(), q[..., :32], torch.randn(3, 4, 128, device=DEV).bfloat16()[..., ::2], q.cpu(), q[0], None, q[:, :3], torch.randn(3, 4, 65, device=DEV).bfloat16()[..., 1:]):
+        with pytest.raises((ofa.OfaError, AttributeError, ValueError)):
+            sv.paged_attention(cache, batch, bad)
+    for more in ({"window": -1}, {"window": 3, "causal": False}, {"scale": math.nan}, {"out": q.float()}, {"out": torch.empty_like(q)[:2]}):
+        with pytest.raises(ofa.OfaError):
+            sv.paged_attention(cache, batch, q, **more)
+    with pytest.raises(ofa.OfaError):
+        sv.kv_read(cache, batch)
+    with pytest.raises(ofa.OfaError):
+        sv.kv_read(cache, batch, 3, k=k)
+    with pytest.raises(ofa.OfaError):
+        sv.kv_read(cache, batch, 3, k=k, v=k.float())
+    x, n = torch.randn(3, 100, device=DEV), i32([1, 2, 3])
+    t, f = i32([[1, 2], [3, 4], [5, 6]]), torch.ones(3, device=DEV)
+    for more in ({"n_tokens": n}, {"repetition": f}, {"tokens": t.long()}, {"tokens": t, "n_tokens": n.long()}, {"tokens": t[:2]}, {"tokens": t, "repetition": f.double()}, {"tokens": t, "presence": f[:2]},
+                 {"bias_ids": t}, {"bias": torch.ones(3, 2, device=DEV)}, {"bias_ids": t, "bias": torch.ones(3, 3, device=DEV)}, {"mask": i32([[1] * 3] * 3)}, {"mask": i32([[1] * 4] * 2)},
+                 {"out": x.bfloat16()}, {"out": x[:2]}, {"out": x.t()}, {"tokens": t.t().contiguous().t()}, {"mask": torch.zeros(3, 4, dtype=torch.int32)}):
+        with pytest.raises(ofa.OfaError):
+            sv.logits_process(x, **more)
+    for bad in (x.half(), x[0], x.cpu(), x.t(), x[:, ::2]):
+        with pytest.raises(ofa.OfaError):
+            sv.logits_process(bad)
+    assert torch.equal(before[0], cache.k) and torch.equal(before[1], cache.v)
+    kk, vv = cache.k, cache.v
+    for args in ((kk, vv.transpose(1, 2).contiguous().transpose(1, 2)), (kk, vv[:, :1]), (kk, vv.float()), (kk[..., :32], vv[..., :32]), (kk, vv, n, n), (kk.to(torch.float8_e4m3fn), vv.to(torch.float8_e4m3fn)),
+                 (torch.zeros(2, 1, 16, 96, dtype=torch.bfloat16, device=DEV),) * 2):
+        with pytest.raises(ofa.OfaError):
+            sv.KVCache(*args)
+    for args in ((n, n, t), (i32([0, 1, 2, 3]).long(), n, t), (i32([0, 1, 2, 3]), n, t.long()), (i32([0, 1, 2, 3]), n.cpu(), t)):
+        with pytest.raises(ofa.OfaError):
+            sv.KVBatch(*args)
+    with pytest.raises(ofa.OfaError):
+        sv.KVBatch(i32([0, 1, 2, 3]), n, t, status=torch.zeros(0, dtype=torch.int32, device=DEV))
+    with pytest.raises(ofa.OfaError):
+        sv.KVBatch(i32([0, 1, 2, 3]), n, t, max_new=-1)
