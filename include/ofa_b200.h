@@ -246,7 +246,7 @@ typedef struct {
  * rows that none brings (behind the last, padding) are neither read nor written. The arrays are read on the device, so a replayed graph sees their current values.
  * What is wrong there cannot be refused on the host; it never becomes an access out of range, and sets bits of *status (or-ed; may be NULL):
  * 1 a page number outside the cache, 2 a length below 0 or beyond the page table, 4 q_start not rising or beyond n_rows (that sequence is left out), 8 a wait inside a kernel
- * ran out (2 s; the call's output is not valid). */
+ * ran out (some seconds; the call's output is not valid). */
 enum { OFA_KV_BAD_PAGE = 1, OFA_KV_BAD_LENGTH = 2, OFA_KV_BAD_ROWS = 4, OFA_KV_TIMEOUT = 8 };
 typedef struct {
   int n_seqs, max_pages;              /* rows and columns of the page table */
@@ -259,7 +259,7 @@ typedef struct {
 
 /* Keys and values (bf16, [n_rows][n_kv_heads][head_dim]) to their pages, in the cache's type: to 8 bits with the smallest power of two by which the row's largest
  * magnitude fits 448, rounded to nearest even. Rows whose position is negative or has no page are not kept. No two rows of a call may have the same
- * place. */
+ * place (which of them it then holds is open), and the cache's rows may not overlap. */
 int ofa_kv_append(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const void* k, const void* v, int n_rows,
                   long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream);
 /* The reverse: the rows of the call are read from their pages (all of a context with q_start counting kv_len) and are exact in bf16. Rows
@@ -270,7 +270,7 @@ int ofa_kv_read(const ofa_kv_cache* cache, const ofa_kv_batch* batch, void* k, v
 /* out[row][h] = softmax over the cached keys that the row sees of scale * q.k, times their values; heads h of [g * n_heads / n_kv_heads ...) share key/value head g.
  * causal: a row at position p sees positions <= p, and with window > 0 only those > p - window; otherwise all kv_len. The rows' own keys
  * have to be in the cache (ofa_kv_append). lse (may be NULL, [n_rows][n_heads] fp32): the natural logarithm of the sum of exponentials. A row
- * that sees no key gets zeros and -inf. Keys without a page are not seen. What a row does not see does not reach it, infinities and NaN included.
+ * that sees no key gets zeros and -inf. out may be q itself, otherwise they do not overlap. Keys without a page are not seen. What a row does not see does not reach it, infinities and NaN included.
  * workspace: ofa_paged_attention_workspace() bytes, 16-byte aligned, contents of no interest before and after; calls that may overlap need one each. */
 typedef struct {
   int n_rows, n_heads;
@@ -284,7 +284,7 @@ typedef struct {
 int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const ofa_paged_attention_args* args, void* stream);
 size_t ofa_paged_attention_workspace(const ofa_kv_cache* cache, const ofa_kv_batch* batch, int n_rows, int n_heads);
 
-/* One pass over logits [n_rows][vocab] (OFA_DTYPE_BF16 or OFA_DTYPE_F32; out may be in), in fp32, in this order:
+/* One pass over logits [n_rows][vocab] (OFA_DTYPE_BF16 or OFA_DTYPE_F32; out may be in, otherwise they do not overlap; at most 65,535 rows), in fp32, in this order:
  *   a token that stands in the row's history:  x > 0 ? x / repetition : x * repetition
  *   x - frequency * n - presence * (n > 0), n = how often it stands there behind the prompt
  *   x + the sum of the row's biases with this id

@@ -36,7 +36,6 @@ namespace ofa {
 namespace paged {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int MAX_SPLIT = 64;
 constexpr float RESCALE_LOG2 = 8.f;
 
 struct AttnArgs {
@@ -59,12 +58,6 @@ struct AttnArgs {
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -571,7 +564,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   }
 }
 
-// Joins the splits of a row and head, in their order: a warp each. Rows that no sequence brought have no parts and are left as they are.
+// Joins the splits (at most 64) of a row and head, in their order: a warp each. Rows that no sequence brought have no parts and are left as they are.
 template <int D> __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ AttnArgs P) {
   const long long g = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;

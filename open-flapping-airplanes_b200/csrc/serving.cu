@@ -28,6 +28,18 @@ int launched(const char* what) {
   return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
 }
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// Whether places of `unit` elements at these strides lie upon one another: from the smallest stride up, each has to pass what lies inside it
+struct Axis { long long stride, count; };
+bool overlap(Axis a, Axis b, Axis c, long long unit) {
+  Axis x[3] = {a, b, c};
+  std::sort(x, x + 3, [](const Axis& u, const Axis& v) { return u.stride < v.stride; });
+  for (const Axis& i : x)
+    if (i.count > 1) {
+      if (i.stride < unit) return true;
+      unit += i.stride * (i.count - 1);
+    }
+  return false;
+}
 
 // ---- checks shared by the operators over a cache
 int check_cache(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, paged::Batch& B, paged::Pool& C) {
@@ -38,6 +50,7 @@ int check_cache(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, paged:
   if (c->page_size < 1 || c->n_pages < 0) return fail(OFA_BAD_ARGUMENT, "page_size %d, n_pages %d", c->page_size, c->n_pages);
   if (n_rows < 0 || b->n_seqs < 0 || b->max_pages < 0 || b->max_new < 0 || b->max_kv < 0)
     return fail(OFA_BAD_ARGUMENT, "negative size: n_rows %d, n_seqs %d, max_pages %d, max_new %d, max_kv %d", n_rows, b->n_seqs, b->max_pages, b->max_new, b->max_kv);
+  if (n_rows > 0x7fffff00) return fail(OFA_BAD_ARGUMENT, "%d rows are too many for one call", n_rows);
   const bool e4m3 = c->dtype == OFA_KV_E4M3;
   const long long es = e4m3 ? 1 : 2;
   if (n_rows > 0 && b->n_seqs > 0) {
@@ -57,9 +70,10 @@ int check_cache(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, paged:
   C.s_page = c->scale_page_stride; C.s_head = c->scale_head_stride; C.s_row = c->scale_row_stride;
   return OFA_OK;
 }
-int check_rows(const char* name, const void* p, long long row, long long head) {
+int check_rows(const char* name, const void* p, Axis row, Axis head, int dim, bool written) {
   if (!p) return fail(OFA_BAD_ARGUMENT, "%s is null", name);
-  if (!aligned(p, 16) || row % 8 || head % 8 || row < 0 || head < 0) return fail(OFA_BAD_ARGUMENT, "rows of %s start on 16-byte boundaries: pointer and strides", name);
+  if (!aligned(p, 16) || row.stride % 8 || head.stride % 8 || row.stride < 0 || head.stride < 0) return fail(OFA_BAD_ARGUMENT, "rows of %s start on 16-byte boundaries: pointer and strides", name);
+  if (written && overlap(row, head, {0, 1}, dim)) return fail(OFA_BAD_ARGUMENT, "rows of %s overlap: strides %lld and %lld", name, row.stride, head.stride);
   return OFA_OK;
 }
 
@@ -68,8 +82,11 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
   paged::MoveArgs P;
   if (int rc = check_cache(c, b, n_rows, P.b, P.c)) return rc;
   if (n_rows == 0 || b->n_seqs == 0) return OFA_OK;
-  if (int rc = check_rows("k", k, k_row, k_head)) return rc;
-  if (int rc = check_rows("v", v, v_row, v_head)) return rc;
+  if (int rc = check_rows("k", k, {k_row, n_rows}, {k_head, c->n_kv_heads}, c->head_dim, READ)) return rc;
+  if (int rc = check_rows("v", v, {v_row, n_rows}, {v_head, c->n_kv_heads}, c->head_dim, READ)) return rc;
+  if (!READ && (overlap({c->page_stride, c->n_pages}, {c->head_stride, c->n_kv_heads}, {c->row_stride, c->page_size}, c->head_dim) ||
+                (c->dtype == OFA_KV_E4M3 && overlap({c->scale_page_stride, c->n_pages}, {c->scale_head_stride, c->n_kv_heads}, {c->scale_row_stride, c->page_size}, 1))))
+    return fail(OFA_BAD_ARGUMENT, "rows of the cache overlap");
   P.k = static_cast<bf16*>(k); P.v = static_cast<bf16*>(v); P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
   P.n_kv_heads = c->n_kv_heads; P.pair.set(2u * (unsigned)c->n_kv_heads);
   // four pieces of 16 bytes for a thread where there are rows for it: a block then amortises the search for its sequences
@@ -218,8 +235,8 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   if ((long long)a->n_rows * group > 0x7fffff00ll || (long long)a->n_rows * a->n_heads > 0x7fffff00ll * 4)
     return fail(OFA_BAD_ARGUMENT, "%d rows of %d heads are too many for one call", a->n_rows, a->n_heads);
   if (a->n_rows == 0 || batch->n_seqs == 0) return OFA_OK;
-  if (int rc = check_rows("q", a->q, a->q_row_stride, a->q_head_stride)) return rc;
-  if (int rc = check_rows("out", a->out, a->out_row_stride, a->out_head_stride)) return rc;
+  if (int rc = check_rows("q", a->q, {a->q_row_stride, a->n_rows}, {a->q_head_stride, a->n_heads}, cache->head_dim, false)) return rc;
+  if (int rc = check_rows("out", a->out, {a->out_row_stride, a->n_rows}, {a->out_head_stride, a->n_heads}, cache->head_dim, true)) return rc;
   if (!aligned(a->lse, 4)) return fail(OFA_BAD_ARGUMENT, "lse is misaligned");
   const Plan p = plan(cache, batch, a->n_rows, a->n_heads);
   if (p.bytes && (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)))
@@ -236,7 +253,9 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   cudaError_t e;
   if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p, s) : attend<128, true>(P, p, s);
   else e = cache->head_dim == 64 ? attend<64, false>(P, p, s) : attend<128, false>(P, p, s);
-  return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
+  if (e == cudaSuccess) return OFA_OK;
+  cudaGetLastError();                                            // reported here, not by the next call
+  return fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
 }
 
 extern "C" size_t ofa_paged_attention_workspace(const ofa_kv_cache* cache, const ofa_kv_batch* batch, int n_rows, int n_heads) {
@@ -251,12 +270,22 @@ extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
   if (a->dtype != OFA_DTYPE_BF16 && a->dtype != OFA_DTYPE_F32) return fail(OFA_BAD_ARGUMENT, "logits dtype %d is neither OFA_DTYPE_BF16 nor OFA_DTYPE_F32", a->dtype);
   if (a->n_rows < 0 || a->vocab < 0 || a->max_tokens < 0 || a->max_bias < 0) return fail(OFA_BAD_ARGUMENT, "negative size: n_rows %d, vocab %d, max_tokens %d, max_bias %d", a->n_rows, a->vocab, a->max_tokens, a->max_bias);
   if (a->n_rows > 65535) return fail(OFA_BAD_ARGUMENT, "n_rows %d: at most 65535", a->n_rows);
+  if (a->vocab > 1 << 30 || a->max_tokens > 1 << 29 || a->max_bias > 1 << 29)
+    return fail(OFA_BAD_ARGUMENT, "vocab %d, max_tokens %d, max_bias %d: at most 2^30, 2^29 and 2^29", a->vocab, a->max_tokens, a->max_bias);
   if (a->n_rows == 0 || a->vocab == 0) return OFA_OK;
   const size_t es = a->dtype == OFA_DTYPE_F32 ? 4 : 2;
   if (!a->in || !a->out) return fail(OFA_BAD_ARGUMENT, "logits are null");
   if (!aligned(a->in, es) || !aligned(a->out, es)) return fail(OFA_BAD_ARGUMENT, "misaligned logits");
   if (a->out_stride < a->vocab && a->n_rows > 1) return fail(OFA_BAD_ARGUMENT, "rows of out overlap: stride %lld, vocab %d", a->out_stride, a->vocab);
   if (a->in_stride < 0 || a->tokens_stride < 0 || a->bias_stride < 0 || a->mask_stride < 0) return fail(OFA_BAD_ARGUMENT, "negative stride");
+  {                                                              // in place, or apart: a row of out that lies on others of in would be read after it was written
+    const intptr_t d = reinterpret_cast<intptr_t>(a->out) - reinterpret_cast<intptr_t>(a->in), row = (intptr_t)(a->vocab * es), st = (intptr_t)(a->out_stride * es);
+    const intptr_t in_end = (intptr_t)((a->n_rows - 1) * a->in_stride * es) + row, out_end = (a->n_rows - 1) * st + row;
+    const bool same = a->n_rows == 1 || a->in_stride == a->out_stride;
+    const intptr_t off = st > 0 ? ((d % st) + st) % st : d;      // with equal strides: how far a row of out begins behind one of in
+    const bool apart = d >= in_end || -d >= out_end || (a->n_rows > 1 && same && off >= row && st - off >= row);
+    if (!apart && !(d == 0 && same)) return fail(OFA_BAD_ARGUMENT, "out and in overlap and are not the same");
+  }
   if ((a->repetition || a->presence || a->frequency) && !a->tokens && a->max_tokens > 0) return fail(OFA_BAD_ARGUMENT, "penalties need tokens");
   if (!a->bias_ids != !a->bias) return fail(OFA_BAD_ARGUMENT, "bias_ids and bias come together");
   if (!aligned(a->tokens, 4) || !aligned(a->n_tokens, 4) || !aligned(a->n_prompt, 4) || !aligned(a->repetition, 4) || !aligned(a->presence, 4) || !aligned(a->frequency, 4) ||

@@ -9,7 +9,7 @@ paged cache" part of include/ofa_b200.h, which says what each computes.
     logits_process(logits, tokens=..., repetition=..., mask=..., out=logits)    # penalties, biases, a grammar's mask
 
 Nothing is copied, cast or made contiguous behind the caller's back: a tensor of another type, device or layout than an operator takes is refused with an
-OfaError. No call waits for the device or reads from it. Index tensors are int32 and are read by the kernels, so a captured graph sees what they hold when it
+OfaError. No call waits for the device or reads from it, and results carry no gradient. Index tensors are int32 and are read by the kernels, so a captured graph sees what they hold when it
 is replayed.
 """
 import ctypes as C
@@ -244,21 +244,21 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
     """Attention of q [n_rows, n_heads, head_dim] (bf16) over the batch's pages; scale: 1/sqrt(head_dim) by default. Returns out, of q's shape, or with
     with_lse (out, lse [n_rows, n_heads] fp32). Rows that no sequence brings are left as they were."""
     _same_device(cache, batch)
+    if out is None:
+        if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype is not _BF16:
+            _rows("q", q, None, cache)
+        out = torch.empty_like(q)
     try:
         n_rows, n_heads, _ = q.shape
     except (AttributeError, ValueError):
         _rows("q", q, None, cache)
         raise
-    if out is None:
-        if not q.is_cuda or q.dtype is not _BF16:
-            _rows("q", q, None, cache)
-        out = torch.empty_like(q)
     lse = torch.empty_strided((n_rows, n_heads), (n_heads, 1), dtype=_F32, device=cache.device) if with_lse else None
     key = (cache.c.dtype, cache.head_dim, cache.n_kv_heads, cache.page_size, n_rows, n_heads)
     need = batch._need.get(key)
     if need is None:
         need = batch._need[key] = _lib().ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
-    # from the caller's allocator: a graph that captures the call keeps its own
+    # from torch's allocator: a graph that captures the call keeps its own
     work = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=cache.device) if need else None
     scale = cache.scale if scale is None else scale
     f = _fast()

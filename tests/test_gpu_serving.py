@@ -602,9 +602,9 @@ def test_tensors_that_do_not_fit_are_refused(sv, ofa, monkeypatch, extension):
         with pytest.raises(ofa.OfaError):
             sv.kv_append(cache, batch, k, bad)
     for bad in (q.float(), q[..., :32], torch.randn(3, 4, 128, device=DEV).bfloat16()[..., ::2], q.cpu(), q[0], None, q[:, :3], torch.randn(3, 4, 65, device=DEV).bfloat16()[..., 1:]):
-        with pytest.raises((ofa.OfaError, AttributeError, ValueError)):
+        with pytest.raises(ofa.OfaError):
             sv.paged_attention(cache, batch, bad)
-    for more in ({"window": -1}, {"window": 3, "causal": False}, {"scale": math.nan}, {"out": q.float()}, {"out": torch.empty_like(q)[:2]}):
+    for more in ({"window": -1}, {"window": 3, "causal": False}, {"scale": math.nan}, {"out": q.float()}, {"out": torch.empty_like(q)[:2]}, {"out": torch.empty_like(q)[:1].expand(3, -1, -1)}):
         with pytest.raises(ofa.OfaError):
             sv.paged_attention(cache, batch, q, **more)
     with pytest.raises(ofa.OfaError):
@@ -617,7 +617,7 @@ def test_tensors_that_do_not_fit_are_refused(sv, ofa, monkeypatch, extension):
     t, f = i32([[1, 2], [3, 4], [5, 6]]), torch.ones(3, device=DEV)
     for more in ({"n_tokens": n}, {"repetition": f}, {"tokens": t.long()}, {"tokens": t, "n_tokens": n.long()}, {"tokens": t[:2]}, {"tokens": t, "repetition": f.double()}, {"tokens": t, "presence": f[:2]},
                  {"bias_ids": t}, {"bias": torch.ones(3, 2, device=DEV)}, {"bias_ids": t, "bias": torch.ones(3, 3, device=DEV)}, {"mask": i32([[1] * 3] * 3)}, {"mask": i32([[1] * 4] * 2)},
-                 {"out": x.bfloat16()}, {"out": x[:2]}, {"out": x.t()}, {"tokens": t.t().contiguous().t()}, {"mask": torch.zeros(3, 4, dtype=torch.int32)}):
+                 {"out": x.bfloat16()}, {"out": x[:2]}, {"out": x.t()}, {"tokens": t.t().contiguous().t()}, {"mask": torch.zeros(3, 4, dtype=torch.int32)}, {"out": x[:1].expand(3, -1)}):
         with pytest.raises(ofa.OfaError):
             sv.logits_process(x, **more)
     for bad in (x.half(), x[0], x.cpu(), x.t(), x[:, ::2]):
@@ -636,3 +636,56 @@ def test_tensors_that_do_not_fit_are_refused(sv, ofa, monkeypatch, extension):
         sv.KVBatch(i32([0, 1, 2, 3]), n, t, status=torch.zeros(0, dtype=torch.int32, device=DEV))
     with pytest.raises(ofa.OfaError):
         sv.KVBatch(i32([0, 1, 2, 3]), n, t, max_new=-1)
+
+
+@pytest.mark.parametrize("new,kv", [([1], [400]), ([1] * 70, [300] * 70), ([3, 1], [40, 900]), ([60], [90]), ([130, 3], [3000, 3])])
+def test_attention_in_the_place_of_its_queries(sv, new, kv):
+    """blocks that share a tile's keys, tiles walked one after the other (a hint that is too small), both kernels"""
+    for hints in ({}, {"max_new": 1, "max_kv": max(kv)}):
+        cache, batch, g = make(sv, new, kv, 2, 64, 16, **hints)
+        q = queries(g, sum(new), 8, 64)
+        want = sv.paged_attention(cache, batch, q)
+        assert sv.paged_attention(cache, batch, q, out=q) is q and torch.equal(q, want)
+
+
+def test_logits_side_by_side_in_one_tensor(sv):
+    x, a, mask = logit_inputs(6, 333, 30, 4, torch.float32)
+    a = {k: v.to(DEV) for k, v in a.items()} | {"mask": mask.to(DEV)}
+    both = torch.zeros(6, 700, device=DEV)
+    both[:, :333] = x.to(DEV)
+    want = sv.logits_process(both[:, :333], **a)
+    sv.logits_process(both[:, :333], **a, out=both[:, 367:])
+    assert torch.equal(both[:, 367:], want) and torch.equal(both[:, :333], x.to(DEV)) and not both[:, 333:367].any()
+    sv.logits_process(both[:, :333], **a, out=both[:, :333])
+    assert torch.equal(both[:, :333], want)
+
+
+def test_two_graphs_share_nothing(sv):
+    """each keeps its own workspace; replayed in turns and on two streams at once, after the eager tensors are gone"""
+    jobs = []
+    for seed, new, kv in ((1, [1, 1], [3000, 2500]), (2, [1, 1, 1], [4000, 100, 2000])):
+        cache, batch, g = make(sv, new, kv, 1, 128, 16, seed=seed, max_new=1)
+        q = queries(g, sum(new), 4, 128)
+        want = sv.paged_attention(cache, batch, q)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = sv.paged_attention(cache, batch, q)
+        jobs.append((graph, out, want, s, (cache, batch, q)))
+    torch.cuda.synchronize()
+    junk = [torch.full((1 << 20,), math.nan, device=DEV) for _ in range(8)]
+    for _ in range(5):
+        for graph, out, *_ in jobs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, out, want, s, _ in jobs:
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, want, *_ in jobs:
+            assert torch.equal(out, want)
+        for graph, out, want, *_ in jobs:
+            graph.replay()
+            assert torch.equal(out, want)
+    del junk

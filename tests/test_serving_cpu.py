@@ -70,11 +70,33 @@ def test_bad_rows(ofa, args):
 @pytest.mark.parametrize("change,say", [({"n_heads": 3}, "multiple"), ({"n_heads": 0}, "multiple"), ({"n_rows": -1}, "negative"), ({"window": -1}, "window"), ({"window": 5, "causal": 0}, "window"),
                                         ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"), ({"q": None}, "q is null"), ({"out": None}, "out is null"),
                                         ({"q": P + 4}, "16-byte"), ({"out_row_stride": 252}, "16-byte"), ({"q_head_stride": -64}, "16-byte"), ({"lse": P + 2}, "lse"),
-                                        ({"n_rows": 2 ** 31 - 1, "n_heads": 2 ** 16}, "too many")])
+                                        ({"n_rows": 2 ** 31 - 1, "n_heads": 2 ** 16}, "too many"), ({"n_rows": 2 ** 30, "n_heads": 2 ** 16}, "too many")])
 def test_bad_attention(ofa, change, say):
     K, lib = ofa.capi, ofa.capi.load()
     assert lib.ofa_paged_attention(C.byref(cache(K)), C.byref(batch(K)), C.byref(attention_args(K, **change)), None) == K.BAD_ARGUMENT
     assert say in lib.ofa_serving_last_error().decode()
+
+
+def test_rows_that_overlap_where_they_are_written(ofa):
+    K, lib = ofa.capi, ofa.capi.load()
+    said = lambda: lib.ofa_serving_last_error().decode()  # noqa: E731
+    for strides in ((0, 64, 128, 64), (128, 0, 128, 64), (128, 64, 64, 64), (128, 64, 128, 56), (128, 64, 64, 128)):
+        assert lib.ofa_kv_read(C.byref(cache(K)), C.byref(batch(K)), P, P, 3, *strides, None) == K.BAD_ARGUMENT and "overlap" in said()
+    for change in ({"row_stride": 0}, {"head_stride": 0}, {"page_stride": 0}, {"row_stride": 56}, {"head_stride": 64}, {"dtype": 1, "k_scale": P, "v_scale": P, "scale_row_stride": 0},
+                   {"dtype": 1, "k_scale": P, "v_scale": P, "scale_page_stride": 16}):
+        assert lib.ofa_kv_append(C.byref(cache(K, **change)), C.byref(batch(K)), P, P, 3, 128, 64, 128, 64, None) == K.BAD_ARGUMENT and "overlap" in said()
+    for change in ({"out_row_stride": 0}, {"out_row_stride": 192}, {"out_head_stride": 0}, {"out_head_stride": 56}):
+        assert lib.ofa_paged_attention(C.byref(cache(K)), C.byref(batch(K)), C.byref(attention_args(K, **change)), None) == K.BAD_ARGUMENT and "overlap" in said()
+
+
+@pytest.mark.parametrize("rows,vocab,ins,outs,off", [(3, 100, 100, 100, 1), (3, 100, 100, 100, -1), (3, 100, 100, 100, 100), (3, 100, 200, 200, 99), (3, 100, 200, 200, 101),
+                                                        (3, 100, 200, 100, 0), (3, 100, 100, 200, 0), (1, 100, 100, 100, 99), (3, 100, 0, 100, 0), (3, 100, 0, 100, 50)])
+def test_logits_that_overlap(ofa, rows, vocab, ins, outs, off):
+    """The calls that are allowed (in place, side by side in one tensor) run in the GPU's tests"""
+    K, lib = ofa.capi, ofa.capi.load()
+    a = K.LogitsArgs()
+    a.dtype, a.n_rows, a.vocab, a.inp, a.out, a.in_stride, a.out_stride = K.DTYPE_F32, rows, vocab, P, P + off * 4, ins, outs
+    assert lib.ofa_logits_process(C.byref(a), None) == K.BAD_ARGUMENT and "overlap" in lib.ofa_serving_last_error().decode()
 
 
 def test_a_workspace_that_is_too_small(ofa):
@@ -99,7 +121,7 @@ def test_empty_calls_launch_nothing(ofa):
 
 @pytest.mark.parametrize("change,say", [({"dtype": 7}, "dtype"), ({"n_rows": -1}, "negative"), ({"n_rows": 70000}, "65535"), ({"inp": None}, "null"), ({"out": P + 2}, "misaligned"),
                                         ({"out_stride": 50}, "overlap"), ({"in_stride": -100}, "negative"), ({"repetition": P, "max_tokens": 4}, "tokens"), ({"bias": P}, "together"),
-                                        ({"mask": P + 1}, "misaligned"), ({"max_bias": -1}, "negative")])
+                                        ({"mask": P + 1}, "misaligned"), ({"max_bias": -1}, "negative"), ({"vocab": 2 ** 30 + 1}, "2^30"), ({"tokens": P, "max_tokens": 2 ** 29 + 1}, "2^29")])
 def test_bad_logits(ofa, change, say):
     K, lib = ofa.capi, ofa.capi.load()
     a = K.LogitsArgs()
