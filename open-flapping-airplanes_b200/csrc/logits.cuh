@@ -5,12 +5,17 @@
 //   x = -inf where the mask's bit is 0
 // In fp32 whatever the logits' type, rounded once. Bound by reading and writing the logits.
 //
-// A block takes a stretch of one row's vocabulary. It streams the logits through with the mask alone, and then changes those few that the history or a bias names:
-// every block reads its row's whole history (from L2 after the first), counts what falls into its stretch in a word for each token in shared memory (integer atomics, whose order does
-// not matter; no sort, no pass over [rows][vocab] counters). Who makes a token's word other than 0 puts it on a list, and the listed tokens are finished from what the stream left in their
-// places (where the list is too short, by a second look at the history). Looking at a token's word for every logit instead, with the arithmetic of a hit inlined 32 times, took 47 us
-// where this takes 29 (192 rows of 100,352 bf16); a second look at the history in every block 31. A bias marks its token's word; the entries of its list are added in their order. Stretches begin where a row's 16-byte vectors do, so a row that starts between two boundaries loses only its first and last vector to single
-// elements.
+// Every stretch of a row needs its own tokens' counts, of the row's whole history. Two ways:
+//   process_kernel alone: a block streams a stretch of one row's vocabulary through with the mask, and then changes those few logits that the history or a bias names: it reads the
+//     row's whole history (from L2 after the first block), counts what falls into its stretch in a word for each token in shared memory (integer atomics, whose order does
+//     not matter) and puts who makes a token's word other than 0 on a list, whose tokens are finished from what the stream left in their places (where the list is
+//     too short, by a second look at the history). One launch, for calls of few rows: 4 rows of 50,304 fp32 in 3.4 us.
+//   process_kernel for the stream and mask, touch_kernel for the named logits: a block a row counts the history in a hash table of shared memory, large enough for every entry to be
+//     another token, while the last blocks of the stream still run. For calls that fill the machine, whose stream is then free of counters: 192 rows of 100,352 bf16 up to 2,000
+//     tokens each take 30 us the first way, 21.5 this way, the stream alone 15. What is left are the named logits' sectors, which go to memory twice. (Looking at a token's word for
+//     every logit, with the arithmetic of a hit inlined 32 times, took 47.)
+// A bias marks its token's word; the entries of its list are added in their order. Stretches begin where a row's 16-byte vectors do, so a row that starts between two boundaries
+// loses only its first and last vector to single elements.
 #pragma once
 #include "common.cuh"
 
@@ -26,11 +31,31 @@ struct Args {
   const float *repetition, *presence, *frequency;
   const int* bias_ids; const float* bias; long long bias_row; int max_bias;
   const unsigned* mask; long long mask_row;
+  int slots_log2;                                              // touch_kernel: of its table
 };
 constexpr int LISTED = 1024;
 constexpr unsigned PROMPT = 1u << 31, BIASED = 1u << 30;      // a token's word: in the prompt, has a bias; the rest counts where it stands behind the prompt
 
-template <class T, int VECS, bool WIDE>
+// A named token's logit with its word c and the sum of its biases
+struct Row { float rep, pres, freq; const int* ids; const float* val; };
+__device__ __forceinline__ Row row_of(const Args& P, int row) {
+  return {P.repetition ? __ldg(P.repetition + row) : 1.f, P.presence ? __ldg(P.presence + row) : 0.f, P.frequency ? __ldg(P.frequency + row) : 0.f,
+          P.bias_ids + (long long)row * P.bias_row, P.bias + (long long)row * P.bias_row};
+}
+__device__ __forceinline__ float bias_of(const Args& P, const Row& R, int t) {
+  float s = 0.f;
+#pragma unroll 4
+  for (int j = 0; j < P.max_bias; j++) if (__ldg(R.ids + j) == t) s += __ldg(R.val + j);
+  return s;
+}
+__device__ __forceinline__ float touched(const Row& R, float f, unsigned c, float bias) {
+  const unsigned made = c & ~(PROMPT | BIASED);
+  if (made || (c & PROMPT)) f = f > 0.f ? f / R.rep : f * R.rep;
+  if (made) f = f - R.freq * (float)made - R.pres;
+  return c & BIASED ? f + bias : f;
+}
+
+template <class T, int VECS, bool WIDE, bool WORDS>
 __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Args P) {
   constexpr int VN = Vec<T>::N, S = 256 * VN * VECS;           // tokens of a block
   extern __shared__ __align__(16) unsigned count[];
@@ -39,7 +64,8 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
   const T* in = reinterpret_cast<const T*>(P.in) + (long long)row * P.in_row;
   T* out = reinterpret_cast<T*>(P.out) + (long long)row * P.out_row;
   const int v0 = (int)blockIdx.x * S - (WIDE ? (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T)) : 0);
-  const bool words = P.tokens || P.bias_ids;
+  const bool words = WORDS && (P.tokens || P.bias_ids);
+  if (!WORDS) cudaTriggerProgrammaticLaunchCompletion();       // touch_kernel may begin to count
   uint4 x[VECS];
 #pragma unroll
   for (int k = 0; k < VECS; k++) {
@@ -64,11 +90,16 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
     if (P.tokens) {
       n = P.n_tokens ? min(max(__ldg(P.n_tokens + row), 0), P.max_tokens) : P.max_tokens;
       const int first = P.n_prompt ? __ldg(P.n_prompt + row) : 0;
-#pragma unroll 4
-      for (int i = tid; i < n; i += 256) {
-        const int t = __ldg(text + i);
-        unsigned* w = word(t);
-        if (w && (i < first ? atomicOr(w, PROMPT) : atomicAdd(w, 1u)) == 0) put(t);
+      for (int base = tid; base < P.max_tokens; base += 1024) {
+        int t[4];                                              // asked for side by side, and without waiting for how many count
+#pragma unroll
+        for (int u = 0; u < 4; u++) t[u] = base + u * 256 < P.max_tokens ? __ldg(text + base + u * 256) : -1;
+        if (base >= n) break;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          unsigned* w = base + u * 256 < n ? word(t[u]) : nullptr;
+          if (w && (base + u * 256 < first ? atomicOr(w, PROMPT) : atomicAdd(w, 1u)) == 0) put(t[u]);
+        }
       }
     }
     if (P.bias_ids)
@@ -97,8 +128,7 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
   }
   if (!words) return;
   __syncthreads();
-  const float* val = P.bias + (long long)row * P.bias_row;
-  const float rep = P.repetition ? __ldg(P.repetition + row) : 1.f, pres = P.presence ? __ldg(P.presence + row) : 0.f, freq = P.frequency ? __ldg(P.frequency + row) : 0.f;
+  const Row R = row_of(P, row);
   const bool all = listed <= LISTED;
 #pragma unroll 1
   for (int i = tid; i < (all ? listed : n + P.max_bias); i += 256) {           // max_bias is 0 without biases
@@ -106,18 +136,81 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
     unsigned* w = word(t);
     const unsigned c = w ? atomicExch(w, 0u) : 0u;
     if (!c || (mask && !(__ldg(mask + (t >> 5)) >> (t & 31) & 1))) continue;
-    const unsigned made = c & ~(PROMPT | BIASED);
-    float f = to_f(out[t]);
-    if (made || (c & PROMPT)) f = f > 0.f ? f / rep : f * rep;
-    if (made) f = f - freq * (float)made - pres;
-    if (c & BIASED) {
-      float s = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < P.max_bias; j++) if (__ldg(ids + j) == t) s += __ldg(val + j);
-      f += s;
-    }
-    out[t] = from_f<T>(f);
+    out[t] = from_f<T>(touched(R, to_f(out[t]), c, c & BIASED ? bias_of(P, R, t) : 0.f));
   }
+}
+
+// The named logits of a row, behind the stream. The table holds a token + 1, its word and the sum of its biases, which each thread with one of them forms (the same
+// value). With a quarter of the slots in use few lanes probe twice; at a half a warp's longest chain of atomics took 6 us. All that needs only the tokens is
+// asked for side by side, before it is known how many count and while the stream still runs.
+template <class T> __global__ void __launch_bounds__(512) touch_kernel(const __grid_constant__ Args P) {
+  extern __shared__ __align__(16) unsigned table[];
+  const int tid = threadIdx.x, row = blockIdx.x, slots = 1 << P.slots_log2, most = P.tokens ? P.max_tokens : 0, named = most + P.max_bias;
+  unsigned *keys = table, *words = table + slots;
+  float* sums = reinterpret_cast<float*>(words + slots);
+  const T* in = reinterpret_cast<const T*>(P.in) + (long long)row * P.in_row;
+  T* out = reinterpret_cast<T*>(P.out) + (long long)row * P.out_row;
+  const unsigned* mask = P.mask ? P.mask + (long long)row * P.mask_row : nullptr;
+  const int* text = P.tokens + (long long)row * P.tokens_row;
+  const Row R = row_of(P, row);
+  const int n = !P.tokens ? 0 : P.n_tokens ? __ldg(P.n_tokens + row) : most, first = P.tokens && P.n_prompt ? __ldg(P.n_prompt + row) : 0;
+  constexpr int U = 4;                                         // entries of a thread: of the history, then the biases
+  int t[U];
+  T x[U];
+  unsigned allowed[U];
+  auto ask = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = base + u * 512;
+      t[u] = i < most ? __ldg(text + i) : i < named ? __ldg(R.ids + i - most) : -1;
+      if ((unsigned)t[u] >= (unsigned)P.vocab || (i < most && i >= n)) t[u] = -1;
+    }
+  };
+  auto count = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (t[u] < 0) continue;
+      const int i = base + u * 512;
+      unsigned at = (unsigned)t[u] * 2654435769u >> (32 - P.slots_log2);        // Fibonacci hashing
+      while (true) {                                           // ends: there are more slots than entries
+        const unsigned was = atomicCAS(keys + at, 0u, (unsigned)t[u] + 1);
+        if (was == 0 || was == (unsigned)t[u] + 1) break;
+        at = (at + 1) & (slots - 1);
+      }
+      if (i >= most) { sums[at] = bias_of(P, R, t[u]); atomicOr(words + at, BIASED); }
+      else if (i < first) atomicOr(words + at, PROMPT);
+      else atomicAdd(words + at, 1u);
+    }
+  };
+  auto look = [&] {                                            // the logits as they came: in place the stream writes back what it read
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      allowed[u] = t[u] < 0 ? 0u : mask ? __ldg(mask + (t[u] >> 5)) >> (t[u] & 31) : 1u;
+      x[u] = in[max(t[u], 0)];
+    }
+  };
+  auto finish = [&] {                                          // by the first thread that comes for a token
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (!(allowed[u] & 1)) continue;
+      unsigned at = (unsigned)t[u] * 2654435769u >> (32 - P.slots_log2);
+      while (keys[at] != (unsigned)t[u] + 1) at = (at + 1) & (slots - 1);      // it is there
+      if (const unsigned c = atomicExch(words + at, 0u)) out[t[u]] = from_f<T>(touched(R, to_f(x[u]), c, sums[at]));
+    }
+  };
+  ask(tid);
+  for (int i = tid; i < slots / 2; i += 512) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  if (named > 512 * U)
+    for (int base = tid + 512 * U; base < named; base += 512 * U) { ask(base); count(base); }
+  if (named > 512 * U) ask(tid);
+  look();
+  count(tid);
+  __syncthreads();
+  cudaGridDependencySynchronize();
+  finish();
+  if (named > 512 * U)
+    for (int base = tid + 512 * U; base < named; base += 512 * U) { ask(base); look(); finish(); }
 }
 
 }  // namespace logits

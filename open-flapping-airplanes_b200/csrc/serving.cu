@@ -201,14 +201,29 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   return e;
 }
 
-// Four vectors a thread where that still gives every SM several blocks, else one: each block reads its row's whole history
-template <class T, bool WIDE> void process(const logits::Args& P, int rows, cudaStream_t s) {
+// Where four vectors a thread still give every SM several blocks: the stream, and a block for each row's named tokens if they fit its table; else one kernel, with one
+// vector a thread for few rows, since each block reads its row's whole history.
+template <class T, bool WIDE> cudaError_t process(logits::Args& P, int rows, cudaStream_t s) {
   const int vn = Vec<T>::N, span = P.vocab + (WIDE ? vn - 1 : 0);
-  const bool large = (long long)rows * ((span + 1024 * vn - 1) / (1024 * vn)) >= 4 * 148;
+  const bool large = (long long)rows * ((span + 1024 * vn - 1) / (1024 * vn)) >= 4 * 148, words = P.tokens || P.bias_ids;
   const int stretch = (large ? 1024 : 256) * vn;
   const dim3 grid((unsigned)((span + stretch - 1) / stretch), (unsigned)rows);
-  const unsigned smem = P.tokens || P.bias_ids ? (unsigned)stretch * 4 : 0;
-  if (large) logits::process_kernel<T, 4, WIDE><<<grid, 256, smem, s>>>(P); else logits::process_kernel<T, 1, WIDE><<<grid, 256, smem, s>>>(P);
+  const long long named = (P.tokens ? P.max_tokens : 0) + (long long)P.max_bias;
+  if (!large || (words && named > 8192)) {
+    const unsigned smem = words ? (unsigned)stretch * 4 : 0;
+    if (large) logits::process_kernel<T, 4, WIDE, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<T, 1, WIDE, true><<<grid, 256, smem, s>>>(P);
+    return cudaGetLastError();
+  }
+  logits::process_kernel<T, 4, WIDE, false><<<grid, 256, 0, s>>>(P);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !words) return e;
+  for (P.slots_log2 = 9; P.slots_log2 < 14 && 1ll << P.slots_log2 < 4 * named;) P.slots_log2++;
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization; at.val.programmaticStreamSerializationAllowed = 1;
+  lc.gridDim = dim3((unsigned)rows); lc.blockDim = dim3(512); lc.dynamicSmemBytes = (size_t)12 << P.slots_log2; lc.stream = s; lc.attrs = &at; lc.numAttrs = 1;
+  e = allow<logits::touch_kernel<T>>(12 << 14);
+  return e == cudaSuccess ? cudaLaunchKernelEx(&lc, logits::touch_kernel<T>, P) : e;
 }
 
 }  // namespace
@@ -300,7 +315,9 @@ extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // whole 16-byte vectors where rows of in and out lie alike against their boundaries (an odd vocabulary moves both from row to row)
   const bool wide = (reinterpret_cast<uintptr_t>(a->in) - reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 && (a->n_rows == 1 || ((a->in_stride - a->out_stride) * (long long)es) % 16 == 0);
-  if (a->dtype == OFA_DTYPE_F32) wide ? process<float, true>(P, a->n_rows, s) : process<float, false>(P, a->n_rows, s);
-  else wide ? process<bf16, true>(P, a->n_rows, s) : process<bf16, false>(P, a->n_rows, s);
-  return launched("ofa_logits_process");
+  const cudaError_t e = a->dtype == OFA_DTYPE_F32 ? wide ? process<float, true>(P, a->n_rows, s) : process<float, false>(P, a->n_rows, s)
+                                                  : wide ? process<bf16, true>(P, a->n_rows, s) : process<bf16, false>(P, a->n_rows, s);
+  if (e == cudaSuccess) return OFA_OK;
+  cudaGetLastError();
+  return fail(OFA_CUDA_ERROR, "ofa_logits_process: %s", cudaGetErrorString(e));
 }

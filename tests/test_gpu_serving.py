@@ -365,6 +365,33 @@ def test_logits(sv, rows, vocab, history, biases, masked, dtype):
     assert (got[fine & over] == -math.inf).all() or (got[fine & over] == torch.finfo(dtype).min).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,history,biases,masked", [(700, 1000, 50, 6, True), (700, 300, 5000, 0, False), (620, 2000, 8300, 3, True), (170, 33001, 8000, 192, True), (170, 33001, 0, 7, False),
+                                                              (170, 33000, 0, 0, True), (9000, 5, 3, 1, True)])
+def test_logits_of_many_rows(sv, rows, vocab, history, biases, masked, dtype):
+    """bit by bit what a few of the rows give alone; some against the plain form"""
+    x, a, mask = logit_inputs(rows, vocab, history, biases, dtype, seed=3)
+    if masked:
+        a["mask"] = mask
+    dev, x = {k: v.to(DEV) for k, v in a.items()}, x.to(DEV)
+    got = sv.logits_process(x, **dev)
+    for r in range(0, rows, 8 if rows < 1000 else 500):
+        part = slice(r, r + 8)
+        assert torch.equal(got[part], sv.logits_process(x[part], **{k: v[part] for k, v in dev.items()}))
+    some = slice(rows - 3, rows)
+    want, tol = ref.logits(x[some], **{k: v[some] for k, v in a.items()})
+    tol = tol + (ref.F32_HALF if dtype == torch.float32 else ref.BF16_HALF) * (want.abs() + tol)
+    fine, have = torch.isfinite(want), got[some].double().cpu()
+    assert torch.equal(have[~fine], want[~fine]) and ((have - want).abs()[fine] <= tol[fine]).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = sv.logits_process(x, **dev)
+    again.zero_()
+    graph.replay()
+    assert torch.equal(again, got)
+    assert sv.logits_process(x, out=x, **dev) is x and torch.equal(x, got)
+
+
 def test_logits_of_strided_rows(sv):
     wide = torch.randn(4, 3000, device=DEV)
     x = wide[:, 5:1006]
