@@ -75,13 +75,6 @@ __device__ __forceinline__ int scale_byte(unsigned amax_bits) {
 // The bits of an e4m3 number, moved to where bf16 has sign, exponent and mantissa, are 2^-120 times its value (subnormals too); this is 2^120 times the
 // scale, as bf16 bits. One multiplication, exact, then gives the held value.
 __device__ __forceinline__ uint32_t scale_bits(int b) { return b == SCALE_NAN ? 0x7fc0u : (uint32_t)(min(b, E_MAX + 127) + 120) << 7; }
-// bytes 1 and 3 of w are e4m3 numbers; f holds the scale_bits of each -> two bf16
-__device__ __forceinline__ uint32_t widen(uint32_t w, uint32_t f) {
-  const uint32_t t = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(f));
-  return r;
-}
 // the largest magnitude's bits of eight bf16 numbers; an infinity or a NaN is the largest
 __device__ __forceinline__ unsigned max_bits(uint4 u) {
   unsigned m = 0;
@@ -90,17 +83,17 @@ __device__ __forceinline__ unsigned max_bits(uint4 u) {
   for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
   return m;
 }
-// Without the multiplication: two e4m3 numbers as bf16 of 2^-120 times their codes' values, three instructions. sel places them in bytes 0 and 2 with their signs
-// in the bytes above, so that one shift moves both. Factors are then applied to what is computed from them.
+// Two e4m3 numbers as bf16 of 2^-120 times their codes' values, three instructions. sel places them in bytes 0 and 2 with their signs in the bytes above, so that one shift moves both.
 __device__ __forceinline__ uint32_t raw_pair(uint32_t x, uint32_t y, uint32_t sel) {
   uint32_t w;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(x), "r"(y), "r"(sel));
   return (w << 4) & 0x87f087f0u;
 }
 __host__ __device__ constexpr uint32_t raw_sel(int a, int b) { return (uint32_t)(a | (8 | a) << 4 | b << 8 | (8 | b) << 12); }      // of bytes a and b of the eight in (x, y)
-// elements 2x, 2x+1 of the four in w
-__device__ __forceinline__ uint32_t widen_lo(uint32_t w, uint32_t f) { return widen(__byte_perm(w, 0, 0x1404), f); }
-__device__ __forceinline__ uint32_t widen_hi(uint32_t w, uint32_t f) { return widen(__byte_perm(w, 0, 0x3424), f); }
+// elements 0 and 1, or 2 and 3, of the four in w; f holds the scale_bits of each
+__device__ __forceinline__ uint32_t scaled(uint32_t t, uint32_t f) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(f)); return r; }
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w, uint32_t f) { return scaled(raw_pair(w, w, raw_sel(0, 1)), f); }
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w, uint32_t f) { return scaled(raw_pair(w, w, raw_sel(2, 3)), f); }
 
 }  // namespace paged
 }  // namespace ofa

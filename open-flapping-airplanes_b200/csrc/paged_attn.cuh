@@ -135,7 +135,7 @@ template <int D, bool E4M3, int NR> struct Few {
 
 // one held element as a float (the rare path)
 template <bool E4M3> __device__ float held(const char* row, int d, int scale) {
-  if constexpr (E4M3) return __uint_as_float(widen((uint32_t)*reinterpret_cast<const unsigned char*>(row + d) << 8, scale_bits(scale)) << 16);
+  if constexpr (E4M3) return __uint_as_float(widen_lo(*reinterpret_cast<const unsigned char*>(row + d), scale_bits(scale)) << 16);
   return to_f(reinterpret_cast<const bf16*>(row)[d]);
 }
 

@@ -12,7 +12,7 @@
 //              One thread a tile because one issues a tcgen05.mma only every ~96 clocks and a 128 x 128 x 16 product takes 64
 //   copies     one warp asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
 //              (128-byte swizzle), 8-bit rows into a ring of their own
-//   workers    widen 8-bit rows from there into the tiles, once for the block's rows; look at values that some row must not meet; and gather the rows of pages that are no
+//   workers    widen 8-bit rows from there into the tiles, once for the block's rows, a worker on each scheduler; look at values that some row must not meet; and gather the rows of pages that are no
 //              multiple of 8 by cp.async, 16 bytes a lane
 // What bounds it: 128 keys of two tiles of heads of 128 take 3,400 clocks, of which the tensor pipe works 2,048 and the special-function unit, for 32,768 exponentials, as many.
 // Tensor memory: S of a tile in 128 columns (P in their last 64), O behind all S.
@@ -32,7 +32,7 @@ namespace paged {
 
 template <int D, bool E4M3> struct Tc {
   static constexpr int NT = D == 64 && !E4M3 ? 1 : 2, BLOCKS = 3 - NT;      // tiles of 128 rows a block, blocks an SM
-  static constexpr int WORKERS = NT == 1 ? 2 : 5, WARPS = 5 * NT + 1 + WORKERS, THREADS = 32 * WARPS;
+  static constexpr int WORKERS = NT == 1 ? 2 : E4M3 ? 4 : 5, WARPS = NT == 1 ? 8 : 16, THREADS = 32 * WARPS;      // 8-bit rows: a worker on each scheduler, one warp idle
   static constexpr int SOFT_REGS = 184, REST_REGS = 72;         // of a softmax thread, of another: together twice the launch's 128
   static constexpr int TMEM = NT * 256, O_AT = NT * 128;        // columns; S of a tile at tile * 128, O behind them
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
@@ -453,6 +453,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
       uses += 2u * (uint32_t)(k.B - k.A);
       if (!next(ok)) break;
     }
+  } else if (warp > 5 * NT + WK) {
+    set_regs<false, F::REST_REGS>();
+    for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) if (!next(true)) break;
   } else {
     // ------------------------------------------------------------------------------------------ workers
     set_regs<false, F::REST_REGS>();
@@ -489,8 +492,11 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         return x;
       };
       auto offset = [&](const Row& x) { return x.page >= 0 ? (long long)x.page * P.c.page_b + (long long)x.at * P.c.row_b : -1ll; };
+      // A row's scale byte as it comes from memory: anything done with it here would wait for it
       auto scale = [&](const Row& x, int item) {
-        return x.page >= 0 ? 256u | __ldg((item & 1 ? P.c.vs : P.c.ks) + (long long)x.page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)x.at * P.c.s_row) : 0u;
+        unsigned char s = 0;
+        if (x.page >= 0) s = __ldg((item & 1 ? P.c.vs : P.c.ks) + (long long)x.page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)x.at * P.c.s_row);
+        return s;
       };
       auto odd_at = [&](int key) { atomicMin(&ct.odd_lo, key); atomicMax(&ct.odd_hi, min(k.hi - 1, key)); };
       auto tile_free = [&](int item) {
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {
                 const int u = unit0(item) + (gr * 4 + y) * WK;
-                if (u >= 16) break;
+                if (16 % WK && u >= 16) break;
                 if (!(item & 1) && lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][u] = (uint8_t)(there >> y * 8);
                 long long o[IT];
 #pragma unroll
@@ -530,37 +536,43 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         };
         if (!P.run) for (int i = 0; i < F::RS - 1; i++) gather(i);
         Row ahead[GROUPS];
-        uint32_t next_f[GROUPS];
+        unsigned char next_f[GROUPS];
+        bool next_there[GROUPS];
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; gr++) { next_f[gr] = scale(known(row_of(0, gr)), 0); ahead[gr] = row_of(1, gr); }
+        for (int gr = 0; gr < GROUPS; gr++) {
+          const Row x = known(row_of(0, gr));
+          next_f[gr] = scale(x, 0); next_there[gr] = x.page >= 0; ahead[gr] = row_of(1, gr);
+        }
         for (int item = 0; item < total && ok; item++) {
           const uint32_t n = uses + (uint32_t)item, rs = n % F::RS;
           const int j = k.A + (item >> 1);
           const bool check = (item & 1) && partial(k, j);
-          uint32_t f[GROUPS];
-#pragma unroll
-          for (int gr = 0; gr < GROUPS; gr++) {
-            f[gr] = next_f[gr];
-            next_f[gr] = scale(known(ahead[gr]), item + 1);
-            ahead[gr] = row_of(item + 2, gr);
-          }
           if (P.run) ok = wait_for(smem_u32(&ct.raw_full[rs]), (n / F::RS) & 1);
           else { gather(item + F::RS - 1); cp_wait<F::RS - 1>(); __syncwarp(); }
           if (!__all_sync(0xffffffffu, ok) || !tile_free(item)) { ok = false; break; }
+          uint32_t f[GROUPS];                                    // 2^120 times the scale, as bf16; 0: rows that are not there become zeros
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; gr++) {
+            f[gr] = next_there[gr] ? scale_bits((int)next_f[gr]) : 0u;
+            const Row x = known(ahead[gr]);
+            next_f[gr] = scale(x, item + 1); next_there[gr] = x.page >= 0;
+            ahead[gr] = row_of(item + 2, gr);
+          }
           const unsigned char* src = smem + F::RAW_AT + rs * F::RAW;
           unsigned char* dst = smem + F::RING_AT + n % F::NST * F::TILE;
 #pragma unroll
           for (int gr = 0; gr < GROUPS; gr++) {
-            uint32_t mine = f[gr] ? scale_bits((int)(f[gr] & 255)) : 0u;      // rows that are not there become zeros
+            uint32_t mine = f[gr];
             if (check && mine == 0x7fc0u) { odd_at(j * 128 + (unit0(item) + (gr * 4 + (lane >> 3)) * WK) * 8 + (lane & 7)); mine = 0; }
             mine |= mine << 16;
 #pragma unroll
             for (int y = 0; y < 4; y++) {
               const int u = unit0(item) + (gr * 4 + y) * WK;
-              if (u >= 16) break;
+              if (16 % WK && u >= 16) break;
 #pragma unroll
               for (int i = 0; i < IT; i++) {
-                const int row = (i * 32 + lane) / CH, q = lane % CH, r = u * 8 + row;
+                // rows of 8 pieces in pairs, half of each to eight lanes, which then write to all the banks: two pieces of a tile's row lie side by side
+                const int row = CH == 8 ? i * 4 + ((lane >> 3) ^ (lane >> 2 & 1)) : (i * 32 + lane) / CH, q = lane % CH, r = u * 8 + row;
                 const uint32_t fr = __shfl_sync(0xffffffffu, mine, y * 8 + row);
                 const uint4 v = *reinterpret_cast<const uint4*>(src + F::raw_at(r, q));
                 *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * q)) = make_uint4(widen_lo(v.x, fr), widen_hi(v.x, fr), widen_lo(v.y, fr), widen_hi(v.y, fr));
@@ -614,7 +626,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {
                 const int u = unit0(item) + (gr * 4 + y) * WK;
-                if (u >= 16) break;
+                if (16 % WK && u >= 16) break;
                 if (!(item & 1) && lane == 0) ct.valid[j % F::NV][u] = (uint8_t)(there >> y * 8);
                 long long o[IT];                                 // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll
