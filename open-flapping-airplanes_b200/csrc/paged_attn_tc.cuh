@@ -2,12 +2,14 @@
 //
 // The rows of a key/value head (new tokens x the query heads that share it) are taken 128 at a time, a tile, and walk their keys 128 at a time. A block has two tiles, half
 // a step apart, so that the tensor pipe works for one while the softmax warps of the other do; heads of 64 with bf16 rows, whose tiles are small, have one tile a block and two blocks
-// an SM, which also covers a block's start and end (four prompts of 1,024 tokens, 12 heads: 32.1 -> 29.0 us). Roles of a block's warps:
+// an SM, which also covers a block's start and end (four prompts of 1,024 tokens, 12 heads: 32.1 -> 29.0 us). So have up to 64 rows of heads of 128 (drafts): their tile is 64 rows high, and warps
+// without rows only pass their signals on (5 tokens of 24 sequences over up to 2,000 keys, 32 heads over 8: 54.4 -> 41.2 us; of 64 sequences over 4,096: 236 -> 176, 6.1 TB/s; with two
+// tiles of keys and values instead of three on an SM's half 55 and 204). A block's start and end take 6 us, most of it instructions that are fetched for the first time: they are kept short, in rolled loops. Roles of a block's warps:
 //   softmax    four warps a tile, a thread per row (= tensor-memory lane): reads its 128 scores once, keeps maximum and sum, writes the probabilities
 //              back over the second half of them as bf16, the A operand of the second product
 //   products   a warp a tile, one thread of which issues, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
 //              soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores. (4,096 tokens over
-//              16,384 keys, heads of 128: 843 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
+//              16,384 keys, heads of 128: 838 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
 //              two threads a row, four softmax warps a scheduler: 910, bound by issue; a third of the exponentials by a polynomial on the multiply-add pipe: 970 and more, for registers and issue.)
 //              One thread a tile because one issues a tcgen05.mma only every ~96 clocks and a 128 x 128 x 16 product takes 64
 //   copies     one warp asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
@@ -30,18 +32,23 @@
 namespace ofa {
 namespace paged {
 
-template <int D, bool E4M3> struct Tc {
-  static constexpr int NT = D == 64 && !E4M3 ? 1 : 2, BLOCKS = 3 - NT;      // tiles of 128 rows a block, blocks an SM
+template <int D, bool E4M3, int NT> struct Tc {                 // NT tiles of 128 rows a block
+  static constexpr int BLOCKS = 3 - NT;                         // of an SM
+  // Rows of a tile that are used: 64 where two blocks of wide rows share an SM. Q's parts then lie 64 rows apart, which leaves room for a third tile of keys or values (products read
+  // the other 64 rows from whatever lies behind, and nobody looks at what comes of them)
+  static constexpr int ROWS = NT == 1 && D == 128 ? 64 : 128, Q_PART = ROWS * 128, Q_TILE = ROWS * D * 2;
   static constexpr int WORKERS = NT == 1 ? 2 : E4M3 ? 4 : 5, WARPS = NT == 1 ? 8 : 16, THREADS = 32 * WARPS;      // 8-bit rows: a worker on each scheduler, one warp idle
   static constexpr int SOFT_REGS = 184, REST_REGS = 72;         // of a softmax thread, of another: together twice the launch's 128
   static constexpr int TMEM = NT * 256, O_AT = NT * 128;        // columns; S of a tile at tile * 128, O behind them
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
-  static constexpr int NST = E4M3 ? (D == 128 ? 3 : 6) : 4;           // ring of K and V tiles
+  static constexpr int NST = E4M3 ? (D == 128 ? 3 : 6) : NT == 1 && D == 128 ? 3 : 4;           // ring of K and V tiles
   static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 4 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
   static constexpr int LAG = 1;                                 // gathered tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
-  static constexpr int Q_AT = 0, RING_AT = NT * TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
-  static constexpr int SMEM = CTRL_AT + 640 + 1024;             // 1,024 for the alignment of the swizzle's atoms
+  static constexpr int Q_AT = 0, RING_AT = NT * Q_TILE, RAW_AT = RING_AT + NST * TILE, CTRL_AT = RAW_AT + RS * RAW;
+  static constexpr int SMEM = CTRL_AT + 640;
+  static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "blocks of an SM");
+  static __device__ __forceinline__ uint32_t q_at(int row, int chunk) { return (uint32_t)((chunk >> 3) * Q_PART + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
   static __device__ __forceinline__ uint32_t raw_at(int row, int chunk) {      // a 16-byte piece of an 8-bit row
     return D == 64 ? (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)) : (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
   }
@@ -74,12 +81,11 @@ __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, int n) { asm volatil
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }      // the lowest n bits
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) { return (uint32_t)((chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
 
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) many_rows_kernel(const __grid_constant__ AttnArgs P) {
-  using F = Tc<D, E4M3>;
-  constexpr int NT = F::NT, WK = F::WORKERS;
-  extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* smem = raw + (-(int)smem_u32(raw) & 1023);      // by an offset: through an integer the pointer would lose its address space
+template <int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLOCKS) many_rows_kernel(const __grid_constant__ AttnArgs P) {
+  using F = Tc<D, E4M3, NT>;
+  constexpr int WK = F::WORKERS;
+  extern __shared__ __align__(1024) unsigned char smem[];       // the swizzle's atoms
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -89,7 +95,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);
-  const int npair = (ch.n * group + NT * 128 - 1) / (NT * 128);      // pairs of tiles, or tiles
+  const int npair = (ch.n * group + NT * F::ROWS - 1) / (NT * F::ROWS);      // pairs of tiles, or tiles
   if (turn >= npair) return;
   if (tid == 0) {
     mbar_init(smem_u32(&ct.q_full), 4 * NT);
@@ -114,9 +120,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
     k.lo = 0x7fffffff; k.hi = 0; k.p_low = k.p_high = 0;
 #pragma unroll
     for (int i = 0; i < NT; i++) {
-      const int r0 = (pair * NT + i) * 128;
+      const int r0 = (pair * NT + i) * F::ROWS;
       if (r0 >= ch.n * group) { k.a[i] = k.b[i] = 0; continue; }
-      const int pmin = ch.p0 + (int)P.group.quot(r0), pmax = ch.p0 + min(ch.n - 1, (int)P.group.quot(r0 + 127));
+      const int pmin = ch.p0 + (int)P.group.quot(r0), pmax = ch.p0 + min(ch.n - 1, (int)P.group.quot(r0 + F::ROWS - 1));
       const int h = min(cap, P.causal ? pmax + 1 : ch.len), l = P.window ? max(0, pmin - P.window + 1) : 0;
       if (i == 0) k.p_low = pmin;
       k.p_high = pmax;
@@ -153,33 +159,38 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
     uint32_t done = 0;                                           // steps of this tile so far: phases of its barriers
     for (int pair = npair - 1 - turn; pair >= 0; pair -= P.tiles) {
       const Walk k = walk(pair);
-      const int rr = (pair * NT + tile) * 128 + r, t = (int)P.group.quot(rr);
-      const bool on = t < ch.n;
+      const int rr = (pair * NT + tile) * F::ROWS + r, t = (int)P.group.quot(rr);
+      const bool on = r < F::ROWS && t < ch.n;
       const int pos = ch.p0 + (on ? t : ch.n - 1), head = kvh * group + rr - t * group;
-      unsigned char* qt = smem + F::Q_AT + tile * F::TILE;
+      unsigned char* qt = smem + F::Q_AT + tile * F::Q_TILE;
       constexpr int CQ = D / 8;                                  // 16-byte pieces of a row
-      {                                                          // the warp's 32 rows of Q, whole rows side by side, their sign turned if scores are scaled by a negative number
-        const uint32_t flip = P.flip ? 0x80008000u : 0u;
+      const bool idle = e * 32 >= F::ROWS || (pair * NT + tile) * F::ROWS + e * 32 >= ch.n * group;      // none of the warp's rows is there: whatever is computed for them is not looked at
+      if (!idle) {                                               // the warp's 32 rows of Q, whole rows side by side
         const long long at = on ? (long long)(ch.s + t) * P.q_row + (long long)head * P.q_head : -1;
-        uint4 u[CQ];
-#pragma unroll
+#pragma unroll 4
         for (int q = 0; q < CQ; q++) {
           const long long o = __shfl_sync(0xffffffffu, at, (q * 32 + lane) / CQ);
-          u[q] = o >= 0 ? *reinterpret_cast<const uint4*>(P.q + o + lane % CQ * 8) : make_uint4(0, 0, 0, 0);
+          cp16(smem_u32(qt) + F::q_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ), P.q + (o >= 0 ? o : 0) + lane % CQ * 8, o >= 0);
         }
-#pragma unroll
-        for (int q = 0; q < CQ; q++) {
-          u[q].x ^= flip; u[q].y ^= flip; u[q].z ^= flip; u[q].w ^= flip;
-          *reinterpret_cast<uint4*>(qt + tile_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ)) = u[q];
-        }
+        cp_commit();
+        cp_wait<0>();
         fence_async_shared();
-        attn_tc::warp_arrive(smem_u32(&ct.q_full));
       }
+      attn_tc::warp_arrive(smem_u32(&ct.q_full));
       const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + F::O_AT + tile * D;
       float m = -INFINITY, l = 0.f;
       const int n = k.b[tile] - k.a[tile];
       for (int c = 0; c < n; c++) {
         const int j = k.a[tile] + c, k0 = j * 128;
+        if (idle) {
+          ok = wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          attn_tc::warp_arrive(smem_u32(&ct.s_free[tile]));
+          attn_tc::warp_arrive(smem_u32(&ct.pa_full[tile]));
+          attn_tc::warp_arrive(smem_u32(&ct.p_full[tile]));
+          continue;
+        }
         uint32_t s[4][32];
         ok = wait_for(smem_u32(&ct.s_full[tile]), (done + c) & 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
-      if (ok) {                                                  // the row's result, or its part for combine_kernel
+      if (ok && !idle) {                                         // the row's result, or its part for combine_kernel
         const int olo = *reinterpret_cast<volatile int*>(&ct.odd_lo), ohi = *reinterpret_cast<volatile int*>(&ct.odd_hi);
         const long long g = (long long)(ch.s + t) * P.n_heads + head;
         const float inv = P.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
@@ -286,7 +297,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
               float f[8];
 #pragma unroll
               for (int y = 0; y < 8; y++) f[y] = __uint_as_float(o[x + y]) * inv;
-              *reinterpret_cast<uint4*>(qt + tile_at(r, (q * 32 + x) / 8)) = pack8(f);
+              *reinterpret_cast<uint4*>(qt + F::q_at(r, (q * 32 + x) / 8)) = pack8(f);
             }
           } else {                                               // 128 bytes of each of the warp's rows, the same way
             unsigned char* mine = qt + e * 4096;
@@ -305,10 +316,10 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         if (P.nsplit == 1) {
           __syncwarp();
           const long long at = on ? (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head : -1;
-#pragma unroll
+#pragma unroll 4
           for (int q = 0; q < CQ; q++) {
             const long long d = __shfl_sync(0xffffffffu, at, (q * 32 + lane) / CQ);
-            if (d >= 0) *reinterpret_cast<uint4*>(P.out + d + lane % CQ * 8) = *reinterpret_cast<const uint4*>(qt + tile_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ));
+            if (d >= 0) *reinterpret_cast<uint4*>(P.out + d + lane % CQ * 8) = *reinterpret_cast<const uint4*>(qt + F::q_at(e * 32 + (q * 32 + lane) / CQ, lane % CQ));
           }
         }
         if (on && P.nsplit > 1) reinterpret_cast<float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D)[g * P.nsplit + split] = make_float2(m, l);
@@ -330,8 +341,9 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
       const Walk k = walk(pair);
       const int ka = k.a[tile], kb = k.b[tile];
       const uint32_t ts = tmem + tile * 128, to = tmem + F::O_AT + tile * D;
-      const u64 dq = umma_smem_desc(base + F::Q_AT + tile * F::TILE, 16, 1024);
-      constexpr uint32_t I_S = umma_idesc(false, false, 128, 64), I_O = umma_idesc(false, true, 128, D);
+      const u64 dq = umma_smem_desc(base + F::Q_AT + tile * F::Q_TILE, 16, 1024);
+      const uint32_t I_S = umma_idesc(false, false, 128, 64) | (uint32_t)P.flip << 13;      // negates Q where scores are scaled by a negative number
+      constexpr uint32_t I_O = umma_idesc(false, true, 128, D);
       uint32_t c = 0;
       auto slot_of = [&](int item) { return (uses + (uint32_t)item) % F::NST; };
       auto filled = [&](int item) { return wait_for(smem_u32(&ct.full[slot_of(item)]), ((uses + (uint32_t)item) / F::NST) & 1); };
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3>::THREADS, Tc<D, E4M3>::BLOCKS) man
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++)
-            umma_bf16(ts + half * 64, dq + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
+            umma_bf16(ts + half * 64, dq + ((kk >> 2) * F::Q_PART + (kk & 3) * 32) / 16, dk + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, I_S, kk > 0 ? 1u : 0u);
           if (half) { umma_commit(smem_u32(&ct.s_full[tile])); umma_commit(smem_u32(&ct.empty[slot])); }
         }
       };

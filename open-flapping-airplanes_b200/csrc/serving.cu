@@ -105,7 +105,7 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
 }
 
 // ---- attention
-struct Plan { bool many, cluster, by_head; int rows, tiles, nsplit; size_t bytes; };      // rows: of a tile
+struct Plan { bool many, cluster, by_head; int pair, rows, tiles, nsplit; size_t bytes; };      // rows: of a tile
 
 // A chunk of more than 16 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 128 or 256 rows; fewer to the one that keeps more bytes
 // in flight. max_new and max_kv are what the caller says; without them one sequence with all rows and the page table's width are assumed.
@@ -120,15 +120,17 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   const long long group = n_heads / c->n_kv_heads;
   const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
   p.many = rows > 16;
-  const int tiles_of = c->head_dim == 64 && c->dtype == OFA_KV_BF16 ? 1 : 2;      // tiles of 128 rows a block of the tensor-core kernel, of which an SM holds 2 / tiles_of
-  p.rows = p.many ? 128 * tiles_of : rows > 8 ? 16 : 8;
+  // Tiles a block of the tensor-core kernel, of which an SM holds 2 / pair. One where tiles are small, or where the rows are few: two blocks then cover each other's waits
+  // (12 tokens of 24 sequences over 2,000 keys: 50 us with one, 69 with two; 8-bit rows need the room for their own ring).
+  p.pair = c->dtype == OFA_KV_BF16 && (c->head_dim == 64 || rows <= 64) ? 1 : 2;
+  p.rows = p.many ? (p.pair == 1 && c->head_dim == 128 ? 64 : 128 * p.pair) : rows > 8 ? 16 : 8;
   long long tiles = (rows + p.rows - 1) / p.rows;
   if (tiles > 4096) tiles = 4096;
   if (tiles < 1) tiles = 1;
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
   const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles, units = (kv + 127) / 128;
   const long long fewer = p.many ? std::min(rows / group, kv) / 256 : 0;       // units that a chunk's blocks have less on average than the last one
-  const long long slots = 148 * (p.many ? 2 / tiles_of : p.rows == 8 ? 3 : 2), fixed = p.many ? 3 : 6;
+  const long long slots = 148 * (p.many ? 2 / p.pair : p.rows == 8 ? 3 : 2), fixed = p.many ? 3 : 6;
   const size_t part = (size_t)n_rows * n_heads * (c->head_dim + 2) * 4;      // bytes of one split's parts
   p.nsplit = 1;
   double best = 0;
@@ -182,12 +184,13 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute at = {};
   lc.gridDim = dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads); lc.stream = s; lc.attrs = &at;
-  cudaError_t e;
+  cudaError_t e = cudaSuccess;
   if (p.many) {
     lc.gridDim = dim3(lc.gridDim.x * lc.gridDim.y);             // heads among the tiles, for the order in which blocks start
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    e = launch<paged::many_rows_kernel<D, E4M3>>(lc, paged::Tc<D, E4M3>::THREADS, paged::Tc<D, E4M3>::SMEM, P);
+    if constexpr (!E4M3) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(lc, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, P);
+    if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(lc, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, P);
   } else {
     if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
     e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(lc, 128, paged::Few<D, E4M3, 1>::SMEM, P) : launch<paged::few_rows_kernel<D, E4M3, 2>>(lc, 128, paged::Few<D, E4M3, 2>::SMEM, P);
