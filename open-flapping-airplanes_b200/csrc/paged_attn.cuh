@@ -8,8 +8,8 @@
 // every fourth step of 16 or 32 keys and meet once, at the end; up to eight blocks that share the keys of a tile are a cluster and meet in shared memory, more leave their
 // parts in the workspace for combine_kernel.
 //
-// Each warp has a ring of steps in shared memory. Where a page holds a multiple of 8 rows, boxes of 8 or 16 rows come through the copy engine, one instruction for
-// 1 or 2 KB; other pages are gathered by cp.async, 16 bytes a lane. (Gathering everything kept the load/store pipe busy with the copies themselves: 29 clocks for
+// Each warp has a ring of steps in shared memory. Where a page holds a multiple of 8 rows, boxes of 8 to 32 rows come through the copy engine, one instruction for
+// 1 to 4 KB; other pages are gathered by cp.async, 16 bytes a lane. (Gathering everything kept the load/store pipe busy with the copies themselves: 29 clocks for
 // 512 bytes, with the reads behind them, 4.8 TB/s over long contexts.) Rows lie 128 bytes wide, their 16-byte pieces permuted by the row number (the copy engine's
 // swizzle), and operands are read in an order that meets no bank conflict; the order of the sum over head dims and the order of the output's dims are free as long as both
 // operands agree:
@@ -49,7 +49,7 @@ struct AttnArgs {
   float scale_log2;                 // of many_rows_kernel: its magnitude, flip = the scale is negative
   int flip, wide;                   // wide: offsets of 2^35 bytes and more
   alignas(64) CUtensorMap km, vm;   // the pages in boxes of `run` rows x 128 bytes (64: 8-bit rows of 64)
-  int run;                          // 16, 8, or 0: pages of other sizes, no maps
+  int run;                          // a power of two, 8 .. 64 (few_rows_kernel: .. KEYS), or 0: pages of other sizes, no maps
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
   int by_head;                      // many_rows_kernel: the order of its blocks
   int cluster;                      // ... which are a cluster and meet in shared memory

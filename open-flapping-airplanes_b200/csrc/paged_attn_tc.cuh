@@ -9,10 +9,10 @@
 //              back over the second half of them as bf16, the A operand of the second product
 //   products   a warp a tile, one thread of which issues, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
 //              soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores. (4,096 tokens over
-//              16,384 keys, heads of 128: 838 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
+//              16,384 keys, heads of 128: 843 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
 //              two threads a row, four softmax warps a scheduler: 910, bound by issue; a third of the exponentials by a polynomial on the multiply-add pipe: 970 and more, for registers and issue.)
 //              One thread a tile because one issues a tcgen05.mma only every ~96 clocks and a 128 x 128 x 16 product takes 64
-//   copies     one warp asks the copy engine for keys and values, in boxes of 8 or 16 rows of a page: bf16 rows into a ring of tiles in the layout the products read
+//   copies     one warp asks the copy engine for keys and values, in boxes of 8 to 64 rows of a page: bf16 rows into a ring of tiles in the layout the products read
 //              (128-byte swizzle), 8-bit rows into a ring of their own
 //   workers    widen 8-bit rows from there into the tiles, once for the block's rows, a worker on each scheduler; look at values that some row must not meet; and gather the rows of pages that are no
 //              multiple of 8 by cp.async, 16 bytes a lane
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
           const bool there = (unsigned)pg < (unsigned)P.b.n_pages, bad = reaches(j) && !there;
           if (bad) flag(P.b.status, ST_PAGE);
           const bool any_bad = __any_sync(0xffffffffu, bad);
-          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * (uint32_t)(run * D * (E4M3 ? 1 : 2));
+          const uint32_t there_runs = __ballot_sync(0xffffffffu, there), bytes = __popc(there_runs) * (uint32_t)(run * D * (E4M3 ? 1 : 2));
 #pragma unroll
           for (int half = 0; half < 2; half++) {
             const uint32_t n = uses + 2 * (uint32_t)(j - k.A) + half, slot = n % F::NST, rs = n % F::RS;
@@ -428,10 +428,10 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
             else ok = wait_for(smem_u32(&ct.empty[slot]), ((n / F::NST) & 1) ^ 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            if (half == 0 && lane < nrun) {                      // which keys are there
-              const uint32_t bits = there ? below(k.hi - key) & ~below(k.lo - key) : 0u;
-              if (run == 16) *reinterpret_cast<uint16_t*>(&ct.valid[j % F::NV][lane * 2]) = (uint16_t)bits;
-              else ct.valid[j % F::NV][lane] = (uint8_t)bits;
+            if (half == 0) {                                     // which keys are there, eight a lane
+              const int key8 = j * 128 + lane * 8;
+              const bool t8 = (there_runs >> (lane * 8 / run & 31)) & 1;
+              if (lane < 16) ct.valid[j % F::NV][lane] = t8 ? (uint8_t)(below(k.hi - key8) & ~below(k.lo - key8)) : 0;
             }
             const CUtensorMap* map = half ? &P.vm : &P.km;
             if constexpr (E4M3) {

@@ -265,7 +265,9 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
   P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0;
   P.wide = (long long)cache->n_pages * P.c.page_b + (long long)cache->page_size * P.c.row_b >= 1ll << 35; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.by_head = p.by_head; P.part = static_cast<float*>(a->workspace);
-  P.run = cache->n_pages == 0 ? 0 : cache->page_size % 16 == 0 ? 16 : cache->page_size % 8 == 0 ? 8 : 0;
+  // rows of a box of the copy engine: as many as divide a page and are of use at once, since a lane asks for one after the other
+  P.run = std::min(cache->page_size & -cache->page_size, p.many ? 64 : cache->head_dim == 128 && cache->dtype == OFA_KV_BF16 ? 16 : 32);
+  if (P.run < 8 || cache->n_pages == 0) P.run = 0;
   if (P.run && !(map_pages(&P.km, cache->k, cache, P.c, P.run) && map_pages(&P.vm, cache->v, cache, P.c, P.run))) P.run = 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
