@@ -71,13 +71,28 @@ def build_cli(force=False):
 
 
 def build_host(force=False):
-    """Compile csrc/serving_py.cpp for this Python next to the package's modules. Returns the path, or None where Python's headers are missing: serving.py then makes the same
-    calls itself, more slowly."""
+    """Compile csrc/serving_py.cpp for this Python and torch next to the package's modules. Returns the path, or None where their headers or a compiler are missing: serving.py then
+    makes the same calls itself, more slowly."""
     hdr = os.path.join(CSRC, "..", "..", "include", "ofa_b200.h")
     inc = sysconfig.get_paths()["include"]
     cxx = shutil.which("g++") or shutil.which("c++")
     if not force and os.path.exists(HOST) and os.path.getmtime(HOST) >= max(os.path.getmtime(HOST_SRC), os.path.getmtime(hdr)):
         return HOST
+    try:
+        import torch
+        root = os.path.dirname(torch.__file__)
+    except ImportError:
+        return None
+    cuda = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
+    dirs = [inc, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
+    needed = (os.path.join(inc, "Python.h"), os.path.join(root, "include", "ATen", "Functions.h"), os.path.join(cuda, "include", "cuda_runtime_api.h"))
+    if not cxx or not all(os.path.exists(f) for f in needed):
+        return None
+    r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *["-I" + d for d in dirs], "-o", HOST, HOST_SRC,
+                        "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building " + HOST + " failed:\n" + r.stdout + r.stderr)
+    return HOST
     if not cxx or not os.path.exists(os.path.join(inc, "Python.h")):
         return None
     r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + inc, "-o", HOST, HOST_SRC], capture_output=True, text=True)

@@ -72,15 +72,15 @@ def _lib():
 
 
 def _bind():
-    """The extension that build.build_host() compiles, bound to the loaded library; None where there is none. Its functions return an entry point's code, or None for
-    arguments that are not plainly right: the code below then finds out what is wrong with them."""
+    """The extension that build.build_host() compiles, bound to the loaded library; None where there is none. Its functions return results, the code of an entry point that
+    refused, or None for arguments that are not plainly right: the code below then finds out what is wrong with them."""
     try:
         from . import _serving
     except ImportError:
         return None
     lib = _lib()
     addr = lambda f: C.cast(f, C.c_void_p).value  # noqa: E731
-    _serving.bind(addr(lib.ofa_kv_append), addr(lib.ofa_kv_read), addr(lib.ofa_paged_attention), addr(lib.ofa_logits_process), _BF16, _F32, _I32, torch.uint8, _stream, _current)
+    _serving.bind(addr(lib.ofa_kv_append), addr(lib.ofa_kv_read), addr(lib.ofa_paged_attention), addr(lib.ofa_paged_attention_workspace), addr(lib.ofa_logits_process))
     return _serving
 
 
@@ -195,7 +195,6 @@ class KVBatch:
         if max_new < 0 or max_kv < 0:
             _refuse(f"max_new {max_new}, max_kv {max_kv}")
         self.q_start, self.kv_len, self.pages, self.status, self.device, self.index = q_start, kv_len, pages, status, pages.device, pages.get_device()
-        self._need = {}                                         # workspace sizes by what they depend on beside the batch
         c = self.c = capi.KvBatch()
         c.n_seqs, c.max_pages, c.pages_stride = n, pages.shape[1], pages.stride(0)
         c.q_start, c.kv_len, c.pages = q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr()
@@ -213,14 +212,17 @@ def _move(read, cache, batch, k, v, n_rows):
     _same_device(cache, batch)
     f = _fast()
     if f is not None:
-        rc = f.move(read, cache.address, batch.address, cache.n_kv_heads, cache.head_dim, cache.index, -1 if n_rows is None else n_rows, k, v)
-        if rc is not None:
-            return _done(rc)
+        got = f.move(read, cache.address, batch.address, cache.index, -1 if n_rows is None else n_rows, k, v)
+        if got is not None:
+            return _done(got) if type(got) is int else got
     fn = _lib().ofa_kv_read if read else _lib().ofa_kv_append
     rows = k.shape[0] if n_rows is None and isinstance(k, torch.Tensor) and k.dim() else n_rows
     shape = (rows, cache.n_kv_heads, cache.head_dim)
+    if k is None and read:
+        k, v = torch.empty(shape, dtype=_BF16, device=cache.device), torch.empty(shape, dtype=_BF16, device=cache.device)
     a, b = _rows("k", k, shape, cache), _rows("v", v, shape, cache)
     _call(fn, cache.index, cache.ref, batch.ref, k.data_ptr(), v.data_ptr(), shape[0], a[0], a[1], b[0], b[1])
+    return k, v
 
 
 def kv_append(cache, batch, k, v):
@@ -231,11 +233,9 @@ def kv_append(cache, batch, k, v):
 def kv_read(cache, batch, n_rows=None, k=None, v=None):
     """The batch's n_rows rows out of their pages, as bf16 [n_rows, n_kv_heads, head_dim] pairs (written into k and v where these are given)."""
     if k is None or v is None:
-        if n_rows is None or k is not None or v is not None:
+        if n_rows is None or n_rows < 0 or k is not None or v is not None:
             _refuse("kv_read needs n_rows, or k and v to write to")
-        shape = (n_rows, cache.n_kv_heads, cache.head_dim)
-        k = torch.empty_strided(shape, (cache.n_kv_heads * cache.head_dim, cache.head_dim, 1), dtype=_BF16, device=cache.device)
-        v = torch.empty_like(k)
+        return _move(True, cache, batch, None, None, n_rows)
     _move(True, cache, batch, k, v, n_rows)
     return k, v
 
@@ -244,32 +244,24 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
     """Attention of q [n_rows, n_heads, head_dim] (bf16) over the batch's pages; scale: 1/sqrt(head_dim) by default. Returns out, of q's shape, or with
     with_lse (out, lse [n_rows, n_heads] fp32). Rows that no sequence brings are left as they were."""
     _same_device(cache, batch)
-    if out is None:
-        if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype is not _BF16:
-            _rows("q", q, None, cache)
-        out = torch.empty_like(q)
-    try:
-        n_rows, n_heads, _ = q.shape
-    except (AttributeError, ValueError):
-        _rows("q", q, None, cache)
-        raise
-    lse = torch.empty_strided((n_rows, n_heads), (n_heads, 1), dtype=_F32, device=cache.device) if with_lse else None
-    key = (cache.c.dtype, cache.head_dim, cache.n_kv_heads, cache.page_size, n_rows, n_heads)
-    need = batch._need.get(key)
-    if need is None:
-        need = batch._need[key] = _lib().ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
-    # from torch's allocator: a graph that captures the call keeps its own
-    work = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=cache.device) if need else None
     scale = cache.scale if scale is None else scale
     f = _fast()
-    rc = f.attend(cache.address, batch.address, cache.head_dim, cache.index, q, out, lse, work, scale, causal, window) if f is not None else None
-    if rc is not None:
-        _done(rc)
-    else:
-        sq, so = _rows("q", q, None, cache), _rows("out", out, q.shape, cache)
-        a = capi.PagedAttentionArgs(n_rows, n_heads, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse.data_ptr() if with_lse else None, scale, bool(causal), window,
-                                    work.data_ptr() if need else None, need)
-        _call(_lib().ofa_paged_attention, cache.index, cache.ref, batch.ref, C.byref(a))
+    if f is not None:
+        got = f.attend(cache.address, batch.address, cache.index, q, out, scale, causal, window, with_lse)
+        if got is not None:
+            return _done(got) if type(got) is int else got
+    sq = _rows("q", q, None, cache)
+    n_rows, n_heads, _ = q.shape
+    if out is None:
+        out = torch.empty_like(q, requires_grad=False)
+    so = _rows("out", out, q.shape, cache)
+    lse = torch.empty((n_rows, n_heads), dtype=_F32, device=cache.device) if with_lse else None
+    need = _lib().ofa_paged_attention_workspace(cache.ref, batch.ref, n_rows, n_heads)
+    # from torch's allocator: a graph that captures the call keeps its own
+    work = torch.empty((need,), dtype=torch.uint8, device=cache.device) if need else None
+    a = capi.PagedAttentionArgs(n_rows, n_heads, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse.data_ptr() if with_lse else None, scale, bool(causal), window,
+                                work.data_ptr() if need else None, need)
+    _call(_lib().ofa_paged_attention, cache.index, cache.ref, batch.ref, C.byref(a))
     return (out, lse) if with_lse else out
 
 
@@ -279,18 +271,16 @@ def logits_process(logits, tokens=None, n_tokens=None, n_prompt=None, repetition
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F32, _BF16):
         _refuse("logits have to be a bf16 or fp32 tensor")
     f = _fast()
-    if f is not None and logits.is_cuda:
-        y = torch.empty_like(logits) if out is None else out
-        rc = f.process(logits, y, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias, mask)
-        if rc is not None:
-            _done(rc)
-            return y
+    if f is not None:
+        got = f.process(logits, out, tokens, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias, mask)
+        if got is not None:
+            return _done(got) if type(got) is int else got
     kind, dev, index = logits.dtype, logits.device, logits.get_device()
     if index < 0 or logits.dim() != 2:
         _want("logits", logits, kind, (None, None), None)
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty_like(logits)
+        out = torch.empty_like(logits, requires_grad=False)
     src, src_row = _table("logits", logits, kind, (rows, vocab), index, dev)
     dst, dst_row = _table("out", out, kind, (rows, vocab), index, dev)
     text = text_row = most = made = first = ids = bias_row = n_bias = weight = words = words_row = 0
