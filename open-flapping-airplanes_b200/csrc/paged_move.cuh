@@ -4,7 +4,9 @@
 // A thread holds 8 values of a row (16 of an 8-bit one: 16 bytes where it is held), so a row is 4 to 16 neighbouring lanes: the largest magnitude is found as an
 // unsigned maximum of the bits without signs (an infinity or a NaN is then the largest) and shared by shuffles; scaling by a power of two is exact, so the
 // only rounding is the one to e4m3 (to nearest, half a step 2^-4 relative). A block takes consecutive rows of the call; its threads compare the starts of
-// all sequences with them once and leave each row's page in shared memory. Four pieces a thread are asked for before the first is worked on.
+// all sequences with them once and leave each row's page in shared memory. Two pieces a thread are asked for before the first is worked
+// on, in 32 registers, so that an SM holds eight blocks (73,000 rows of 8 heads of 128 out of 8 bits 42.6 us; four pieces and five blocks 45; asking for new rows before their places are
+// known, which keeps them in registers meanwhile, 13.2 -> 15.7 for 8,192 rows to 8 bits).
 #pragma once
 #include <cuda_fp8.h>
 #include "paged.cuh"
@@ -30,7 +32,7 @@ __device__ __forceinline__ uint32_t to_e4m3(uint32_t lo, uint32_t hi, float f) {
 }
 
 template <int D, bool E4M3, bool READ>
-__global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ MoveArgs P) {
+__global__ void __launch_bounds__(256, 8) move_kernel(const __grid_constant__ MoveArgs P) {
   constexpr int PIECE = E4M3 ? 16 : 8, LANES = D / PIECE;      // values a thread holds of a row, lanes of a row
   __shared__ int2 place[MOVE_ROWS];                   // page and row in it; x = -1: nowhere, -2: no sequence's row
   const int tid = threadIdx.x, r0 = blockIdx.x * P.rows, r1 = min(r0 + P.rows, P.b.n_rows);
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ MoveA
     place[tid] = make_int2(page, at);
   }
   __syncthreads();
-  constexpr int U = 4;                                // pieces that a thread has on their way
+  constexpr int U = 2;                                // pieces that a thread has on their way
   const int total = (r1 - r0) * 2 * P.n_kv_heads * LANES;
   for (int base = 0; base < total; base += 256 * U) {
     bf16* x[U];

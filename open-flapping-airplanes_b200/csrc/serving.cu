@@ -89,7 +89,7 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
     return fail(OFA_BAD_ARGUMENT, "rows of the cache overlap");
   P.k = static_cast<bf16*>(k); P.v = static_cast<bf16*>(v); P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
   P.n_kv_heads = c->n_kv_heads; P.pair.set(2u * (unsigned)c->n_kv_heads);
-  // four pieces of 16 bytes for a thread where there are rows for it: a block then amortises the search for its sequences
+  // four pieces of 16 bytes for a thread, in two turns, where there are rows for it: a block then amortises the search for its sequences
   const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / (c->dtype == OFA_KV_E4M3 ? 16 : 8));
   long long rows = (1024 + per_row - 1) / per_row;
   while (rows > 1 && (n_rows + rows - 1) / rows < 148) rows--;
