@@ -5,7 +5,7 @@
 // unsigned maximum of the bits without signs (an infinity or a NaN is then the largest) and shared by shuffles; scaling by a power of two is exact, so the
 // only rounding is the one to e4m3 (to nearest, half a step 2^-4 relative). A block takes consecutive rows of the call; its threads compare the starts of
 // all sequences with them once and leave each row's page in shared memory. Two pieces a thread are asked for before the first is worked
-// on, in 32 registers, so that an SM holds eight blocks (73,000 rows of 8 heads of 128 out of 8 bits 42.6 us; four pieces and five blocks 45; asking for new rows before their places are
+// on, in 32 registers, so that an SM holds eight blocks (39,000 rows of 8 heads of 128 out of 8 bits 42.6 us; four pieces and five blocks 45; asking for new rows before their places are
 // known, which keeps them in registers meanwhile, 13.2 -> 15.7 for 8,192 rows to 8 bits).
 #pragma once
 #include <cuda_fp8.h>
