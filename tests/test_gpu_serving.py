@@ -716,3 +716,39 @@ def test_two_graphs_share_nothing(sv):
             graph.replay()
             assert torch.equal(out, want)
     del junk
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [8, 24, 32, 64, 128, 192])
+def test_pages_of_many_sizes(sv, page, dim, dtype):
+    """boxes of 8 to 64 rows, contexts and windows that begin and end inside them"""
+    for new, kv, window in (([1, 1, 1], [1, 63, 300], 0), ([1, 1], [200, 129], 70), ([3, 2], [65, 190], 0), ([40, 9], [40, 333], 0), ([40, 70], [260, 139], 50)):
+        cache, batch, g = make(sv, new, kv, 2, dim, page, dtype)
+        check_attention(sv, cache, batch, queries(g, sum(new), 8, dim), window=window)
+
+
+@pytest.mark.parametrize("page", [16, 64, 33])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_missing_page_among_others(sv, page, new):
+    """its keys are not seen, whatever the box size; the others are"""
+    for dtype in ("bf16", "e4m3"):
+        cache, batch, g = make(sv, [new], [400], 2, 64, page, dtype)
+        bad = batch.pages.clone()
+        bad[0, 2] = cache.n_pages + 5
+        status = i32([0])
+        b2 = sv.KVBatch(batch.q_start, batch.kv_len, bad, status=status)
+        q = queries(g, new, 4, 64)
+        got, lse = sv.paged_attention(cache, b2, q, with_lse=True)
+        assert int(status) == sv.BAD_PAGE
+        want, wl, tol, ltol = ref.attention(cache, [0, new], [400], bad.cpu(), q, cache.scale)
+        assert ((got.double().cpu() - want).abs() <= tol).all() and ((lse.double().cpu() - wl).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("dim,heads", [(128, 8), (64, 8), (128, 2)])
+@pytest.mark.parametrize("hint", [3, 5, 12, 30])
+def test_chunks_longer_than_the_hint(sv, dim, heads, hint):
+    """every form of the kernels walks on through the tiles that the hint did not count"""
+    for dtype in ("bf16", "e4m3"):
+        cache, batch, g = make(sv, [200, 7, 70], [300, 7, 500], 2, dim, 16, dtype, max_new=hint, max_kv=40)
+        check_attention(sv, cache, batch, queries(g, 277, heads, dim))
