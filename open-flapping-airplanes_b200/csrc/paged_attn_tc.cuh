@@ -33,15 +33,16 @@ namespace ofa {
 namespace paged {
 
 template <int D, bool E4M3, int NT> struct Tc {                 // NT tiles of 128 rows a block
-  static constexpr int BLOCKS = 3 - NT;                         // of an SM
+  static constexpr int BLOCKS = E4M3 ? 1 : 3 - NT;              // of an SM
   // Rows of a tile that are used: 64 where two blocks of wide rows share an SM. Q's parts then lie 64 rows apart, which leaves room for a third tile of keys or values (products read
   // the other 64 rows from whatever lies behind, and nobody looks at what comes of them)
   static constexpr int ROWS = NT == 1 && D == 128 ? 64 : 128, Q_PART = ROWS * 128, Q_TILE = ROWS * D * 2;
-  static constexpr int WORKERS = NT == 1 ? 2 : E4M3 ? 4 : 5, WARPS = NT == 1 ? 8 : 16, THREADS = 32 * WARPS;      // 8-bit rows: a worker on each scheduler, one warp idle
+  // 8-bit rows: one or two workers on each scheduler, the rest idle
+  static constexpr int WORKERS = E4M3 ? (NT == 1 ? 8 : 4) : NT == 1 ? 2 : 5, WARPS = BLOCKS == 2 ? 8 : 16, THREADS = 32 * WARPS;
   static constexpr int SOFT_REGS = 184, REST_REGS = 72;         // of a softmax thread, of another: together twice the launch's 128
   static constexpr int TMEM = NT * 256, O_AT = NT * 128;        // columns; S of a tile at tile * 128, O behind them
   static constexpr int TILE = 128 * D * 2;                      // a tile of rows: D / 64 parts of 128 rows x 128 bytes
-  static constexpr int NST = E4M3 ? (D == 128 ? 3 : 6) : NT == 1 && D == 128 ? 3 : 4;           // ring of K and V tiles
+  static constexpr int NST = E4M3 ? (D == 64 ? 6 : 5 - NT) : NT == 1 && D == 128 ? 3 : 4;           // ring of K and V tiles
   static constexpr int RAW = E4M3 ? 128 * D : 0, RS = D == 64 ? 4 : 3;      // ring of 8-bit tiles, rows D bytes apart, pieces permuted as the copy engine does
   static constexpr int LAG = 1;                                 // gathered tiles whose copies may be in flight when the next is begun
   static constexpr int NV = 8;                                  // ring of the keys' validity, by step
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {
                 const int u = unit0(item) + (gr * 4 + y) * WK;
-                if (16 % WK && u >= 16) break;
+                if (GROUPS * 4 * WK != 16 && u >= 16) break;
                 if (!(item & 1) && lane == 0) ct.valid[(k.A + (item >> 1)) % F::NV][u] = (uint8_t)(there >> y * 8);
                 long long o[IT];
 #pragma unroll
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
 #pragma unroll
             for (int y = 0; y < 4; y++) {
               const int u = unit0(item) + (gr * 4 + y) * WK;
-              if (16 % WK && u >= 16) break;
+              if (GROUPS * 4 * WK != 16 && u >= 16) break;
 #pragma unroll
               for (int i = 0; i < IT; i++) {
                 // rows of 8 pieces in pairs, half of each to eight lanes, which then write to all the banks: two pieces of a tile's row lie side by side
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
 #pragma unroll 1
               for (int y = 0; y < 4; y++) {
                 const int u = unit0(item) + (gr * 4 + y) * WK;
-                if (16 % WK && u >= 16) break;
+                if (GROUPS * 4 * WK != 16 && u >= 16) break;
                 if (!(item & 1) && lane == 0) ct.valid[j % F::NV][u] = (uint8_t)(there >> y * 8);
                 long long o[IT];                                 // all the exchanges before the first copy: in turns each copy would wait for its own
 #pragma unroll

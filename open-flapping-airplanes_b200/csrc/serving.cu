@@ -120,9 +120,9 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   const long long group = n_heads / c->n_kv_heads;
   const long long rows = (b->max_new > 0 && b->max_new < n_rows ? b->max_new : n_rows) * group;
   p.many = rows > 16;
-  // Tiles a block of the tensor-core kernel, of which an SM holds 2 / pair. One where tiles are small, or where the rows are few: two blocks then cover each other's waits
-  // (12 tokens of 24 sequences over 2,000 keys: 50 us with one, 69 with two; 8-bit rows need the room for their own ring).
-  p.pair = c->dtype == OFA_KV_BF16 && (c->head_dim == 64 || rows <= 64) ? 1 : 2;
+  // Tiles a block of the tensor-core kernel. One where bf16 tiles are small, or where the rows are few: two blocks an SM then cover each other's waits (12 tokens of 24 sequences over
+  // 2,000 keys: 50 us with one, 69 with two). 8-bit rows need the room for their own ring, one block an SM has twice the workers (83 -> 78; for heads of 64 no gain).
+  p.pair = c->head_dim == 64 ? (c->dtype == OFA_KV_BF16 ? 1 : 2) : rows <= 64 ? 1 : 2;
   p.rows = p.many ? (p.pair == 1 && c->head_dim == 128 ? 64 : 128 * p.pair) : rows > 8 ? 16 : 8;
   long long tiles = (rows + p.rows - 1) / p.rows;
   if (tiles > 4096) tiles = 4096;
@@ -130,7 +130,7 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   const long long cap = (long long)b->max_pages * c->page_size, kv = b->max_kv > 0 && b->max_kv < cap ? b->max_kv : cap;
   const long long blocks = (long long)(b->n_seqs > 0 ? b->n_seqs : 1) * c->n_kv_heads * tiles, units = (kv + 127) / 128;
   const long long fewer = p.many ? std::min(rows / group, kv) / 256 : 0;       // units that a chunk's blocks have less on average than the last one
-  const long long slots = 148 * (p.many ? 2 / p.pair : p.rows == 8 ? 3 : 2), fixed = p.many ? 3 : 6;
+  const long long slots = 148 * (p.many ? (c->dtype == OFA_KV_BF16 ? 2 / p.pair : 1) : p.rows == 8 ? 3 : 2), fixed = p.many ? 3 : 6;
   const size_t part = (size_t)n_rows * n_heads * (c->head_dim + 2) * 4;      // bytes of one split's parts
   p.nsplit = 1;
   double best = 0;
@@ -189,7 +189,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
     lc.gridDim = dim3(lc.gridDim.x * lc.gridDim.y);             // heads among the tiles, for the order in which blocks start
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    if constexpr (!E4M3) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(lc, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, P);
+    if constexpr (!E4M3 || D == 128) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(lc, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, P);
     if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(lc, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, P);
   } else {
     if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
