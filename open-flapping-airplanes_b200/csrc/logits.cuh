@@ -17,10 +17,11 @@
 // A bias marks its token's word; the entries of its list are added in their order. Stretches begin where a row's 16-byte vectors do, so a row that starts between two boundaries
 // loses only its first and last vector to single elements.
 #pragma once
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace ofa {
 namespace logits {
+using paged::after_the_kernel_before;
 
 struct Args {
   const void* in; void* out;
@@ -58,6 +59,7 @@ __device__ __forceinline__ float touched(const Row& R, float f, unsigned c, floa
 template <class T, int VECS, bool WIDE, bool WORDS>
 __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Args P) {
   constexpr int VN = Vec<T>::N, S = 256 * VN * VECS;           // tokens of a block
+  after_the_kernel_before();
   extern __shared__ __align__(16) unsigned count[];
   __shared__ int list[LISTED], listed;
   const int tid = threadIdx.x, row = blockIdx.y;

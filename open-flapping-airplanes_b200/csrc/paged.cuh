@@ -41,6 +41,10 @@ struct Pool {
   long long s_page, s_head, s_row;                    // strides of ks and vs
 };
 
+// The serving kernels are launched as dependents of whatever runs before them in the stream: their launch is then prepared while that still runs, and every block waits here,
+// before it touches memory, until it has ended (a block that left without waiting would let the next kernel run ahead of the one before).
+__device__ __forceinline__ void after_the_kernel_before() { cudaGridDependencySynchronize(); }
+
 static __device__ __noinline__ void flag(int* status, int bits) { if (status) atomicOr(status, bits); }
 
 // Rows [s, s + n) of the call belong to sequence i, the first of them at position p0 (negative: the sequence is shorter than what it brings).

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   if (lane < F::STAGES) mbar_init(bars + lane * 8, 1);
   mbar_fence_init();
   __syncwarp();
+  after_the_kernel_before();
   uint32_t used = 0;                                             // steps of this warp so far: phases of its barriers
   const int split = (int)blockIdx.x % P.nsplit, tile0 = (int)blockIdx.x / P.nsplit % P.tiles, seq = (int)blockIdx.x / P.nsplit / P.tiles, kvh = blockIdx.y;
   const Chunk ch = chunk_of(P.b, seq);

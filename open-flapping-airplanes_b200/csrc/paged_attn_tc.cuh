@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
   TcCtrl& ct = *reinterpret_cast<TcCtrl*>(smem + F::CTRL_AT);
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  after_the_kernel_before();
   // The last tiles, which have the most keys, start first: over all sequences and heads, or, where their keys and values together would not stay in L2, head by head
   const int split = (int)blockIdx.x % P.nsplit, rest = (int)blockIdx.x / P.nsplit, streams = P.n_kv_heads * P.b.n_seqs;
   const int turn = P.by_head ? rest % P.tiles : rest / streams, stream = P.by_head ? rest / P.tiles : rest % streams, kvh = stream % P.n_kv_heads, seq = stream / P.n_kv_heads;

@@ -34,6 +34,7 @@ __device__ __forceinline__ uint32_t to_e4m3(uint32_t lo, uint32_t hi, float f) {
 template <int D, bool E4M3, bool READ>
 __global__ void __launch_bounds__(256, 8) move_kernel(const __grid_constant__ MoveArgs P) {
   constexpr int PIECE = E4M3 ? 16 : 8, LANES = D / PIECE;      // values a thread holds of a row, lanes of a row
+  after_the_kernel_before();
   __shared__ int2 place[MOVE_ROWS];                   // page and row in it; x = -1: nowhere, -2: no sequence's row
   const int tid = threadIdx.x, r0 = blockIdx.x * P.rows, r1 = min(r0 + P.rows, P.b.n_rows);
   if (tid < MOVE_ROWS) place[tid] = make_int2(-2, 0);

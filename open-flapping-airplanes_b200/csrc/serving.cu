@@ -23,9 +23,10 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? OFA_OK : fail(OFA_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
+int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return OFA_OK;
+  cudaGetLastError();                                            // reported here, not by the next call
+  return fail(OFA_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
 }
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 // Whether places of `unit` elements at these strides lie upon one another: from the smallest stride up, each has to pass what lies inside it
@@ -77,6 +78,27 @@ int check_rows(const char* name, const void* p, Axis row, Axis head, int dim, bo
   return OFA_OK;
 }
 
+// The limit of dynamic shared memory, raised once for each kernel and device to all an SM has
+template <auto KERNEL> cudaError_t allow() {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+// A launch as a dependent of the kernel before (paged.cuh: after_the_kernel_before), in clusters of `cluster` blocks
+template <auto KERNEL, class Args> cudaError_t launch(dim3 grid, int threads, int smem, cudaStream_t s, const Args& P, int cluster = 1) {
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = (unsigned)cluster; at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  lc.gridDim = grid; lc.blockDim = dim3((unsigned)threads); lc.dynamicSmemBytes = (size_t)smem; lc.stream = s; lc.attrs = at; lc.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = smem > 48 * 1024 ? allow<KERNEL>() : cudaSuccess;
+  return e == cudaSuccess ? cudaLaunchKernelEx(&lc, KERNEL, P) : e;
+}
+
 template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void* k, void* v, int n_rows, long long k_row, long long k_head, long long v_row,
                               long long v_head, void* stream) {
   paged::MoveArgs P;
@@ -96,12 +118,10 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
   P.rows = (int)(rows < paged::MOVE_ROWS ? rows : paged::MOVE_ROWS);
   const unsigned grid = (unsigned)((n_rows + P.rows - 1) / P.rows);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (c->dtype == OFA_KV_E4M3) {
-    if (c->head_dim == 64) paged::move_kernel<64, true, READ><<<grid, 256, 0, s>>>(P); else paged::move_kernel<128, true, READ><<<grid, 256, 0, s>>>(P);
-  } else {
-    if (c->head_dim == 64) paged::move_kernel<64, false, READ><<<grid, 256, 0, s>>>(P); else paged::move_kernel<128, false, READ><<<grid, 256, 0, s>>>(P);
-  }
-  return launched(READ ? "ofa_kv_read" : "ofa_kv_append");
+  const bool e4m3 = c->dtype == OFA_KV_E4M3, small = c->head_dim == 64;
+  const cudaError_t e = e4m3 ? small ? launch<paged::move_kernel<64, true, READ>>(grid, 256, 0, s, P) : launch<paged::move_kernel<128, true, READ>>(grid, 256, 0, s, P)
+                             : small ? launch<paged::move_kernel<64, false, READ>>(grid, 256, 0, s, P) : launch<paged::move_kernel<128, false, READ>>(grid, 256, 0, s, P);
+  return launched(e, READ ? "ofa_kv_read" : "ofa_kv_append");
 }
 
 // ---- attention
@@ -165,42 +185,22 @@ bool map_pages(CUtensorMap* m, const void* base, const ofa_kv_cache* c, const pa
   return encode && encode(m, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           e4m3 && c->head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// The limit of dynamic shared memory, raised once for each kernel and device
-template <auto KERNEL> cudaError_t allow(int bytes) {
-  static std::atomic<unsigned long long> done{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
-  return e;
-}
-template <auto KERNEL> cudaError_t launch(cudaLaunchConfig_t& lc, int threads, int smem, const paged::AttnArgs& P) {
-  lc.blockDim = dim3((unsigned)threads); lc.dynamicSmemBytes = (size_t)smem;
-  const cudaError_t e = allow<KERNEL>(smem);
-  return e == cudaSuccess ? cudaLaunchKernelEx(&lc, KERNEL, P) : e;
-}
 template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p, cudaStream_t s) {
-  cudaLaunchConfig_t lc = {};
-  cudaLaunchAttribute at = {};
-  lc.gridDim = dim3((unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit), (unsigned)P.n_kv_heads); lc.stream = s; lc.attrs = &at;
+  const unsigned blocks = (unsigned)((long long)P.b.n_seqs * P.tiles * P.nsplit);
   cudaError_t e = cudaSuccess;
   if (p.many) {
-    lc.gridDim = dim3(lc.gridDim.x * lc.gridDim.y);             // heads among the tiles, for the order in which blocks start
+    const dim3 grid(blocks * (unsigned)P.n_kv_heads);           // heads among the tiles, for the order in which blocks start
     P.flip = P.scale_log2 < 0.f;
     P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
-    if constexpr (!E4M3 || D == 128) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(lc, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, P);
-    if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(lc, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, P);
+    if constexpr (!E4M3 || D == 128) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(grid, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, s, P);
+    if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(grid, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, s, P);
   } else {
-    if (P.cluster) { at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = (unsigned)P.nsplit; at.val.clusterDim.y = at.val.clusterDim.z = 1; lc.numAttrs = 1; }
-    e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(lc, 128, paged::Few<D, E4M3, 1>::SMEM, P) : launch<paged::few_rows_kernel<D, E4M3, 2>>(lc, 128, paged::Few<D, E4M3, 2>::SMEM, P);
+    const dim3 grid(blocks, (unsigned)P.n_kv_heads);
+    const int cluster = P.cluster ? P.nsplit : 1;
+    e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(grid, 128, paged::Few<D, E4M3, 1>::SMEM, s, P, cluster)
+                    : launch<paged::few_rows_kernel<D, E4M3, 2>>(grid, 128, paged::Few<D, E4M3, 2>::SMEM, s, P, cluster);
   }
-  if (e == cudaSuccess && P.nsplit > 1 && !P.cluster) {
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    lc.gridDim = dim3((unsigned)(((long long)P.b.n_rows * P.n_heads + 3) / 4)); lc.blockDim = dim3(128); lc.dynamicSmemBytes = 0; lc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&lc, paged::combine_kernel<D>, P);
-  }
+  if (e == cudaSuccess && P.nsplit > 1 && !P.cluster) e = launch<paged::combine_kernel<D>>(dim3((unsigned)(((long long)P.b.n_rows * P.n_heads + 3) / 4)), 128, 0, s, P);
   return e;
 }
 
@@ -213,20 +213,13 @@ template <class T, bool WIDE> cudaError_t process(logits::Args& P, int rows, cud
   const dim3 grid((unsigned)((span + stretch - 1) / stretch), (unsigned)rows);
   const long long named = (P.tokens ? P.max_tokens : 0) + (long long)P.max_bias;
   if (!large || (words && named > 8192)) {
-    const unsigned smem = words ? (unsigned)stretch * 4 : 0;
-    if (large) logits::process_kernel<T, 4, WIDE, true><<<grid, 256, smem, s>>>(P); else logits::process_kernel<T, 1, WIDE, true><<<grid, 256, smem, s>>>(P);
-    return cudaGetLastError();
+    const int smem = words ? stretch * 4 : 0;
+    return large ? launch<logits::process_kernel<T, 4, WIDE, true>>(grid, 256, smem, s, P) : launch<logits::process_kernel<T, 1, WIDE, true>>(grid, 256, smem, s, P);
   }
-  logits::process_kernel<T, 4, WIDE, false><<<grid, 256, 0, s>>>(P);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch<logits::process_kernel<T, 4, WIDE, false>>(grid, 256, 0, s, P);
   if (e != cudaSuccess || !words) return e;
   for (P.slots_log2 = 9; P.slots_log2 < 14 && 1ll << P.slots_log2 < 4 * named;) P.slots_log2++;
-  cudaLaunchConfig_t lc = {};
-  cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization; at.val.programmaticStreamSerializationAllowed = 1;
-  lc.gridDim = dim3((unsigned)rows); lc.blockDim = dim3(512); lc.dynamicSmemBytes = (size_t)12 << P.slots_log2; lc.stream = s; lc.attrs = &at; lc.numAttrs = 1;
-  e = allow<logits::touch_kernel<T>>(12 << 14);
-  return e == cudaSuccess ? cudaLaunchKernelEx(&lc, logits::touch_kernel<T>, P) : e;
+  return launch<logits::touch_kernel<T>>(dim3((unsigned)rows), 512, 12 << P.slots_log2, s, P);
 }
 
 }  // namespace
@@ -273,9 +266,7 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   cudaError_t e;
   if (cache->dtype == OFA_KV_E4M3) e = cache->head_dim == 64 ? attend<64, true>(P, p, s) : attend<128, true>(P, p, s);
   else e = cache->head_dim == 64 ? attend<64, false>(P, p, s) : attend<128, false>(P, p, s);
-  if (e == cudaSuccess) return OFA_OK;
-  cudaGetLastError();                                            // reported here, not by the next call
-  return fail(OFA_CUDA_ERROR, "ofa_paged_attention: %s", cudaGetErrorString(e));
+  return launched(e, "ofa_paged_attention");
 }
 
 extern "C" size_t ofa_paged_attention_workspace(const ofa_kv_cache* cache, const ofa_kv_batch* batch, int n_rows, int n_heads) {
@@ -322,7 +313,5 @@ extern "C" int ofa_logits_process(const ofa_logits_args* a, void* stream) {
   const bool wide = (reinterpret_cast<uintptr_t>(a->in) - reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 && (a->n_rows == 1 || ((a->in_stride - a->out_stride) * (long long)es) % 16 == 0);
   const cudaError_t e = a->dtype == OFA_DTYPE_F32 ? wide ? process<float, true>(P, a->n_rows, s) : process<float, false>(P, a->n_rows, s)
                                                   : wide ? process<bf16, true>(P, a->n_rows, s) : process<bf16, false>(P, a->n_rows, s);
-  if (e == cudaSuccess) return OFA_OK;
-  cudaGetLastError();
-  return fail(OFA_CUDA_ERROR, "ofa_logits_process: %s", cudaGetErrorString(e));
+  return launched(e, "ofa_logits_process");
 }
