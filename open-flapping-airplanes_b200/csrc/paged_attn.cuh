@@ -51,7 +51,7 @@ struct AttnArgs {
   alignas(64) CUtensorMap km, vm;   // the pages in boxes of `run` rows x 128 bytes (64: 8-bit rows of 64)
   int run;                          // a power of two, 8 .. 64 (few_rows_kernel: .. KEYS), or 0: pages of other sizes, no maps
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
-  int by_head;                      // many_rows_kernel: the order of its blocks
+  int by_head, ranked;              // the order of blocks in many_rows_kernel; few_rows_kernel: sequences by length (at most 128)
   int cluster;                      // ... which are a cluster and meet in shared memory
   float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
 };
@@ -152,7 +152,21 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   __syncwarp();
   after_the_kernel_before();
   uint32_t used = 0;                                             // steps of this warp so far: phases of its barriers
-  const int split = (int)blockIdx.x % P.nsplit, tile0 = (int)blockIdx.x / P.nsplit % P.tiles, seq = (int)blockIdx.x / P.nsplit / P.tiles, kvh = blockIdx.y;
+  const int split = (int)blockIdx.x % P.nsplit, rest = (int)blockIdx.x / P.nsplit, kvh = rest % P.n_kv_heads, tile0 = rest / P.n_kv_heads % P.tiles;
+  int seq = rest / P.n_kv_heads / P.tiles;
+  if (P.ranked) {                                                // the longest first
+    int *lens = reinterpret_cast<int*>(smem), *pick = lens + 128;      // where the rings will be
+    const int len = threadIdx.x < P.b.n_seqs ? __ldg(P.b.kv_len + threadIdx.x) : -1;
+    lens[threadIdx.x] = len;
+    __syncthreads();
+    int rank = 0;
+    for (int j = 0; j < P.b.n_seqs; j++) rank += lens[j] > len || (lens[j] == len && j < (int)threadIdx.x);
+    if ((int)threadIdx.x < P.b.n_seqs && rank == seq) *pick = threadIdx.x;
+    __syncthreads();
+    seq = *pick;
+    fence_async_shared();                                        // read, before the copy engine writes there
+    __syncthreads();
+  }
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && threadIdx.x == 0) flag(P.b.status, ST_LENGTH);

@@ -125,7 +125,7 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
 }
 
 // ---- attention
-struct Plan { bool many, cluster, by_head; int pair, rows, tiles, nsplit; size_t bytes; };      // rows: of a tile
+struct Plan { bool many, cluster, by_head, ranked; int pair, rows, tiles, nsplit; size_t bytes; };      // rows: of a tile
 
 // A chunk of more than 16 rows for a key/value head goes to the tensor-core kernel, which reads the keys once for 128 or 256 rows; fewer to the one that keeps more bytes
 // in flight. max_new and max_kv are what the caller says; without them one sequence with all rows and the page table's width are assumed.
@@ -133,7 +133,7 @@ struct Plan { bool many, cluster, by_head; int pair, rows, tiles, nsplit; size_t
 // How many blocks share a tile's keys: the number for which the call should take least, in units of 128 keys of a block: one block's time where all run at once, else all blocks' time over
 // the places for them and half a block's more for the end. What a block costs beside its keys (its first loads one after the other, the meeting at its end) measured 3 units of the tensor-core
 // kernel and 6 of the other, a second launch to join parts 3, and parts pass through memory at 5 TB/s, a unit being 1.6 us. Up to eight blocks of the few-row kernel are a cluster and need no parts.
-// (64 tokens over 1,024 to 4,096 8-bit keys: 88 us with one block a tile, 84 with two, 97 with four; a token over 1,000 keys, 12 heads of 64: 11.1, 8.7, 6.9 and 6.3 us with one, two, four and
+// (64 tokens over 2,048 to 4,096 8-bit keys: 99 us with one block a tile, 97 with two, 112 with four; a token over 1,000 keys, 12 heads of 64: 11.1, 8.7, 6.9 and 6.3 us with one, two, four and
 // eight; 4,096 tokens over 16,384 keys: 889 us with one, 914 with two.)
 Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
   Plan p;
@@ -164,6 +164,9 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   // Keys and values of all heads above 48 MB are taken head by head (4,096 tokens over 16,384 keys of 8 heads, 67 MB: 850 us, 897 with all heads side by side); below that the longest
   // tiles of all heads go first (prompts of 1,024 tokens, 12.6 MB: 22.8 us, 29.4 head by head).
   p.by_head = (double)b->n_seqs * c->n_kv_heads * kv * c->head_dim * (c->dtype == OFA_KV_E4M3 ? 2 : 4) > 48e6;
+  // Where blocks start one after the other, those of the longest sequences do so first (64 tokens over 1 to 4,096 8-bit keys: 76 us in the order of the table, 67 so; every block ranks the
+  // lengths itself, 0.3 us)
+  p.ranked = b->n_seqs > 1 && b->n_seqs <= 128 && blocks * p.nsplit > slots;
   p.tiles = (int)tiles;
   p.bytes = p.nsplit > 1 && !p.cluster ? part * p.nsplit : 0;
   return p;
@@ -195,7 +198,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
     if constexpr (!E4M3 || D == 128) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(grid, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, s, P);
     if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(grid, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, s, P);
   } else {
-    const dim3 grid(blocks, (unsigned)P.n_kv_heads);
+    const dim3 grid(blocks * (unsigned)P.n_kv_heads);
     const int cluster = P.cluster ? P.nsplit : 1;
     e = p.rows == 8 ? launch<paged::few_rows_kernel<D, E4M3, 1>>(grid, 128, paged::Few<D, E4M3, 1>::SMEM, s, P, cluster)
                     : launch<paged::few_rows_kernel<D, E4M3, 2>>(grid, 128, paged::Few<D, E4M3, 2>::SMEM, s, P, cluster);
@@ -252,12 +255,12 @@ extern "C" int ofa_paged_attention(const ofa_kv_cache* cache, const ofa_kv_batch
   const Plan p = plan(cache, batch, a->n_rows, a->n_heads);
   if (p.bytes && (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)))
     return fail(OFA_BAD_ARGUMENT, "workspace of %zu bytes on a 16-byte boundary needed, %zu given", p.bytes, a->workspace ? a->workspace_bytes : 0);
-  if ((long long)batch->n_seqs * p.tiles * p.nsplit * (p.many ? cache->n_kv_heads : 1) > 0x7fffffffll) return fail(OFA_BAD_ARGUMENT, "%d sequences are too many for one call", batch->n_seqs);
+  if ((long long)batch->n_seqs * p.tiles * p.nsplit * cache->n_kv_heads > 0x7fffffffll) return fail(OFA_BAD_ARGUMENT, "%d sequences are too many for one call", batch->n_seqs);
   P.q = static_cast<const bf16*>(a->q); P.q_row = a->q_row_stride; P.q_head = a->q_head_stride;
   P.out = static_cast<bf16*>(a->out); P.o_row = a->out_row_stride; P.o_head = a->out_head_stride; P.lse = a->lse;
   P.n_heads = a->n_heads; P.n_kv_heads = cache->n_kv_heads; P.causal = a->causal != 0; P.window = a->window; P.group.set((unsigned)group);
   P.scale_log2 = a->scale * paged::LOG2E; P.flip = 0;
-  P.wide = (long long)cache->n_pages * P.c.page_b + (long long)cache->page_size * P.c.row_b >= 1ll << 35; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.by_head = p.by_head; P.part = static_cast<float*>(a->workspace);
+  P.wide = (long long)cache->n_pages * P.c.page_b + (long long)cache->page_size * P.c.row_b >= 1ll << 35; P.tiles = p.tiles; P.nsplit = p.nsplit; P.cluster = p.cluster; P.by_head = p.by_head; P.ranked = p.ranked; P.part = static_cast<float*>(a->workspace);
   // rows of a box of the copy engine: as many as divide a page and are of use at once, since a lane asks for one after the other
   P.run = std::min(cache->page_size & -cache->page_size, p.many ? 64 : cache->head_dim == 128 && cache->dtype == OFA_KV_BF16 ? 16 : 32);
   if (P.run < 8 || cache->n_pages == 0) P.run = 0;

@@ -589,6 +589,19 @@ def test_thousands_of_sequences(sv):
         assert ((o[st[i]:st[i + 1]].double().cpu() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [128, 129])
+def test_sequences_by_length(sv, n, dtype):
+    """enough of them that blocks start one after the other; equal and missing lengths among them"""
+    g = torch.Generator().manual_seed(n)
+    kv = [int(x) for x in torch.randint(1, 500, (n,), generator=g)]
+    kv[3] = kv[7] = kv[90] = 499
+    new = [1] * n
+    new[5], kv[5], new[6] = 0, 0, 0
+    cache, batch, g = make(sv, new, kv, 8, 64, 16, dtype, max_new=1, max_kv=500)
+    check_attention(sv, cache, batch, queries(g, sum(new), 8, 64))
+
+
 def dense(q, k, v):
     """attention of one sequence whose keys and values lie side by side"""
     class One:
