@@ -51,7 +51,7 @@ struct AttnArgs {
   alignas(64) CUtensorMap km, vm;   // the pages in boxes of `run` rows x 128 bytes (64: 8-bit rows of 64)
   int run;                          // a power of two, 8 .. 64 (few_rows_kernel: .. KEYS), or 0: pages of other sizes, no maps
   int tiles, nsplit;                // of the launch: row tiles per sequence (more are walked through), blocks that share a tile's keys
-  int by_head, ranked;              // the order of blocks in many_rows_kernel; few_rows_kernel: sequences by length (at most 128)
+  int by_head, ranked;              // the order of blocks: in many_rows_kernel; sequences by length (at most 128)
   int cluster;                      // ... which are a cluster and meet in shared memory
   float* part;                      // otherwise, nsplit > 1: [row][head][split][D], and behind them float2 [row][head][split] = {m, l}
 };
@@ -113,6 +113,20 @@ __device__ __forceinline__ float4 peer_f32x4(uint32_t a) {
   return v;
 }
 
+// The sequence (of at most 128) with this place in their order by length, the longest first; scratch: 129 words of shared memory. For all threads of a block of 128 or more.
+__device__ __forceinline__ int by_length(const Batch& B, int place, int* scratch) {
+  const int t = threadIdx.x, len = t < B.n_seqs ? __ldg(B.kv_len + t) : -1;
+  if (t < 128) scratch[t] = len;
+  __syncthreads();
+  if (t < B.n_seqs) {
+    int rank = 0;
+    for (int j = 0; j < B.n_seqs; j++) rank += scratch[j] > len || (scratch[j] == len && j < t);
+    if (rank == place) scratch[128] = t;
+  }
+  __syncthreads();
+  return scratch[128];
+}
+
 template <int D, bool E4M3, int NR> struct Few {
   static constexpr int RB = D * (E4M3 ? 1 : 2);                 // bytes of a row
   static constexpr int KEYS = RB > 128 ? 16 : 32, WARPS = 4, ROWS = 8 * NR;      // of a step: at most 8 KB of keys and values a warp
@@ -154,16 +168,8 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   uint32_t used = 0;                                             // steps of this warp so far: phases of its barriers
   const int split = (int)blockIdx.x % P.nsplit, rest = (int)blockIdx.x / P.nsplit, kvh = rest % P.n_kv_heads, tile0 = rest / P.n_kv_heads % P.tiles;
   int seq = rest / P.n_kv_heads / P.tiles;
-  if (P.ranked) {                                                // the longest first
-    int *lens = reinterpret_cast<int*>(smem), *pick = lens + 128;      // where the rings will be
-    const int len = threadIdx.x < P.b.n_seqs ? __ldg(P.b.kv_len + threadIdx.x) : -1;
-    lens[threadIdx.x] = len;
-    __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < P.b.n_seqs; j++) rank += lens[j] > len || (lens[j] == len && j < (int)threadIdx.x);
-    if ((int)threadIdx.x < P.b.n_seqs && rank == seq) *pick = threadIdx.x;
-    __syncthreads();
-    seq = *pick;
+  if (P.ranked) {
+    seq = by_length(P.b, seq, reinterpret_cast<int*>(smem));     // where the rings will be
     fence_async_shared();                                        // read, before the copy engine writes there
     __syncthreads();
   }

@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
   after_the_kernel_before();
   // The last tiles, which have the most keys, start first: over all sequences and heads, or, where their keys and values together would not stay in L2, head by head
   const int split = (int)blockIdx.x % P.nsplit, rest = (int)blockIdx.x / P.nsplit, streams = P.n_kv_heads * P.b.n_seqs;
-  const int turn = P.by_head ? rest % P.tiles : rest / streams, stream = P.by_head ? rest / P.tiles : rest % streams, kvh = stream % P.n_kv_heads, seq = stream / P.n_kv_heads;
+  const int turn = P.by_head ? rest % P.tiles : rest / streams, stream = P.by_head ? rest / P.tiles : rest % streams, kvh = stream % P.n_kv_heads;
+  const int seq = P.ranked ? by_length(P.b, stream / P.n_kv_heads, reinterpret_cast<int*>(smem)) : stream / P.n_kv_heads;      // where Q will be
   const Chunk ch = chunk_of(P.b, seq);
   const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);

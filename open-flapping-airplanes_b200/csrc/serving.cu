@@ -164,8 +164,8 @@ Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads)
   // Keys and values of all heads above 48 MB are taken head by head (4,096 tokens over 16,384 keys of 8 heads, 67 MB: 850 us, 897 with all heads side by side); below that the longest
   // tiles of all heads go first (prompts of 1,024 tokens, 12.6 MB: 22.8 us, 29.4 head by head).
   p.by_head = (double)b->n_seqs * c->n_kv_heads * kv * c->head_dim * (c->dtype == OFA_KV_E4M3 ? 2 : 4) > 48e6;
-  // Where blocks start one after the other, those of the longest sequences do so first (64 tokens over 1 to 4,096 8-bit keys: 76 us in the order of the table, 67 so; every block ranks the
-  // lengths itself, 0.3 us)
+  // Where blocks start one after the other, those of the longest sequences do so first (64 sequences over 1 to 4,096 keys: a token, 8-bit keys 76 us in the order of the table,
+  // 67 so; five tokens 117 and 104, 8-bit keys 170 and 146). Every block ranks the lengths itself, 0.3 us.
   p.ranked = b->n_seqs > 1 && b->n_seqs <= 128 && blocks * p.nsplit > slots;
   p.tiles = (int)tiles;
   p.bytes = p.nsplit > 1 && !p.cluster ? part * p.nsplit : 0;

@@ -598,8 +598,8 @@ def test_sequences_by_length(sv, n, dtype):
     kv[3] = kv[7] = kv[90] = 499
     new = [1] * n
     new[5], kv[5], new[6] = 0, 0, 0
-    cache, batch, g = make(sv, new, kv, 8, 64, 16, dtype, max_new=1, max_kv=500)
-    check_attention(sv, cache, batch, queries(g, sum(new), 8, 64))
+    cache, batch, g = make(sv, new, kv, 4, 64, 16, dtype, max_new=1, max_kv=500)
+    check_attention(sv, cache, batch, queries(g, sum(new), 4, 64))
 
 
 def dense(q, k, v):
