@@ -224,7 +224,8 @@ const char* ofa_noalloc_last_error(void);
 /* ---- serving over a paged cache ---------------------------------------------------------------------------------------
  * No counterpart in the reference (its decoder keeps one contiguous cache and serves one sequence). Operators for hosts that serve many
  * sequences from a model trained here: each is one or two ordinary kernel launches on `stream` (a cudaStream_t, or NULL) of the current device,
- * allocates nothing, keeps nothing between calls, can be captured into a graph, and returns without waiting. All pointers are device pointers of the
+ * allocates nothing, keeps nothing between calls, can be captured into a graph, and returns without waiting.
+ * Kernels are launched as programmatic dependents of the one before them in the stream and wait for its end before they touch memory. All pointers are device pointers of the
  * current device unless stated; strides are counted in elements and not negative. Errors: OFA_BAD_ARGUMENT or OFA_CUDA_ERROR, nothing launched, text
  * in ofa_serving_last_error() (per thread).
  *
