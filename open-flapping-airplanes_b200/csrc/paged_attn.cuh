@@ -585,12 +585,17 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
   }
 }
 
-// Joins the splits (at most 64) of a row and head, in their order: a warp each. Rows that no sequence brought have no parts and are left as they are.
+// Joins the splits (at most 64) of a row and head, in their order: a warp each. Rows that no sequence brings, or one that chunk_of leaves out, have no parts and are left as they are: the
+// warp looks for the row's sequence by chunk_of's rule (32 at once; calls whose keys are split into parts have few sequences).
 template <int D> __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ AttnArgs P) {
   const long long g = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int row = (int)(g / P.n_heads), head = (int)(g - (long long)row * P.n_heads);
-  const bool mine = row >= __ldg(P.b.q_start) && row < min(__ldg(P.b.q_start + P.b.n_seqs), P.b.n_rows);
+  bool mine = false;
+  for (int i0 = 0; i0 < P.b.n_seqs && !mine; i0 += 32) {
+    const int i = min(i0 + lane, P.b.n_seqs - 1), s = __ldg(P.b.q_start + i), e = __ldg(P.b.q_start + i + 1);
+    mine = __any_sync(0xffffffffu, s >= 0 && e <= P.b.n_rows && s <= row && row < e);
+  }
   cudaGridDependencySynchronize();
   if (!mine) return;
   const float2* ml = reinterpret_cast<const float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D) + g * P.nsplit;

@@ -1,0 +1,53 @@
+"""Serving operators on the GPU where calls leave the ordinary: rows that no sequence brings beside split keys, scores without a finite one, the widest windows and longest contexts, queries of
+any range, long lists of biases."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import serving_reference as ref
+from test_gpu_serving import DEV, check_attention, i32, make, queries, sv  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# Forms of the attention kernels by new tokens and context of a sequence, with two query heads on one key/value head: one block, a cluster of blocks, parts that a second launch joins; few
+# rows and many
+FORMS = {"few": (2, 20), "few_cluster": (1, 1000), "few_parts": (2, 6000), "many": (40, 90), "many_parts": (40, 6000)}
+
+
+def call(sv, ofa, cache, batch, q, out, lse, fill=7.0, **more):  # noqa: F811
+    """ofa_paged_attention with a workspace that holds something; its size in bytes"""
+    lib, K = ofa.capi.load(), ofa.capi
+    n, heads, dim = q.shape
+    need = lib.ofa_paged_attention_workspace(cache.ref, batch.ref, n, heads)
+    work = torch.full((need // 4 + 4,), fill, device=DEV)
+    a = K.PagedAttentionArgs(n, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), cache.scale, True, 0, work.data_ptr(), need)
+    for k, v in more.items():
+        setattr(a, k, v)
+    assert lib.ofa_paged_attention(cache.ref, batch.ref, C.byref(a), torch.cuda.current_stream().cuda_stream) == K.OK
+    return need
+
+
+@pytest.mark.parametrize("status", [True, False])
+@pytest.mark.parametrize("form", ["few_cluster", "few_parts", "many", "many_parts"])
+@pytest.mark.parametrize("kind", ["beyond", "falling", "negative", "alone_beyond", "behind_the_first"])
+def test_rows_of_sequences_that_are_left_out_stay_as_they_were(sv, ofa, kind, form, status):  # noqa: F811
+    g, kv = FORMS[form]
+    n = g + 6
+    st, first = {"beyond": ([0, g, n + 90], 0), "falling": ([0, g, g - 1], 0), "negative": ([-1, g], None), "alone_beyond": ([0, n + 1], None), "behind_the_first": ([3, 3 + g], 3)}[kind]
+    cache, made, gen = make(sv, [g], [kv], 1, 64, 16)
+    seqs = len(st) - 1
+    word = i32([0])
+    batch = sv.KVBatch(i32(st), i32([kv] * seqs), made.pages.expand(seqs, -1), max_new=g, max_kv=kv, status=word if status else None)
+    q = queries(gen, n, 2, 64)
+    out, lse = torch.full((n, 2, 64), 3.0, dtype=torch.bfloat16, device=DEV), torch.full((n, 2), 3.0, device=DEV)
+    assert (call(sv, ofa, cache, batch, q, out, lse) > 0) == form.endswith("parts")
+    have = torch.zeros(n, dtype=torch.bool)
+    if first is not None:
+        have[first:first + g] = True
+        want, want_lse, tol, tol_lse = ref.attention(cache, [first, first + g], [kv], made.pages.cpu(), q, cache.scale)
+        assert ((out.double().cpu() - want).abs() <= tol)[have].all() and ((lse.double().cpu() - want_lse).abs() <= tol_lse)[have].all()
+    assert (out.cpu()[~have] == 3).all() and (lse.cpu()[~have] == 3).all()
+    if status:
+        assert int(word) == (0 if kind == "behind_the_first" else sv.BAD_ROWS)
