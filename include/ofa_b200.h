@@ -271,7 +271,7 @@ int ofa_kv_read(const ofa_kv_cache* cache, const ofa_kv_batch* batch, void* k, v
 /* out[row][h] = softmax over the cached keys that the row sees of scale * q.k, times their values; heads h of [g * n_heads / n_kv_heads ...) share key/value head g.
  * causal: a row at position p sees positions <= p, and with window > 0 only those > p - window; otherwise all kv_len. The rows' own keys
  * have to be in the cache (ofa_kv_append). lse (may be NULL, [n_rows][n_heads] fp32): the natural logarithm of the sum of exponentials. A row
- * that sees no key gets zeros and -inf. out may be q itself, otherwise they do not overlap. Keys without a page are not seen. What a row does not see does not reach it, infinities and NaN included.
+ * that sees no key gets zeros and -inf; one that sees keys, but whose scores are all -inf, gets NaN and -inf. out may be q itself, otherwise they do not overlap. Keys without a page are not seen. What a row does not see does not reach it, infinities and NaN included.
  * workspace: ofa_paged_attention_workspace() bytes, 16-byte aligned, contents of no interest before and after; calls that may overlap need one each. */
 typedef struct {
   int n_rows, n_heads;

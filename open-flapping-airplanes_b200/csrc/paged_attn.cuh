@@ -127,6 +127,20 @@ __device__ __forceinline__ int by_length(const Batch& B, int place, int* scratch
   return scratch[128];
 }
 
+// Whether a row at position pos of sequence i sees any key. Asked only where the sum of a row's exponentials is 0: a row that sees nothing gets zeros, one whose scores are all
+// -inf has no softmax, and gets NaN.
+__device__ __forceinline__ bool sees_any(const AttnArgs& P, int i, int pos) {
+  const int cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)__ldg(P.b.kv_len + i)), hi = P.causal ? min(cap, pos + 1) : cap, lo = P.window ? max(0, pos - P.window + 1) : 0;
+  if (hi <= lo) return false;
+  const unsigned last = P.b.page.quot((unsigned)(hi - 1));
+#pragma unroll 1
+  for (unsigned idx = P.b.page.quot((unsigned)lo); idx <= last; idx++)
+    if ((unsigned)__ldg(P.b.pages + (long long)i * P.b.pages_stride + idx) < (unsigned)P.b.n_pages) return true;
+  return false;
+}
+// What a row's sums are multiplied by, for l the sum of its exponentials
+__device__ __forceinline__ float over(const AttnArgs& P, float l, int i, int pos) { return l != 0.f ? 1.f / l : sees_any(P, i, pos) ? __int_as_float(0x7fc00000) : 0.f; }
+
 template <int D, bool E4M3, int NR> struct Few {
   static constexpr int RB = D * (E4M3 ? 1 : 2);                 // bytes of a row
   static constexpr int KEYS = RB > 128 ? 16 : 32, WARPS = 4, ROWS = 8 * NR;      // of a step: at most 8 KB of keys and values a warp
@@ -567,7 +581,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         }
       }
       if (last && (P.cluster || P.nsplit == 1)) {
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        const float inv = over(P, ll, seq, ch.p0 + t);
         bf16* dst = P.out + (long long)(ch.s + t) * P.o_row + (long long)head * P.o_head + part * 4;
 #pragma unroll
         for (int x = 0; x < DP; x += 4) *reinterpret_cast<uint2*>(dst + x * TPR) = make_uint2(pack2f(acc[x] * inv, acc[x + 1] * inv), pack2f(acc[x + 2] * inv, acc[x + 3] * inv));
@@ -591,13 +605,14 @@ template <int D> __global__ void __launch_bounds__(128) combine_kernel(const __g
   const long long g = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int row = (int)(g / P.n_heads), head = (int)(g - (long long)row * P.n_heads);
-  bool mine = false;
-  for (int i0 = 0; i0 < P.b.n_seqs && !mine; i0 += 32) {
+  int seq = -1;
+  for (int i0 = 0; i0 < P.b.n_seqs && seq < 0; i0 += 32) {
     const int i = min(i0 + lane, P.b.n_seqs - 1), s = __ldg(P.b.q_start + i), e = __ldg(P.b.q_start + i + 1);
-    mine = __any_sync(0xffffffffu, s >= 0 && e <= P.b.n_rows && s <= row && row < e);
+    const uint32_t here = __ballot_sync(0xffffffffu, s >= 0 && e <= P.b.n_rows && s <= row && row < e);
+    if (here) seq = min(i0 + __ffs(here) - 1, P.b.n_seqs - 1);
   }
   cudaGridDependencySynchronize();
-  if (!mine) return;
+  if (seq < 0) return;
   const float2* ml = reinterpret_cast<const float2*>(P.part + (long long)P.b.n_rows * P.n_heads * P.nsplit * D) + g * P.nsplit;
   float2 a = lane < P.nsplit ? ml[lane] : make_float2(-INFINITY, 0.f), b = lane + 32 < P.nsplit ? ml[lane + 32] : make_float2(-INFINITY, 0.f);
   const float mm = warp_max(fmaxf(a.x, b.x));
@@ -611,7 +626,7 @@ template <int D> __global__ void __launch_bounds__(128) combine_kernel(const __g
 #pragma unroll
     for (int x = 0; x < DP; x++) acc[x] += src[(long long)s * D + x] * f;
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const float inv = over(P, ll, seq, __ldg(P.b.kv_len + seq) - __ldg(P.b.q_start + seq + 1) + row);
   bf16* dst = P.out + (long long)row * P.o_row + (long long)head * P.o_head + lane * DP;
 #pragma unroll
   for (int x = 0; x < DP; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack2f(acc[x] * inv, acc[x + 1] * inv);

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
       if (ok && !idle) {                                         // the row's result, or its part for combine_kernel
         const int olo = *reinterpret_cast<volatile int*>(&ct.odd_lo), ohi = *reinterpret_cast<volatile int*>(&ct.odd_hi);
         const long long g = (long long)(ch.s + t) * P.n_heads + head;
-        const float inv = P.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float inv = P.nsplit > 1 || !on ? 1.f : over(P, l, seq, pos);
 #pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
           uint32_t o[32];

@@ -51,3 +51,38 @@ def test_rows_of_sequences_that_are_left_out_stay_as_they_were(sv, ofa, kind, fo
     assert (out.cpu()[~have] == 3).all() and (lse.cpu()[~have] == 3).all()
     if status:
         assert int(word) == (0 if kind == "behind_the_first" else sv.BAD_ROWS)
+
+
+def infinite_query(dtype, form, sv):  # noqa: F811
+    """A cache whose keys are all below zero in their first dim, queries of which one, (0, 0), is infinite there"""
+    n, kv = FORMS[form]
+    cache, batch, gen = make(sv, [n], [kv], 1, 64, 16, dtype, max_new=n, max_kv=kv)
+    if dtype == "e4m3":
+        cache.k.view(torch.uint8)[..., 0] = 0xb8                         # -1
+    else:
+        cache.k[..., 0] = -1
+    q = queries(gen, n, 2, 64)
+    q[0, 0, 0] = math.inf
+    return cache, batch, q, n, kv
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_without_a_finite_one(sv, form, dtype):  # noqa: F811
+    """exp(x - max x) has no value where every score that a row sees is -inf; a row that sees no key is another matter"""
+    cache, batch, q, n, kv = infinite_query(dtype, form, sv)
+    out, lse = sv.paged_attention(cache, batch, q, with_lse=True)
+    out, lse = out.double().cpu(), lse.double().cpu()
+    assert torch.isnan(out[0, 0]).all()
+    clean = q.clone()
+    clean[0, 0, 0] = 0
+    want, want_lse, tol, tol_lse = ref.attention(cache, [0, n], [kv], batch.pages.cpu(), clean, cache.scale)
+    some = torch.ones(n, 2, dtype=torch.bool)
+    some[0, 0] = False
+    assert ((out - want).abs() <= tol)[some].all() and ((lse - want_lse).abs() <= tol_lse)[some].all()
+    if dtype == "bf16" or n > 16:
+        assert lse[0, 0] == -math.inf
+    none = sv.KVBatch(batch.q_start, batch.kv_len, torch.full_like(batch.pages, -1), max_new=n, max_kv=kv)
+    for b in (none, sv.KVBatch(batch.q_start, i32([n - 1]), batch.pages, max_new=n, max_kv=kv)):     # no page; one position less than rows
+        out, lse = sv.paged_attention(cache, b, q, with_lse=True)
+        assert (out[0] == 0).all() and (lse[0] == -math.inf).all()
