@@ -127,10 +127,12 @@ __device__ __forceinline__ int by_length(const Batch& B, int place, int* scratch
   return scratch[128];
 }
 
+// The first key that a row at position pos sees; without a difference that leaves 32 bits (positions may be negative, and windows as large as an int)
+__device__ __forceinline__ int first_seen(const AttnArgs& P, int pos) { return P.window && pos >= P.window ? pos - P.window + 1 : 0; }
 // Whether a row at position pos of sequence i sees any key. Asked only where the sum of a row's exponentials is 0: a row that sees nothing gets zeros, one whose scores are all
 // -inf has no softmax, and gets NaN.
 __device__ __forceinline__ bool sees_any(const AttnArgs& P, int i, int pos) {
-  const int cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)__ldg(P.b.kv_len + i)), hi = P.causal ? min(cap, pos + 1) : cap, lo = P.window ? max(0, pos - P.window + 1) : 0;
+  const int cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)__ldg(P.b.kv_len + i)), hi = P.causal ? min(cap, pos + 1) : cap, lo = first_seen(P, pos);
   if (hi <= lo) return false;
   const unsigned last = P.b.page.quot((unsigned)(hi - 1));
 #pragma unroll 1
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         for (int h = 0; h < 2; h++) rowf[n][h] *= __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
       }
     }
-    const int hi = min(cap, P.causal ? p_max + 1 : ch.len), lo = P.window ? max(0, p_min - P.window + 1) : 0;
+    const int hi = min(cap, P.causal ? p_max + 1 : ch.len), lo = first_seen(P, p_min);
     const int first = lo / F::KEYS, nst = max(0, (hi + F::KEYS - 1) / F::KEYS - first);
     const int a = first + (int)((long long)nst * split / P.nsplit) + warp, b = first + (int)((long long)nst * (split + 1) / P.nsplit);
     const int mine = b > a ? (b - a + F::WARPS - 1) / F::WARPS : 0;
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         kf = __uint_as_float(k8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)min(max(k8, 1), E_MAX + 127) << 23);
         vf = __uint_as_float(v8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)(min(v8, E_MAX + 127) + 100) << 23);
       }
-      const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 <= p_max - P.window);
+      const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || k0 < first_seen(P, p_max);
       float s[F::NB][NR][4];
       float fk[F::NB][2], fv[F::NB][2];
 #pragma unroll
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             if constexpr (E4M3) x *= fk[kk][e >> 1];
             if (mask) {
               const int at = kk * 16 + (e >> 1) * 8 + r, p = k0 + at, q = pos[n][e & 1];
-              if (!((valid >> at) & 1) || (P.causal && p > q) || (P.window && p <= q - P.window)) x = -INFINITY;
+              if (!((valid >> at) & 1) || (P.causal && p > q) || p < first_seen(P, q)) x = -INFINITY;
             }
             mx[n][e & 1] = fmaxf(mx[n][e & 1], x);
           }
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 #pragma unroll
                 for (int n = 0; n < NR; n++)
 #pragma unroll
-                  for (int h = 0; h < 2; h++) if (!(P.causal && p > pos[n][h]) && !(P.window && p <= pos[n][h] - P.window)) o[n][t][2 * e + h] += x;
+                  for (int h = 0; h < 2; h++) if (!(P.causal && p > pos[n][h]) && p >= first_seen(P, pos[n][h])) o[n][t][2 * e + h] += x;
               }
           }
         }

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
       const int r0 = (pair * NT + i) * F::ROWS;
       if (r0 >= ch.n * group) { k.a[i] = k.b[i] = 0; continue; }
       const int pmin = ch.p0 + (int)P.group.quot(r0), pmax = ch.p0 + min(ch.n - 1, (int)P.group.quot(r0 + F::ROWS - 1));
-      const int h = min(cap, P.causal ? pmax + 1 : ch.len), l = P.window ? max(0, pmin - P.window + 1) : 0;
+      const int h = min(cap, P.causal ? pmax + 1 : ch.len), l = first_seen(P, pmin);
       if (i == 0) k.p_low = pmin;
       k.p_high = pmax;
       k.a[i] = l / 128; k.b[i] = h > l ? (h + 127) / 128 : k.a[i];
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
   };
   // a step that not every row of the block sees whole
   auto partial = [&](const Walk& k, int j) {
-    return j * 128 < k.lo || j * 128 + 128 > k.hi || (P.causal && j * 128 + 127 > k.p_low) || (P.window && j * 128 <= k.p_high - P.window);
+    return j * 128 < k.lo || j * 128 + 128 > k.hi || (P.causal && j * 128 + 127 > k.p_low) || j * 128 < first_seen(P, k.p_high);
   };
   // the end of a pair for all warps: tiles, control words and tensor memory are free for the next; false: a wait ran out somewhere
   auto next = [&](bool ok) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
         attn_tc::warp_arrive(smem_u32(&ct.s_free[tile]));        // the first half of the next scores may overwrite these
         const uint4 vw = *reinterpret_cast<const uint4*>(ct.valid[j % F::NV]);
         if (partial(k, j) || (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu) {
-          const int x1 = P.causal ? pos - k0 : 127, x0 = P.window ? pos - P.window + 1 - k0 : 0;       // of the step's keys the row sees x0 .. x1
+          const int x1 = P.causal ? pos - k0 : 127, x0 = first_seen(P, pos) - k0;       // of the step's keys the row sees x0 .. x1
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const uint32_t w = (q == 0 ? vw.x : q == 1 ? vw.y : q == 2 ? vw.z : vw.w) & below(x1 + 1 - q * 32) & ~below(x0 - q * 32);
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
           if (ohi >= olo) {                                      // rare: what the loaders left out
             for (int key = olo; key <= ohi; key++) {
               int page, at;
-              if ((P.causal && key > pos) || (P.window && key <= pos - P.window) || key / 128 < k.a[tile] || key / 128 >= k.b[tile] || !locate(P.b, seq, key, page, at)) continue;
+              if ((P.causal && key > pos) || key < first_seen(P, pos) || key / 128 < k.a[tile] || key / 128 >= k.b[tile] || !locate(P.b, seq, key, page, at)) continue;
               const char* row = P.c.v + (long long)kvh * P.c.head_b + (long long)page * P.c.page_b + (long long)at * P.c.row_b;
               const int sc = E4M3 ? P.c.vs[(long long)page * P.c.s_page + (long long)kvh * P.c.s_head + (long long)at * P.c.s_row] : 0;
 #pragma unroll

@@ -86,3 +86,15 @@ def test_scores_without_a_finite_one(sv, form, dtype):  # noqa: F811
     for b in (none, sv.KVBatch(batch.q_start, i32([n - 1]), batch.pages, max_new=n, max_kv=kv)):     # no page; one position less than rows
         out, lse = sv.paged_attention(cache, b, q, with_lse=True)
         assert (out[0] == 0).all() and (lse[0] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 7, 2 ** 31 - 128, 2 ** 30])
+@pytest.mark.parametrize("new,kv", [(8, 2), (8, 200), (150, 3), (150, 140), (40, 6000), (4, 6000)])
+def test_a_window_wider_than_any_context(sv, new, kv, window, dtype):  # noqa: F811
+    """sees what no window sees, in sequences shorter than what they bring too"""
+    cache, batch, gen = make(sv, [new], [kv], 1, 64, 16, dtype, max_new=new)
+    q = queries(gen, new, 2, 64)
+    got, lse = check_attention(sv, cache, batch, q, window=window)
+    want, want_lse = sv.paged_attention(cache, batch, q, with_lse=True)
+    assert torch.equal(got, want.double().cpu()) and torch.equal(lse, want_lse.double().cpu())
