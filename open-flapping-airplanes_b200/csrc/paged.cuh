@@ -55,6 +55,8 @@ __device__ __forceinline__ Chunk chunk_of(const Batch& B, int i) {
   if (len < 0) { flag(B.status, ST_LENGTH); return {s, e - s, s - e, 0}; }
   return {s, e - s, len - (e - s), len};
 }
+// Keys that attention over a context of this length reaches: those that the page table has, at most 2^31 - 1024: what is looked up ahead of a step has a position of 31 bits too
+__device__ __forceinline__ int reach(const Batch& B, int len) { return (int)min(min((long long)B.max_pages * B.page.d, 0x7ffffc00ll), (long long)len); }
 // page and row of position pos (>= 0) of sequence i; false, and a bit in the status word, where the table has none
 __device__ __forceinline__ bool locate(const Batch& B, int i, int pos, int& page, int& at) {
   const unsigned idx = B.page.quot((unsigned)pos);

@@ -132,7 +132,7 @@ __device__ __forceinline__ int first_seen(const AttnArgs& P, int pos) { return P
 // Whether a row at position pos of sequence i sees any key. Asked only where the sum of a row's exponentials is 0: a row that sees nothing gets zeros, one whose scores are all
 // -inf has no softmax, and gets NaN.
 __device__ __forceinline__ bool sees_any(const AttnArgs& P, int i, int pos) {
-  const int cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)__ldg(P.b.kv_len + i)), hi = P.causal ? min(cap, pos + 1) : cap, lo = first_seen(P, pos);
+  const int cap = reach(P.b, __ldg(P.b.kv_len + i)), hi = P.causal ? min(cap, pos + 1) : cap, lo = first_seen(P, pos);
   if (hi <= lo) return false;
   const unsigned last = P.b.page.quot((unsigned)(hi - 1));
 #pragma unroll 1
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
     __syncthreads();
   }
   const Chunk ch = chunk_of(P.b, seq);
-  const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
+  const int group = (int)P.group.d, cap = reach(P.b, ch.len);
   if (ch.len > cap && threadIdx.x == 0) flag(P.b.status, ST_LENGTH);
   unsigned char* ring = smem + warp * F::STAGES * F::STAGE;
   const uint32_t ring_s = smem_u32(ring);

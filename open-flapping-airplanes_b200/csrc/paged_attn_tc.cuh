@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
   const int turn = P.by_head ? rest % P.tiles : rest / streams, stream = P.by_head ? rest / P.tiles : rest % streams, kvh = stream % P.n_kv_heads;
   const int seq = P.ranked ? by_length(P.b, stream / P.n_kv_heads, reinterpret_cast<int*>(smem)) : stream / P.n_kv_heads;      // where Q will be
   const Chunk ch = chunk_of(P.b, seq);
-  const int group = (int)P.group.d, cap = (int)min((long long)P.b.max_pages * P.b.page.d, (long long)ch.len);
+  const int group = (int)P.group.d, cap = reach(P.b, ch.len);
   if (ch.len > cap && tid == 0) flag(P.b.status, ST_LENGTH);
   const int npair = (ch.n * group + NT * F::ROWS - 1) / (NT * F::ROWS);      // pairs of tiles, or tiles
   if (turn >= npair) return;

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256, 8) move_kernel(const __grid_constant__ Mo
   if (tid < MOVE_ROWS && place[tid].x >= 0) {
     const int i = place[tid].x;
     const Chunk ch = chunk_of(P.b, i);
-    const int pos = ch.p0 + r0 + tid - ch.s;
+    const int pos = ch.p0 + (r0 + tid - ch.s);
     int page, at;
     if (pos < 0 || !locate(P.b, i, pos, page, at)) page = -1, at = 0;
     place[tid] = make_int2(page, at);

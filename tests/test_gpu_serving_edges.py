@@ -98,3 +98,41 @@ def test_a_window_wider_than_any_context(sv, new, kv, window, dtype):  # noqa: F
     got, lse = check_attention(sv, cache, batch, q, window=window)
     want, want_lse = sv.paged_attention(cache, batch, q, with_lse=True)
     assert torch.equal(got, want.double().cpu()) and torch.equal(lse, want_lse.double().cpu())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [1 << 16, 100003])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_context_as_long_as_an_int(sv, new, page, dtype):  # noqa: F811
+    """One page that stands throughout a table of 2^31 positions; the last of them, behind 2^31 - 1024, are beyond what a context may have"""
+    top, length, window = 2 ** 31 - 1024, 2 ** 31 - 1, 3000
+    gen = torch.Generator().manual_seed(page + new)
+    cols = -(-2 ** 31 // page)
+    table = torch.zeros(1, cols, dtype=torch.int32, device=DEV)
+    shape = (1, 1, page, 64)
+    if dtype == "e4m3":
+        cache = sv.KVCache(*(torch.randn(shape, generator=gen).to(torch.float8_e4m3fn).to(DEV) for _ in range(2)), *(torch.full(shape[:3], 127, dtype=torch.uint8, device=DEV) for _ in range(2)))
+    else:
+        cache = sv.KVCache(*(torch.randn(shape, generator=gen).bfloat16().to(DEV) for _ in range(2)))
+    q = queries(gen, new, 2, 64)
+    for kv, status in ((top, 0), (length, sv.BAD_LENGTH)):
+        batch = sv.KVBatch(i32([0, new]), i32([kv]), table, max_new=new, max_kv=window, status=i32([0]))
+        got, lse = sv.paged_attention(cache, batch, q, window=window, with_lse=True)
+        assert int(batch.status) == status
+        k, v = (x[0, 0].double().cpu() for x in (cache.k, cache.v))
+        for t in range(0, new, 13):
+            pos = kv - new + t
+            at = torch.arange(pos - window + 1, min(pos + 1, top)) % page
+            for h in range(2):
+                want, want_lse, tol, tol_lse = one_row(q[t, h].double().cpu(), k[at], v[at], 1 / 8)
+                assert ((got[t, h].double().cpu() - want).abs() <= tol).all() and abs(float(lse[t, h]) - want_lse) <= tol_lse
+
+
+def one_row(q, k, v, scale):
+    """(out, lse, their bounds) of one row that sees all of k and v, as serving_reference counts them"""
+    x = k @ q * scale
+    z = torch.logsumexp(x, 0)
+    p = torch.exp(x - z)
+    off = float((k.abs() @ q.abs()).max()) * abs(scale) * (len(q) + 16) * 2.0 ** -23 + 2.0 ** -20
+    out = p @ v
+    return out, float(z), p @ v.abs() * (ref.BF16_HALF + 2 * off) + out.abs() * ref.BF16_HALF * (1 + ref.BF16_HALF) + 1e-37, off + abs(float(z)) * 2.0 ** -22
