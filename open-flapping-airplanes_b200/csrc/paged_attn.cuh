@@ -382,8 +382,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             float& x = s[kk][n][e];
-            x *= rowf[n][e & 1];
-            if constexpr (E4M3) x *= fk[kk][e >> 1];
+            x *= E4M3 ? rowf[n][e & 1] * fk[kk][e >> 1] : rowf[n][e & 1];      // a key's scale is a power of two: first with the row's factor, a large query's sum may not have room for it
             if (mask) {
               const int at = kk * 16 + (e >> 1) * 8 + r, p = k0 + at, q = pos[n][e & 1];
               if (!((valid >> at) & 1) || (P.causal && p > q) || p < first_seen(P, q)) x = -INFINITY;

@@ -136,3 +136,33 @@ def one_row(q, k, v, scale):
     off = float((k.abs() @ q.abs()).max()) * abs(scale) * (len(q) + 16) * 2.0 ** -23 + 2.0 ** -20
     out = p @ v
     return out, float(z), p @ v.abs() * (ref.BF16_HALF + 2 * off) + out.abs() * ref.BF16_HALF * (1 + ref.BF16_HALF) + 1e-37, off + abs(float(z)) * 2.0 ** -22
+
+
+def held_cache(sv, codes, exponents):  # noqa: F811
+    """An 8-bit cache of one page: keys and values of these codes (as floats) [n, dim] and scales 2^e [n]"""
+    n, dim = codes[0].shape
+    pools = [c.to(torch.float8_e4m3fn).view(1, 1, n, dim).to(DEV) for c in codes]
+    return sv.KVCache(*pools, *((e + 127).to(torch.uint8).view(1, 1, n).to(DEV) for e in exponents))
+
+
+def large_scores(sv, rows, exponent):  # noqa: F811
+    """Queries of 2^120 to 2^127 over 8-bit keys of this scale: the row's result is the value of the key whose score is largest by far, its lse that score"""
+    gen = torch.Generator().manual_seed(rows)
+    n, dim = 50, 64
+    k = torch.zeros(n, dim)
+    k[:, 3], k[20, 3] = 416.0, 448.0
+    v = torch.randn(n, dim, generator=gen)
+    cache = held_cache(sv, [k, v], [torch.full((n,), float(exponent)), torch.zeros(n)])
+    q = torch.zeros(rows, 1, dim)
+    q[:, 0, 3] = 2.0 ** torch.arange(120, 128).float().repeat(-(-rows // 8))[:rows]
+    q = q.bfloat16().to(DEV)
+    out, lse = sv.paged_attention(cache, sv.KVBatch(i32([0, rows]), i32([n]), i32([[0]]), max_new=rows), q, causal=False, with_lse=True)
+    assert (out[:, 0].cpu() == v[20].to(torch.float8_e4m3fn).bfloat16()).all()
+    want = q[:, 0, 3].double().cpu() * 448 * 2.0 ** exponent / 8
+    assert ((lse[:, 0].double().cpu() - want).abs() <= want * 2.0 ** -21).all()      # at most eight roundings of 32 bits
+
+
+@pytest.mark.parametrize("rows", [1, 16])
+def test_large_queries_over_keys_of_the_smallest_scales(sv, rows):  # noqa: F811
+    """2^127 times 448 leaves 32 bits before a key's scale of 2^-100 is applied, the score does not"""
+    large_scores(sv, rows, -100)
