@@ -64,6 +64,8 @@ struct TcCtrl {
 };
 static_assert(sizeof(TcCtrl) <= 640, "control area");
 
+constexpr float BIG = 268435456.f;                              // 2^28
+
 __device__ __forceinline__ bool elect_one() {                  // one thread of a converged warp
   uint32_t e;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
@@ -182,6 +184,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
       attn_tc::warp_arrive(smem_u32(&ct.q_full));
       const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + F::O_AT + tile * D;
       float m = -INFINITY, l = 0.f;
+      bool big = false;
       const int n = k.b[tile] - k.a[tile];
       for (int c = 0; c < n; c++) {
         const int j = k.a[tile] + c, k0 = j * 128;
@@ -222,12 +225,13 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
 #pragma unroll
           for (int q = 0; q < 4; q++) mx[q] = attn_tc::max3(mx[q], __uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1]));
         const float m_true = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2);
-        if (c == 0) m = m_true;
+        if (c == 0) { m = m_true; big = __any_sync(0xffffffffu, fabsf(m) > BIG && m != -INFINITY); }
         else {
           const bool grow = m_true > m + RESCALE_LOG2;
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? ex2_approx(m - m_true) : 1.f;
             if (grow) { m = m_true; l *= alpha; }
+            big = __any_sync(0xffffffffu, fabsf(m) > BIG && m != -INFINITY);
 #pragma unroll 1
             for (int q = 0; q < D / 16; q++) {
               uint32_t o[16];
@@ -239,7 +243,17 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;              // no key seen yet: 2^(-inf - 0) = 0
-        const u64 sc2 = attn_tc::f2(P.scale_log2, P.scale_log2), nm2 = attn_tc::f2(-ref, -ref);
+        // A multiply-add forms the product exactly, the reference is a rounded one: the largest score's exponent is half a step of the reference off 0, which beyond 2^28 may be
+        // more than sums have room for. There the scores are rounded first.
+        float sc = P.scale_log2;
+        if (big) [[unlikely]] {
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int x = 0; x < 32; x++) s[q][x] = __float_as_uint(__uint_as_float(s[q][x]) * sc);
+          sc = 1.f;
+        }
+        const u64 sc2 = attn_tc::f2(sc, sc), nm2 = attn_tc::f2(-ref, -ref);
         u64 sum[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; q++) {

@@ -166,3 +166,10 @@ def large_scores(sv, rows, exponent):  # noqa: F811
 def test_large_queries_over_keys_of_the_smallest_scales(sv, rows):  # noqa: F811
     """2^127 times 448 leaves 32 bits before a key's scale of 2^-100 is applied, the score does not"""
     large_scores(sv, rows, -100)
+
+
+@pytest.mark.parametrize("exponent", [-100, -60, -20])
+@pytest.mark.parametrize("rows", [40, 150])
+def test_scores_beyond_the_range_of_an_exponential(sv, rows, exponent):  # noqa: F811
+    """of 2^26 to 2^113"""
+    large_scores(sv, rows, exponent)
