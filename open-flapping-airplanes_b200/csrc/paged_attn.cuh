@@ -18,18 +18,16 @@
 //            of the t-th product are two neighbouring dims
 // The scores' accumulator has keys down the lanes, the second product wants them along a lane: movmatrix turns 8 x 8 of them.
 //
-// Keys of the 8-bit cache are operands as they are: a row of q is brought to 128 .. 256 by a power of two and split into two e4m3 numbers, the second holding
-// 16 times what the first leaves, which is all 8 bits of a bf16 number down to 2^-13 of the row's largest and 2^-21 of that below (products of e4m3 numbers are summed in fp32 as
-// exactly as those of bf16). Values enter as bf16 of 2^-120 times their codes (paged::raw_pair, three instructions for two elements). Keys' scales multiply the scores, values'
-// scales the probabilities, which carry 2^100 so that nothing underflows (the result is 2^-20 of what it should be, made good at the end). Widening the keys like the
-// values left the byte and logic instructions of the integer pipe, two clocks each, as the bound: 10 of them for four elements.
+// Rows of the 8-bit cache enter the products as bf16 of 2^-120 times their codes (paged::raw_pair, three instructions for two elements), which is exact, and so are the queries: bf16 as
+// they came, a row's largest magnitude brought to 2^127 by a power of two. Keys' scales multiply the scores, values' scales the probabilities, which carry 2^100 so that nothing
+// underflows (the result is 2^-20 of what it should be, made good at the end). Queries split into two e4m3 numbers against the keys as they are saved the widening, lost bits of elements
+// below 2^-13 of a row's largest, and was no faster: 64 tokens over 4,096 keys, 32 heads over 8, 114 us against 112; four tokens each 160 against 144.
 //
 // A key that a row does not see counts nothing, whatever is stored there: its score is replaced, and where some rows of the tile see it and others do not,
 // infinities and NaN are taken out of its values and added to the rows that see it. What lies behind the context in its last page may be fetched and counts nowhere; nothing
 // of a bad page is read.
 #pragma once
 #include <cuda.h>
-#include <cuda_fp8.h>
 #include "paged.cuh"
 
 namespace ofa {
@@ -64,20 +62,6 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16832_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// four values as e4m3 numbers, to nearest; what they leave comes back in their place
-__device__ __forceinline__ uint32_t split_e4m3(float (&v)[4]) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)((i < 2 ? lo : hi) >> (i & 1) * 8 & 255), __NV_E4M3);
-    v[i] -= __half2float(*reinterpret_cast<const __half*>(&h));
-  }
-  return lo | hi << 16;
 }
 __device__ __forceinline__ bool odd_bits(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }   // an infinity or a NaN in the pair
 __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
@@ -204,7 +188,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 
   for (int tile = tile0; tile * F::ROWS < ch.n * group; tile += P.tiles) {
     const int t_last = min(ch.n - 1, (int)P.group.quot(tile * F::ROWS + F::ROWS - 1)), p_min = ch.p0 + (int)P.group.quot(tile * F::ROWS), p_max = ch.p0 + t_last;
-    uint32_t qf[NR][KS][2], ql[NR][KS][2];                       // row r of every eight; 8-bit keys: 16 times what qf leaves
+    uint32_t qf[NR][D / 16][2];                                  // row r of every eight
     float rowf[NR][2];                                           // what the raw scores of rows 2c and 2c + 1 of every eight are multiplied by
     int pos[NR][2];                                              // and where they stand
 #pragma unroll
@@ -227,29 +211,17 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         pos[n][h] = t2 < ch.n ? ch.p0 + t2 : p_max;
         rowf[n][h] = P.scale_log2;
       }
-      if constexpr (E4M3) {
+      if constexpr (E4M3) {                                      // the row's largest magnitude to 2^127, since widened keys are 2^-120 of theirs
         unsigned mag = 0;
 #pragma unroll
         for (int s = 0; s < KS; s++) mag = max(mag, max_bits(qv[s]));
         mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
         mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
-        const int shift = min(7 - ((int)(mag >> 7) - 127), 120);                     // largest magnitude to 2^7 ..
-        const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
-        float down = __uint_as_float((uint32_t)(127 - shift) << 23);
-        if (mag >= 0x7f80u) down = __uint_as_float(0x7fc00000u);                     // an infinity or a NaN in the row
+        const int shift = min(max(127 - ((int)(mag >> 7) - 127), 0), 127);
+        const float up = __uint_as_float((uint32_t)(127 + shift) << 23), down = __uint_as_float((uint32_t)(247 - shift) << 23);      // 2^(120 - shift)
+        auto times_up = [&](uint32_t w) { const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); return pack2f(x.x * up, x.y * up); };
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-          const uint32_t w[4] = {qv[s].x, qv[s].y, qv[s].z, qv[s].w};
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[2 * h])), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[2 * h + 1]));
-            float v[4] = {x.x * up, x.y * up, y.x * up, y.y * up};
-            qf[n][s][h] = split_e4m3(v);
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] *= 16.f;
-            ql[n][s][h] = split_e4m3(v);
-          }
-        }
+        for (int s = 0; s < KS; s++) { qf[n][2 * s][0] = times_up(qv[s].x); qf[n][2 * s][1] = times_up(qv[s].y); qf[n][2 * s + 1][0] = times_up(qv[s].z); qf[n][2 * s + 1][1] = times_up(qv[s].w); }
 #pragma unroll
         for (int h = 0; h < 2; h++) rowf[n][h] *= __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
       }
@@ -351,13 +323,12 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
           const unsigned char* src = sk + (x & 1 ? ka1 : ka0) + x / 2 * (F::KEYS * 128) + kk * 16 * F::W;
           const uint4 wa = *reinterpret_cast<const uint4*>(src), wb = *reinterpret_cast<const uint4*>(src + 8 * F::W);
           if constexpr (E4M3) {
-            const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
+            const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-            for (int n = 0; n < NR; n++) {
-              mma16832_e4m3(s[kk][n], a0, qf[n][2 * x][0], qf[n][2 * x][1]);
-              mma16832_e4m3(s2[n], a0, ql[n][2 * x][0], ql[n][2 * x][1]);
-              mma16832_e4m3(s[kk][n], a1, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
-              mma16832_e4m3(s2[n], a1, ql[n][2 * x + 1][0], ql[n][2 * x + 1][1]);
+            for (int i = 0; i < 4; i++) {
+              const uint32_t a0[4] = {raw_pair(ua[i], ua[i], raw_sel(0, 1)), raw_pair(ub[i], ub[i], raw_sel(0, 1)), raw_pair(ua[i], ua[i], raw_sel(2, 3)), raw_pair(ub[i], ub[i], raw_sel(2, 3))};
+#pragma unroll
+              for (int n = 0; n < NR; n++) mma16816(i % 2 ? s2[n] : s[kk][n], a0, qf[n][4 * x + i][0], qf[n][4 * x + i][1]);
             }
           } else {
             const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
@@ -371,7 +342,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
 #pragma unroll
         for (int n = 0; n < NR; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[kk][n][e] += E4M3 ? s2[n][e] * 0.0625f : s2[n][e];
+          for (int e = 0; e < 4; e++) s[kk][n][e] += s2[n][e];
       }
       float mx[NR][2];
 #pragma unroll

@@ -145,6 +145,28 @@ def held_cache(sv, codes, exponents):  # noqa: F811
     return sv.KVCache(*pools, *((e + 127).to(torch.uint8).view(1, 1, n).to(DEV) for e in exponents))
 
 
+@pytest.mark.parametrize("rows", [1, 3, 5, 8, 16, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_of_a_wide_range_over_8_bit_keys(sv, dim, rows):  # noqa: F811
+    """Scores come from elements far below a row's largest, whose keys are zero: 2^30 below, 2^100 below, and spread over all of it"""
+    gen = torch.Generator().manual_seed(dim + rows)
+    n = 70
+    for low, high, e in ((-6, 24, 7), (-6, 100, 7), (-100, -70, 7), (-6, None, 0)):
+        k = torch.randn(n, dim, generator=gen)
+        big = torch.arange(dim) % 16 == 5
+        if high is not None:
+            k[:, big] = 0
+        cache = held_cache(sv, [k, torch.randn(n, dim, generator=gen)], [torch.full((n,), float(e)), torch.zeros(n)])
+        q = torch.randn(rows, 2, dim, generator=gen) * 2.0 ** low
+        if high is None:
+            q = q * torch.exp2(torch.randint(-18, 9, (rows, 2, dim), generator=gen).float())
+        else:
+            q[..., big] = 2.0 ** high * (1 + torch.rand(rows, 2, int(big.sum()), generator=gen))
+        q = q.bfloat16().to(DEV)
+        batch = sv.KVBatch(i32([0, rows]), i32([n]), i32([[0]]), max_new=rows)
+        check_attention(sv, cache, batch, q, scale=0.125 if low > -20 else 2.0 ** 90)
+
+
 def large_scores(sv, rows, exponent):  # noqa: F811
     """Queries of 2^120 to 2^127 over 8-bit keys of this scale: the row's result is the value of the key whose score is largest by far, its lse that score"""
     gen = torch.Generator().manual_seed(rows)
@@ -173,3 +195,11 @@ def test_large_queries_over_keys_of_the_smallest_scales(sv, rows):  # noqa: F811
 def test_scores_beyond_the_range_of_an_exponential(sv, rows, exponent):  # noqa: F811
     """of 2^26 to 2^113"""
     large_scores(sv, rows, exponent)
+
+
+def test_infinite_queries_over_8_bit_keys(sv):  # noqa: F811
+    """give what they give over others: no value, and the logarithm of a sum of zeros"""
+    for form in FORMS:
+        cache, batch, q, n, kv = infinite_query("e4m3", form, sv)
+        out, lse = sv.paged_attention(cache, batch, q, with_lse=True)
+        assert torch.isnan(out[0, 0]).all() and float(lse[0, 0]) == -math.inf and torch.isfinite(out[0, 1]).all()
