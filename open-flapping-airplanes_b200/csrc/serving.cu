@@ -61,7 +61,7 @@ int check_cache(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, paged:
   }
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || (c->page_stride * es) % 16 || (c->head_stride * es) % 16 || (c->row_stride * es) % 16)
     return fail(OFA_BAD_ARGUMENT, "cached rows start on 16-byte boundaries: pointers and strides");
-  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->scale_page_stride < 0 || c->scale_head_stride < 0 || c->scale_row_stride < 0)
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->scale_page_stride < 0 || c->scale_head_stride < 0 || c->scale_row_stride < 0 || b->pages_stride < 0)
     return fail(OFA_BAD_ARGUMENT, "negative stride");
   if (!aligned(b->q_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->pages, 4) || !aligned(b->status, 4)) return fail(OFA_BAD_ARGUMENT, "misaligned index array");
   B.q_start = b->q_start; B.kv_len = b->kv_len; B.pages = b->pages; B.pages_stride = b->pages_stride;
