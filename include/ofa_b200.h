@@ -246,7 +246,7 @@ typedef struct {
  * them: row t of its n rows is position kv_len[i] - n + t, and position p is row p % page_size of page pages[i][p / page_size]. Sequences may bring no rows;
  * rows that none brings (behind the last, padding) are neither read nor written. The arrays are read on the device, so a replayed graph sees their current values.
  * What is wrong there cannot be refused on the host; it never becomes an access out of range, and sets bits of *status (or-ed; may be NULL):
- * 1 a page number outside the cache, 2 a length below 0 or beyond the page table (in attention, above 2^31 - 1024 too), 4 q_start not rising or beyond n_rows (that sequence is left out), 8 a wait inside a kernel
+ * 1 a page number outside the cache, 2 a length below 0 or beyond the page table (in attention, above 2^31 - 1024 too; in ofa_kv_append, below the number of rows that the sequence brings, unless it is 0: a place in a batch that is not in use), 4 q_start not rising or beyond n_rows (that sequence is left out), 8 a wait inside a kernel
  * ran out (some seconds; the call's output is not valid). */
 enum { OFA_KV_BAD_PAGE = 1, OFA_KV_BAD_LENGTH = 2, OFA_KV_BAD_ROWS = 4, OFA_KV_TIMEOUT = 8 };
 typedef struct {

@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(256, 8) move_kernel(const __grid_constant__ Mo
     const Chunk ch = chunk_of(P.b, i);
     const int pos = ch.p0 + (r0 + tid - ch.s);
     int page, at;
+    if (!READ && pos < 0 && ch.len > 0) flag(P.b.status, ST_LENGTH);           // a row is lost, unless the sequence is a place in a batch that nobody uses; one that is read is zeros
     if (pos < 0 || !locate(P.b, i, pos, page, at)) page = -1, at = 0;
     place[tid] = make_int2(page, at);
   }

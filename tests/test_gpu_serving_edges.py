@@ -203,3 +203,17 @@ def test_infinite_queries_over_8_bit_keys(sv):  # noqa: F811
         cache, batch, q, n, kv = infinite_query("e4m3", form, sv)
         out, lse = sv.paged_attention(cache, batch, q, with_lse=True)
         assert torch.isnan(out[0, 0]).all() and float(lse[0, 0]) == -math.inf and torch.isfinite(out[0, 1]).all()
+
+
+def test_rows_that_a_sequence_is_too_short_for(sv):  # noqa: F811
+    """are not kept, and that is said; sequences of length 0 are places that a padded batch does not use"""
+    cache, batch, gen = make(sv, [6, 2], [4, 2], 1, 64, 8)
+    k = torch.randn(8, 1, 64, generator=gen).bfloat16().to(DEV)
+    before, idle = cache.k.clone(), sv.KVBatch(batch.q_start, i32([0, 0]), batch.pages, status=i32([0]))
+    sv.kv_append(cache, idle, k, k)
+    assert int(idle.status) == 0 and torch.equal(cache.k, before)
+    sv.kv_append(cache, batch, k, k)
+    assert int(batch.status) == sv.BAD_LENGTH
+    batch.status.zero_()
+    back, _ = sv.kv_read(cache, batch, 8)
+    assert int(batch.status) == 0 and (back[:2] == 0).all() and torch.equal(back[2:], k[2:])
