@@ -22,6 +22,7 @@ from .tasks import OfaError
 
 E4M3 = torch.float8_e4m3fn
 _TYPES = {"bf16": torch.bfloat16, "e4m3": E4M3}
+_INT_MAX = 2 ** 31 - 1                                        # ctypes cuts what is larger to 32 bits without a word
 BAD_PAGE, BAD_LENGTH, BAD_ROWS, TIMEOUT = 1, 2, 4, 8          # bits of a batch's status word
 
 
@@ -38,6 +39,8 @@ def _want(name, t, dtype, shape, device, inner=True):
     s = t.shape
     if len(s) != len(shape) or any(w is not None and w != n for w, n in zip(shape, s)):
         _refuse(f"{name} has shape {tuple(s)}, not {tuple('any' if w is None else w for w in shape)}")
+    if max(s, default=0) > _INT_MAX:
+        _refuse(f"{name} has shape {tuple(s)}: at most 2^31 - 1 along an axis")
     if device is not None and t.device != device:
         _refuse(f"{name} is on {t.device}, not on {device}")
     if inner and len(s) and s[-1] > 1 and t.stride(-1) != 1:
@@ -102,7 +105,7 @@ def _done(rc):
 def _rows(name, t, shape, cache):
     """The strides of bf16 rows [n_rows, heads, head_dim] on the cache's device; what is wrong with them otherwise."""
     try:
-        if t.dtype is _BF16 and t.get_device() == cache.index and (shape is None or t.shape == shape):
+        if t.dtype is _BF16 and t.get_device() == cache.index and (shape is None or t.shape == shape) and t.shape[0] <= _INT_MAX:
             s = t.stride()
             if len(s) == 3 and s[2] == 1 and t.shape[2] == cache.head_dim:
                 return s
@@ -128,7 +131,7 @@ def _table(name, t, dtype, shape, index, device):
     try:
         if t.dtype is dtype and t.get_device() == index:
             s = t.stride()
-            if len(s) == 2 and s[1] == 1 and t.shape[0] == shape[0] and (shape[1] is None or t.shape[1] == shape[1]):
+            if len(s) == 2 and s[1] == 1 and t.shape[0] == shape[0] and (shape[1] is None or t.shape[1] == shape[1]) and max(t.shape) <= _INT_MAX:
                 return t.data_ptr(), s[0]
     except AttributeError:
         pass
@@ -198,7 +201,7 @@ class KVBatch:
         c = self.c = capi.KvBatch()
         c.n_seqs, c.max_pages, c.pages_stride = n, pages.shape[1], pages.stride(0)
         c.q_start, c.kv_len, c.pages = q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr()
-        c.max_new, c.max_kv = min(max_new, 2 ** 31 - 1), min(max_kv, 2 ** 31 - 1)
+        c.max_new, c.max_kv = min(max_new, _INT_MAX), min(max_kv, _INT_MAX)
         c.status = status.data_ptr() if status is not None else None
         self.ref, self.address = C.byref(c), C.addressof(c)
 
@@ -250,6 +253,7 @@ def paged_attention(cache, batch, q, out=None, scale=None, causal=True, window=0
         got = f.attend(cache.address, batch.address, cache.index, q, out, scale, causal, window, with_lse)
         if got is not None:
             return _done(got) if type(got) is int else got
+    window = max(-1, min(window, _INT_MAX))                      # as wide as that: wider than any context
     sq = _rows("q", q, None, cache)
     n_rows, n_heads, _ = q.shape
     if out is None:

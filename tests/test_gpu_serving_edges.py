@@ -205,6 +205,23 @@ def test_infinite_queries_over_8_bit_keys(sv):  # noqa: F811
         assert torch.isnan(out[0, 0]).all() and float(lse[0, 0]) == -math.inf and torch.isfinite(out[0, 1]).all()
 
 
+def test_windows_and_sizes_beyond_32_bits(sv, ofa, monkeypatch):  # noqa: F811
+    cache, batch, gen = make(sv, [4], [60], 1, 64, 16)
+    q = queries(gen, 4, 2, 64)
+    want = sv.paged_attention(cache, batch, q)
+    for fast in (True, False):
+        if not fast:
+            monkeypatch.setattr(sv, "_fast_module", None)
+        for window in (2 ** 31, 2 ** 32 + 5, 2 ** 40):
+            assert torch.equal(sv.paged_attention(cache, batch, q, window=window), want)
+        many = 2 ** 32 + 4
+        k, x = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV).expand(many, -1, -1), torch.zeros(1, 8, device=DEV).expand(many, -1)
+        for bad in (lambda: sv.paged_attention(cache, batch, q, window=-2 ** 40), lambda: sv.kv_append(cache, batch, k, k), lambda: sv.kv_read(cache, batch, k=k, v=k),
+                    lambda: sv.logits_process(x, out=x), lambda: sv.KVCache(k[None], k[None]), lambda: sv.KVBatch(i32([0] * 3), i32([1, 1]), i32([[0]]).expand(many, 1))):
+            with pytest.raises(ofa.OfaError):
+                bad()
+
+
 def test_rows_that_a_sequence_is_too_short_for(sv):  # noqa: F811
     """are not kept, and that is said; sequences of length 0 are places that a padded batch does not use"""
     cache, batch, gen = make(sv, [6, 2], [4, 2], 1, 64, 8)
