@@ -14,7 +14,9 @@
 //     another token, while the last blocks of the stream still run. For calls that fill the machine, whose stream is then free of counters: 192 rows of 100,352 bf16 up to 2,000
 //     tokens each take 30 us the first way, 21.5 this way, the stream alone 15. What is left are the named logits' sectors, which go to memory twice. (Looking at a token's word for
 //     every logit, with the arithmetic of a hit inlined 32 times, took 47.)
-// A bias marks its token's word; the entries of its list are added in their order. Stretches begin where a row's 16-byte vectors do, so a row that starts between two boundaries
+// A bias marks its token's word; the entries of its list are added in their order: by process_kernel in shared memory, in one pass over the list; in touch_kernel by each thread with one of them,
+// who looks through the list. That is quadratic, so lists of more than 128 take the first way whatever the call's size (192 rows of 100,352 bf16 with 96 biases 22.5 us, the first way 27.8; with
+// 160 35.4 and 32.4; with 5,000 8,680 and 260). Stretches begin where a row's 16-byte vectors do, so a row that starts between two boundaries
 // loses only its first and last vector to single elements.
 #pragma once
 #include "paged.cuh"
@@ -34,7 +36,8 @@ struct Args {
   const unsigned* mask; long long mask_row;
   int slots_log2;                                              // touch_kernel: of its table
 };
-constexpr int LISTED = 1024;
+constexpr int LISTED = 1024, SHORT_LIST = 128;
+enum { STREAM, WORDS, SUMS };                                   // process_kernel: the stream alone; the history's logits too; and the biases'
 constexpr unsigned PROMPT = 1u << 31, BIASED = 1u << 30;      // a token's word: in the prompt, has a bias; the rest counts where it stands behind the prompt
 
 // A named token's logit with its word c and the sum of its biases
@@ -56,7 +59,7 @@ __device__ __forceinline__ float touched(const Row& R, float f, unsigned c, floa
   return c & BIASED ? f + bias : f;
 }
 
-template <class T, int VECS, bool WIDE, bool WORDS>
+template <class T, int VECS, bool WIDE, int MODE>
 __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Args P) {
   constexpr int VN = Vec<T>::N, S = 256 * VN * VECS;           // tokens of a block
   after_the_kernel_before();
@@ -66,8 +69,9 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
   const T* in = reinterpret_cast<const T*>(P.in) + (long long)row * P.in_row;
   T* out = reinterpret_cast<T*>(P.out) + (long long)row * P.out_row;
   const int v0 = (int)blockIdx.x * S - (WIDE ? (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T)) : 0);
-  const bool words = WORDS && (P.tokens || P.bias_ids);
-  if (!WORDS) cudaTriggerProgrammaticLaunchCompletion();       // touch_kernel may begin to count
+  const bool words = MODE == SUMS || (MODE == WORDS && P.tokens);
+  float* sums = reinterpret_cast<float*>(count + S);           // SUMS: by token of the stretch
+  if (MODE == STREAM) cudaTriggerProgrammaticLaunchCompletion();       // touch_kernel may begin to count
   uint4 x[VECS];
 #pragma unroll
   for (int k = 0; k < VECS; k++) {
@@ -86,7 +90,7 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
   auto put = [&](int t) { const int at = atomicAdd(&listed, 1); if (at < LISTED) list[at] = t; };
   if (words) {
 #pragma unroll
-    for (int i = 0; i < S / 1024; i++) reinterpret_cast<uint4*>(count)[i * 256 + tid] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < S / 1024 * (MODE == SUMS ? 2 : 1); i++) reinterpret_cast<uint4*>(count)[i * 256 + tid] = make_uint4(0, 0, 0, 0);
     if (tid == 0) listed = 0;
     __syncthreads();
     if (P.tokens) {
@@ -104,8 +108,31 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
         }
       }
     }
-    if (P.bias_ids)
-      for (int i = tid; i < P.max_bias; i += 256) { const int t = __ldg(ids + i); unsigned* w = word(t); if (w && atomicOr(w, BIASED) == 0) put(t); }
+    if constexpr (MODE == SUMS) {
+      // A warp sums the tokens of every eighth place, so that a token's entries are added by one warp, in the order of the list: 32 entries at once, the same token's in turns
+      const int lane = tid & 31, warp = tid >> 5;
+      const float* val = P.bias + (long long)row * P.bias_row;
+#pragma unroll 1
+      for (int base = lane; base - lane < P.max_bias; base += 128) {
+        int t[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) t[u] = base + u * 32 < P.max_bias ? __ldg(ids + base + u * 32) : -1;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          unsigned* w = word(t[u]);
+          const int at = w ? (int)(w - count) : -1;
+          const bool mine = w && (at & 7) == warp;
+          if (!__any_sync(0xffffffffu, mine)) continue;
+          const float v = mine ? __ldg(val + base + u * 32) : 0.f;
+          const int turn = __popc(__match_any_sync(0xffffffffu, mine ? at : -1) & ((1u << lane) - 1)), turns = (int)__reduce_max_sync(0xffffffffu, mine ? turn : 0);
+          if (mine && turn == 0 && atomicOr(w, BIASED) == 0) put(t[u]);
+          for (int i = 0; i <= turns; i++) {
+            if (mine && turn == i) sums[at] += v;
+            __syncwarp();
+          }
+        }
+      }
+    }
   }
 #pragma unroll
   for (int k = 0; k < VECS; k++) {
@@ -133,12 +160,12 @@ __global__ void __launch_bounds__(256) process_kernel(const __grid_constant__ Ar
   const Row R = row_of(P, row);
   const bool all = listed <= LISTED;
 #pragma unroll 1
-  for (int i = tid; i < (all ? listed : n + P.max_bias); i += 256) {           // max_bias is 0 without biases
+  for (int i = tid; i < (all ? listed : n + (MODE == SUMS ? P.max_bias : 0)); i += 256) {
     const int t = all ? list[i] : i < n ? __ldg(text + i) : __ldg(ids + i - n);
     unsigned* w = word(t);
     const unsigned c = w ? atomicExch(w, 0u) : 0u;
     if (!c || (mask && !(__ldg(mask + (t >> 5)) >> (t & 31) & 1))) continue;
-    out[t] = from_f<T>(touched(R, to_f(out[t]), c, c & BIASED ? bias_of(P, R, t) : 0.f));
+    out[t] = from_f<T>(touched(R, to_f(out[t]), c, MODE == SUMS && (c & BIASED) ? sums[w - count] : 0.f));
   }
 }
 

@@ -78,13 +78,15 @@ int check_rows(const char* name, const void* p, Axis row, Axis head, int dim, bo
   return OFA_OK;
 }
 
-// The limit of dynamic shared memory, raised once for each kernel and device to all an SM has
+// The limit of dynamic shared memory, raised once for each kernel and device to all a block may have beside the kernel's own
 template <auto KERNEL> cudaError_t allow() {
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  cudaFuncAttributes own;
+  e = cudaFuncGetAttributes(&own, KERNEL);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)own.sharedSizeBytes);
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }
@@ -207,19 +209,21 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   return e;
 }
 
-// Where four vectors a thread still give every SM several blocks: the stream, and a block for each row's named tokens if they fit its table; else one kernel, with one
-// vector a thread for few rows, since each block reads its row's whole history.
+// Where four vectors a thread still give every SM several blocks: the stream, and a block for each row's named tokens if they fit its table and the list of biases is short; else one kernel,
+// with one vector a thread for few rows, since each block reads its row's whole history.
 template <class T, bool WIDE> cudaError_t process(logits::Args& P, int rows, cudaStream_t s) {
   const int vn = Vec<T>::N, span = P.vocab + (WIDE ? vn - 1 : 0);
   const bool large = (long long)rows * ((span + 1024 * vn - 1) / (1024 * vn)) >= 4 * 148, words = P.tokens || P.bias_ids;
   const int stretch = (large ? 1024 : 256) * vn;
   const dim3 grid((unsigned)((span + stretch - 1) / stretch), (unsigned)rows);
   const long long named = (P.tokens ? P.max_tokens : 0) + (long long)P.max_bias;
-  if (!large || (words && named > 8192)) {
+  if (P.bias_ids && (!large || named > 8192 || P.max_bias > logits::SHORT_LIST))
+    return large ? launch<logits::process_kernel<T, 4, WIDE, logits::SUMS>>(grid, 256, stretch * 8, s, P) : launch<logits::process_kernel<T, 1, WIDE, logits::SUMS>>(grid, 256, stretch * 8, s, P);
+  if (!large || named > 8192) {
     const int smem = words ? stretch * 4 : 0;
-    return large ? launch<logits::process_kernel<T, 4, WIDE, true>>(grid, 256, smem, s, P) : launch<logits::process_kernel<T, 1, WIDE, true>>(grid, 256, smem, s, P);
+    return large ? launch<logits::process_kernel<T, 4, WIDE, logits::WORDS>>(grid, 256, smem, s, P) : launch<logits::process_kernel<T, 1, WIDE, logits::WORDS>>(grid, 256, smem, s, P);
   }
-  const cudaError_t e = launch<logits::process_kernel<T, 4, WIDE, false>>(grid, 256, 0, s, P);
+  const cudaError_t e = launch<logits::process_kernel<T, 4, WIDE, logits::STREAM>>(grid, 256, 0, s, P);
   if (e != cudaSuccess || !words) return e;
   for (P.slots_log2 = 9; P.slots_log2 < 14 && 1ll << P.slots_log2 < 4 * named;) P.slots_log2++;
   return launch<logits::touch_kernel<T>>(dim3((unsigned)rows), 512, 12 << P.slots_log2, s, P);

@@ -205,6 +205,35 @@ def test_infinite_queries_over_8_bit_keys(sv):  # noqa: F811
         assert torch.isnan(out[0, 0]).all() and float(lse[0, 0]) == -math.inf and torch.isfinite(out[0, 1]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,history,biases", [(2, 1000, 30, 129), (1, 5000, 0, 5000), (3, 9000, 100, 3001), (700, 1000, 20, 600), (400, 3001, 9000, 700), (2, 50, 5, 4096), (150, 33001, 500, 2000)])
+def test_long_lists_of_biases(sv, rows, vocab, history, biases, dtype):  # noqa: F811
+    """as long as the vocabulary and longer, the same id many times: sums in the order of the list, whatever the call's size"""
+    gen = torch.Generator().manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, generator=gen) * 4).to(dtype).to(DEV)
+    a = {"bias_ids": torch.randint(-2, vocab + 2, (rows, biases), generator=gen).int(), "bias": torch.randn(rows, biases, generator=gen) * 5,
+         "mask": torch.randint(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32), generator=gen).int()}
+    a["bias_ids"][:, biases // 2:] %= max(1, vocab // 3)
+    if history:
+        a["tokens"] = torch.randint(0, vocab, (rows, history), generator=gen).int()
+        a["repetition"], a["frequency"] = 1 + torch.rand(rows, generator=gen), torch.rand(rows, generator=gen)
+    dev = {k: v.to(DEV) for k, v in a.items()}
+    got = sv.logits_process(x, **dev)
+    some = sorted({0, rows // 2, rows - 1})
+    want, tol = ref.logits(x[some], **{k: v[some] for k, v in a.items()})
+    tol = tol + (ref.F32_HALF if dtype == torch.float32 else ref.BF16_HALF) * (want.abs() + tol)
+    fine, have = torch.isfinite(want), got[some].double().cpu()
+    assert torch.equal(have[~fine], want[~fine]) and ((have - want).abs()[fine] <= tol[fine]).all()
+    for r in some:
+        part = slice(r, r + 1)
+        assert torch.equal(got[part], sv.logits_process(x[part], **{k: v[part] for k, v in dev.items()}))
+    assert sv.logits_process(x, out=x, **dev) is x and torch.equal(x, got)
+    # one more entry than a short list may have, the last without weight: the same sums
+    short = {"bias_ids": dev["bias_ids"][:, :128].contiguous(), "bias": dev["bias"][:, :128].contiguous()}
+    longer = {"bias_ids": torch.cat([short["bias_ids"], torch.full((rows, 1), -1, dtype=torch.int32, device=DEV)], 1), "bias": torch.cat([short["bias"], torch.ones(rows, 1, device=DEV)], 1)}
+    assert torch.equal(sv.logits_process(got, **short), sv.logits_process(got, **longer))
+
+
 def test_windows_and_sizes_beyond_32_bits(sv, ofa, monkeypatch):  # noqa: F811
     cache, batch, gen = make(sv, [4], [60], 1, 64, 16)
     q = queries(gen, 4, 2, 64)
