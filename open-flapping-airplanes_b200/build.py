@@ -93,9 +93,3 @@ def build_host(force=False):
     if r.returncode != 0:
         raise RuntimeError("building " + HOST + " failed:\n" + r.stdout + r.stderr)
     return HOST
-    if not cxx or not os.path.exists(os.path.join(inc, "Python.h")):
-        return None
-    r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + inc, "-o", HOST, HOST_SRC], capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("building " + HOST + " failed:\n" + r.stdout + r.stderr)
-    return HOST
