@@ -17,7 +17,11 @@ HEADERS = ["common.cuh", "task_api.h", "tickets.h", "elementwise.cuh", "gemm_tc.
 
 
 HOST_SRC = os.path.join(CSRC, "serving_py.cpp")  # the torch view's calls of the serving operators, a CPython extension
-HOST = os.path.join(HERE, "_serving" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def host_path(torch_version):
+    """Where the extension for this torch lies. It looks at tensors in place, so one that was built for another torch is another file, and is not taken."""
+    return os.path.join(HERE, f"_serving-torch{torch_version}" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
 def nvcc_path():
@@ -76,20 +80,21 @@ def build_host(force=False):
     hdr = os.path.join(CSRC, "..", "..", "include", "ofa_b200.h")
     inc = sysconfig.get_paths()["include"]
     cxx = shutil.which("g++") or shutil.which("c++")
-    if not force and os.path.exists(HOST) and os.path.getmtime(HOST) >= max(os.path.getmtime(HOST_SRC), os.path.getmtime(hdr)):
-        return HOST
     try:
         import torch
         root = os.path.dirname(torch.__file__)
     except ImportError:
         return None
+    host = host_path(torch.__version__)
+    if not force and os.path.exists(host) and os.path.getmtime(host) >= max(os.path.getmtime(HOST_SRC), os.path.getmtime(hdr)):
+        return host
     cuda = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
     dirs = [inc, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
     needed = (os.path.join(inc, "Python.h"), os.path.join(root, "include", "ATen", "Functions.h"), os.path.join(cuda, "include", "cuda_runtime_api.h"))
     if not cxx or not all(os.path.exists(f) for f in needed):
         return None
-    r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *["-I" + d for d in dirs], "-o", HOST, HOST_SRC,
+    r = subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *["-I" + d for d in dirs], "-o", host, HOST_SRC,
                         "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"], capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("building " + HOST + " failed:\n" + r.stdout + r.stderr)
-    return HOST
+        raise RuntimeError("building " + host + " failed:\n" + r.stdout + r.stderr)
+    return host

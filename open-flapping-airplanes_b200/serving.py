@@ -13,11 +13,13 @@ OfaError. No call waits for the device or reads from it, and results carry no gr
 is replayed.
 """
 import ctypes as C
+import importlib.util
 import math
 
 import torch
 
 from . import capi
+from .build import host_path
 from .tasks import OfaError
 
 E4M3 = torch.float8_e4m3fn
@@ -75,10 +77,12 @@ def _lib():
 
 
 def _bind():
-    """The extension that build.build_host() compiles, bound to the loaded library; None where there is none. Its functions return results, the code of an entry point that
+    """The extension that build.build_host() compiled for this torch, bound to the loaded library; None where there is none. Its functions return results, the code of an entry point that
     refused, or None for arguments that are not plainly right: the code below then finds out what is wrong with them."""
+    spec = importlib.util.spec_from_file_location("_serving", host_path(torch.__version__))
     try:
-        from . import _serving
+        _serving = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_serving)
     except ImportError:
         return None
     lib = _lib()
