@@ -87,8 +87,8 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint3
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// Shared memory of the cluster's other blocks
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Shared memory of the cluster's other blocks. The barrier's instructions are for whole warps: their lanes come together first, from code that some of them had to themselves.
+__device__ __forceinline__ void cluster_sync() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
 __device__ __forceinline__ float peer_f32(uint32_t a) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory"); return v; }
 __device__ __forceinline__ float4 peer_f32x4(uint32_t a) {
@@ -425,6 +425,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
                   for (int h = 0; h < 2; h++) if (!(P.causal && p > pos[n][h]) && p >= first_seen(P, pos[n][h])) o[n][t][2 * e + h] += x;
               }
           }
+          __syncwarp();                                          // the products below are whole warps' too
         }
       }
 #pragma unroll

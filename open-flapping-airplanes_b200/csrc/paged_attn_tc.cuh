@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
                 if (!isfinite(v)) o[x] = __float_as_uint(__uint_as_float(o[x]) + v);
               }
             }
+            __syncwarp();                                        // tensor memory is read by whole warps
           }
           if (P.nsplit == 1) {                                   // through the tile of Q, which is not needed any more, so that rows leave whole
 #pragma unroll
