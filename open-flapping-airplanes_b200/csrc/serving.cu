@@ -196,7 +196,7 @@ template <int D, bool E4M3> cudaError_t attend(paged::AttnArgs& P, const Plan& p
   if (p.many) {
     const dim3 grid(blocks * (unsigned)P.n_kv_heads);           // heads among the tiles, for the order in which blocks start
     P.flip = P.scale_log2 < 0.f;
-    P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1e-30f);           // -inf times it has to stay -inf
+    P.scale_log2 = fmaxf(fabsf(P.scale_log2), 1.17549435e-38f);      // the smallest normal number instead of 0: -inf times it has to stay -inf
     if constexpr (!E4M3 || D == 128) if (p.pair == 1) e = launch<paged::many_rows_kernel<D, E4M3, 1>>(grid, paged::Tc<D, E4M3, 1>::THREADS, paged::Tc<D, E4M3, 1>::SMEM, s, P);
     if constexpr (E4M3 || D == 128) if (p.pair == 2) e = launch<paged::many_rows_kernel<D, E4M3, 2>>(grid, paged::Tc<D, E4M3, 2>::THREADS, paged::Tc<D, E4M3, 2>::SMEM, s, P);
   } else {

@@ -263,3 +263,16 @@ def test_rows_that_a_sequence_is_too_short_for(sv):  # noqa: F811
     batch.status.zero_()
     back, _ = sv.kv_read(cache, batch, 8)
     assert int(batch.status) == 0 and (back[:2] == 0).all() and torch.equal(back[2:], k[2:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 8, 40, 150])
+def test_the_smallest_scales(sv, rows, dtype):  # noqa: F811
+    """scores of order one from large queries and a scale below 1e-30"""
+    cache, batch, gen = make(sv, [rows], [170], 1, 64, 16, dtype, max_new=rows)
+    q = (torch.randn(rows, 2, 64, generator=gen) * 2.0 ** 112).bfloat16().to(DEV)
+    for scale in (2.0 ** -115, -2.0 ** -115):
+        check_attention(sv, cache, batch, q, scale=scale)
+    out = sv.paged_attention(cache, batch, q, causal=False, scale=0.0)
+    want = sv.kv_read(cache, sv.KVBatch(i32([0, 170]), i32([170]), batch.pages), 170)[1].double()[:, 0]
+    assert ((out.double() - want.mean(0)).abs() <= (want.abs().mean(0) + want.mean(0).abs()) * ref.BF16_HALF * 1.01).all()
