@@ -64,7 +64,7 @@ struct TcCtrl {
 };
 static_assert(sizeof(TcCtrl) <= 640, "control area");
 
-constexpr float BIG = 268435456.f;                              // 2^28
+constexpr float BIG = 1073741824.f;                             // 2^30
 
 __device__ __forceinline__ bool elect_one() {                  // one thread of a converged warp
   uint32_t e;
@@ -183,8 +183,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
       }
       attn_tc::warp_arrive(smem_u32(&ct.q_full));
       const uint32_t tl = tmem + ((uint32_t)(e * 32) << 16), ts = tl + tile * 128, to = tl + F::O_AT + tile * D;
-      float m = -INFINITY, l = 0.f;
-      bool big = false;
+      float m = -INFINITY, l = 0.f, sc = P.scale_log2;
       const int n = k.b[tile] - k.a[tile];
       for (int c = 0; c < n; c++) {
         const int j = k.a[tile] + c, k0 = j * 128;
@@ -224,14 +223,20 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
         for (int x = 0; x < 32; x += 2)
 #pragma unroll
           for (int q = 0; q < 4; q++) mx[q] = attn_tc::max3(mx[q], __uint_as_float(s[q][x]), __uint_as_float(s[q][x + 1]));
-        const float m_true = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2);
-        if (c == 0) { m = m_true; big = __any_sync(0xffffffffu, fabsf(m) > BIG && m != -INFINITY); }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m_true = fmaxf(m, top * sc);
+        // The multiply-add below forms products exactly, the reference is a rounded one: the largest score's exponent is up to half a step of the reference off 0, which from 2^31 on is more
+        // than sums have room for. Beyond 2^30, where two scores that are not alike lie 2^6 or more apart, the factor is its power of two instead, whose products are exact.
+        auto factor = [&](float x) { return fabsf(x * P.scale_log2) > BIG && x != -INFINITY ? __uint_as_float(__float_as_uint(P.scale_log2) & 0xff800000u) : P.scale_log2; };
+        if (c == 0) { sc = factor(top); m = top * sc; }
         else {
           const bool grow = m_true > m + RESCALE_LOG2;
           if (__any_sync(0xffffffffu, grow)) {
-            const float alpha = grow ? ex2_approx(m - m_true) : 1.f;
-            if (grow) { m = m_true; l *= alpha; }
-            big = __any_sync(0xffffffffu, fabsf(m) > BIG && m != -INFINITY);
+            float alpha = grow ? ex2_approx(m - m_true) : 1.f;
+            if (grow) {
+              const float f = factor(top);
+              if (f != sc) alpha = 0.f;                          // the old reference is 2^5 or more below the new one
+              sc = f; m = top * sc; l *= alpha;
+            }
 #pragma unroll 1
             for (int q = 0; q < D / 16; q++) {
               uint32_t o[16];
@@ -243,16 +248,6 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;              // no key seen yet: 2^(-inf - 0) = 0
-        // A multiply-add forms the product exactly, the reference is a rounded one: the largest score's exponent is half a step of the reference off 0, which beyond 2^28 may be
-        // more than sums have room for. There the scores are rounded first.
-        float sc = P.scale_log2;
-        if (big) [[unlikely]] {
-#pragma unroll
-          for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int x = 0; x < 32; x++) s[q][x] = __float_as_uint(__uint_as_float(s[q][x]) * sc);
-          sc = 1.f;
-        }
         const u64 sc2 = attn_tc::f2(sc, sc), nm2 = attn_tc::f2(-ref, -ref);
         u64 sum[2] = {0, 0};
 #pragma unroll
@@ -283,6 +278,7 @@ __global__ void __launch_bounds__(Tc<D, E4M3, NT>::THREADS, Tc<D, E4M3, NT>::BLO
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
+      if (sc != P.scale_log2) m = m / sc * P.scale_log2;
       if (ok && !idle) {                                         // the row's result, or its part for combine_kernel
         const int olo = *reinterpret_cast<volatile int*>(&ct.odd_lo), ohi = *reinterpret_cast<volatile int*>(&ct.odd_hi);
         const long long g = (long long)(ch.s + t) * P.n_heads + head;

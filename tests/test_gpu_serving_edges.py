@@ -276,3 +276,30 @@ def test_the_smallest_scales(sv, rows, dtype):  # noqa: F811
     out = sv.paged_attention(cache, batch, q, causal=False, scale=0.0)
     want = sv.kv_read(cache, sv.KVBatch(i32([0, 170]), i32([170]), batch.pages), 170)[1].double()[:, 0]
     assert ((out.double() - want.mean(0)).abs() <= (want.abs().mean(0) + want.mean(0).abs()) * ref.BF16_HALF * 1.01).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("order", ["rising", "falling", "any"])
+@pytest.mark.parametrize("hints", [{}, {"max_kv": 6000}])
+def test_scores_of_every_size_over_many_steps(sv, hints, order, dtype):  # noqa: F811
+    """One dim alone counts, so that scores are exact: rows of 2^-4 to 2^100, of either sign, over keys that rise, fall and repeat; with a scale that is no power of two"""
+    gen = torch.Generator().manual_seed(7)
+    n, rows, dim = 6000, 150, 64
+    k = torch.zeros(n, dim)
+    x = torch.randn(n, generator=gen).to(torch.float8_e4m3fn).float() if dtype == "e4m3" else torch.randn(n, generator=gen).bfloat16().float()
+    k[:, 3] = x if order == "any" else x.sort(descending=order == "falling").values
+    v = torch.randn(n, dim, generator=gen)
+    cache = held_cache(sv, [k, v], [torch.zeros(n)] * 2) if dtype == "e4m3" else sv.KVCache(k.bfloat16().view(1, 1, n, dim).to(DEV), v.bfloat16().view(1, 1, n, dim).to(DEV))
+    q = torch.zeros(rows, 1, dim)
+    q[:, 0, 3] = torch.exp2(torch.arange(rows) * 104 / (rows - 1) - 4) * (1 - 2 * (torch.arange(rows) % 2))
+    q = q.bfloat16().to(DEV)
+    batch = sv.KVBatch(i32([0, rows]), i32([n]), i32([[0]]), max_new=rows, **hints)
+    for scale in (0.17, -0.17):
+        out, lse = sv.paged_attention(cache, batch, q, causal=False, scale=scale, with_lse=True)
+        s = q[:, 0, 3].double().cpu()[:, None] * k[:, 3].double() * C.c_float(scale).value
+        want, p = torch.logsumexp(s, 1), torch.softmax(s, 1)
+        held = cache.v[0, 0].double().cpu()
+        # a score's exponent: the scale times log2 e and the product rounded (2^-23 of it), which moves a probability by as much of its distance from the largest
+        off = (p * (s.max(1, keepdim=True).values - s)).sum(1)[:, None] * 2.0 ** -22 + 2.0 ** -18
+        assert ((out[:, 0].double().cpu() - p @ held).abs() <= (p @ held.abs()) * (ref.BF16_HALF + 2 * off) + (p @ held).abs() * ref.BF16_HALF * 1.01 + 1e-37).all()
+        assert ((lse[:, 0].double().cpu() - want).abs() <= want.abs() * 2.0 ** -21 + 2.0 ** -18).all()
