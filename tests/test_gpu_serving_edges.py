@@ -191,7 +191,7 @@ def test_large_queries_over_keys_of_the_smallest_scales(sv, rows):  # noqa: F811
 
 
 @pytest.mark.parametrize("exponent", [-100, -60, -20])
-@pytest.mark.parametrize("rows", [40, 150])
+@pytest.mark.parametrize("rows", [1, 16, 40, 150])
 def test_scores_beyond_the_range_of_an_exponential(sv, rows, exponent):  # noqa: F811
     """of 2^26 to 2^113"""
     large_scores(sv, rows, exponent)
