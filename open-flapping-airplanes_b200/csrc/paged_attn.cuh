@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
         kf = __uint_as_float(k8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)min(max(k8, 1), E_MAX + 127) << 23);
         vf = __uint_as_float(v8 == SCALE_NAN ? 0x7fc00000u : (uint32_t)(min(v8, E_MAX + 127) + 100) << 23);
       }
-      const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || k0 < first_seen(P, p_max);
+      const bool mask = valid != F::ALL || (P.causal && k0 + F::KEYS - 1 > p_min) || (P.window && k0 < first_seen(P, p_max));
       float s[F::NB][NR][4];
       float fk[F::NB][2], fv[F::NB][2];
 #pragma unroll
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(128, NR == 1 ? 3 : 2) few_rows_kernel(const __
             x *= E4M3 ? rowf[n][e & 1] * fk[kk][e >> 1] : rowf[n][e & 1];      // a key's scale is a power of two: first with the row's factor, a large query's sum may not have room for it
             if (mask) {
               const int at = kk * 16 + (e >> 1) * 8 + r, p = k0 + at, q = pos[n][e & 1];
-              if (!((valid >> at) & 1) || (P.causal && p > q) || p < first_seen(P, q)) x = -INFINITY;
+              if (!((valid >> at) & 1) || (P.causal && p > q) || (P.window && p < first_seen(P, q))) x = -INFINITY;
             }
             mx[n][e & 1] = fmaxf(mx[n][e & 1], x);
           }
