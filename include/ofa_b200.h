@@ -260,11 +260,11 @@ typedef struct {
 
 /* Keys and values (bf16, [n_rows][n_kv_heads][head_dim]) to their pages, in the cache's type: to 8 bits with the smallest power of two by which the row's largest
  * magnitude fits 448, rounded to nearest even. Rows whose position is negative or has no page are not kept. No two rows of a call may have the same
- * place (which of them it then holds is open), and the cache's rows may not overlap. */
+ * place (which of them it then holds is open), and the cache's rows, of keys and values together, may not overlap. */
 int ofa_kv_append(const ofa_kv_cache* cache, const ofa_kv_batch* batch, const void* k, const void* v, int n_rows,
                   long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream);
 /* The reverse: the rows of the call are read from their pages (all of a context with q_start counting kv_len) and are exact in bf16. Rows
- * without a place read as zeros. */
+ * without a place read as zeros. k and v do not overlap. */
 int ofa_kv_read(const ofa_kv_cache* cache, const ofa_kv_batch* batch, void* k, void* v, int n_rows,
                 long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride, void* stream);
 

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 using namespace ofa;
 
@@ -31,15 +32,23 @@ int launched(cudaError_t e, const char* what) {
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 // Whether places of `unit` elements at these strides lie upon one another: from the smallest stride up, each has to pass what lies inside it
 struct Axis { long long stride, count; };
-bool overlap(Axis a, Axis b, Axis c, long long unit) {
-  Axis x[3] = {a, b, c};
-  std::sort(x, x + 3, [](const Axis& u, const Axis& v) { return u.stride < v.stride; });
+bool overlap(Axis a, Axis b, Axis c, long long unit, Axis d = {0, 1}) {
+  Axis x[4] = {a, b, c, d};
+  std::sort(x, x + 4, [](const Axis& u, const Axis& v) { return u.stride < v.stride; });
   for (const Axis& i : x)
     if (i.count > 1) {
       if (i.stride < unit) return true;
       unit += i.stride * (i.count - 1);
     }
   return false;
+}
+
+// Whether two sets of such places, which start at p and q and are alike otherwise, lie upon one another: the second is one more axis, as far as it begins inside the longest step of the first
+bool twins(Axis a, Axis b, Axis c, long long unit, const void* p, const void* q, long long size) {
+  long long d = std::abs((long long)(reinterpret_cast<intptr_t>(p) - reinterpret_cast<intptr_t>(q))) / size, step = 0, end = unit;
+  for (const Axis& i : {a, b, c})
+    if (i.count > 1) { step = std::max(step, i.stride); end += i.stride * (i.count - 1); }
+  return d < end && overlap(a, b, c, unit, {step ? d % step : d, 2});
 }
 
 // ---- checks shared by the operators over a cache
@@ -106,21 +115,26 @@ template <bool READ> int move(const ofa_kv_cache* c, const ofa_kv_batch* b, void
   paged::MoveArgs P;
   if (int rc = check_cache(c, b, n_rows, P.b, P.c)) return rc;
   if (n_rows == 0 || b->n_seqs == 0) return OFA_OK;
+  const bool e4m3 = c->dtype == OFA_KV_E4M3;
   if (int rc = check_rows("k", k, {k_row, n_rows}, {k_head, c->n_kv_heads}, c->head_dim, READ)) return rc;
   if (int rc = check_rows("v", v, {v_row, n_rows}, {v_head, c->n_kv_heads}, c->head_dim, READ)) return rc;
   if (!READ && (overlap({c->page_stride, c->n_pages}, {c->head_stride, c->n_kv_heads}, {c->row_stride, c->page_size}, c->head_dim) ||
-                (c->dtype == OFA_KV_E4M3 && overlap({c->scale_page_stride, c->n_pages}, {c->scale_head_stride, c->n_kv_heads}, {c->scale_row_stride, c->page_size}, 1))))
+                (e4m3 && overlap({c->scale_page_stride, c->n_pages}, {c->scale_head_stride, c->n_kv_heads}, {c->scale_row_stride, c->page_size}, 1))))
     return fail(OFA_BAD_ARGUMENT, "rows of the cache overlap");
+  if (READ ? k_row == v_row && k_head == v_head && twins({k_row, n_rows}, {k_head, c->n_kv_heads}, {0, 1}, c->head_dim, k, v, 2)
+           : c->n_pages > 0 && (twins({c->page_stride, c->n_pages}, {c->head_stride, c->n_kv_heads}, {c->row_stride, c->page_size}, c->head_dim, c->k, c->v, e4m3 ? 1 : 2) ||
+                                (e4m3 && twins({c->scale_page_stride, c->n_pages}, {c->scale_head_stride, c->n_kv_heads}, {c->scale_row_stride, c->page_size}, 1, c->k_scale, c->v_scale, 1))))
+    return fail(OFA_BAD_ARGUMENT, "keys and values overlap where they are written");
   P.k = static_cast<bf16*>(k); P.v = static_cast<bf16*>(v); P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
   P.n_kv_heads = c->n_kv_heads; P.pair.set(2u * (unsigned)c->n_kv_heads);
   // four pieces of 16 bytes for a thread, in two turns, where there are rows for it: a block then amortises the search for its sequences
-  const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / (c->dtype == OFA_KV_E4M3 ? 16 : 8));
+  const long long per_row = 2ll * c->n_kv_heads * (c->head_dim / (e4m3 ? 16 : 8));
   long long rows = (1024 + per_row - 1) / per_row;
   while (rows > 1 && (n_rows + rows - 1) / rows < 148) rows--;
   P.rows = (int)(rows < paged::MOVE_ROWS ? rows : paged::MOVE_ROWS);
   const unsigned grid = (unsigned)((n_rows + P.rows - 1) / P.rows);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool e4m3 = c->dtype == OFA_KV_E4M3, small = c->head_dim == 64;
+  const bool small = c->head_dim == 64;
   const cudaError_t e = e4m3 ? small ? launch<paged::move_kernel<64, true, READ>>(grid, 256, 0, s, P) : launch<paged::move_kernel<128, true, READ>>(grid, 256, 0, s, P)
                              : small ? launch<paged::move_kernel<64, false, READ>>(grid, 256, 0, s, P) : launch<paged::move_kernel<128, false, READ>>(grid, 256, 0, s, P);
   return launched(e, READ ? "ofa_kv_read" : "ofa_kv_append");

@@ -303,3 +303,33 @@ def test_scores_of_every_size_over_many_steps(sv, hints, order, dtype):  # noqa:
         off = (p * (s.max(1, keepdim=True).values - s)).sum(1)[:, None] * 2.0 ** -22 + 2.0 ** -18
         assert ((out[:, 0].double().cpu() - p @ held).abs() <= (p @ held.abs()) * (ref.BF16_HALF + 2 * off) + (p @ held).abs() * ref.BF16_HALF * 1.01 + 1e-37).all()
         assert ((lse[:, 0].double().cpu() - want).abs() <= want.abs() * 2.0 ** -21 + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("layout", ["two_pools", "by_page", "by_head", "by_row", "v_first"])
+def test_keys_and_values_in_one_tensor(sv, layout, dtype):  # noqa: F811
+    """and rows read into one: whatever lies beside one another is taken"""
+    pages, heads, page, dim = 9, 2, 16, 64
+    t = torch.bfloat16 if dtype == "bf16" else torch.float8_e4m3fn
+
+    def pair(last, t):
+        both = {"two_pools": (2, pages, heads, page, *last), "v_first": (2, pages, heads, page, *last), "by_page": (pages, 2, heads, page, *last), "by_head": (pages, heads, 2, page, *last),
+                "by_row": (pages, heads, page, 2, *last)}[layout]
+        x = torch.zeros(both, dtype=torch.uint8 if t != torch.bfloat16 else t, device=DEV)
+        x = x.view(t) if t != torch.uint8 else x
+        axis = {"two_pools": 0, "v_first": 0, "by_page": 1, "by_head": 2, "by_row": 3}[layout]
+        k, v = x.select(axis, 0), x.select(axis, 1)
+        return (v, k) if layout == "v_first" else (k, v)
+    k, v = pair((dim,), t)
+    cache = sv.KVCache(k, v, *(pair((), torch.uint8) if dtype == "e4m3" else ()))
+    plain = sv.KVCache.empty(pages, page, heads, dim, dtype)
+    gen = torch.Generator().manual_seed(1)
+    rows = torch.randn(100, 2, 2, dim, generator=gen).bfloat16().to(DEV)
+    batch = sv.KVBatch(i32([0, 100]), i32([100]), i32([[4, 2, 8, 0, 1, 3, 7]]))
+    for c in (cache, plain):
+        sv.kv_append(c, batch, rows[:, 0], rows[:, 1])
+    into = torch.zeros(100, 2, 3, dim, dtype=torch.bfloat16, device=DEV)
+    got, want = sv.kv_read(cache, batch, k=into[:, :, 0], v=into[:, :, 2]), sv.kv_read(plain, batch, 100)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not into[:, :, 1].any()
+    q = queries(gen, 100, 4, dim)
+    assert torch.equal(sv.paged_attention(cache, batch, q), sv.paged_attention(plain, batch, q))
