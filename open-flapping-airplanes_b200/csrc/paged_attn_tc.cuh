@@ -9,7 +9,7 @@
 //              back over the second half of them as bf16, the A operand of the second product
 //   products   a warp a tile, one thread of which issues, in halves of 64 keys so that little of a step waits for all of the one before: the first half of the next scores as
 //              soon as the present ones are in registers, O += P V of each half when its probabilities are written, then the second half of the next scores. (4,096 tokens over
-//              16,384 keys, heads of 128: 843 us; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
+//              16,384 keys, heads of 128: 843 us, 860 now; without the early half 1,075. Steps of 64 keys with two buffers of scores waited least, but their fixed cost of 420 clocks came twice: 928;
 //              two threads a row, four softmax warps a scheduler: 910, bound by issue; a third of the exponentials by a polynomial on the multiply-add pipe: 970 and more, for registers and issue.)
 //              One thread a tile because one issues a tcgen05.mma only every ~96 clocks and a 128 x 128 x 16 product takes 64
 //   copies     one warp asks the copy engine for keys and values, in boxes of 8 to 64 rows of a page: bf16 rows into a ring of tiles in the layout the products read

@@ -149,8 +149,9 @@ struct Plan { bool many, cluster, by_head, ranked; int pair, rows, tiles, nsplit
 // How many blocks share a tile's keys: the number for which the call should take least, in units of 128 keys of a block: one block's time where all run at once, else all blocks' time over
 // the places for them and half a block's more for the end. What a block costs beside its keys (its first loads one after the other, the meeting at its end) measured 3 units of the tensor-core
 // kernel and 6 of the other, a second launch to join parts 3, and parts pass through memory at 5 TB/s, a unit being 1.6 us. Up to eight blocks of the few-row kernel are a cluster and need no parts.
-// (64 tokens over 2,048 to 4,096 8-bit keys: 99 us with one block a tile, 97 with two, 112 with four; a token over 1,000 keys, 12 heads of 64: 11.1, 8.7, 6.9 and 6.3 us with one, two, four and
-// eight; 4,096 tokens over 16,384 keys: 889 us with one, 914 with two.)
+// (64 tokens over 4,096 8-bit keys: 112 us with one block a tile, 108 with two, 121 with four; a token over 1,000 keys, 12 heads of 64: 10.3, 8.5, 6.8 and 6.2 us with one, two, four and
+// eight; two over 131,072 keys: 176 with twelve, 158 with 16, 170 with 24, 200 with 32; five tokens of 64 sequences over 4,096 keys 176 and 224. It takes the second, the last, 24 and the first
+// of these. Contexts are all taken for the longest: 64 uneven ones of up to 4,096 8-bit keys, the longest first, take 62 with one and 75 with two, which it chooses.)
 Plan plan(const ofa_kv_cache* c, const ofa_kv_batch* b, int n_rows, int n_heads) {
   Plan p;
   const long long group = n_heads / c->n_kv_heads;
